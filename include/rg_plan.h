@@ -78,6 +78,27 @@
  *     BODIES       n_bodies, per body: n_words, then a whole plan descriptor (header included)
  *                  whose constants lie in the same blob (scan: body; while: condition, body;
  *                  cond: then, else)
+ *   CAUSAL_CONV, CAUSAL_CONV_GRAD, SELECTIVE_SCAN, SELECTIVE_SCAN_GRAD, ROTARY_NORM,
+ *   ROTARY_NORM_GRAD
+ *                  flags, rotary dims, base (f64 bits), eps (f64 bits), n_sections, sections...,
+ *                  n_results, per result the program reads: result index, slot
+ *   Sequence operators (no reference counterpart; `sequence_of` says which operands follow which
+ *   flags, and their shapes). ROTARY_NORM writes `dst`; the others' `dst` is -1.
+ *     CAUSAL_CONV  in x[B,T,D], w[K,D] (, bias[D]) (, state[B,K-1,D]) (, lengths[B])
+ *                  out 0: y[t] = act(bias + sum_k w[k] past[t + k]), past = state (zeros without
+ *                  one) then x; 1: the K - 1 rows of past that end the sequence
+ *       _GRAD      in the same, dy (, d of result 1); out dx, dw, dbias, dstate
+ *     SELECTIVE_SCAN in x, dt[B,T,D], a[D,N], b, c[B,T,G,N] (, d[D]) (, z[B,T,D]) (, state[B,D,N])
+ *                  (, lengths[B]); h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t];
+ *                  out 0: (c[t] . h[t] + d x[t]) silu(z[t]); 1: the last h; 2: marks, h before
+ *                  positions 0, RG_SCAN_MARK, 2 RG_SCAN_MARK, ..., for the gradient alone
+ *       _GRAD      in the same, marks, dy (, d of result 1); out dx, ddt, da, db, dc, dd, dz, dstate
+ *     ROTARY_NORM  in x[B,T,H,hd], positions[T] or [B,T] (, gain[S,hd]); out x with the heads of
+ *                  section s divided by their root mean square and scaled by gain[s], and their
+ *                  pairs (i, i + R / 2), i < R / 2, turned by position * base^(-2 i / R)
+ *       _GRAD      in the same, dy; out dx, dgain
+ *   With lengths, positions from lengths[b] on (clamped to 0..T) are outside sequence b: their
+ *   results and gradients are 0, their inputs are not read into any other value.
  *   Control flow (plan.rs:737-831): the step's `dst` is -1 and its results go to the listed
  *   slots. Scan runs its body `length` times (from the last position when `reverse`) over
  *   inputs (carries, one slice of each x, captures); its results by index are the final
@@ -112,8 +133,23 @@ enum rg_op {
   RG_OP_CAST, RG_OP_STOP_GRADIENT, RG_OP_FLOOR, RG_OP_TAKE, RG_OP_TAKE_ALONG, RG_OP_TAKE_GRAD,
   RG_OP_TAKE_ALONG_GRAD, RG_OP_CONCAT, RG_OP_ARGMAX, RG_OP_RAND_UNIFORM, RG_OP_RAND_NORMAL,
   RG_OP_KEY_SPLIT, RG_OP_ARG_TOP_K, RG_OP_CUMSUM, RG_OP_SCAN, RG_OP_WHILE, RG_OP_COND,
-  RG_OP_OUTPUT, RG_OP_PLACEHOLDER, RG_OP_CUSTOM, RG_OP_COUNT
+  RG_OP_OUTPUT, RG_OP_PLACEHOLDER, RG_OP_CUSTOM, RG_OP_CAUSAL_CONV, RG_OP_CAUSAL_CONV_GRAD,
+  RG_OP_SELECTIVE_SCAN, RG_OP_SELECTIVE_SCAN_GRAD, RG_OP_ROTARY_NORM, RG_OP_ROTARY_NORM_GRAD,
+  RG_OP_COUNT
 };
+
+/* Flags of the sequence operators: which optional operands are present, and the variants. */
+enum rg_conv_flags { RG_CONV_BIAS = 1, RG_CONV_STATE = 2, RG_CONV_LENGTHS = 4, RG_CONV_SILU = 8, RG_CONV_CARRY = 16 };
+enum rg_scan_flags {
+  RG_SCAN_SKIP = 1, RG_SCAN_GATE = 2, RG_SCAN_STATE = 4, RG_SCAN_LENGTHS = 8, RG_SCAN_SOFTPLUS = 16, RG_SCAN_CARRY = 32
+};
+enum rg_rotary_flags { RG_ROTARY_GAIN = 1 };
+/* Taps of a causal convolution, states of a selective scan, and the length of a head. */
+#define RG_CONV_MAX_TAPS 8
+#define RG_SCAN_MAX_STATES 64
+#define RG_ROTARY_MAX_HEAD 256
+/* A selective scan keeps its state before every RG_SCAN_MARK-th position for its gradient. */
+#define RG_SCAN_MARK 16
 
 enum rg_reduce_kind { RG_REDUCE_SUM = 0, RG_REDUCE_MAX = 1, RG_REDUCE_MIN = 2 };
 /* Added to a row group's RG_OP_REDUCE `aux`: the reduction runs over the rows (a column reduction). */
@@ -140,13 +176,160 @@ struct Arg {
   std::vector<int64_t> shape;
 };
 
+/* The attributes of a sequence operator, before its results. */
+struct SequenceAttr {
+  int64_t flags = 0, turn = 0;
+  double base = 0, eps = 0;
+  std::vector<int64_t> sections;
+};
+
 struct Instr {
   int32_t op, dtype;
   int64_t dst, n, mode, node;
   std::vector<int64_t> shape;
   std::vector<Arg> args;
   std::vector<int64_t> attr;
+  SequenceAttr sequence;                         /* sequence operators */
+  std::vector<std::pair<int64_t, int64_t>> outs; /* theirs: (result index, slot) */
 };
+
+inline bool is_sequence(int32_t op) { return op >= RG_OP_CAUSAL_CONV && op <= RG_OP_ROTARY_NORM_GRAD; }
+/* Those whose results are numbered; ROTARY_NORM has one, in `dst`. */
+inline bool is_multi_result(int32_t op) { return is_sequence(op) && op != RG_OP_ROTARY_NORM; }
+
+/* A sequence operator's sizes, where its operands are among the arguments (-1: absent), and the
+ * shapes of its results. The one definition that the engine, the backend and the parser share. */
+struct Sequence {
+  int64_t batch = 0, length = 0, width = 0, taps = 0, states = 0, groups = 0, heads = 0, head = 0, used = 0;
+  int x = 0, w = -1, bias = -1, dt = -1, a = -1, b = -1, c = -1, skip = -1, gate = -1, state = -1, lengths = -1, marks = -1, dy = -1,
+      carry = -1, positions = -1, gain = -1;
+  bool shared_positions = false; /* positions of [length], the same for every sequence */
+  std::vector<std::vector<int64_t>> results;
+  std::string wrong; /* empty when the operands fit */
+};
+
+inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vector<std::vector<int64_t>>& s) {
+  Sequence q;
+  auto fail = [&](const char* what) {
+    if (q.wrong.empty()) q.wrong = what;
+  };
+  auto dims = [&](int k, const std::vector<int64_t>& want, const char* what) {
+    if (s[(size_t)k] != want) fail(what);
+  };
+  const int64_t f = at.flags;
+  int next = 1;
+  auto take = [&](bool present) { return present ? next++ : -1; };
+  const bool conv = op == RG_OP_CAUSAL_CONV || op == RG_OP_CAUSAL_CONV_GRAD, rotary = op == RG_OP_ROTARY_NORM || op == RG_OP_ROTARY_NORM_GRAD;
+  const bool grad = op == RG_OP_CAUSAL_CONV_GRAD || op == RG_OP_SELECTIVE_SCAN_GRAD || op == RG_OP_ROTARY_NORM_GRAD;
+  if (conv) {
+    q.w = take(true);
+    q.bias = take(f & RG_CONV_BIAS);
+    q.state = take(f & RG_CONV_STATE);
+    q.lengths = take(f & RG_CONV_LENGTHS);
+    q.dy = take(grad);
+    q.carry = take(grad && (f & RG_CONV_CARRY));
+  } else if (rotary) {
+    q.positions = take(true);
+    q.gain = take(f & RG_ROTARY_GAIN);
+    q.dy = take(grad);
+  } else {
+    q.dt = take(true);
+    q.a = take(true);
+    q.b = take(true);
+    q.c = take(true);
+    q.skip = take(f & RG_SCAN_SKIP);
+    q.gate = take(f & RG_SCAN_GATE);
+    q.state = take(f & RG_SCAN_STATE);
+    q.lengths = take(f & RG_SCAN_LENGTHS);
+    q.marks = take(grad);
+    q.dy = take(grad);
+    q.carry = take(grad && (f & RG_SCAN_CARRY));
+  }
+  if ((int)s.size() != next) {
+    fail("operand_count_does_not_match_the_flags");
+    return q;
+  }
+  const std::vector<int64_t>& x = s[0];
+  if (x.size() != (rotary ? 4u : 3u)) {
+    fail(rotary ? "x_must_be_batch_length_heads_head" : "x_must_be_batch_length_width");
+    return q;
+  }
+  for (const auto& v : s)
+    for (int64_t d : v)
+      if (d < 1) {
+        fail("empty_operand");
+        return q;
+      }
+  q.batch = x[0];
+  q.length = x[1];
+  q.width = x[2];
+  if (q.dy >= 0) dims(q.dy, x, "cotangent_shape_differs_from_x");
+  if (q.lengths >= 0) dims(q.lengths, {q.batch}, "lengths_must_be_one_per_sequence");
+  if (conv) {
+    const std::vector<int64_t>& w = s[(size_t)q.w];
+    if (w.size() != 2 || w[1] != q.width) {
+      fail("weights_must_be_taps_width");
+      return q;
+    }
+    q.taps = w[0];
+    if (q.taps < 2 || q.taps > RG_CONV_MAX_TAPS) fail("taps_must_be_two_to_eight");
+    const std::vector<int64_t> past = {q.batch, q.taps - 1, q.width};
+    if (q.bias >= 0) dims(q.bias, {q.width}, "bias_must_be_width");
+    if (q.state >= 0) dims(q.state, past, "state_must_be_batch_taps_less_one_width");
+    if (q.carry >= 0) dims(q.carry, past, "state_cotangent_shape");
+    if (grad) q.results = {x, w, {q.width}, past};
+    else q.results = {x, past};
+  } else if (rotary) {
+    q.heads = x[2];
+    q.head = x[3];
+    q.width = q.heads * q.head;
+    for (int64_t n : at.sections) {
+      if (n < 1) fail("sections_must_be_positive");
+      q.used += n;
+    }
+    if (at.sections.empty() || at.sections.size() > 4 || q.used > q.heads || q.used < 1) fail("sections_must_be_one_to_four_within_the_heads");
+    if (q.head % 2 != 0 || q.head > RG_ROTARY_MAX_HEAD) fail("head_must_be_even_and_at_most_256");
+    if (at.turn < 0 || at.turn % 2 != 0 || at.turn > q.head) fail("rotary_dims_must_be_even_and_within_the_head");
+    const std::vector<int64_t>& p = s[(size_t)q.positions];
+    q.shared_positions = p.size() == 1;
+    if (q.shared_positions) dims(q.positions, {q.length}, "positions_must_be_length_or_batch_length");
+    else dims(q.positions, {q.batch, q.length}, "positions_must_be_length_or_batch_length");
+    const std::vector<int64_t> gain = {(int64_t)at.sections.size(), q.head};
+    if (q.gain >= 0) dims(q.gain, gain, "gain_must_be_sections_head");
+    q.results = {x};
+    if (grad) q.results.push_back(gain);
+  } else {
+    const std::vector<int64_t>&a = s[(size_t)q.a], &b = s[(size_t)q.b];
+    if (a.size() != 2 || a[0] != q.width || a[1] > RG_SCAN_MAX_STATES) {
+      fail("a_must_be_width_by_at_most_64_states");
+      return q;
+    }
+    q.states = a[1];
+    if (b.size() != 4 || b[0] != q.batch || b[1] != q.length || b[3] != q.states || q.width % b[2] != 0) {
+      fail("b_must_be_batch_length_groups_states_with_groups_dividing_the_width");
+      return q;
+    }
+    q.groups = b[2];
+    const std::vector<int64_t> state = {q.batch, q.width, q.states};
+    const std::vector<int64_t> marks = {q.batch, (q.length + RG_SCAN_MARK - 1) / RG_SCAN_MARK, q.width, q.states};
+    dims(q.dt, x, "dt_shape_differs_from_x");
+    dims(q.c, b, "c_shape_differs_from_b");
+    if (q.skip >= 0) dims(q.skip, {q.width}, "d_must_be_width");
+    if (q.gate >= 0) dims(q.gate, x, "z_shape_differs_from_x");
+    if (q.state >= 0) dims(q.state, state, "state_must_be_batch_width_states");
+    if (q.carry >= 0) dims(q.carry, state, "state_cotangent_shape");
+    if (q.marks >= 0) dims(q.marks, marks, "marks_shape");
+    if (grad) q.results = {x, x, a, b, b, {q.width}, x, state};
+    else q.results = {x, state, marks};
+  }
+  return q;
+}
+
+inline Sequence sequence_of(const Instr& in) {
+  std::vector<std::vector<int64_t>> shapes;
+  for (const Arg& a : in.args) shapes.push_back(a.shape);
+  return sequence_of(in.op, in.sequence, shapes);
+}
 
 struct FusedInput {
   int64_t slot, kind, row_len, reg;
@@ -263,6 +446,22 @@ inline void check_refs(const Plan& pl) {
       if (in.dst != -1) fits(in.dst, in.n, (at + " output").c_str());
       for (const Arg& a : in.args)
         if (a.slot != -1) fits(a.slot, prod_of(a.shape), (at + " argument").c_str());
+      if (is_sequence(in.op)) {
+        const Sequence q = sequence_of(in);
+        if (!q.wrong.empty()) fail(at + ": " + q.wrong);
+        if (in.dtype != RG_F32 && in.dtype != RG_F64) fail(at + " is not of a floating-point dtype");
+        for (size_t j = 0; j < in.args.size(); j++) {
+          const int32_t want = (int)j == q.lengths || (int)j == q.positions ? (int32_t)RG_I32 : in.dtype;
+          if (in.args[j].slot < 0 || pl.slots[(size_t)in.args[j].slot].dtype != want) fail(at + " has an argument of another dtype");
+        }
+        if (!is_multi_result(in.op) && (in.dst < 0 || in.n != prod_of(q.results[0]) || pl.slots[(size_t)in.dst].dtype != in.dtype))
+          fail(at + " has a result of another size or dtype");
+        for (const auto& o : in.outs) {
+          if (o.first < 0 || (size_t)o.first >= q.results.size()) fail(at + " names a result it does not have");
+          fits(o.second, prod_of(q.results[(size_t)o.first]), (at + " result").c_str());
+          if (pl.slots[(size_t)o.second].dtype != in.dtype) fail(at + " has a result of another dtype");
+        }
+      }
     } else if (st.kind == RG_STEP_FUSED || st.kind == RG_STEP_ROWS) {
       const Fused& f = st.fused;
       const int64_t rows = f.row_len > 0 ? f.n / f.row_len : 0;
@@ -362,6 +561,30 @@ inline Plan parse(const int64_t* w, size_t nw) {
         in.args.push_back(arg);
       }
       in.attr = vec(next());
+      if (is_sequence(in.op)) {
+        size_t q = 0;
+        auto word = [&]() -> int64_t {
+          if (q >= in.attr.size()) throw std::runtime_error("sequence attributes truncated");
+          return in.attr[q++];
+        };
+        auto real = [&]() {
+          const int64_t bits = word();
+          double v;
+          memcpy(&v, &bits, 8);
+          return v;
+        };
+        in.sequence.flags = word();
+        in.sequence.turn = word();
+        in.sequence.base = real();
+        in.sequence.eps = real();
+        const int64_t ns2 = word();
+        for (int64_t j = 0; j < ns2; j++) in.sequence.sections.push_back(word());
+        const int64_t nr = word();
+        for (int64_t j = 0; j < nr; j++) {
+          const int64_t index = word();
+          in.outs.push_back({index, word()});
+        }
+      }
     } else if (st.kind == RG_STEP_FUSED || st.kind == RG_STEP_ROWS) {
       const bool rows = st.kind == RG_STEP_ROWS;
       Fused& f = st.fused;

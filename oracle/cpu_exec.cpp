@@ -27,6 +27,7 @@
 #include <vector>
 
 #include "../include/rg_plan.h"
+#include "sequence_ops.h"
 
 using namespace rgplan;
 
@@ -944,6 +945,12 @@ void step_float(const Instr& i, std::vector<Buf>& s) {
 }
 
 void exec_instr(const Plan& p, const Instr& i, std::vector<Buf>& s) {
+  if (is_sequence(i.op)) {
+    auto bytes = [&](int64_t slot) { return (void*)s[(size_t)slot].bytes.data(); };
+    if (i.dtype == RG_F32) rgseq::run<float>(i, bytes);
+    else rgseq::run<double>(i, bytes);
+    return;
+  }
   int arg_dtype = i.args.empty() ? i.dtype : p.slots[(size_t)i.args[0].slot].dtype;
   switch (i.op) {
     case RG_OP_CAST: cast(i, arg_dtype, s); return;

@@ -20,6 +20,7 @@ from .ops import (
 )
 from .transforms import custom_vjp, grad, hessian, jvp, value_and_grad
 from .control import cond, scan, while_loop
+from .sequence import causal_conv, rotary_norm, selective_scan
 from .program import Compiled, Report, RunResult, compile, devices, inspect, run
 from .checkpoint import load, save
 from . import nn, optim, random, tree

@@ -204,6 +204,17 @@ std::vector<std::pair<uint32_t, uint32_t>> vjp(Graph& g, size_t i, uint32_t ct, 
       break;
     }
     case RG_OP_TAKE_ALONG_GRAD: out.push_back({x, g.add(mk(RG_OP_TAKE_ALONG), {ct, y})}); break;
+    case RG_OP_ROTARY_NORM: {
+      Op o = node.op;
+      o.kind = RG_OP_ROTARY_NORM_GRAD;
+      std::vector<uint32_t> ins = node.inputs;
+      ins.push_back(ct);
+      const uint32_t grads = g.add(o, ins);
+      const int gain = g.sequence(node.op, node.inputs).gain;
+      if (rel[x]) out.push_back({x, g.result(grads, 0)});
+      if (gain >= 0 && rel[node.inputs[(size_t)gain]]) out.push_back({node.inputs[(size_t)gain], g.result(grads, 1)});
+      break;
+    }
     case RG_OP_CONCAT: {
       Shape shape = node.shape;
       size_t axis = node.op.a, at = 0;
@@ -505,6 +516,37 @@ std::vector<std::pair<uint32_t, uint32_t>> vjp_control(Graph& g, size_t i, const
   return out;
 }
 
+// Reverse rules of the sequence operators with several results: one gradient operator over the
+// operands and the results' cotangents (the scan's also reads the marks its forward kept).
+std::vector<std::pair<uint32_t, uint32_t>> vjp_sequence(Graph& g, size_t i, const std::map<size_t, uint32_t>& cots,
+                                                        const std::vector<bool>& rel) {
+  const Node node = g.nodes[i];
+  const bool conv = node.op.kind == RG_OP_CAUSAL_CONV;
+  if (!conv && node.op.kind != RG_OP_SELECTIVE_SCAN) {
+    Json obs = Json::obj();
+    obs["operation"] = node.op.name();
+    throw DiagError{diag("GRAD_UNSUPPORTED", "error", g.node_json((uint32_t)i), obs, "no_vjp_rule_for_operation", "verified")};
+  }
+  const rgplan::Sequence q = g.sequence(node.op, node.inputs);
+  Op o = node.op;
+  o.kind = conv ? RG_OP_CAUSAL_CONV_GRAD : RG_OP_SELECTIVE_SCAN_GRAD;
+  std::vector<uint32_t> ins = node.inputs;
+  if (!conv) ins.push_back(g.result((uint32_t)i, 2));
+  auto dy = cots.find(0), carry = cots.find(1);
+  ins.push_back(dy != cots.end() ? dy->second : zeros(g, g.shape(node.inputs[0]), node.dtype));
+  if (carry != cots.end()) {
+    o.a |= (size_t)(conv ? (int)RG_CONV_CARRY : (int)RG_SCAN_CARRY);
+    ins.push_back(carry->second);
+  }
+  const uint32_t grads = g.add(o, ins);
+  std::vector<std::pair<uint32_t, uint32_t>> out;
+  const std::vector<int> operands = conv ? std::vector<int>{q.x, q.w, q.bias, q.state}
+                                         : std::vector<int>{q.x, q.dt, q.a, q.b, q.c, q.skip, q.gate, q.state};
+  for (size_t k = 0; k < operands.size(); k++)
+    if (operands[k] >= 0 && rel[node.inputs[(size_t)operands[k]]]) out.push_back({node.inputs[(size_t)operands[k]], g.result(grads, k)});
+  return out;
+}
+
 }  // namespace
 
 std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wrts) {
@@ -545,7 +587,7 @@ std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wr
   std::vector<int64_t> cot(end + 1, -1);
   if (rel[end]) cot[end] = g.constant(Tensor::full(g.dtype(y), g.shape(y), 1.0));
   for (size_t i = end + 1; i-- > 0;) {
-    if (g.nodes[i].op.is_control_flow()) {
+    if (g.nodes[i].op.has_results()) {
       if (!rel[i]) continue;
       // The node's results are its later RG_OP_OUTPUT readers, whose cotangents are complete.
       std::map<size_t, uint32_t> cots;
@@ -556,7 +598,7 @@ std::vector<uint32_t> grad(Graph& g, uint32_t y, const std::vector<uint32_t>& wr
       if (cots.empty()) continue;
       g.cur_source = g.nodes[i].source;
       g.cur_origin = (int64_t)i;
-      for (auto& [input, c] : vjp_control(g, i, cots, rel))
+      for (auto& [input, c] : g.nodes[i].op.is_sequence() ? vjp_sequence(g, i, cots, rel) : vjp_control(g, i, cots, rel))
         cot[input] = cot[input] >= 0 ? (int64_t)bin(g, RG_OP_ADD, (uint32_t)cot[input], c) : (int64_t)c;
       continue;
     }

@@ -2,6 +2,7 @@
 #include "graph.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdio>
 
 namespace rg {
@@ -65,6 +66,12 @@ const char* Op::name() const {
     case RG_OP_OUTPUT: return "output";
     case RG_OP_PLACEHOLDER: return "placeholder";
     case RG_OP_CUSTOM: return "custom_vjp";
+    case RG_OP_CAUSAL_CONV: return "causal_conv";
+    case RG_OP_CAUSAL_CONV_GRAD: return "causal_conv_grad";
+    case RG_OP_SELECTIVE_SCAN: return "selective_scan";
+    case RG_OP_SELECTIVE_SCAN_GRAD: return "selective_scan_grad";
+    case RG_OP_ROTARY_NORM: return "rotary_norm";
+    case RG_OP_ROTARY_NORM_GRAD: return "rotary_norm_grad";
     default: return "unknown";
   }
 }
@@ -137,6 +144,11 @@ std::string Op::key() const {
   if (kind == RG_OP_CUSTOM) {
     k += ":C" + std::to_string(placeholder);
     for (auto& r : rules) k += "," + std::to_string(r.first) + "/" + std::to_string(r.second);
+  }
+  if (is_sequence()) {
+    char reals[80];
+    snprintf(reals, sizeof reals, ":R%zu,%a,%a", turn, base, eps);
+    k += reals;
   }
   if (is_control_flow()) {
     char ids[64];
@@ -237,7 +249,7 @@ uint32_t Graph::add(const Op& op, const std::vector<uint32_t>& inputs) {
       arity = 2; break;
     case RG_OP_CONCAT: arity = std::max<size_t>(inputs.size(), 1); break;
     default:
-      if (op.is_control_flow()) arity = inputs.size();
+      if (op.is_control_flow() || op.is_sequence()) arity = inputs.size();
       else if (op.is_binary_elementwise()) arity = 2;
       else arity = 1;
   }
@@ -251,11 +263,28 @@ uint32_t Graph::add(const Op& op, const std::vector<uint32_t>& inputs) {
     check_control_flow(op, inputs);
     return push(op, inputs, {}, DType::F32);
   }
+  if (op.is_sequence()) {
+    check_sequence(op, inputs);
+    const DType d = dtype(inputs[0]);
+    return push(op, inputs, op.has_results() ? Shape{} : shape(inputs[0]), d);
+  }
   if (op.kind == RG_OP_OUTPUT) {
-    if (inputs.size() != 1 || !nodes[inputs[0]].op.is_control_flow()) {
+    if (inputs.size() != 1 || !nodes[inputs[0]].op.has_results()) {
       Json obs = Json::obj();
       obs["input"] = inputs.empty() ? Json() : Json(nodes[inputs[0]].op.name());
       static_err("INVALID_NODE_REF", op, obs, "output_reads_a_control_flow_node");
+    }
+    const Node& of = nodes[inputs[0]];
+    if (of.op.is_sequence()) {
+      const rgplan::Sequence q = sequence(of.op, of.inputs);
+      Shape want;
+      if (op.a < q.results.size()) want.assign(q.results[op.a].begin(), q.results[op.a].end());
+      if (op.a >= q.results.size() || op.v != want || op.dt != of.dtype) {
+        Json obs = Json::obj();
+        obs["input"] = of.op.name();
+        obs["index"] = (long long)op.a;
+        static_err("INVALID_NODE_REF", op, obs, "output_differs_from_the_operators_result");
+      }
     }
     return push(op, inputs, op.v, op.dt);
   }
@@ -627,6 +656,57 @@ void Graph::check_control_flow(const Op& op, const std::vector<uint32_t>& inputs
     }
     default: break;
   }
+}
+
+rgplan::SequenceAttr Op::sequence_attr() const {
+  rgplan::SequenceAttr at;
+  at.flags = (int64_t)a;
+  at.turn = (int64_t)turn;
+  at.base = base;
+  at.eps = eps;
+  at.sections.assign(v.begin(), v.end());
+  return at;
+}
+
+rgplan::Sequence Graph::sequence(const Op& op, const std::vector<uint32_t>& inputs) const {
+  std::vector<std::vector<int64_t>> shapes;
+  for (uint32_t i : inputs) shapes.emplace_back(shape(i).begin(), shape(i).end());
+  return rgplan::sequence_of(op.kind, op.sequence_attr(), shapes);
+}
+
+// Sequence operators: shapes by the definition all executors share, one floating-point dtype, and
+// int32 lengths and positions.
+void Graph::check_sequence(const Op& op, const std::vector<uint32_t>& inputs) const {
+  Json shapes = Json::arr(), names = Json::arr();
+  for (uint32_t i : inputs) {
+    shapes.push(shape_json(shape(i)));
+    names.push(dname(dtype(i)));
+  }
+  auto fail = [&](const char* code, const char* cause) {
+    Json obs = Json::obj();
+    obs["input_shapes"] = shapes;
+    obs["input_dtypes"] = names;
+    static_err(code, op, obs, cause);
+  };
+  if (inputs.empty()) fail("ARITY_MISMATCH", "wrong_input_count");
+  const rgplan::Sequence q = sequence(op, inputs);
+  if (!q.wrong.empty()) fail("SHAPE_MISMATCH", q.wrong.c_str());
+  const DType d = dtype(inputs[0]);
+  if (d == DType::I32) fail("UNSUPPORTED_DTYPE", "operation_is_float_only_cast_first");
+  for (size_t k = 0; k < inputs.size(); k++) {
+    const bool index = (int)k == q.lengths || (int)k == q.positions;
+    if (index && dtype(inputs[k]) != DType::I32) fail("DTYPE_MISMATCH", "lengths_and_positions_must_be_int32");
+    if (!index && dtype(inputs[k]) != d) fail("DTYPE_MISMATCH", "implicit_promotion_not_allowed");
+  }
+  const bool rotary = op.kind == RG_OP_ROTARY_NORM || op.kind == RG_OP_ROTARY_NORM_GRAD;
+  if (rotary && (!(op.base > 0) || !std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)))
+    fail("INVALID_ARGUMENT", "base_must_be_positive_and_eps_not_negative");
+}
+
+uint32_t Graph::result(uint32_t node, size_t index) {
+  const Node& n = nodes[node];
+  const rgplan::Sequence q = sequence(n.op, n.inputs);
+  return output(node, index, Shape(q.results[index].begin(), q.results[index].end()), n.dtype);
 }
 
 uint32_t Graph::output(uint32_t node, size_t index, const Shape& s, DType d) {

@@ -126,6 +126,9 @@ struct Op {
   // branch's. The node itself has shape [] and each result is an RG_OP_OUTPUT node reading it.
   std::shared_ptr<const Body> body, body2;
   size_t n_carry = 0, n_x = 0, length = 0, max_iter = 0;
+  // Sequence operators (include/rg_plan.h): `a` holds the flags, `v` the sections.
+  size_t turn = 0;
+  double base = 0, eps = 0;
 
   static Op make(rg_op k) {
     Op o;
@@ -138,6 +141,10 @@ struct Op {
   bool is_control_flow() const {
     return kind == RG_OP_SCAN || kind == RG_OP_WHILE || kind == RG_OP_COND;
   }
+  bool is_sequence() const { return rgplan::is_sequence(kind); }
+  // Operations whose node has shape [] and whose results are RG_OP_OUTPUT nodes reading it.
+  bool has_results() const { return is_control_flow() || rgplan::is_multi_result(kind); }
+  rgplan::SequenceAttr sequence_attr() const;
   bool int_ok() const;
   bool is_nonsmooth() const;
   // The identity of an operation with its attributes, for common-subexpression elimination.
@@ -180,6 +187,10 @@ class Graph {
   std::vector<bool> reachable(const std::vector<uint32_t>& outputs) const;
   // The RG_OP_OUTPUT node reading result `index` of control-flow node `node`.
   uint32_t output(uint32_t node, size_t index, const Shape& shape, DType dtype);
+  // Result `index` of sequence operator `node`.
+  uint32_t result(uint32_t node, size_t index);
+  // Sizes, operands and results of a sequence operator on these inputs.
+  rgplan::Sequence sequence(const Op& op, const std::vector<uint32_t>& inputs) const;
   Graph to_f64() const;
   Json node_json(uint32_t id) const;
 
@@ -188,6 +199,7 @@ class Graph {
   Json pending_json(const Op& op) const;
   [[noreturn]] void static_err(const char* code, const Op& op, Json obs, const char* cause) const;
   Shape infer(const Op& op, const std::vector<Shape>& s) const;
+  void check_sequence(const Op& op, const std::vector<uint32_t>& inputs) const;
   void check_control_flow(const Op& op, const std::vector<uint32_t>& inputs) const;
 };
 

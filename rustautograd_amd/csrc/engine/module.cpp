@@ -147,6 +147,16 @@ Op parse_op(const std::string& name, const py::object& a) {
   } else if (name == "take_along_grad") {
     o.kind = RG_OP_TAKE_ALONG_GRAD;
     o.v = attr<Shape>(a, "shape");
+  } else if (name == "causal_conv" || name == "selective_scan") {
+    o.kind = name == "causal_conv" ? RG_OP_CAUSAL_CONV : RG_OP_SELECTIVE_SCAN;
+    o.a = attr<size_t>(a, "flags");
+  } else if (name == "rotary_norm") {
+    o.kind = RG_OP_ROTARY_NORM;
+    o.a = attr<size_t>(a, "flags");
+    o.v = attr<Shape>(a, "sections");
+    o.turn = attr<size_t>(a, "rotary_dims");
+    o.base = attr<double>(a, "base");
+    o.eps = attr<double>(a, "eps");
   } else {
     throw py::value_error("unknown op " + name);
   }
@@ -279,6 +289,12 @@ PYBIND11_MODULE(_rg, m) {
              return g.g.output(node, index, shape, dtype_of(dtype));
            },
            py::arg("node"), py::arg("index"), py::arg("shape"), py::arg("dtype"), py::arg("source") = py::none())
+      .def("result",
+           [](PyGraph& g, uint32_t node, size_t index, std::optional<std::string> source) {
+             g.set_source(source);
+             return g.g.result(node, index);
+           },
+           py::arg("node"), py::arg("index"), py::arg("source") = py::none())
       .def_property_readonly("n_inputs", [](const PyGraph& g) { return g.g.n_inputs; })
       .def("placeholder",
            [](PyGraph& g, const std::vector<size_t>& shape, const std::string& dtype) {
@@ -391,6 +407,7 @@ PYBIND11_MODULE(_rg, m) {
                  d["shape"] = s.instr.shape;
                  d["arg_shapes"] = s.instr.arg_shapes;
                  d["dst"] = s.instr.dst;
+                 d["outs"] = s.instr.outs;
                  d["args"] = s.instr.args;
                }
                out.append(d);

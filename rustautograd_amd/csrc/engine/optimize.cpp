@@ -236,7 +236,7 @@ Simplified simplify(const Graph& g, const std::vector<uint32_t>& outputs, bool d
         r.st.simplified++;
       }
     }
-    bool foldable = !op.is_control_flow() && op.kind != RG_OP_OUTPUT && !ins.empty() && node.n() <= FOLD_LIMIT;
+    bool foldable = !op.has_results() && op.kind != RG_OP_OUTPUT && !ins.empty() && node.n() <= FOLD_LIMIT;
     for (uint32_t x : ins) foldable = foldable && ng.nodes[x].op.kind == RG_OP_CONST;
     if (foldable) {
       Graph tmp;

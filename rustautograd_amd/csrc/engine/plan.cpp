@@ -1138,7 +1138,7 @@ Plan build_with(const Graph& g, const std::vector<uint32_t>& outputs, bool reuse
       in.arg_shapes.push_back(g.shape(x));
       in.args.push_back(value_slot[x]);
     }
-    if (node.op.is_control_flow()) {
+    if (node.op.has_results()) {
       // Results get slots before the inputs are released, so none lands on an input's buffer
       // (plan.rs:611-620); the bodies are planned like the program itself.
       for (uint32_t x : node.inputs) uses[x]--;
@@ -1348,6 +1348,24 @@ StepWork step_work(const Step& s, const PriceFn& price) {
       if (w.compute) w.peak_factor = factor;
       return w;
     }
+    case RG_OP_CAUSAL_CONV: case RG_OP_CAUSAL_CONV_GRAD: case RG_OP_SELECTIVE_SCAN: case RG_OP_SELECTIVE_SCAN_GRAD: {
+      // Operands once and the results that are read; a scan's marks are the operator's own.
+      std::vector<std::vector<int64_t>> shapes;
+      for (auto& a : i.arg_shapes) shapes.emplace_back(a.begin(), a.end());
+      const rgplan::Sequence q = rgplan::sequence_of(i.op.kind, i.op.sequence_attr(), shapes);
+      double elems = in_elems - (q.marks >= 0 ? (double)numel(i.arg_shapes[(size_t)q.marks]) : 0.0);
+      for (auto& o : i.outs)
+        if (i.op.kind != RG_OP_SELECTIVE_SCAN || o.first != 2) {
+          double n = 1;
+          for (int64_t d : q.results[o.first]) n *= (double)d;
+          elems += n;
+        }
+      w.bytes = elems * ds;
+      return w;
+    }
+    case RG_OP_ROTARY_NORM_GRAD:
+      w.bytes = (in_elems + (double)numel(i.arg_shapes[0])) * ds;
+      return w;
     case RG_OP_TAKE:
     case RG_OP_TAKE_ALONG:
       // The indices, and each gathered element read once and written once.
@@ -1395,6 +1413,7 @@ std::vector<size_t> step_writes(const Step& st) {
     for (auto& o : st.group.outputs) w.push_back(o.second);
   } else {
     w.push_back(st.instr.dst);
+    for (auto& o : st.instr.outs) w.push_back(o.second);
   }
   return w;
 }
@@ -1485,6 +1504,26 @@ static void put_op_attr(std::vector<int64_t>& a, const Op& op) {
     case RG_OP_RAND_UNIFORM: case RG_OP_RAND_NORMAL: a.push_back((int64_t)op.dt); vec(op.v); break;
     case RG_OP_CUMSUM: a.push_back(op.reverse); break;
     default: break;
+  }
+}
+
+// Sequence operators: their attributes, then the result slots.
+static void put_sequence_attr(std::vector<int64_t>& a, const Instr& in) {
+  auto real = [&](double v) {
+    int64_t bits;
+    memcpy(&bits, &v, 8);
+    a.push_back(bits);
+  };
+  a.push_back((int64_t)in.op.a);
+  a.push_back((int64_t)in.op.turn);
+  real(in.op.base);
+  real(in.op.eps);
+  a.push_back((int64_t)in.op.v.size());
+  for (auto n : in.op.v) a.push_back((int64_t)n);
+  a.push_back((int64_t)in.outs.size());
+  for (auto& [index, slot] : in.outs) {
+    a.push_back((int64_t)index);
+    a.push_back((int64_t)slot);
   }
 }
 
@@ -1618,6 +1657,7 @@ static void write_plan(const Plan& plan, std::vector<int64_t>* words, std::vecto
       }
       std::vector<int64_t> attr;
       if (in.op.is_control_flow()) put_control_attr(attr, in, blob);
+      else if (in.op.is_sequence()) put_sequence_attr(attr, in);
       else put_op_attr(attr, in.op);
       w.push_back((int64_t)attr.size());
       w.insert(w.end(), attr.begin(), attr.end());

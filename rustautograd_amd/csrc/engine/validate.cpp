@@ -339,7 +339,20 @@ struct Observer {
       }
     }
     if (i.dtype == DType::I32) return;
-    Tensor dst = e.prefix(i.dst, i.n, i.shape);
+    Tensor dst;
+    if (i.op.has_results()) {
+      // The first result with a value that is not finite, if any.
+      std::vector<std::vector<int64_t>> shapes;
+      for (auto& a : i.arg_shapes) shapes.emplace_back(a.begin(), a.end());
+      const rgplan::Sequence q = rgplan::sequence_of(i.op.kind, i.op.sequence_attr(), shapes);
+      for (auto& [index, slot] : i.outs) {
+        const Shape s(q.results[index].begin(), q.results[index].end());
+        dst = e.prefix(slot, numel(s), s);
+        if (any_nonfinite(dst)) break;
+      }
+    } else {
+      dst = e.prefix(i.dst, i.n, i.shape);
+    }
     if (!any_nonfinite(dst)) return;
     std::vector<Stats> args;
     std::vector<Tensor> argv;
@@ -354,7 +367,7 @@ struct Observer {
       return;
     }
     if (o.roots.size() == MAX_ROOTS) return;
-    Stats out = stats_of(dst, i.n);
+    Stats out = stats_of(dst, dst.n());
     Classified c = classify(i, args, out);
     int64_t bad = out.first_bad;
     bool elementwise = i.op.is_unary_elementwise() || i.op.is_binary_elementwise();
@@ -380,7 +393,7 @@ struct Observer {
       ins.push(a);
     }
     obs["inputs"] = ins;
-    obs["output_shape"] = Json(i.shape);
+    obs["output_shape"] = Json(dst.shape);
     obs["output_contains_inf"] = out.inf > 0;
     obs["output_contains_nan"] = out.nan > 0;
     obs["nonfinite_count"] = out.nan + out.inf;

@@ -24,6 +24,7 @@
 #include "jit.h"
 #include "kernels.h"
 #include "noalloc.h"
+#include "sequence.h"
 
 using namespace rgplan;
 
@@ -550,6 +551,159 @@ StepFn lower_instr(Program& prog, const Instr& i) {
   }
 }
 
+// A sequence operator (sequence.hip). Results that nothing reads have no slot and are not written;
+// sums over the batch and its positions leave partial rows in the fold area, folded with the other
+// deferred folds.
+StepFn lower_sequence(Program& prog, const Instr& i) {
+  const Sequence q = sequence_of(i);
+  const int dtype = i.dtype;
+  std::vector<int64_t> args, outs(std::max<size_t>(q.results.size(), 1), -1);
+  for (auto& a : i.args) args.push_back(a.slot);
+  for (auto& o : i.outs) outs[(size_t)o.first] = o.second;
+  const bool conv = i.op == RG_OP_CAUSAL_CONV || i.op == RG_OP_CAUSAL_CONV_GRAD;
+  const bool rotary = i.op == RG_OP_ROTARY_NORM || i.op == RG_OP_ROTARY_NORM_GRAD;
+  const Program* pp = &prog;
+  auto slot = [](void* const* sl, int64_t s) { return s < 0 ? nullptr : sl[s]; };
+  auto arg = [args, slot](void* const* sl, int k) { return k < 0 ? nullptr : slot(sl, args[(size_t)k]); };
+  // Where result r's `rows` partial rows of k values go: -1 nowhere, else their place in the fold
+  // area.
+  auto partial = [&](size_t r, uint32_t rows, uint64_t k) {
+    if (outs[r] < 0) return (int64_t)-1;
+    if (k >= (1ull << 31)) throw std::runtime_error("a partial row of " + std::to_string(k) + " values exceeds the 2^31 element index range");
+    const uint64_t off = prog.fold_bytes;
+    Program::Fold fd{off, outs[r], rows, (uint32_t)k, RG_REDUCE_SUM, dtype};
+    fd.wide = dtype == RG_F32 && k % 4 == 0 && rows <= 16;
+    prog.folds.push_back(fd);
+    prog.fold_bytes += ((uint64_t)rows * k * esize(dtype) + 255) / 256 * 256;
+    return (int64_t)off;
+  };
+  auto place = [pp](void* ws, int64_t off) { return off < 0 ? nullptr : (void*)((char*)ws + pp->fold_base() + off); };
+  if (conv) {
+    rgk::ConvArgs base{};
+    base.batch = (uint32_t)q.batch;
+    base.length = (uint32_t)q.length;
+    base.width = (uint32_t)q.width;
+    base.taps = (uint32_t)q.taps;
+    base.silu = (i.sequence.flags & RG_CONV_SILU) != 0;
+    const bool grad = i.op == RG_OP_CAUSAL_CONV_GRAD;
+    const uint32_t rows = rgk::conv_grad_rows(dtype, base);
+    const int64_t dw = grad ? partial(1, rows, (uint64_t)q.taps * q.width) : -1, db = grad ? partial(2, rows, (uint64_t)q.width) : -1;
+    return [=](hipStream_t s, void* const* sl, void* ws) {
+      rgk::ConvArgs a = base;
+      a.x = arg(sl, q.x);
+      a.w = arg(sl, q.w);
+      a.bias = arg(sl, q.bias);
+      a.state = arg(sl, q.state);
+      a.lengths = (const int32_t*)arg(sl, q.lengths);
+      if (!grad) {
+        a.y = slot(sl, outs[0]);
+        a.next = slot(sl, outs[1]);
+        rgk::causal_conv(s, dtype, a);
+        return;
+      }
+      a.dy = arg(sl, q.dy);
+      a.carry = arg(sl, q.carry);
+      a.dx = slot(sl, outs[0]);
+      a.dstate = slot(sl, outs[3]);
+      a.dw_rows = place(ws, dw);
+      a.db_rows = place(ws, db);
+      rgk::causal_conv_grad(s, dtype, a);
+    };
+  }
+  if (rotary) {
+    rgk::RotaryArgs base{};
+    base.batch = (uint32_t)q.batch;
+    base.length = (uint32_t)q.length;
+    base.heads = (uint32_t)q.heads;
+    base.head = (uint32_t)q.head;
+    base.turn = (uint32_t)i.sequence.turn;
+    base.sections = (uint32_t)i.sequence.sections.size();
+    uint32_t last = 0;
+    for (size_t k = 0; k < i.sequence.sections.size(); k++) base.last[k] = last += (uint32_t)i.sequence.sections[k];
+    base.eps = i.sequence.eps;
+    base.normed = q.gain >= 0;
+    base.shared_positions = q.shared_positions;
+    if ((uint64_t)q.batch * q.length >= (1ull << 31)) throw std::runtime_error("more than 2^31 positions in one rotation");
+    if (base.turn > 0) {
+      // Turns per position of each pair, its double and what that leaves out.
+      std::vector<double> turns;
+      for (uint32_t k = 0; k < base.turn / 2; k++) {
+        const long double v = powl((long double)i.sequence.base, -2.0L * k / base.turn) / (2.0L * 3.14159265358979323846264338327950288L);
+        turns.push_back((double)v);
+        turns.push_back((double)(v - (long double)(double)v));
+      }
+      void* table = nullptr;
+      HIP_OK(hipMalloc(&table, turns.size() * 8));
+      prog.device_tables.push_back(table);
+      HIP_OK(hipMemcpy(table, turns.data(), turns.size() * 8, hipMemcpyHostToDevice));
+      base.turns = (const double2*)table;
+    }
+    const bool grad = i.op == RG_OP_ROTARY_NORM_GRAD;
+    const int64_t dst = i.dst, dgain = grad && base.normed ? partial(1, rgk::rotary_grad_rows(dtype, base), (uint64_t)base.sections * q.head) : -1;
+    return [=](hipStream_t s, void* const* sl, void* ws) {
+      rgk::RotaryArgs a = base;
+      a.x = arg(sl, q.x);
+      a.positions = (const int32_t*)arg(sl, q.positions);
+      a.gain = arg(sl, q.gain);
+      if (!grad) {
+        a.y = sl[dst];
+        rgk::rotary_norm(s, dtype, a);
+        return;
+      }
+      a.dy = arg(sl, q.dy);
+      a.dx = slot(sl, outs[0]);
+      a.dgain_rows = place(ws, dgain);
+      rgk::rotary_norm_grad(s, dtype, a);
+    };
+  }
+  rgk::ScanArgs base{};
+  base.batch = (uint32_t)q.batch;
+  base.length = (uint32_t)q.length;
+  base.width = (uint32_t)q.width;
+  base.states = (uint32_t)q.states;
+  base.groups = (uint32_t)q.groups;
+  base.softplus = (i.sequence.flags & RG_SCAN_SOFTPLUS) != 0;
+  const bool grad = i.op == RG_OP_SELECTIVE_SCAN_GRAD;
+  const uint32_t tiles = rgk::scan_group_tiles(dtype, base), rows = rgk::scan_rows(dtype, base);
+  const uint64_t maps = (uint64_t)q.batch * q.length * q.groups * q.states;
+  // One tile of channels a group: its sums are the results.
+  const bool direct = tiles == 1;
+  const int64_t db = grad && !direct ? partial(3, tiles, maps) : -1, dc = grad && !direct ? partial(4, tiles, maps) : -1;
+  const int64_t da = grad ? partial(2, rows, (uint64_t)q.width * q.states) : -1;
+  const int64_t dd = grad && q.skip >= 0 ? partial(5, rows, (uint64_t)q.width) : -1;
+  return [=](hipStream_t s, void* const* sl, void* ws) {
+    rgk::ScanArgs a = base;
+    a.x = arg(sl, q.x);
+    a.dt = arg(sl, q.dt);
+    a.a = arg(sl, q.a);
+    a.b = arg(sl, q.b);
+    a.c = arg(sl, q.c);
+    a.skip = arg(sl, q.skip);
+    a.gate = arg(sl, q.gate);
+    a.state = arg(sl, q.state);
+    a.lengths = (const int32_t*)arg(sl, q.lengths);
+    if (!grad) {
+      a.y = slot(sl, outs[0]);
+      a.last = slot(sl, outs[1]);
+      a.marks = slot(sl, outs[2]);
+      rgk::selective_scan(s, dtype, a);
+      return;
+    }
+    a.marks = arg(sl, q.marks);
+    a.dy = arg(sl, q.dy);
+    a.carry = arg(sl, q.carry);
+    a.dx = slot(sl, outs[0]);
+    a.ddt = slot(sl, outs[1]);
+    a.db_rows = direct ? slot(sl, outs[3]) : place(ws, db);
+    a.dc_rows = direct ? slot(sl, outs[4]) : place(ws, dc);
+    a.da_rows = place(ws, da);
+    a.dd_rows = place(ws, dd);
+    a.dz = slot(sl, outs[6]);
+    a.dstate = slot(sl, outs[7]);
+    rgk::selective_scan_grad(s, dtype, a);
+  };
+}
+
 // A fused attention step (attention.hip). The statistics slot holds the per-query max, sum and
 // rowsum(dO * O), then the packed mask bits.
 StepFn lower_attention(Program& prog, const rgplan::Attn& at, int64_t col_off = -1) {
@@ -749,6 +903,8 @@ std::vector<int64_t> step_writes(const Step& st) {
     if (st.attn.build_bits) w.push_back(st.attn.mask_bits_slot);
   } else if (st.instr.dst >= 0) {
     w.push_back(st.instr.dst);
+  } else {
+    for (auto& o : st.instr.outs) w.push_back(o.second);  // a sequence operator's results
   }
   return w;
 }
@@ -1359,6 +1515,8 @@ void build_program(Program& prog) {
         const bool ta = in.op == RG_OP_MATMUL_T && in.attr[0] != 0, tb = in.op == RG_OP_MATMUL_T && in.attr[1] != 0;
         gemm_fills[k] = gemm_fill(prog, in, ta, tb, &gemm_base[k]);
         prog.steps.push_back(gemm_step(gemm_fills[k]));
+      } else if (is_sequence(in.op)) {
+        prog.steps.push_back(lower_sequence(prog, in));
       } else {
         prog.steps.push_back(lower_instr(prog, in));
       }

@@ -10,8 +10,9 @@ reference's python/rg/nn.py; the code is this package's own.
 import math
 
 from . import random
-from .ops import (abs, argmax, argsort, concatenate, cumsum, equal, exp, eye, maximum, ones, stop_gradient, swapaxes,
-                  take, take_along_axis, tanh, top_k, where, zeros)
+from .ops import (abs, arange, argmax, argsort, broadcast_to, concatenate, cumsum, equal, exp, eye, log, maximum, ones,
+                  stop_gradient, swapaxes, take, take_along_axis, tanh, top_k, where, zeros)
+from .sequence import causal_conv, rotary_norm, selective_scan
 
 _GELU_C = math.sqrt(2.0 / math.pi)
 _MASKED = -1e9  # the score of a position a mask hides, and the logit of a filtered token
@@ -228,26 +229,38 @@ class LayerNorm(Layer):
 
 class MultiHeadAttention(Layer):
     """Self-attention over `heads` heads of `d // heads`. `mask` broadcasts to (T, T); nonzero
-    means visible. With `key` and a dropout rate, the weights and the output are dropped out."""
+    means visible. With `key` and a dropout rate, the weights and the output are dropped out.
+    `qk_norm` divides each head's queries and keys by their root mean square, with a learned gain;
+    `rotary` turns them by position with that base (`positions` as in `rotary_norm`)."""
 
-    def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32"):
+    def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
         if d % heads != 0:
             raise ValueError(f"{heads} heads cannot split a model dimension of {d}")
         self.d = d
         self.heads = heads
         self.rate = dropout_rate
+        self.qk_norm = qk_norm
+        self.rotary = rotary
         self.qkv = Linear(d, 3 * d, bias, init, dtype)
         self.out = Linear(d, d, bias, init, dtype)
 
     def init(self, key):
         k_qkv, k_out = _spend(key, 2)
-        return {"qkv": self.qkv.init(k_qkv), "out": self.out.init(k_out)}
+        params = {"qkv": self.qkv.init(k_qkv), "out": self.out.init(k_out)}
+        if self.qk_norm:
+            params["gain"] = ones((2, self.d // self.heads), self.qkv.dtype)
+        return params
 
-    def __call__(self, params, x, mask=None, key=None):
+    def __call__(self, params, x, mask=None, key=None, positions=None):
         b, t, d = x.shape
         hd = d // self.heads
+        qkv = self.qkv(params["qkv"], x)
+        if self.qk_norm or self.rotary:
+            # Queries and keys in place in the fused projection; the values pass.
+            qkv = rotary_norm(qkv.reshape(b, t, 3 * self.heads, hd), params["gain"] if self.qk_norm else None, positions,
+                              (self.heads, self.heads), None if self.rotary else 0, self.rotary or 10000.0)
         # (b, t, 3d) -> (3, b, heads, t, hd): q, k and v for every head.
-        qkv = self.qkv(params["qkv"], x).reshape(b, t, 3, self.heads, hd).transpose(2, 0, 3, 1, 4)
+        qkv = qkv.reshape(b, t, 3, self.heads, hd).transpose(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
         scores = q @ swapaxes(k, -1, -2) / math.sqrt(hd)
         if mask is not None:
@@ -264,13 +277,13 @@ class MultiHeadAttention(Layer):
 
 class TransformerBlock(Layer):
     """Pre-norm transformer block: x + attention(norm(x)), then x + mlp(norm(x)) with a GELU
-    MLP of `mlp_ratio * d` hidden units."""
+    MLP of `mlp_ratio * d` hidden units. `qk_norm` and `rotary` are the attention's."""
 
-    def __init__(self, d, heads, mlp_ratio=4, dropout_rate=0.0, init=None, dtype="float32"):
+    def __init__(self, d, heads, mlp_ratio=4, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
         self.rate = dropout_rate
         self.norm1 = LayerNorm(d, dtype=dtype)
         self.norm2 = LayerNorm(d, dtype=dtype)
-        self.attn = MultiHeadAttention(d, heads, True, dropout_rate, init, dtype)
+        self.attn = MultiHeadAttention(d, heads, True, dropout_rate, init, dtype, qk_norm, rotary)
         self.fc1 = Linear(d, mlp_ratio * d, True, init, dtype)
         self.fc2 = Linear(mlp_ratio * d, d, True, init, dtype)
 
@@ -279,11 +292,77 @@ class TransformerBlock(Layer):
         return {"norm1": self.norm1.init(), "attn": self.attn.init(k_attn), "norm2": self.norm2.init(),
                 "fc1": self.fc1.init(k_fc1), "fc2": self.fc2.init(k_fc2)}
 
-    def __call__(self, params, x, mask=None, key=None):
+    def __call__(self, params, x, mask=None, key=None, positions=None):
         k_attn, k_mlp = (None, None) if key is None else random.split(key)
-        x = x + self.attn(params["attn"], self.norm1(params["norm1"], x), mask, k_attn)
+        x = x + self.attn(params["attn"], self.norm1(params["norm1"], x), mask, k_attn, positions)
         hidden = self.fc2(params["fc2"], gelu(self.fc1(params["fc1"], self.norm2(params["norm2"], x))))
         return x + (dropout(k_mlp, hidden, self.rate) if key is not None else hidden)
+
+
+class SelectiveSSM(Layer):
+    """A selective state space layer, the linear-time counterpart of attention: a projection to
+    `width` channels (2 d by default), a short causal convolution with SiLU, step sizes and the
+    maps into and out of `states` states per channel computed from its result, the scan, a SiLU
+    gate and a projection back. The maps, one pair for each of `groups` groups of channels, are
+    normed like an attention's queries and keys, and turned by position with `rotary`.
+
+    `layer(params, x)` reads whole sequences from an empty state. `layer.extend(params, x, state,
+    lengths)` returns `(y, state)` for prompts, padded ones too, and for single tokens: the state
+    (`conv`, `scan` and the position `pos` of each sequence) is what the next call takes."""
+
+    def __init__(self, d, width=None, states=16, taps=4, dt_rank=None, groups=1, rotary=False, base=10000.0, init=None, dtype="float32"):
+        self.d = d
+        self.width = 2 * d if width is None else width
+        if self.width % groups != 0:
+            raise ValueError(f"{groups} groups cannot split {self.width} channels")
+        if rotary and states % 2 != 0:
+            raise ValueError(f"an odd number of states ({states}) cannot be turned in pairs")
+        self.states = states
+        self.taps = taps
+        self.groups = groups
+        self.rank = max(1, d // 16) if dt_rank is None else dt_rank
+        self.rotary = rotary
+        self.base = base
+        self.dtype = dtype
+        self.inward = Linear(d, self.width, False, init, dtype)
+        self.gate = Linear(d, self.width, False, init, dtype)
+        self.proj = Linear(self.width, self.rank + 2 * groups * states, False, init, dtype)
+        self.dt = Linear(self.rank, self.width, True, init, dtype)
+        self.out = Linear(self.width, d, False, init, dtype)
+
+    def init(self, key):
+        k_in, k_gate, k_conv, k_proj, k_dt, k_step, k_out = _spend(key, 7)
+        # Steps from 0.001 to 0.1, evenly over their logarithm, as the softplus of the bias.
+        step = exp(random.uniform(k_step, (self.width,), self.dtype) * math.log(100.0) + math.log(0.001))
+        dt = {**self.dt.init(k_dt), "b": step + log(1.0 - exp(-step))}
+        rates = log(arange(self.states).cast(self.dtype) + 1.0)
+        conv = {"w": random.normal(k_conv, (self.taps, self.width), self.dtype) / math.sqrt(self.taps), "b": zeros(self.width, self.dtype)}
+        return {"in": self.inward.init(k_in), "gate": self.gate.init(k_gate), "conv": conv, "proj": self.proj.init(k_proj), "dt": dt,
+                "a_log": broadcast_to(rates, (self.width, self.states)), "d": ones(self.width, self.dtype),
+                "gain": ones((2, self.states), self.dtype), "out": self.out.init(k_out)}
+
+    def state(self, batch):
+        """The state of sequences not yet begun."""
+        return {"conv": zeros((batch, self.taps - 1, self.width), self.dtype), "scan": zeros((batch, self.width, self.states), self.dtype),
+                "pos": zeros((batch,), "int32")}
+
+    def __call__(self, params, x):
+        return self.extend(params, x)[0]
+
+    def extend(self, params, x, state=None, lengths=None):
+        b, t, _ = x.shape
+        conv, scan, pos = (None, None, None) if state is None else (state["conv"], state["scan"], state["pos"])
+        u, conv = causal_conv(self.inward(params["in"], x), params["conv"]["w"], params["conv"]["b"], conv, lengths, "silu")
+        maps = self.proj(params["proj"], u)
+        dt = self.dt(params["dt"], maps[..., :self.rank])
+        positions = arange(t) if pos is None or not self.rotary else pos.reshape(b, 1) + arange(t)
+        maps = rotary_norm(maps[..., self.rank:].reshape(b, t, 2 * self.groups, self.states), params["gain"], positions,
+                           (self.groups, self.groups), None if self.rotary else 0, self.base)
+        y, scan = selective_scan(u, dt, -exp(params["a_log"]), maps[:, :, :self.groups], maps[:, :, self.groups:], params["d"],
+                                 self.gate(params["gate"], x), scan, lengths, softplus=True)
+        read = t if lengths is None else lengths
+        pos = zeros((b,), "int32") + read if pos is None else pos + read
+        return self.out(params["out"], y), {"conv": conv, "scan": scan, "pos": pos}
 
 
 class GRUCell(Layer):

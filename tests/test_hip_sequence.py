@@ -1,0 +1,188 @@
+"""The sequence operators' kernels on the device: values and gradients against the formulas in 64
+bits, captured and replayed step loops against the same steps one by one, bodies of control flow, and
+the three operators run together as the layers call them."""
+
+import numpy as np
+import pytest
+
+import rustautograd_amd as rg
+from rustautograd_amd import nn, random
+import sequence_reference as ref
+
+pytestmark = pytest.mark.gpu
+F = np.float32
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", ref.CONV_CASES, ids=str)
+def test_conv(case, dtype):
+    ref.check_conv(case, dtype, "hip")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", ref.SCAN_CASES, ids=str)
+def test_scan(case, dtype):
+    ref.check_scan(case, dtype, "hip")
+
+
+@pytest.mark.parametrize("case", [ref.SCAN_CASES[i] for i in (2, 7, 12, 16)], ids=str)
+def test_scan_whose_last_state_nobody_reads(case):
+    ref.check_scan(case, "float32", "hip", with_last=False)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", ref.ROTARY_CASES, ids=str)
+def test_rotary(case, dtype):
+    ref.check_rotary(case, dtype, "hip")
+
+
+def _inputs(case, names):
+    v, lengths, soft = ref.scan_inputs(case, "float32")
+    return {k: rg.tensor(v[k]) for k in names if v[k] is not None}, v, lengths, soft
+
+
+def test_infinite_rates_and_values_stay_where_they_are():
+    """A rate of minus infinity forgets the state at once; an infinite input reaches the positions after
+    it in its own channel and sequence, and no other; padded NaN reaches none."""
+    v, lengths, _ = ref.scan_inputs((2, 21, 6, 4, 1, "l"), "float32")
+    v["a"][1] = -np.inf
+    v["x"][0, 5, 3] = np.inf
+    lengths = np.array([21, 9], np.int32)
+    ref.fill_outside(v, lengths, ["x", "dt", "b", "c"])
+    args = [rg.tensor(v[k]) for k in ("x", "dt", "a", "b", "c")]
+    y, last = (o.numpy() for o in rg.compile(lambda *a: rg.selective_scan(*a, lengths=lengths), tuple(args), validate="none")(*args))
+    clean = np.ones((2, 21, 6), bool)
+    clean[0, 5:, 3] = False
+    assert np.isfinite(y[clean]).all() and not np.isfinite(y[~clean]).any()
+    assert (y[1, 9:] == 0).all()
+    want = v["dt"][0, :, 1] * v["x"][0, :, 1] * (v["b"] * v["c"])[0, :, 0].sum(-1)
+    # No state: four products and sums, of magnitudes that the same sum of absolute values bounds.
+    size = np.abs(v["dt"][0, :, 1] * v["x"][0, :, 1]) * np.abs(v["b"] * v["c"])[0, :, 0].sum(-1)
+    ref.agree(y[0, :, 1], want.astype(np.float64), size.astype(np.float64), 24, "float32", "forgetting channel")
+
+
+def _steps(program, state, data, n):
+    """The state after n calls of `program`, one by one, and their scalars."""
+    seen = []
+    for _ in range(n):
+        state, aux = program(state, data)
+        seen.append([float(a) for a in (aux if isinstance(aux, tuple) else (aux,))])
+    return state, np.array(seen)
+
+
+def _same(a, b):
+    if isinstance(a, dict):
+        return a.keys() == b.keys() and all(_same(a[k], b[k]) for k in a)
+    return np.array_equal(a.numpy(), b.numpy(), equal_nan=True)
+
+
+def test_a_replayed_training_loop_is_its_steps_one_by_one():
+    """Every operator's gradient in one step, run as captured graphs and call by call: the same bits, also
+    on a second run of the same program after other work."""
+    layer = nn.SelectiveSSM(24, states=8, dt_rank=3, groups=2, rotary=True)
+    attn = nn.MultiHeadAttention(24, 2, qk_norm=True, rotary=10000.0)
+    params = {"ssm": layer.init(random.key(0)), "attn": attn.init(random.key(1))}
+    r = np.random.default_rng(0)
+    data = (rg.tensor(r.standard_normal((2, 37, 24)).astype(F)), rg.tensor(r.standard_normal((2, 37, 24)).astype(F)))
+    mask = rg.tril(37)
+
+    def loss(p, x, t):
+        h = x + attn(p["attn"], x, mask)
+        return nn.mse_loss(h + layer(p["ssm"], h), t)
+
+    def step(p, batch):
+        value, grads = rg.value_and_grad(loss)(p, *batch)
+        return rg.tree.map(lambda a, g: a - 0.1 * g, p, grads), value
+
+    program = rg.compile(step, (params, data), validate="none")
+    want, seen = _steps(program, params, data, 7)
+    for _ in range(2):
+        got = rg.run(program, params, [data], steps=7)
+        assert _same(got.state, want)
+        assert np.array_equal(np.array(got.history["aux"], F), seen[:, 0].astype(F))
+    assert seen[-1, 0] < seen[0, 0]
+
+
+def test_a_replayed_token_loop_is_its_tokens_one_by_one():
+    layer = nn.SelectiveSSM(16, states=16, rotary=True)
+    params = layer.init(random.key(2))
+    state = {"x": rg.tensor(np.random.default_rng(1).standard_normal((3, 1, 16)).astype(F)), **layer.state(3)}
+
+    def step(s, p):
+        y, carried = layer.extend(p, s["x"], {k: s[k] for k in ("conv", "scan", "pos")})
+        return {"x": rg.tanh(y + s["x"]), **carried}, (y.sum(),)
+
+    program = rg.compile(step, (state, params), validate="none")
+    want, _ = _steps(program, state, params, 70)
+    for _ in range(2):
+        got = rg.run(program, state, [params], steps=70)
+        assert _same(got.state, want)
+        assert got.state["pos"].tolist() == [70, 70, 70]
+
+
+def test_prompts_and_tokens_agree():
+    """A prompt read at once, and the same positions in parts down to single tokens: the same sums in the
+    same order, but for parts' own tiles; bound as the scan's, twice over."""
+    case = (2, 50, 70, 16, 1, "dzp")
+    given, v, _, _ = _inputs(case, ("x", "dt", "a", "b", "c", "d", "z"))
+    whole = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g["d"], g["z"], softplus=True), (given,), validate="none")
+    y, last = whole(given)
+    args = (v["x"], v["dt"], v["a"], v["b"], v["c"], v["d"], v["z"], None, None, True, v["dy"], None)
+    size = ref.scan(*args, mag=True)
+    k = 2 * ref.scan_roundings(v["x"], v["dt"], v["a"], True)
+    state, parts, lo = rg.zeros((2, 70, 16)), [], 0
+    for n in (17, 1, 1, 2, 3, 5, 21):
+        part = {q: rg.tensor(t.numpy()[:, lo:lo + n]) if q in ("x", "dt", "b", "c", "z") else t for q, t in given.items()}
+        out, state = rg.compile(lambda g, s: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g["d"], g["z"], s, softplus=True), (part, state),
+                                validate="none")(part, state)
+        parts.append(out.numpy())
+        lo += n
+    ref.agree(np.concatenate(parts, 1), y.numpy().astype(np.float64), size["y"], k, "float32", "y")
+    ref.agree(state.numpy(), last.numpy().astype(np.float64), size["last"], k, "float32", "state")
+
+
+def test_inside_control_flow():
+    """Tokens through a `scan` body, whose slots and workspace are the enclosing program's, with gradients."""
+    r = np.random.default_rng(4)
+    x = rg.tensor(r.standard_normal((6, 2, 3, 8)).astype(F))
+    w = rg.tensor((0.5 * r.standard_normal((3, 8))).astype(F))
+
+    def looped(w, x):
+        def body(s, v):
+            y, s = rg.causal_conv(v, w, state=s, activation="silu")
+            return s, y
+        _, ys = rg.scan(body, rg.zeros((2, 2, 8)), x)
+        return (ys * ys).sum()
+
+    def at_once(w, x):
+        rows = x.transpose(1, 0, 2, 3).reshape(2, 18, 8)
+        y, _ = rg.causal_conv(rows, w, activation="silu")
+        return (y * y).sum()
+
+    a, b = (rg.compile(lambda *v: rg.value_and_grad(f)(*v), (w, x), validate="none")(w, x) for f in (looped, at_once))
+    # One sum of 288 squares and of their slopes, in another order: 288 u of the sum of magnitudes.
+    assert abs(float(a[0]) - float(b[0])) <= 288 * 2.0 ** -24 * float(b[0])
+    assert np.allclose(a[1].numpy(), b[1].numpy(), rtol=0, atol=400 * 2.0 ** -24 * 36 * np.abs(x.numpy()).max() ** 2)
+
+
+def test_two_programs_at_once_keep_to_their_own_buffers():
+    """Programs of the same operators with other sizes and data, called in turn."""
+    programs = []
+    for k, case in enumerate([(2, 130, 70, 16, 1, "dz"), (1, 40, 200, 16, 1, "dz")]):
+        given, v, _, _ = _inputs(case, ("x", "dt", "a", "b", "c", "d", "z"))
+
+        def fn(g):
+            return rg.grad(lambda q: (rg.selective_scan(q["x"], q["dt"], q["a"], q["b"], q["c"], q["d"], q["z"])[0] ** 2.0).sum())(g)
+        programs.append((rg.compile(fn, (given,), validate="none"), given))
+    first = [p(g) for p, g in programs]
+    for _ in range(3):
+        assert all(_same(p(g), want) for (p, g), want in zip(programs, first))
+
+
+def test_the_oracle_agrees_at_standard_validation():
+    """compile(validate="standard") holds the device against the CPU oracle."""
+    layer = nn.SelectiveSSM(16, states=8, rotary=True)
+    params = layer.init(random.key(5))
+    x = rg.tensor(np.random.default_rng(7).standard_normal((2, 19, 16)).astype(F))
+    c = rg.compile(lambda p, v: rg.value_and_grad(lambda q: (layer(q, v) ** 2.0).sum())(p), (params, x))
+    assert c.report.ok, c.report
