@@ -665,6 +665,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
   base.softplus = (i.sequence.flags & RG_SCAN_SOFTPLUS) != 0;
   const bool grad = i.op == RG_OP_SELECTIVE_SCAN_GRAD;
   const uint32_t tiles = rgk::scan_group_tiles(dtype, base), rows = rgk::scan_rows(dtype, base);
+  prog.workspace_bytes = std::max(prog.workspace_bytes, rgk::scan_workspace(dtype, base));
   const uint64_t maps = (uint64_t)q.batch * q.length * q.groups * q.states;
   // One tile of channels a group: its sums are the results.
   const bool direct = tiles == 1;
@@ -682,6 +683,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     a.gate = arg(sl, q.gate);
     a.state = arg(sl, q.state);
     a.lengths = (const int32_t*)arg(sl, q.lengths);
+    a.workspace = ws;
     if (!grad) {
       a.y = slot(sl, outs[0]);
       a.last = slot(sl, outs[1]);

@@ -35,7 +35,12 @@ struct ScanArgs {
   // Partial rows: of b and c one per tile of a group's channels, each [batch, length, groups,
   // states]; of a ([width, states]) and the skip ([width]) scan_rows of them.
   void *db_rows, *dc_rows, *da_rows, *dd_rows;
+  void* workspace;              // scan_workspace bytes
+  // Set by the launchers: tiles of positions a chunk, and the chunks' ends and sums of steps.
+  uint32_t chunk_tiles;
+  void *ends, *totals;
 };
+uint64_t scan_workspace(int dtype, const ScanArgs& a);
 uint32_t scan_rows(int dtype, const ScanArgs& a);
 uint32_t scan_group_tiles(int dtype, const ScanArgs& a);
 void selective_scan(hipStream_t s, int dtype, const ScanArgs& a);

@@ -248,49 +248,97 @@ constexpr int TILE = RG_SCAN_MARK;
 // NL neighbouring lanes share a channel, NS of its states each; a block holds CH channels, of one
 // group. Tiles of TILE positions pass through LDS, channels' values transposed so that a lane
 // reads four positions at once.
-template <class T, int NL_, int NS_>
+template <class T_, int NL_, int NS_>
 struct ScanShape {
+  using T = T_;
   static constexpr int NL = NL_, NS = NS_, NP = NL * NS, CH = TPB / NL, EPT = CH / 16, LD = TILE + 16 / sizeof(T);
+  static constexpr int MAPS = (TILE * NP + TPB - 1) / TPB;  // values of b or c a thread brings in a tile
 };
 
+// What a block works on: a tile of CH channels of a group, over one chunk of a sequence.
 struct ScanPlace {
-  uint32_t b, group, ch0, chs;  // sequence, group, first channel of the tile and how many
-  uint32_t tile;                // tile of the group's channels
+  uint32_t b, group, tile, chunk;
+  uint32_t ch0, chs;        // first channel and how many
+  uint32_t first, last;     // tiles of positions, [first, last)
+  uint32_t n, marks;        // positions of the sequence; tiles of the padded one
 };
 template <class S>
-__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tiles) {
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tiles, uint32_t first_chunk, uint32_t chunks) {
   ScanPlace p;
   const uint32_t per = a.width / a.groups;
-  p.tile = blockIdx.x % tiles;
-  p.group = blockIdx.x / tiles % a.groups;
-  p.b = blockIdx.x / tiles / a.groups;
+  uint32_t at = blockIdx.x;
+  p.tile = at % tiles;
+  at /= tiles;
+  p.group = at % a.groups;
+  at /= a.groups;
+  p.chunk = at % chunks + first_chunk;
+  p.b = at / chunks;
   p.ch0 = p.group * per + p.tile * S::CH;
   p.chs = min((uint32_t)S::CH, per - p.tile * S::CH);
+  p.n = end_of(a.lengths, p.b, a.length);
+  p.marks = (a.length + TILE - 1) / TILE;
+  p.first = p.chunk * a.chunk_tiles;
+  p.last = min(p.marks, p.first + a.chunk_tiles);
   return p;
 }
 
-// EPT neighbouring channels of one position of a [batch, length, width] value; zeros outside.
-template <class S, class T>
-__device__ __forceinline__ Vec<T, S::EPT> scan_load(const T* p, bool inside, uint32_t left, bool vec) {
-  Vec<T, S::EPT> v{};
-  if (!inside) return v;
-  if (vec && left >= (uint32_t)S::EPT) return load<T, S::EPT>(p);
-#pragma unroll
-  for (int j = 0; j < S::EPT; j++)
-    if ((uint32_t)j < left) v.v[j] = p[j];
-  return v;
-}
-template <class S, class T>
-__device__ __forceinline__ void scan_store(T* p, const Vec<T, S::EPT>& v, bool inside, uint32_t left, bool vec) {
-  if (!inside) return;
-  if (vec && left >= (uint32_t)S::EPT) {
-    store<T, S::EPT>(p, v);
-    return;
+// The part of a tile that a thread moves: EPT neighbouring channels of one position.
+template <class S>
+struct ScanMover {
+  uint32_t row, col, left;
+  bool vec;
+  __device__ __forceinline__ ScanMover(const ScanPlace& p, bool v) : row(threadIdx.x / 16), col(threadIdx.x % 16 * S::EPT), vec(v) {
+    left = col < p.chs ? p.chs - col : 0;
   }
+  __device__ __forceinline__ uint64_t at(const ScanArgs& a, const ScanPlace& p, uint32_t m) const {
+    return ((uint64_t)p.b * a.length + m * TILE + row) * a.width + p.ch0 + col;
+  }
+  __device__ __forceinline__ bool inside(const ScanPlace& p, uint32_t m) const { return m * TILE + row < p.n && left > 0; }
+  // Zeros outside the sequence.
+  template <class T>
+  __device__ __forceinline__ Vec<T, S::EPT> load_from(const void* src, uint64_t at, bool inside) const {
+    Vec<T, S::EPT> v{};
+    if (!inside) return v;
+    const T* p = (const T*)src + at;
+    if (vec && left >= (uint32_t)S::EPT) return load<T, S::EPT>(p);
 #pragma unroll
-  for (int j = 0; j < S::EPT; j++)
-    if ((uint32_t)j < left) p[j] = v.v[j];
-}
+    for (int j = 0; j < S::EPT; j++)
+      if ((uint32_t)j < left) v.v[j] = p[j];
+    return v;
+  }
+  template <class T>
+  __device__ __forceinline__ void store_to(void* dst, uint64_t at, const Vec<T, S::EPT>& v, bool within) const {
+    if (!dst || !within) return;
+    T* p = (T*)dst + at;
+    if (vec && left >= (uint32_t)S::EPT) {
+      store<T, S::EPT>(p, v);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < S::EPT; j++)
+      if ((uint32_t)j < left) p[j] = v.v[j];
+  }
+};
+
+// The values of b or c of a tile that a thread brings; zeros outside the sequence.
+template <class S>
+struct ScanMaps {
+  typename S::T v[S::MAPS];
+  __device__ __forceinline__ void read(const ScanArgs& a, const ScanPlace& p, const void* src, uint32_t m) {
+#pragma unroll
+    for (int q = 0; q < S::MAPS; q++) {
+      const uint32_t i = threadIdx.x + q * TPB, t = m * TILE + i / S::NP, k = i % S::NP;
+      v[q] = typename S::T(0);
+      if (i < TILE * S::NP && t < p.n && k < a.states)
+        v[q] = ((const typename S::T*)src)[(((uint64_t)p.b * a.length + t) * a.groups + p.group) * a.states + k];
+    }
+  }
+  __device__ __forceinline__ void put(typename S::T* dst) const {
+#pragma unroll
+    for (int q = 0; q < S::MAPS; q++)
+      if (threadIdx.x + q * TPB < TILE * S::NP) dst[threadIdx.x + q * TPB] = v[q];
+  }
+};
 
 // The decay e^(dt a) of one position. In 32 bits `a` comes multiplied by log2 e, for the
 // hardware's power of two.
@@ -298,36 +346,167 @@ __device__ __forceinline__ float decay(float dt, float a) { return __builtin_amd
 __device__ __forceinline__ double decay(double dt, double a) { return exp(dt * a); }
 __device__ __forceinline__ float decay_rate(float a) { return a * 1.44269504088896341f; }
 __device__ __forceinline__ double decay_rate(double a) { return a; }
-// An infinite rate becomes the largest finite one: the decay of a step is the same 0 (or infinity),
+// Keeps the scheduler from bringing in the operands of later positions of an unrolled tile early,
+// which costs more registers than a wave has.
+__device__ __forceinline__ void hold(int position) {
+  if (position % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+}
+// An infinite rate becomes a very large finite one: the decay of a step is the same 0 (or infinity),
 // and positions outside the sequence, whose steps are 0, leave the state as it is.
-template <class T>
-__device__ __forceinline__ T finite_rate(T a, T most) { return a > most ? most : a < -most ? -most : a; }
+__device__ __forceinline__ float finite_rate(float a) { return a > 2e38f ? 2e38f : a < -2e38f ? -2e38f : a; }
+__device__ __forceinline__ double finite_rate(double a) { return a > 1e308 ? 1e308 : a < -1e308 ? -1e308 : a; }
 
-// The sum over the NL lanes of a channel, in all of them.
+template <int C>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), C, 0xf, 0xf, false));
+}
+template <int C>
+__device__ __forceinline__ double dpp(double x) {
+  const int2 v = __builtin_bit_cast(int2, x);
+  return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(0, v.x, C, 0xf, 0xf, false), __builtin_amdgcn_update_dpp(0, v.y, C, 0xf, 0xf, false)));
+}
+// The sum over the NL lanes of a channel, in all of them: exchanges within quads, then mirrors.
 template <int NL, class T>
 __device__ __forceinline__ T channel_sum(T v) {
-#pragma unroll
-  for (int m = 1; m < NL; m <<= 1) v += __shfl_xor(v, m);
+  v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+  if (NL >= 8) v += dpp<0x141>(v);   // row_half_mirror
+  if (NL >= 16) v += dpp<0x140>(v);  // row_mirror
   return v;
 }
 
-template <class S, class T>
-__device__ __forceinline__ void scan_maps(const ScanArgs& a, const ScanPlace& p, uint32_t t0, uint32_t n, const T* src, T (*dst)[S::NP]) {
-  for (uint32_t i = threadIdx.x; i < TILE * S::NP; i += TPB) {
-    const uint32_t row = i / S::NP, k = i % S::NP;
-    T v = T(0);
-    if (t0 + row < n && k < a.states) v = src[(((uint64_t)p.b * a.length + t0 + row) * a.groups + p.group) * a.states + k];
-    dst[row][k] = v;
+// a + b over both halves (rows) of the wave: a's sum in the lower half (even rows), b's in the
+// upper (odd).
+__device__ __forceinline__ float halves(float a, float b) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float rows(float a, float b) {
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+__device__ __forceinline__ double halves(double a, double b) {
+  const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+  const auto lo = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false), hi = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+  return __builtin_bit_cast(double, make_uint2(lo[0], hi[0])) + __builtin_bit_cast(double, make_uint2(lo[1], hi[1]));
+}
+__device__ __forceinline__ double rows(double a, double b) {
+  const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+  const auto lo = __builtin_amdgcn_permlane16_swap(x.x, y.x, false, false), hi = __builtin_amdgcn_permlane16_swap(x.y, y.y, false, false);
+  return __builtin_bit_cast(double, make_uint2(lo[0], hi[0])) + __builtin_bit_cast(double, make_uint2(lo[1], hi[1]));
+}
+
+// M values of every lane summed over a wave's channels (lanes q, q + NL, q + 2 NL, ...). The sums
+// are spread as they halve: out[i] is that of value value_at<M>(i) of this lane, the same in the
+// 16 / NL lanes of a row with equal q.
+template <int M>
+constexpr int SUMS = M >= 4 ? M / 4 : 1;
+template <int M>
+__device__ __forceinline__ int value_at(int i) {
+  const int lane = threadIdx.x % 64, odd = lane / 16 % 2, upper = lane / 32;
+  return i + (M >= 4 ? M / 4 * odd : 0) + M / 2 * upper;
+}
+template <int NL, int M, class T>
+__device__ __forceinline__ void sum_channels(const T (&v)[M], T (&out)[SUMS<M>]) {
+  T half[M / 2];
+#pragma unroll
+  for (int i = 0; i < M / 2; i++) half[i] = halves(v[i], v[i + M / 2]);
+#pragma unroll
+  for (int i = 0; i < SUMS<M>; i++) {
+    out[i] = M >= 4 ? rows(half[i], half[(i + M / 4) % (M / 2)]) : rows(half[0], half[0]);
+    if (NL <= 8) out[i] += dpp<0x128>(out[i]);  // row_ror:8
+    if (NL <= 4) out[i] += dpp<0x124>(out[i]);  // row_ror:4
+  }
+}
+
+// A long sequence is cut into chunks. What a chunk makes of an empty state (k_scan_ends) and the
+// sum of its steps suffice to start every chunk: its block folds those of the chunks before it,
+// which for a decay that is an exponential of the steps' sum is one product a chunk.
+//   forward:  end[c]  = state after the chunk's last position, from zero before its first
+//   backward: end[c]  = gradient carried out of the chunk's first position, from zero after its last
+template <class T, int NL, int NS, bool BACK>
+__global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
+  using S = ScanShape<T, NL, NS>;
+  __shared__ __align__(16) T sdt[S::CH][S::LD], su[S::CH][S::LD], smap[TILE][S::NP];
+  const ScanPlace p = scan_place<S>(a, tiles, BACK ? 1 : 0, chunks - 1);
+  const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
+  const bool on = c < p.chs;
+  T rate[NS], h[NS], total = T(0);
+#pragma unroll
+  for (int j = 0; j < NS; j++) {
+    const uint32_t k = q * NS + j;
+    rate[j] = on && k < a.states ? decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k])) : T(0);
+    h[j] = T(0);
+  }
+  const ScanMover<S> mv(p, vec);
+  const uint32_t count = p.last - p.first;
+  Vec<T, S::EPT> dt, u, z{};
+  ScanMaps<S> map;
+  auto read = [&](uint32_t i) {
+    const uint32_t m = BACK ? p.last - 1 - i : p.first + i;
+    const bool in = mv.inside(p, m);
+    const uint64_t at = mv.at(a, p, m);
+    dt = mv.template load_from<T>(a.dt, at, in);
+    u = mv.template load_from<T>(BACK ? a.dy : a.x, at, in);
+    if (BACK && a.gate) z = mv.template load_from<T>(a.gate, at, in);
+    if (a.softplus && in)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) dt.v[j] = softplus(dt.v[j]);
+    map.read(a, p, BACK ? a.c : a.b, m);
+  };
+  read(0);
+  for (uint32_t i = 0; i < count; i++) {
+#pragma unroll
+    for (int j = 0; j < S::EPT; j++) {
+      sdt[mv.col + j][mv.row] = dt.v[j];
+      su[mv.col + j][mv.row] = BACK && a.gate ? u.v[j] * silu(z.v[j]) : u.v[j];
+    }
+    map.put(&smap[0][0]);
+    __syncthreads();
+    if (i + 1 < count) read(i + 1);
+#pragma unroll
+    for (int k = 0; k < TILE; k++) {
+      hold(k);
+      const int t = BACK ? TILE - 1 - k : k;
+      const T step = sdt[c][t], v = su[c][t];
+      total += step;
+#pragma unroll
+      for (int j = 0; j < NS; j++) {
+        const T e = decay(step, rate[j]), w = smap[t][q * NS + j];
+        h[j] = BACK ? e * fma_(v, w, h[j]) : fma_(e, h[j], step * v * w);
+      }
+    }
+    __syncthreads();
+  }
+  if (!on) return;
+  const uint64_t at = ((uint64_t)p.b * chunks + p.chunk) * a.width + d;
+#pragma unroll
+  for (int j = 0; j < NS; j++)
+    if (q * NS + j < a.states) ((T*)a.ends)[at * a.states + q * NS + j] = h[j];
+  if (q == 0) ((T*)a.totals)[at] = total;
+}
+
+// `h` carried from the sequence's start (or, backward, its end) to this block's chunk.
+template <class T, int NS, bool BACK>
+__device__ __forceinline__ void scan_start(const ScanArgs& a, const ScanPlace& p, uint32_t chunks, uint32_t d, uint32_t k0, const T (&rate)[NS], T (&h)[NS]) {
+  const uint32_t count = BACK ? chunks - 1 - p.chunk : p.chunk;
+#pragma unroll 4
+  for (uint32_t i = 0; i < count; i++) {
+    const uint32_t c = BACK ? chunks - 1 - i : i;
+    const uint64_t at = ((uint64_t)p.b * chunks + c) * a.width + d;
+    const T total = ((const T*)a.totals)[at];
+#pragma unroll
+    for (int j = 0; j < NS; j++)
+      if (k0 + j < a.states) h[j] = fma_(decay(total, rate[j]), h[j], ((const T*)a.ends)[at * a.states + k0 + j]);
   }
 }
 
 // Forward: h[t] = e^(dt a) h[t - 1] + dt x b, y = c . h + d x, gated.
 template <class T, int NL, int NS>
-__global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, bool vec) {
+__global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
-  const ScanPlace p = scan_place<S>(a, tiles);
-  const uint32_t n = end_of(a.lengths, p.b, a.length);
+  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
   T rate[NS], h[NS];
@@ -335,37 +514,44 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, bool v
   for (int j = 0; j < NS; j++) {
     const uint32_t k = q * NS + j;
     const bool has = on && k < a.states;
-    rate[j] = has ? decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k], sizeof(T) == 4 ? T(2e38f) : T(1e308))) : T(0);
+    rate[j] = has ? decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k])) : T(0);
     h[j] = has && a.state ? ((const T*)a.state)[((uint64_t)p.b * a.width + d) * a.states + k] : T(0);
   }
   const T skip = on && q == 0 && a.skip ? ((const T*)a.skip)[d] : T(0);
-  const uint32_t row = threadIdx.x / 16, col = threadIdx.x % 16 * S::EPT;
-  const uint32_t left = col < p.chs ? p.chs - col : 0;
-  const uint32_t marks = (a.length + TILE - 1) / TILE;
-  for (uint32_t m = 0; m < marks; m++) {
-    const uint32_t t0 = m * TILE, t = t0 + row;
-    const uint64_t at = ((uint64_t)p.b * a.length + t) * a.width + p.ch0 + col;
-    const bool inside = t < n && left > 0;
-    const auto x = scan_load<S>((const T*)a.x + at, inside, left, vec);
-    auto dt = scan_load<S>((const T*)a.dt + at, inside, left, vec);
-    Vec<T, S::EPT> z{};
-    if (a.gate) z = scan_load<S>((const T*)a.gate + at, inside, left, vec);
+  const ScanMover<S> mv(p, vec);
+  Vec<T, S::EPT> x, dt, z{};
+  ScanMaps<S> bs, cs;
+  auto read = [&](uint32_t m) {
+    const bool in = mv.inside(p, m);
+    const uint64_t at = mv.at(a, p, m);
+    x = mv.template load_from<T>(a.x, at, in);
+    dt = mv.template load_from<T>(a.dt, at, in);
+    if (a.gate) z = mv.template load_from<T>(a.gate, at, in);
+    bs.read(a, p, a.b, m);
+    cs.read(a, p, a.c, m);
+  };
+  read(p.first);
+  if (on) scan_start<T, NS, false>(a, p, chunks, d, q * NS, rate, h);
+  for (uint32_t m = p.first; m < p.last; m++) {
+    const bool in = mv.inside(p, m);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
-      if (a.softplus && inside) dt.v[j] = softplus(dt.v[j]);
-      sx[col + j][row] = x.v[j];
-      sdt[col + j][row] = dt.v[j];
+      sx[mv.col + j][mv.row] = x.v[j];
+      sdt[mv.col + j][mv.row] = a.softplus && in ? softplus(dt.v[j]) : dt.v[j];
     }
-    scan_maps<S>(a, p, t0, n, (const T*)a.b, sb);
-    scan_maps<S>(a, p, t0, n, (const T*)a.c, sc);
+    bs.put(&sb[0][0]);
+    cs.put(&sc[0][0]);
+    const Vec<T, S::EPT> gate = z;
     __syncthreads();
+    if (m + 1 < p.last) read(m + 1);
     if (a.marks && on)
 #pragma unroll
       for (int j = 0; j < NS; j++)
-        if (q * NS + j < a.states) ((T*)a.marks)[(((uint64_t)p.b * marks + m) * a.width + d) * a.states + q * NS + j] = h[j];
+        if (q * NS + j < a.states) ((T*)a.marks)[(((uint64_t)p.b * p.marks + m) * a.width + d) * a.states + q * NS + j] = h[j];
     T mine = T(0);
-#pragma unroll 4
+#pragma unroll
     for (int i = 0; i < TILE; i++) {
+      hold(i);
       const T step = sdt[c][i], u = sx[c][i], drive = step * u;
       T y = skip * u;
 #pragma unroll
@@ -378,73 +564,82 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, bool v
       if (i % NL == NL - 1) sx[c][i - (NL - 1) + q] = mine;
     }
     __syncthreads();
-    if (a.y) {
-      Vec<T, S::EPT> y;
+    Vec<T, S::EPT> y;
 #pragma unroll
-      for (int j = 0; j < S::EPT; j++) y.v[j] = !inside ? T(0) : a.gate ? sx[col + j][row] * silu(z.v[j]) : sx[col + j][row];
-      scan_store<S>((T*)a.y + at, y, t < a.length, left, vec);
-    }
+    for (int j = 0; j < S::EPT; j++) y.v[j] = !in ? T(0) : a.gate ? sx[mv.col + j][mv.row] * silu(gate.v[j]) : sx[mv.col + j][mv.row];
+    mv.store_to(a.y, mv.at(a, p, m), y, m * TILE + mv.row < a.length);
     __syncthreads();
   }
-  if (a.last && on)
+  if (a.last && on && p.last == p.marks)
 #pragma unroll
     for (int j = 0; j < NS; j++)
       if (q * NS + j < a.states) ((T*)a.last)[((uint64_t)p.b * a.width + d) * a.states + q * NS + j] = h[j];
 }
 
-// Backward, tile by tile from the last. From the state kept before the tile, its decays e and the
-// decayed states p = e h[t - 1] are formed again, then with G = dL/dh[t] carried back:
+// Backward, tile by tile from the chunk's last. From the state kept before the tile, its decays e
+// and the decayed states p = e h[t - 1] are formed again, then with G = dL/dh[t] carried back:
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
 // The sums over channels that db and dc take leave one partial row per tile of channels.
 template <class T, int NL, int NS>
-__global__ void __launch_bounds__(TPB) k_scan_grad(ScanArgs a, uint32_t tiles, bool vec) {
+__global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_grad(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
-  constexpr int WAVES = TPB / 64;
+  constexpr int WAVES = TPB / 64, COPIES = 16 / NL, M = 2 * NS;
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sg[S::CH][S::LD], sy[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
-  __shared__ T red[WAVES][TILE][2][S::NP];
-  const ScanPlace p = scan_place<S>(a, tiles);
-  const uint32_t n = end_of(a.lengths, p.b, a.length);
+  __shared__ T red[WAVES][TILE][2 * S::NP];
+  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c, wave = threadIdx.x / 64;
+  const int copy = threadIdx.x % 16 / NL;
   const bool on = c < p.chs;
   T rate[NS], rate_e[NS], back[NS], da[NS], dd = T(0);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
     const uint32_t k = q * NS + j;
     const bool has = on && k < a.states;
-    rate[j] = has ? finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k], sizeof(T) == 4 ? T(2e38f) : T(1e308)) : T(0);
+    rate[j] = has ? finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k]) : T(0);
     rate_e[j] = decay_rate(rate[j]);
     back[j] = has && a.carry ? ((const T*)a.carry)[((uint64_t)p.b * a.width + d) * a.states + k] : T(0);
     da[j] = T(0);
   }
   const T skip = on && a.skip ? ((const T*)a.skip)[d] : T(0);
-  const uint32_t row = threadIdx.x / 16, col = threadIdx.x % 16 * S::EPT;
-  const uint32_t left = col < p.chs ? p.chs - col : 0;
-  const uint32_t marks = (a.length + TILE - 1) / TILE;
-  for (uint32_t m = marks; m-- > 0;) {
-    const uint32_t t0 = m * TILE, t = t0 + row;
-    const uint64_t at = ((uint64_t)p.b * a.length + t) * a.width + p.ch0 + col;
-    const bool inside = t < n && left > 0;
-    const auto x = scan_load<S>((const T*)a.x + at, inside, left, vec);
-    const auto raw = scan_load<S>((const T*)a.dt + at, inside, left, vec);
-    const auto g = scan_load<S>((const T*)a.dy + at, inside, left, vec);
-    Vec<T, S::EPT> z{};
-    if (a.gate) z = scan_load<S>((const T*)a.gate + at, inside, left, vec);
-    T h[NS];
+  const ScanMover<S> mv(p, vec);
+  Vec<T, S::EPT> x, raw, g, z{};
+  ScanMaps<S> bs, cs;
+  T start[NS];
+  auto read = [&](uint32_t m) {
+    const bool in = mv.inside(p, m);
+    const uint64_t at = mv.at(a, p, m);
+    x = mv.template load_from<T>(a.x, at, in);
+    raw = mv.template load_from<T>(a.dt, at, in);
+    g = mv.template load_from<T>(a.dy, at, in);
+    if (a.gate) z = mv.template load_from<T>(a.gate, at, in);
+    bs.read(a, p, a.b, m);
+    cs.read(a, p, a.c, m);
 #pragma unroll
     for (int j = 0; j < NS; j++)
-      h[j] = on && q * NS + j < a.states ? ((const T*)a.marks)[(((uint64_t)p.b * marks + m) * a.width + d) * a.states + q * NS + j] : T(0);
+      start[j] = on && q * NS + j < a.states ? ((const T*)a.marks)[(((uint64_t)p.b * p.marks + m) * a.width + d) * a.states + q * NS + j] : T(0);
+  };
+  read(p.last - 1);
+  if (on) scan_start<T, NS, true>(a, p, chunks, d, q * NS, rate_e, back);
+  for (uint32_t m = p.last; m-- > p.first;) {
+    const bool in = mv.inside(p, m);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
-      sx[col + j][row] = x.v[j];
-      sdt[col + j][row] = a.softplus && inside ? softplus(raw.v[j]) : raw.v[j];
-      sg[col + j][row] = a.gate ? g.v[j] * silu(z.v[j]) : g.v[j];
+      sx[mv.col + j][mv.row] = x.v[j];
+      sdt[mv.col + j][mv.row] = a.softplus && in ? softplus(raw.v[j]) : raw.v[j];
+      sg[mv.col + j][mv.row] = a.gate ? g.v[j] * silu(z.v[j]) : g.v[j];
     }
-    scan_maps<S>(a, p, t0, n, (const T*)a.b, sb);
-    scan_maps<S>(a, p, t0, n, (const T*)a.c, sc);
+    bs.put(&sb[0][0]);
+    cs.put(&sc[0][0]);
+    T h[NS];
+#pragma unroll
+    for (int j = 0; j < NS; j++) h[j] = start[j];
+    const Vec<T, S::EPT> raw0 = raw, g0 = g, z0 = z;
     __syncthreads();
+    if (m > p.first) read(m - 1);
     T e[TILE][NS], kept[TILE][NS], mine = T(0), mine2 = T(0);
 #pragma unroll
     for (int i = 0; i < TILE; i++) {
+      hold(i);
       const T step = sdt[c][i], u = sx[c][i], drive = step * u;
       T y = q == 0 ? skip * u : T(0);
 #pragma unroll
@@ -460,30 +655,30 @@ __global__ void __launch_bounds__(TPB) k_scan_grad(ScanArgs a, uint32_t tiles, b
         if (i % NL == NL - 1) sy[c][i - (NL - 1) + q] = mine;
       }
     }
+    T sums[SUMS<M>];
 #pragma unroll
     for (int i = TILE - 1; i >= 0; i--) {
+      hold(i + 1);
       const T step = sdt[c][i], u = sx[c][i], gy = sg[c][i], drive = step * u;
-      T sum_b = T(0), sum_a = T(0);
+      T sum_b = T(0), sum_a = T(0), over[M];
 #pragma unroll
       for (int j = 0; j < NS; j++) {
-        const T bj = sb[i][q * NS + j], G = fma_(gy, sc[i][q * NS + j], back[j]);
-        T dc = gy * fma_(drive, bj, kept[i][j]), db = G * drive;
-        const T gp = G * kept[i][j];
+        const T bj = sb[i][q * NS + j], G = fma_(gy, sc[i][q * NS + j], back[j]), gp = G * kept[i][j];
+        over[j] = G * drive;
+        over[NS + j] = gy * fma_(drive, bj, kept[i][j]);
         sum_b = fma_(G, bj, sum_b);
         sum_a = fma_(gp, rate[j], sum_a);
         da[j] = fma_(gp, step, da[j]);
         back[j] = e[i][j] * G;
-#pragma unroll
-        for (int l = NL; l < 64; l <<= 1) {
-          db += __shfl_xor(db, l);
-          dc += __shfl_xor(dc, l);
-        }
-        if (threadIdx.x % 64 < NL) {
-          red[wave][i][0][q * NS + j] = db;
-          red[wave][i][1][q * NS + j] = dc;
-        }
       }
       dd = fma_(gy, u, dd);
+      T of[SUMS<M>];
+      sum_channels<NL>(over, of);
+#pragma unroll
+      for (int k = 0; k < SUMS<M>; k++) {
+        if (i % COPIES == copy) sums[k] = of[k];
+        if (i % COPIES == 0) red[wave][i + copy][value_at<M>(k) * NL + q] = sums[k];
+      }
       sum_b = channel_sum<NL>(sum_b);
       sum_a = channel_sum<NL>(sum_a);
       const T dx = fma_(step, sum_b, skip * gy), ddt = fma_(u, sum_b, sum_a);
@@ -497,36 +692,39 @@ __global__ void __launch_bounds__(TPB) k_scan_grad(ScanArgs a, uint32_t tiles, b
     Vec<T, S::EPT> dx, ddt, dz;
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
-      dx.v[j] = inside ? sx[col + j][row] : T(0);
-      ddt.v[j] = !inside ? T(0) : a.softplus ? sdt[col + j][row] * sigmoid(raw.v[j]) : sdt[col + j][row];
-      dz.v[j] = inside && a.gate ? g.v[j] * sy[col + j][row] * silu_slope(z.v[j], sigmoid(z.v[j])) : T(0);
+      dx.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
+      ddt.v[j] = !in ? T(0) : a.softplus ? sdt[mv.col + j][mv.row] * sigmoid(raw0.v[j]) : sdt[mv.col + j][mv.row];
+      dz.v[j] = in && a.gate ? g0.v[j] * sy[mv.col + j][mv.row] * silu_slope(z0.v[j], sigmoid(z0.v[j])) : T(0);
     }
-    const bool within = t < a.length;
-    if (a.dx) scan_store<S>((T*)a.dx + at, dx, within, left, vec);
-    if (a.ddt) scan_store<S>((T*)a.ddt + at, ddt, within, left, vec);
-    if (a.dz) scan_store<S>((T*)a.dz + at, dz, within, left, vec);
+    const bool within = m * TILE + mv.row < a.length;
+    const uint64_t at = mv.at(a, p, m);
+    mv.store_to(a.dx, at, dx, within);
+    mv.store_to(a.ddt, at, ddt, within);
+    mv.store_to(a.dz, at, dz, within);
     for (uint32_t i = threadIdx.x; i < TILE * 2 * S::NP; i += TPB) {
-      const uint32_t r = i / (2 * S::NP), w = i / S::NP % 2, k = i % S::NP;
+      // Value w NS + j of lane q is the gradient of b (w = 0) or c of state q NS + j.
+      const uint32_t r = i / (2 * S::NP), w = i / S::NP % 2, k = i % S::NP, t = m * TILE + r;
       T* to = (T*)(w ? a.dc_rows : a.db_rows);
-      if (!to || k >= a.states || t0 + r >= a.length) continue;
+      if (!to || k >= a.states || t >= a.length) continue;
+      const uint32_t from = (w * NS + k % NS) * NL + k / NS;
       T sum = T(0);
-      if (t0 + r < n)
+      if (t < p.n)
 #pragma unroll
-        for (int v = 0; v < WAVES; v++) sum += red[v][r][w][k];
+        for (int v = 0; v < WAVES; v++) sum += red[v][r][from];
       const uint64_t rows = (uint64_t)a.batch * a.length * a.groups * a.states;
-      to[p.tile * rows + (((uint64_t)p.b * a.length + t0 + r) * a.groups + p.group) * a.states + k] = sum;
+      to[p.tile * rows + (((uint64_t)p.b * a.length + t) * a.groups + p.group) * a.states + k] = sum;
     }
     __syncthreads();
   }
   if (!on) return;
+  const uint64_t row = (uint64_t)p.b * chunks + p.chunk;
 #pragma unroll
   for (int j = 0; j < NS; j++) {
     if (q * NS + j >= a.states) continue;
-    const uint64_t at = ((uint64_t)p.b * a.width + d) * a.states + q * NS + j;
-    if (a.da_rows) ((T*)a.da_rows)[at] = da[j];
-    if (a.dstate) ((T*)a.dstate)[at] = back[j];
+    if (a.da_rows) ((T*)a.da_rows)[(row * a.width + d) * a.states + q * NS + j] = da[j];
+    if (a.dstate && p.chunk == 0) ((T*)a.dstate)[((uint64_t)p.b * a.width + d) * a.states + q * NS + j] = back[j];
   }
-  if (a.dd_rows && q == 0) ((T*)a.dd_rows)[(uint64_t)p.b * a.width + d] = dd;
+  if (a.dd_rows && q == 0) ((T*)a.dd_rows)[row * a.width + d] = dd;
 }
 
 // The lanes and states a channel is spread over: f(NL, NS).
@@ -547,40 +745,62 @@ void scan_shape(uint32_t states, F f) {
   }
 }
 
+// Tiles of a group's channels, and the chunks a sequence is cut into: enough blocks to fill the
+// chip, chunks of at least SCAN_CHUNK_MIN tiles, at most SCAN_CHUNKS of them.
+constexpr uint32_t SCAN_BLOCKS = 1024, SCAN_CHUNK_MIN = 4, SCAN_CHUNKS = 64;
+
+struct ScanCut {
+  uint32_t tiles = 1, chunk_tiles = 1, chunks = 1;
+};
 template <class T>
-uint32_t scan_tiles(const ScanArgs& a) {
-  uint32_t tiles = 0;
+ScanCut scan_cut(const ScanArgs& a) {
+  ScanCut cut;
   scan_shape<T>(a.states, [&](auto nl, auto) {
     const uint32_t ch = TPB / decltype(nl)::value;
-    tiles = (a.width / a.groups + ch - 1) / ch;
+    cut.tiles = (a.width / a.groups + ch - 1) / ch;
   });
-  return tiles;
+  const uint32_t marks = (a.length + TILE - 1) / TILE;
+  const uint64_t blocks = (uint64_t)a.batch * a.groups * cut.tiles;
+  const uint32_t wanted = (uint32_t)std::min<uint64_t>((SCAN_BLOCKS + blocks - 1) / blocks, SCAN_CHUNKS);
+  cut.chunk_tiles = std::max((marks + wanted - 1) / wanted, std::min(marks, SCAN_CHUNK_MIN));
+  cut.chunks = (marks + cut.chunk_tiles - 1) / cut.chunk_tiles;
+  return cut;
 }
+ScanCut scan_cut_of(int dtype, const ScanArgs& a) { return dtype == RG_F32 ? scan_cut<float>(a) : scan_cut<double>(a); }
 
-template <class T>
-void launch_scan(hipStream_t s, const ScanArgs& a, bool grad) {
-  const uint32_t tiles = scan_tiles<T>(a);
+template <class T, bool GRAD>
+void launch_scan(hipStream_t s, ScanArgs a) {
+  const ScanCut cut = scan_cut<T>(a);
+  a.chunk_tiles = cut.chunk_tiles;
+  a.ends = a.workspace;
+  a.totals = (T*)a.workspace + (uint64_t)a.batch * cut.chunks * a.width * a.states;
   scan_shape<T>(a.states, [&](auto nl, auto ns) {
     constexpr int NL = decltype(nl)::value, NS = decltype(ns)::value, EPT = ScanShape<T, NL, NS>::EPT;
     const bool vec = a.width % EPT == 0 && (a.width / a.groups) % EPT == 0;
-    const dim3 grid(a.batch * a.groups * tiles);
-    if (grad) hipLaunchKernelGGL((k_scan_grad<T, NL, NS>), grid, dim3(TPB), 0, s, a, tiles, vec);
-    else hipLaunchKernelGGL((k_scan<T, NL, NS>), grid, dim3(TPB), 0, s, a, tiles, vec);
+    const uint32_t blocks = a.batch * a.groups * cut.tiles;
+    if (cut.chunks > 1)
+      hipLaunchKernelGGL((k_scan_ends<T, NL, NS, GRAD>), dim3(blocks * (cut.chunks - 1)), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+    if constexpr (GRAD) hipLaunchKernelGGL((k_scan_grad<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+    else hipLaunchKernelGGL((k_scan<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
   });
 }
 
 }  // namespace
 
-uint32_t scan_rows(int, const ScanArgs& a) { return a.batch; }
-uint32_t scan_group_tiles(int dtype, const ScanArgs& a) { return dtype == RG_F32 ? scan_tiles<float>(a) : scan_tiles<double>(a); }
+uint32_t scan_rows(int dtype, const ScanArgs& a) { return a.batch * scan_cut_of(dtype, a).chunks; }
+uint32_t scan_group_tiles(int dtype, const ScanArgs& a) { return scan_cut_of(dtype, a).tiles; }
+uint64_t scan_workspace(int dtype, const ScanArgs& a) {
+  const uint32_t chunks = scan_cut_of(dtype, a).chunks;
+  return chunks > 1 ? (uint64_t)a.batch * chunks * a.width * (a.states + 1) * (dtype == RG_F64 ? 8 : 4) : 0;
+}
 
 void selective_scan(hipStream_t s, int dtype, const ScanArgs& a) {
-  if (dtype == RG_F32) launch_scan<float>(s, a, false);
-  else launch_scan<double>(s, a, false);
+  if (dtype == RG_F32) launch_scan<float, false>(s, a);
+  else launch_scan<double, false>(s, a);
 }
 void selective_scan_grad(hipStream_t s, int dtype, const ScanArgs& a) {
-  if (dtype == RG_F32) launch_scan<float>(s, a, true);
-  else launch_scan<double>(s, a, true);
+  if (dtype == RG_F32) launch_scan<float, true>(s, a);
+  else launch_scan<double, true>(s, a);
 }
 
 // ---- norm with rotation -----------------------------------------------------------------------
