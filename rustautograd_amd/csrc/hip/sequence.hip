@@ -11,22 +11,59 @@ constexpr int TPB = 256;
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
-__device__ __forceinline__ float exp_(float v) { return expf(v); }
+// e^v for -infinity <= v <= 88: the hardware's power of two of v log2 e, times what the rounding of
+// that product leaves out (half the instructions of the full range). Below -103 it is 0 or next to it.
+__device__ __forceinline__ float exp_(float v) {
+  constexpr float L = 1.44269504088896341f, REST = 1.92596303e-8f, LN2 = 0.693147180559945309f;  // log2 e = L + REST
+  v = v < -103.0f ? -103.0f : v;
+  const float t = v * L, r = fma_(v, REST, fma_(v, L, -t)), e = __builtin_amdgcn_exp2f(t);
+  return fma_(e, r * LN2, e);
+}
 __device__ __forceinline__ double exp_(double v) { return exp(v); }
-__device__ __forceinline__ float log1p_(float v) { return log1pf(v); }
-__device__ __forceinline__ double log1p_(double v) { return log1p(v); }
 __device__ __forceinline__ float sqrt_(float v) { return sqrtf(v); }
 __device__ __forceinline__ double sqrt_(double v) { return sqrt(v); }
+// a / b for a positive, finite, normal b: the hardware's reciprocal and one step of Newton's method,
+// within a unit in the last place or two (the full division, for every b, takes three times as long).
+__device__ __forceinline__ float over(float a, float b) {
+  const float r = __builtin_amdgcn_rcpf(b), q = a * r;
+  return fma_(fma_(-b, q, a), r, q);
+}
+__device__ __forceinline__ double over(double a, double b) { return a / b; }
+// 1 + e^-v, kept finite: past the bound sigmoid is below 1e-37 (1e-300) either way.
+__device__ __forceinline__ float logistic_base(float v) { return 1.0f + exp_(-v > 86.0f ? 86.0f : -v); }
+__device__ __forceinline__ double logistic_base(double v) { return 1.0 + exp_(-v > 700.0 ? 700.0 : -v); }
 template <class T>
-__device__ __forceinline__ T sigmoid(T v) { return T(1) / (T(1) + exp_(-v)); }
+__device__ __forceinline__ T sigmoid(T v) { return over(T(1), logistic_base(v)); }
 template <class T>
-__device__ __forceinline__ T silu(T v) { return v / (T(1) + exp_(-v)); }
+__device__ __forceinline__ T silu(T v) { return over(v, logistic_base(v)); }
 // silu'(v) from s = sigmoid(v).
 template <class T>
 __device__ __forceinline__ T silu_slope(T v, T s) { return s * fma_(v, T(1) - s, T(1)); }
-// log(1 + e^v) without overflow; log1p keeps the relative precision of small steps.
+// log(1 + u), 0 <= u <= 1, to full relative precision: 2 artanh(s) = 2 s (1 + s^2/3 + s^4/5 + ...)
+// at s = u / (2 + u) <= 1/3, whose terms past s^16/17 are below 2e-10 of the sum.
+__device__ __forceinline__ float log1p_(float u) {
+  const float s = over(u, 2.0f + u), w = s * s;
+  float p = 1.0f / 17.0f;
+  p = fma_(p, w, 1.0f / 15.0f);
+  p = fma_(p, w, 1.0f / 13.0f);
+  p = fma_(p, w, 1.0f / 11.0f);
+  p = fma_(p, w, 1.0f / 9.0f);
+  p = fma_(p, w, 1.0f / 7.0f);
+  p = fma_(p, w, 1.0f / 5.0f);
+  p = fma_(p, w, 1.0f / 3.0f);
+  return fma_(2.0f * s, p * w, 2.0f * s);
+}
+__device__ __forceinline__ double log1p_(double u) { return log1p(u); }
+// log(1 + e^v) without overflow, small steps to full relative precision.
 template <class T>
 __device__ __forceinline__ T softplus(T v) { return (v > T(0) ? v : T(0)) + log1p_(exp_(v > T(0) ? -v : v)); }
+// The same with its slope, the logistic function of v.
+template <class T>
+__device__ __forceinline__ T softplus(T v, T* slope) {
+  const T u = exp_(v > T(0) ? -v : v);
+  *slope = over(v > T(0) ? T(1) : u, T(1) + u);
+  return (v > T(0) ? v : T(0)) + log1p_(u);
+}
 
 __device__ __forceinline__ uint32_t end_of(const int32_t* lengths, uint32_t b, uint32_t length) {
   if (!lengths) return length;
@@ -419,9 +456,40 @@ __device__ __forceinline__ void sum_channels(const T (&v)[M], T (&out)[SUMS<M>])
   }
 }
 
-// A long sequence is cut into chunks. What a chunk makes of an empty state (k_scan_ends) and the
-// sum of its steps suffice to start every chunk: its block folds those of the chunks before it,
-// which for a decay that is an exponential of the steps' sum is one product a chunk.
+// The NS states from k0 on of a row of them, zeros past the last; `whole`: NS divides their number.
+template <class T, int NS>
+__device__ __forceinline__ Vec<T, NS> load_states(const void* src, uint64_t row, uint32_t k0, uint32_t states, bool whole) {
+  const T* p = (const T*)src + row * states;
+  Vec<T, NS> v;
+  if (whole) {
+    v = load<T, NS>(p + (k0 < states ? k0 : 0));
+  } else {
+#pragma unroll
+    for (int j = 0; j < NS; j++) v.v[j] = p[k0 + j < states ? k0 + j : 0];
+  }
+#pragma unroll
+  for (int j = 0; j < NS; j++)
+    if (k0 + j >= states) v.v[j] = T(0);
+  return v;
+}
+template <class T, int NS>
+__device__ __forceinline__ void store_states(void* dst, uint64_t row, uint32_t k0, uint32_t states, bool whole, const T (&h)[NS]) {
+  T* p = (T*)dst + row * states + k0;
+  if (whole) {
+    Vec<T, NS> v;
+#pragma unroll
+    for (int j = 0; j < NS; j++) v.v[j] = h[j];
+    if (k0 < states) store<T, NS>(p, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NS; j++)
+    if (k0 + j < states) p[j] = h[j];
+}
+
+// A long sequence is cut into chunks. What each makes of an empty state (k_scan_ends) and the sum
+// of its steps suffice to start them all: the decay over a chunk is one exponential of that sum,
+// so that joining them (k_scan_join) is one product a chunk and state.
 //   forward:  end[c]  = state after the chunk's last position, from zero before its first
 //   backward: end[c]  = gradient carried out of the chunk's first position, from zero after its last
 template <class T, int NL, int NS, bool BACK>
@@ -431,11 +499,12 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
   const ScanPlace p = scan_place<S>(a, tiles, BACK ? 1 : 0, chunks - 1);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
+  const bool whole = a.states % NS == 0;
   T rate[NS], h[NS], total = T(0);
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    const uint32_t k = q * NS + j;
-    rate[j] = on && k < a.states ? decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k])) : T(0);
+    rate[j] = decay_rate(finite_rate(rates.v[j]));
     h[j] = T(0);
   }
   const ScanMover<S> mv(p, vec);
@@ -480,24 +549,37 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
   }
   if (!on) return;
   const uint64_t at = ((uint64_t)p.b * chunks + p.chunk) * a.width + d;
-#pragma unroll
-  for (int j = 0; j < NS; j++)
-    if (q * NS + j < a.states) ((T*)a.ends)[at * a.states + q * NS + j] = h[j];
+  store_states<T, NS>(a.ends, at, q * NS, a.states, whole, h);
   if (q == 0) ((T*)a.totals)[at] = total;
 }
 
-// `h` carried from the sequence's start (or, backward, its end) to this block's chunk.
-template <class T, int NS, bool BACK>
-__device__ __forceinline__ void scan_start(const ScanArgs& a, const ScanPlace& p, uint32_t chunks, uint32_t d, uint32_t k0, const T (&rate)[NS], T (&h)[NS]) {
-  const uint32_t count = BACK ? chunks - 1 - p.chunk : p.chunk;
-#pragma unroll 4
-  for (uint32_t i = 0; i < count; i++) {
-    const uint32_t c = BACK ? chunks - 1 - i : i;
-    const uint64_t at = ((uint64_t)p.b * chunks + c) * a.width + d;
-    const T total = ((const T*)a.totals)[at];
+// Chunks' ends into their starts, in place: the state carried from the sequence's start (backward:
+// the gradient from its end) to each chunk, a thread a state. Bound by the latency of its loads:
+// the operands of 32 chunks are in flight at a time.
+template <class T, bool BACK>
+__global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
+  const uint32_t i = blockIdx.x * 64 + threadIdx.x;
+  if (i >= a.batch * a.width * a.states) return;
+  const uint32_t k = i % a.states, d = i / a.states % a.width, b = i / a.states / a.width;
+  const T rate = decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k]));
+  const T* given = (const T*)(BACK ? a.carry : a.state);
+  T h = given ? given[i] : T(0);
+  constexpr uint32_t FLIGHT = 32;
+  auto row = [&](uint32_t c) { return ((uint64_t)b * chunks + (BACK ? chunks - 1 - c : c)) * a.width + d; };
+  for (uint32_t c = 0; c < chunks; c += FLIGHT) {
+    T end[FLIGHT], total[FLIGHT];
 #pragma unroll
-    for (int j = 0; j < NS; j++)
-      if (k0 + j < a.states) h[j] = fma_(decay(total, rate[j]), h[j], ((const T*)a.ends)[at * a.states + k0 + j]);
+    for (uint32_t j = 0; j < FLIGHT; j++) {
+      const uint64_t r = row(min(c + j, chunks - 1));
+      total[j] = ((const T*)a.totals)[r];
+      end[j] = ((const T*)a.ends)[r * a.states + k];
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < FLIGHT; j++) {
+      if (c + j >= chunks) break;
+      ((T*)a.ends)[row(c + j) * a.states + k] = h;
+      h = fma_(decay(total[j], rate), h, end[j]);
+    }
   }
 }
 
@@ -509,13 +591,16 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
+  const bool whole = a.states % NS == 0;
   T rate[NS], h[NS];
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
+  Vec<T, NS> from{};
+  if (on && chunks > 1) from = load_states<T, NS>(a.ends, ((uint64_t)p.b * chunks + p.chunk) * a.width + d, q * NS, a.states, whole);
+  else if (on && a.state) from = load_states<T, NS>(a.state, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    const uint32_t k = q * NS + j;
-    const bool has = on && k < a.states;
-    rate[j] = has ? decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k])) : T(0);
-    h[j] = has && a.state ? ((const T*)a.state)[((uint64_t)p.b * a.width + d) * a.states + k] : T(0);
+    rate[j] = decay_rate(finite_rate(rates.v[j]));
+    h[j] = from.v[j];
   }
   const T skip = on && q == 0 && a.skip ? ((const T*)a.skip)[d] : T(0);
   const ScanMover<S> mv(p, vec);
@@ -531,7 +616,6 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
     cs.read(a, p, a.c, m);
   };
   read(p.first);
-  if (on) scan_start<T, NS, false>(a, p, chunks, d, q * NS, rate, h);
   for (uint32_t m = p.first; m < p.last; m++) {
     const bool in = mv.inside(p, m);
 #pragma unroll
@@ -544,10 +628,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
     const Vec<T, S::EPT> gate = z;
     __syncthreads();
     if (m + 1 < p.last) read(m + 1);
-    if (a.marks && on)
-#pragma unroll
-      for (int j = 0; j < NS; j++)
-        if (q * NS + j < a.states) ((T*)a.marks)[(((uint64_t)p.b * p.marks + m) * a.width + d) * a.states + q * NS + j] = h[j];
+    if (a.marks && on) store_states<T, NS>(a.marks, ((uint64_t)p.b * p.marks + m) * a.width + d, q * NS, a.states, whole, h);
     T mine = T(0);
 #pragma unroll
     for (int i = 0; i < TILE; i++) {
@@ -570,10 +651,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
     mv.store_to(a.y, mv.at(a, p, m), y, m * TILE + mv.row < a.length);
     __syncthreads();
   }
-  if (a.last && on && p.last == p.marks)
-#pragma unroll
-    for (int j = 0; j < NS; j++)
-      if (q * NS + j < a.states) ((T*)a.last)[((uint64_t)p.b * a.width + d) * a.states + q * NS + j] = h[j];
+  if (a.last && on && p.last == p.marks) store_states<T, NS>(a.last, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, h);
 }
 
 // Backward, tile by tile from the chunk's last. From the state kept before the tile, its decays e
@@ -590,21 +668,24 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c, wave = threadIdx.x / 64;
   const int copy = threadIdx.x % 16 / NL;
   const bool on = c < p.chs;
+  const bool whole = a.states % NS == 0;
   T rate[NS], rate_e[NS], back[NS], da[NS], dd = T(0);
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
+  Vec<T, NS> from{};
+  if (on && chunks > 1) from = load_states<T, NS>(a.ends, ((uint64_t)p.b * chunks + p.chunk) * a.width + d, q * NS, a.states, whole);
+  else if (on && a.carry) from = load_states<T, NS>(a.carry, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    const uint32_t k = q * NS + j;
-    const bool has = on && k < a.states;
-    rate[j] = has ? finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k]) : T(0);
+    rate[j] = finite_rate(rates.v[j]);
     rate_e[j] = decay_rate(rate[j]);
-    back[j] = has && a.carry ? ((const T*)a.carry)[((uint64_t)p.b * a.width + d) * a.states + k] : T(0);
+    back[j] = from.v[j];
     da[j] = T(0);
   }
   const T skip = on && a.skip ? ((const T*)a.skip)[d] : T(0);
   const ScanMover<S> mv(p, vec);
   Vec<T, S::EPT> x, raw, g, z{};
   ScanMaps<S> bs, cs;
-  T start[NS];
+  Vec<T, NS> start{};
   auto read = [&](uint32_t m) {
     const bool in = mv.inside(p, m);
     const uint64_t at = mv.at(a, p, m);
@@ -614,26 +695,31 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     if (a.gate) z = mv.template load_from<T>(a.gate, at, in);
     bs.read(a, p, a.b, m);
     cs.read(a, p, a.c, m);
-#pragma unroll
-    for (int j = 0; j < NS; j++)
-      start[j] = on && q * NS + j < a.states ? ((const T*)a.marks)[(((uint64_t)p.b * p.marks + m) * a.width + d) * a.states + q * NS + j] : T(0);
+    if (on) start = load_states<T, NS>(a.marks, ((uint64_t)p.b * p.marks + m) * a.width + d, q * NS, a.states, whole);
   };
   read(p.last - 1);
-  if (on) scan_start<T, NS, true>(a, p, chunks, d, q * NS, rate_e, back);
   for (uint32_t m = p.last; m-- > p.first;) {
     const bool in = mv.inside(p, m);
+    Vec<T, S::EPT> slope, gate_g;  // d dt / d raw; dy silu'(z)
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
+      T step = raw.v[j], gy = g.v[j];
+      slope.v[j] = T(1);
+      if (a.softplus && in) step = softplus(raw.v[j], &slope.v[j]);
+      if (a.gate) {
+        const T s = sigmoid(z.v[j]);
+        gate_g.v[j] = gy * silu_slope(z.v[j], s);
+        gy *= z.v[j] * s;
+      }
       sx[mv.col + j][mv.row] = x.v[j];
-      sdt[mv.col + j][mv.row] = a.softplus && in ? softplus(raw.v[j]) : raw.v[j];
-      sg[mv.col + j][mv.row] = a.gate ? g.v[j] * silu(z.v[j]) : g.v[j];
+      sdt[mv.col + j][mv.row] = step;
+      sg[mv.col + j][mv.row] = gy;
     }
     bs.put(&sb[0][0]);
     cs.put(&sc[0][0]);
     T h[NS];
 #pragma unroll
-    for (int j = 0; j < NS; j++) h[j] = start[j];
-    const Vec<T, S::EPT> raw0 = raw, g0 = g, z0 = z;
+    for (int j = 0; j < NS; j++) h[j] = start.v[j];
     __syncthreads();
     if (m > p.first) read(m - 1);
     T e[TILE][NS], kept[TILE][NS], mine = T(0), mine2 = T(0);
@@ -693,8 +779,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       dx.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
-      ddt.v[j] = !in ? T(0) : a.softplus ? sdt[mv.col + j][mv.row] * sigmoid(raw0.v[j]) : sdt[mv.col + j][mv.row];
-      dz.v[j] = in && a.gate ? g0.v[j] * sy[mv.col + j][mv.row] * silu_slope(z0.v[j], sigmoid(z0.v[j])) : T(0);
+      ddt.v[j] = in ? sdt[mv.col + j][mv.row] * slope.v[j] : T(0);
+      dz.v[j] = in && a.gate ? sy[mv.col + j][mv.row] * gate_g.v[j] : T(0);
     }
     const bool within = m * TILE + mv.row < a.length;
     const uint64_t at = mv.at(a, p, m);
@@ -718,12 +804,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   }
   if (!on) return;
   const uint64_t row = (uint64_t)p.b * chunks + p.chunk;
-#pragma unroll
-  for (int j = 0; j < NS; j++) {
-    if (q * NS + j >= a.states) continue;
-    if (a.da_rows) ((T*)a.da_rows)[(row * a.width + d) * a.states + q * NS + j] = da[j];
-    if (a.dstate && p.chunk == 0) ((T*)a.dstate)[((uint64_t)p.b * a.width + d) * a.states + q * NS + j] = back[j];
-  }
+  if (a.da_rows) store_states<T, NS>(a.da_rows, row * a.width + d, q * NS, a.states, whole, da);
+  if (a.dstate && p.chunk == 0) store_states<T, NS>(a.dstate, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, back);
   if (a.dd_rows && q == 0) ((T*)a.dd_rows)[row * a.width + d] = dd;
 }
 
@@ -745,9 +827,11 @@ void scan_shape(uint32_t states, F f) {
   }
 }
 
-// Tiles of a group's channels, and the chunks a sequence is cut into: enough blocks to fill the
-// chip, chunks of at least SCAN_CHUNK_MIN tiles, at most SCAN_CHUNKS of them.
-constexpr uint32_t SCAN_BLOCKS = 1024, SCAN_CHUNK_MIN = 4, SCAN_CHUNKS = 64;
+// Tiles of a group's channels, and the chunks a sequence is cut into: as many as bring the launch to
+// SCAN_BLOCKS blocks, two a CU, but no more than SCAN_CHUNKS. More and shorter chunks cost more
+// joining than they save (2 x 2048 x 512, 16 states, forward and backward: 32 chunks 112 us, 64 chunks
+// 123), fewer leave CUs idle (3 x 777 x 200, 8 states: 25 chunks 46 us, 13 chunks 62).
+constexpr uint32_t SCAN_BLOCKS = 512, SCAN_CHUNKS = 64;
 
 struct ScanCut {
   uint32_t tiles = 1, chunk_tiles = 1, chunks = 1;
@@ -762,7 +846,7 @@ ScanCut scan_cut(const ScanArgs& a) {
   const uint32_t marks = (a.length + TILE - 1) / TILE;
   const uint64_t blocks = (uint64_t)a.batch * a.groups * cut.tiles;
   const uint32_t wanted = (uint32_t)std::min<uint64_t>((SCAN_BLOCKS + blocks - 1) / blocks, SCAN_CHUNKS);
-  cut.chunk_tiles = std::max((marks + wanted - 1) / wanted, std::min(marks, SCAN_CHUNK_MIN));
+  cut.chunk_tiles = (marks + wanted - 1) / wanted;
   cut.chunks = (marks + cut.chunk_tiles - 1) / cut.chunk_tiles;
   return cut;
 }
@@ -778,8 +862,11 @@ void launch_scan(hipStream_t s, ScanArgs a) {
     constexpr int NL = decltype(nl)::value, NS = decltype(ns)::value, EPT = ScanShape<T, NL, NS>::EPT;
     const bool vec = a.width % EPT == 0 && (a.width / a.groups) % EPT == 0;
     const uint32_t blocks = a.batch * a.groups * cut.tiles;
-    if (cut.chunks > 1)
+    if (cut.chunks > 1) {
+      const uint32_t joins = (a.batch * a.width * a.states + 63) / 64;
       hipLaunchKernelGGL((k_scan_ends<T, NL, NS, GRAD>), dim3(blocks * (cut.chunks - 1)), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+      hipLaunchKernelGGL((k_scan_join<T, GRAD>), dim3(joins), dim3(64), 0, s, a, cut.chunks);
+    }
     if constexpr (GRAD) hipLaunchKernelGGL((k_scan_grad<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
     else hipLaunchKernelGGL((k_scan<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
   });
