@@ -89,11 +89,13 @@
  *                  one) then x; 1: the K - 1 rows of past that end the sequence
  *       _GRAD      in the same, dy (, d of result 1); out dx, dw, dbias, dstate
  *     SELECTIVE_SCAN in x, dt[B,T,D], a[D,N], b, c[B,T,G,N] (, d[D]) (, z[B,T,D]) (, state[B,D,N])
- *                  (, lengths[B]); h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t];
+ *                  (, lengths[B]) (with RG_SCAN_JOINED one b[B,T,2 G,N], b's groups then c's, and
+ *                  no c); h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t];
  *                  out 0: (c[t] . h[t] + d x[t]) silu(z[t]); 1: the last h; 2: marks, h before
  *                  positions 0, RG_SCAN_MARK, 2 RG_SCAN_MARK, ..., for the gradient alone
  *       _GRAD      in the same, marks, dy (, d of result 1); out dx, ddt, da, db, dc, dd, dz, dstate
- *     ROTARY_NORM  in x[B,T,H,hd], positions[T] or [B,T] (, gain[S,hd]); out x with the heads of
+ *     ROTARY_NORM  in x[B,T,H,hd], positions[T], [B,T] or [B,1] (the first of each sequence)
+ *                  (, gain[S,hd]); out x with the heads of
  *                  section s divided by their root mean square and scaled by gain[s], and their
  *                  pairs (i, i + R / 2), i < R / 2, turned by position * base^(-2 i / R)
  *       _GRAD      in the same, dy; out dx, dgain
@@ -141,7 +143,8 @@ enum rg_op {
 /* Flags of the sequence operators: which optional operands are present, and the variants. */
 enum rg_conv_flags { RG_CONV_BIAS = 1, RG_CONV_STATE = 2, RG_CONV_LENGTHS = 4, RG_CONV_SILU = 8, RG_CONV_CARRY = 16 };
 enum rg_scan_flags {
-  RG_SCAN_SKIP = 1, RG_SCAN_GATE = 2, RG_SCAN_STATE = 4, RG_SCAN_LENGTHS = 8, RG_SCAN_SOFTPLUS = 16, RG_SCAN_CARRY = 32
+  RG_SCAN_SKIP = 1, RG_SCAN_GATE = 2, RG_SCAN_STATE = 4, RG_SCAN_LENGTHS = 8, RG_SCAN_SOFTPLUS = 16, RG_SCAN_CARRY = 32,
+  RG_SCAN_JOINED = 64 /* b holds b and c: [B,T,2 G,N], and c is no operand */
 };
 enum rg_rotary_flags { RG_ROTARY_GAIN = 1 };
 /* Taps of a causal convolution, states of a selective scan, and the length of a head. */
@@ -204,6 +207,7 @@ struct Sequence {
   int x = 0, w = -1, bias = -1, dt = -1, a = -1, b = -1, c = -1, skip = -1, gate = -1, state = -1, lengths = -1, marks = -1, dy = -1,
       carry = -1, positions = -1, gain = -1;
   bool shared_positions = false; /* positions of [length], the same for every sequence */
+  bool positions_from = false;   /* positions of [batch, 1], the first of each sequence */
   std::vector<std::vector<int64_t>> results;
   std::string wrong; /* empty when the operands fit */
 };
@@ -236,7 +240,7 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
     q.dt = take(true);
     q.a = take(true);
     q.b = take(true);
-    q.c = take(true);
+    q.c = take(!(f & RG_SCAN_JOINED));
     q.skip = take(f & RG_SCAN_SKIP);
     q.gate = take(f & RG_SCAN_GATE);
     q.state = take(f & RG_SCAN_STATE);
@@ -292,7 +296,9 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
     if (at.turn < 0 || at.turn % 2 != 0 || at.turn > q.head) fail("rotary_dims_must_be_even_and_within_the_head");
     const std::vector<int64_t>& p = s[(size_t)q.positions];
     q.shared_positions = p.size() == 1;
+    q.positions_from = p.size() == 2 && p[1] == 1;
     if (q.shared_positions) dims(q.positions, {q.length}, "positions_must_be_length_or_batch_length");
+    else if (q.positions_from) dims(q.positions, {q.batch, 1}, "positions_must_be_length_or_batch_length");
     else dims(q.positions, {q.batch, q.length}, "positions_must_be_length_or_batch_length");
     const std::vector<int64_t> gain = {(int64_t)at.sections.size(), q.head};
     if (q.gain >= 0) dims(q.gain, gain, "gain_must_be_sections_head");
@@ -305,15 +311,16 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
       return q;
     }
     q.states = a[1];
-    if (b.size() != 4 || b[0] != q.batch || b[1] != q.length || b[3] != q.states || q.width % b[2] != 0) {
+    const int64_t maps = q.c < 0 ? 2 : 1;
+    if (b.size() != 4 || b[0] != q.batch || b[1] != q.length || b[3] != q.states || b[2] % maps != 0 || q.width % (b[2] / maps) != 0) {
       fail("b_must_be_batch_length_groups_states_with_groups_dividing_the_width");
       return q;
     }
-    q.groups = b[2];
+    q.groups = b[2] / maps;
     const std::vector<int64_t> state = {q.batch, q.width, q.states};
     const std::vector<int64_t> marks = {q.batch, (q.length + RG_SCAN_MARK - 1) / RG_SCAN_MARK, q.width, q.states};
     dims(q.dt, x, "dt_shape_differs_from_x");
-    dims(q.c, b, "c_shape_differs_from_b");
+    if (q.c >= 0) dims(q.c, b, "c_shape_differs_from_b");
     if (q.skip >= 0) dims(q.skip, {q.width}, "d_must_be_width");
     if (q.gate >= 0) dims(q.gate, x, "z_shape_differs_from_x");
     if (q.state >= 0) dims(q.state, state, "state_must_be_batch_width_states");

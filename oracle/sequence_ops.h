@@ -86,11 +86,14 @@ void selective_scan(const Operands<T>& o) {
   const T *x = o.arg(q.x), *raw = o.arg(q.dt), *a = o.arg(q.a), *bm = o.arg(q.b), *cm = o.arg(q.c), *skip = o.arg(q.skip), *z = o.arg(q.gate),
           *state = o.arg(q.state), *dy = o.arg(q.dy), *carry = o.arg(q.carry);
   const int64_t D = q.width, N = q.states, L = q.length, G = q.groups, per = D / G;
+  const bool joined = q.c < 0;  // c's groups follow b's in one operand
+  const int64_t GM = joined ? 2 * G : G, cg = joined ? G * N : 0;
+  if (joined) cm = bm;
   const bool grad = dy != nullptr, soft = o.has(RG_SCAN_SOFTPLUS);
   std::vector<double> da((size_t)(D * N), 0.0), dd((size_t)D, 0.0);
   std::vector<double> db, dc;
   if (grad) {
-    db.assign((size_t)(q.batch * L * G * N), 0.0);
+    db.assign((size_t)(q.batch * L * GM * N), 0.0);
     dc.assign(db.size(), 0.0);
     for (int r : {0, 1, 6})  // positions outside a sequence
       if (o.out[(size_t)r]) std::fill(o.out[(size_t)r], o.out[(size_t)r] + q.batch * L * D, (T)0);
@@ -107,12 +110,12 @@ void selective_scan(const Operands<T>& o) {
         for (int64_t s = 0; s < N; s++) h[(size_t)s] = (double)state[(b * D + d) * N + s];
       std::vector<double> y((size_t)n, 0.0);
       for (int64_t t = 0; t < n; t++) {
-        const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * G + g) * N;
+        const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * GM + g) * N;
         const double dt = soft ? softplus((double)raw[at]) : (double)raw[at], u = (double)x[at];
         for (int64_t s = 0; s < N; s++) {
           const double v = std::exp(dt * (double)a[d * N + s]) * h[(size_t)(t * N + s)] + dt * u * (double)bm[row + s];
           h[(size_t)((t + 1) * N + s)] = v;
-          y[(size_t)t] += (double)cm[row + s] * v;
+          y[(size_t)t] += (double)cm[row + cg + s] * v;
         }
         if (skip) y[(size_t)t] += (double)skip[d] * u;
         if (!grad && o.out[0]) o.out[0][at] = (T)(z ? y[(size_t)t] * (double)z[at] * sigmoid((double)z[at]) : y[(size_t)t]);
@@ -126,7 +129,7 @@ void selective_scan(const Operands<T>& o) {
       if (carry)
         for (int64_t s = 0; s < N; s++) G_[(size_t)s] = (double)carry[(b * D + d) * N + s];
       for (int64_t t = n; t-- > 0;) {
-        const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * G + g) * N;
+        const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * GM + g) * N;
         const double dt = soft ? softplus((double)raw[at]) : (double)raw[at], u = (double)x[at];
         double gy = (double)dy[at];
         if (z) {
@@ -137,8 +140,8 @@ void selective_scan(const Operands<T>& o) {
         double sb = 0, sa = 0;
         for (int64_t s = 0; s < N; s++) {
           const double e = std::exp(dt * (double)a[d * N + s]), p = e * h[(size_t)(t * N + s)];
-          const double gr = G_[(size_t)s] + gy * (double)cm[row + s];
-          dc[(size_t)(row + s)] += gy * h[(size_t)((t + 1) * N + s)];
+          const double gr = G_[(size_t)s] + gy * (double)cm[row + cg + s];
+          (joined ? db : dc)[(size_t)(row + cg + s)] += gy * h[(size_t)((t + 1) * N + s)];
           db[(size_t)(row + s)] += gr * dt * u;
           sb += gr * (double)bm[row + s];
           sa += gr * p * (double)a[d * N + s];
@@ -160,7 +163,7 @@ void selective_scan(const Operands<T>& o) {
   if (grad) {
     store(2, da);
     store(3, db);
-    store(4, dc);
+    if (!joined) store(4, dc);
     store(5, dd);
   }
 }
@@ -174,7 +177,7 @@ void rotary_norm(const Operands<T>& o) {
   std::vector<double> dgain((size_t)(S * hd), 0.0), v((size_t)hd), u((size_t)hd);
   for (int64_t b = 0; b < q.batch; b++)
     for (int64_t t = 0; t < q.length; t++) {
-      const long double p = (long double)pos[q.shared_positions ? t : b * q.length + t];
+      const long double p = q.positions_from ? (long double)pos[b] + t : (long double)pos[q.shared_positions ? t : b * q.length + t];
       for (int64_t h = 0; h < q.heads; h++) {
         const int64_t at = ((b * q.length + t) * q.heads + h) * hd;
         int64_t s = 0, last = 0;

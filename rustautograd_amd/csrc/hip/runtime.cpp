@@ -623,6 +623,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     base.eps = i.sequence.eps;
     base.normed = q.gain >= 0;
     base.shared_positions = q.shared_positions;
+    base.positions_from = q.positions_from;
     if ((uint64_t)q.batch * q.length >= (1ull << 31)) throw std::runtime_error("more than 2^31 positions in one rotation");
     if (base.turn > 0) {
       // Turns per position of each pair, its double and what that leaves out.
@@ -662,14 +663,18 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
   base.width = (uint32_t)q.width;
   base.states = (uint32_t)q.states;
   base.groups = (uint32_t)q.groups;
+  const bool joined = q.c < 0;
+  base.map_stride = (uint32_t)(joined ? 2 * q.groups : q.groups);
   base.softplus = (i.sequence.flags & RG_SCAN_SOFTPLUS) != 0;
   const bool grad = i.op == RG_OP_SELECTIVE_SCAN_GRAD;
   const uint32_t tiles = rgk::scan_group_tiles(dtype, base), rows = rgk::scan_rows(dtype, base);
   prog.workspace_bytes = std::max(prog.workspace_bytes, rgk::scan_workspace(dtype, base));
-  const uint64_t maps = (uint64_t)q.batch * q.length * q.groups * q.states;
+  const uint64_t maps = (uint64_t)q.batch * q.length * base.map_stride * q.states;
+  // Where c lies after b in one operand, in bytes.
+  const uint64_t after = (uint64_t)q.groups * q.states * esize(dtype);
   // One tile of channels a group: its sums are the results.
   const bool direct = tiles == 1;
-  const int64_t db = grad && !direct ? partial(3, tiles, maps) : -1, dc = grad && !direct ? partial(4, tiles, maps) : -1;
+  const int64_t db = grad && !direct ? partial(3, tiles, maps) : -1, dc = grad && !direct && !joined ? partial(4, tiles, maps) : -1;
   const int64_t da = grad ? partial(2, rows, (uint64_t)q.width * q.states) : -1;
   const int64_t dd = grad && q.skip >= 0 ? partial(5, rows, (uint64_t)q.width) : -1;
   return [=](hipStream_t s, void* const* sl, void* ws) {
@@ -678,7 +683,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     a.dt = arg(sl, q.dt);
     a.a = arg(sl, q.a);
     a.b = arg(sl, q.b);
-    a.c = arg(sl, q.c);
+    a.c = joined ? (const void*)((const char*)a.b + after) : arg(sl, q.c);
     a.skip = arg(sl, q.skip);
     a.gate = arg(sl, q.gate);
     a.state = arg(sl, q.state);
@@ -697,7 +702,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     a.dx = slot(sl, outs[0]);
     a.ddt = slot(sl, outs[1]);
     a.db_rows = direct ? slot(sl, outs[3]) : place(ws, db);
-    a.dc_rows = direct ? slot(sl, outs[4]) : place(ws, dc);
+    a.dc_rows = joined ? (a.db_rows ? (char*)a.db_rows + after : nullptr) : direct ? slot(sl, outs[4]) : place(ws, dc);
     a.da_rows = place(ws, da);
     a.dd_rows = place(ws, dd);
     a.dz = slot(sl, outs[6]);

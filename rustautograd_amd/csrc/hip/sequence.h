@@ -26,13 +26,14 @@ void causal_conv_grad(hipStream_t s, int dtype, const ConvArgs& a);
 
 struct ScanArgs {
   uint32_t batch, length, width, states, groups;
+  uint32_t map_stride;          // rows of states from one position to the next, in b and in c
   bool softplus;
   const void *x, *dt, *a, *b, *c, *skip, *gate, *state;
   const int32_t* lengths;
   void *y, *last, *marks;       // forward; `marks` is read by the backward
   const void *dy, *carry;       // backward
   void *dx, *ddt, *dz, *dstate;
-  // Partial rows: of b and c one per tile of a group's channels, each [batch, length, groups,
+  // Partial rows: of b and c one per tile of a group's channels, each [batch, length, map_stride,
   // states]; of a ([width, states]) and the skip ([width]) scan_rows of them.
   void *db_rows, *dc_rows, *da_rows, *dd_rows;
   void* workspace;              // scan_workspace bytes
@@ -51,7 +52,7 @@ struct RotaryArgs {
   uint32_t batch, length, heads, head, turn;
   uint32_t sections, last[ROTARY_SECTIONS];  // head past the end of each section
   double eps;
-  bool normed, shared_positions;
+  bool normed, shared_positions, positions_from;
   const void *x, *gain;
   const int32_t* positions;
   const double2* turns;         // turns per position of each pair, as high and low parts

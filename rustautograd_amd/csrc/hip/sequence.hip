@@ -40,12 +40,10 @@ __device__ __forceinline__ T silu(T v) { return over(v, logistic_base(v)); }
 template <class T>
 __device__ __forceinline__ T silu_slope(T v, T s) { return s * fma_(v, T(1) - s, T(1)); }
 // log(1 + u), 0 <= u <= 1, to full relative precision: 2 artanh(s) = 2 s (1 + s^2/3 + s^4/5 + ...)
-// at s = u / (2 + u) <= 1/3, whose terms past s^16/17 are below 2e-10 of the sum.
+// at s = u / (2 + u) <= 1/3, whose terms past s^12/13 add up to less than 2e-8, a quarter of a rounding.
 __device__ __forceinline__ float log1p_(float u) {
   const float s = over(u, 2.0f + u), w = s * s;
-  float p = 1.0f / 17.0f;
-  p = fma_(p, w, 1.0f / 15.0f);
-  p = fma_(p, w, 1.0f / 13.0f);
+  float p = 1.0f / 13.0f;
   p = fma_(p, w, 1.0f / 11.0f);
   p = fma_(p, w, 1.0f / 9.0f);
   p = fma_(p, w, 1.0f / 7.0f);
@@ -235,46 +233,77 @@ __global__ void __launch_bounds__(TPB) k_conv_grad(ConvArgs a, uint32_t nx, uint
   }
 }
 
-constexpr int CONV_RUN = 8;
-
-template <class T, int V, class F>
-void conv_taps(const ConvArgs& a, F launch) {
-  switch (a.taps) {
-    case 2: launch(std::integral_constant<int, 2>()); break;
-    case 3: launch(std::integral_constant<int, 3>()); break;
-    case 4: launch(std::integral_constant<int, 4>()); break;
-    case 5: launch(std::integral_constant<int, 5>()); break;
-    case 6: launch(std::integral_constant<int, 6>()); break;
-    case 7: launch(std::integral_constant<int, 7>()); break;
-    case 8: launch(std::integral_constant<int, 8>()); break;
+template <class F>
+void conv_taps(uint32_t taps, F launch) {
+  using std::integral_constant;
+  switch (taps) {
+    case 2: launch(integral_constant<int, 2>()); break;
+    case 3: launch(integral_constant<int, 3>()); break;
+    case 4: launch(integral_constant<int, 4>()); break;
+    case 5: launch(integral_constant<int, 5>()); break;
+    case 6: launch(integral_constant<int, 6>()); break;
+    case 7: launch(integral_constant<int, 7>()); break;
+    case 8: launch(integral_constant<int, 8>()); break;
     default: break;
   }
 }
 
-template <class T, int V>
-void launch_conv(hipStream_t s, const ConvArgs& a, bool grad) {
-  const uint32_t nx = (a.width + 64 * V - 1) / (64 * V), runs = (a.length + 4 * CONV_RUN - 1) / (4 * CONV_RUN);
-  conv_taps<T, V>(a, [&](auto k) {
-    if (grad) hipLaunchKernelGGL((k_conv_grad<T, decltype(k)::value, V, CONV_RUN>), dim3(nx * runs * a.batch), dim3(TPB), 0, s, a, nx, runs);
-    else hipLaunchKernelGGL((k_conv<T, decltype(k)::value, V, CONV_RUN>), dim3(nx * runs * a.batch), dim3(TPB), 0, s, a, nx, runs);
+// Channels a lane takes (wide accesses) and the positions of a run (fewer of them read twice), as far
+// as that leaves eight waves a SIMD, or of runs two: 8 x 4096 x 2048 takes 88 us forward and 144
+// backward with four channels (6.1 and 5.6 TB/s; 95 and 162 with one), 4 x 1024 x 512 5.4 and 9.6 us
+// with one (7.1 and 11.6 with four), 5 x 333 x 77 backward 4.7 us in runs of four, 5.6 in runs of eight.
+struct ConvCut {
+  uint32_t v, r;
+};
+uint32_t conv_runs(const ConvArgs& a, uint32_t r) { return (a.length + 4 * r - 1) / (4 * r); }
+ConvCut conv_cut(int dtype, const ConvArgs& a) {
+  auto waves = [&](uint32_t v, uint32_t r) { return (uint64_t)a.batch * conv_runs(a, r) * 4 * ((a.width + 64 * v - 1) / (64 * v)); };
+  ConvCut cut{1, a.length <= 4 ? 1u : waves(1, 8) < 2048 ? 4u : 8u};
+  for (uint32_t v = dtype == RG_F32 ? 4 : 2; v > 1; v /= 2)
+    if (a.width % v == 0 && waves(v, cut.r) >= 8192) {
+      cut.v = v;
+      break;
+    }
+  return cut;
+}
+
+template <class T, int V, int R, bool GRAD>
+void launch_conv(hipStream_t s, const ConvArgs& a) {
+  const uint32_t nx = (a.width + 64 * V - 1) / (64 * V), runs = conv_runs(a, R);
+  const dim3 grid(nx * runs * a.batch);
+  conv_taps(a.taps, [&](auto k) {
+    if constexpr (GRAD) hipLaunchKernelGGL((k_conv_grad<T, decltype(k)::value, V, R>), grid, dim3(TPB), 0, s, a, nx, runs);
+    else hipLaunchKernelGGL((k_conv<T, decltype(k)::value, V, R>), grid, dim3(TPB), 0, s, a, nx, runs);
   });
+}
+
+template <class T, bool GRAD>
+void conv(hipStream_t s, int dtype, const ConvArgs& a) {
+  constexpr int MOST = sizeof(T) == 4 ? 4 : 2;
+  const ConvCut cut = conv_cut(dtype, a);
+  auto runs = [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    if (cut.r == 8) launch_conv<T, V, 8, GRAD>(s, a);
+    else if (cut.r == 4) launch_conv<T, V, 4, GRAD>(s, a);
+    else launch_conv<T, V, 1, GRAD>(s, a);
+  };
+  if (cut.v == MOST) runs(std::integral_constant<int, MOST>());
+  else if (cut.v == MOST / 2) runs(std::integral_constant<int, MOST / 2>());
+  else runs(std::integral_constant<int, 1>());
 }
 
 }  // namespace
 
-uint32_t conv_grad_rows(int, const ConvArgs& a) { return a.batch * ((a.length + 4 * CONV_RUN - 1) / (4 * CONV_RUN)); }
+uint32_t conv_grad_rows(int dtype, const ConvArgs& a) { return a.batch * conv_runs(a, conv_cut(dtype, a).r); }
 
-static void conv(hipStream_t s, int dtype, const ConvArgs& a, bool grad) {
-  if (dtype == RG_F32) {
-    if (a.width % 4 == 0) launch_conv<float, 4>(s, a, grad);
-    else launch_conv<float, 1>(s, a, grad);
-  } else {
-    if (a.width % 2 == 0) launch_conv<double, 2>(s, a, grad);
-    else launch_conv<double, 1>(s, a, grad);
-  }
+void causal_conv(hipStream_t s, int dtype, const ConvArgs& a) {
+  if (dtype == RG_F32) conv<float, false>(s, dtype, a);
+  else conv<double, false>(s, dtype, a);
 }
-void causal_conv(hipStream_t s, int dtype, const ConvArgs& a) { conv(s, dtype, a, false); }
-void causal_conv_grad(hipStream_t s, int dtype, const ConvArgs& a) { conv(s, dtype, a, true); }
+void causal_conv_grad(hipStream_t s, int dtype, const ConvArgs& a) {
+  if (dtype == RG_F32) conv<float, true>(s, dtype, a);
+  else conv<double, true>(s, dtype, a);
+}
 
 // ---- selective scan ---------------------------------------------------------------------------
 
@@ -367,7 +396,7 @@ struct ScanMaps {
       const uint32_t i = threadIdx.x + q * TPB, t = m * TILE + i / S::NP, k = i % S::NP;
       v[q] = typename S::T(0);
       if (i < TILE * S::NP && t < p.n && k < a.states)
-        v[q] = ((const typename S::T*)src)[(((uint64_t)p.b * a.length + t) * a.groups + p.group) * a.states + k];
+        v[q] = ((const typename S::T*)src)[(((uint64_t)p.b * a.length + t) * a.map_stride + p.group) * a.states + k];
     }
   }
   __device__ __forceinline__ void put(typename S::T* dst) const {
@@ -654,6 +683,48 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   if (a.last && on && p.last == p.marks) store_states<T, NS>(a.last, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, h);
 }
 
+// A few positions, single tokens above all: no tiles, every operand of a position loaded at once.
+// Bound by the latency of one round of loads, and for many sequences by the states, read and
+// written once (16 x 2048 channels, 16 states, one position: 4 MB).
+constexpr uint32_t SCAN_FEW = 4;
+template <class T, int NL, int NS>
+__global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
+  using S = ScanShape<T, NL, NS>;
+  const ScanPlace p = scan_place<S>(a, tiles, 0, 1);
+  const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
+  if (c >= p.chs) return;  // whole channels: the lanes that sum stay together
+  const bool whole = a.states % NS == 0;
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, d, q * NS, a.states, whole);
+  Vec<T, NS> from{};
+  if (a.state) from = load_states<T, NS>(a.state, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
+  const T skip = q == 0 && a.skip ? ((const T*)a.skip)[d] : T(0);
+  T h[NS];
+#pragma unroll
+  for (int j = 0; j < NS; j++) h[j] = from.v[j];
+  for (uint32_t t = 0; t < a.length; t++) {
+    const uint64_t at = ((uint64_t)p.b * a.length + t) * a.width + d, row = ((uint64_t)p.b * a.length + t) * a.map_stride + p.group;
+    T y = T(0);
+    if (t < p.n) {
+      const T u = ((const T*)a.x)[at];
+      T step = ((const T*)a.dt)[at], z = T(0);
+      if (a.gate) z = ((const T*)a.gate)[at];
+      const Vec<T, NS> b = load_states<T, NS>(a.b, row, q * NS, a.states, whole), m = load_states<T, NS>(a.c, row, q * NS, a.states, whole);
+      if (a.softplus) step = softplus(step);
+      const T drive = step * u;
+      y = skip * u;
+#pragma unroll
+      for (int j = 0; j < NS; j++) {
+        h[j] = fma_(decay(step, decay_rate(finite_rate(rates.v[j]))), h[j], drive * b.v[j]);
+        y = fma_(m.v[j], h[j], y);
+      }
+      y = channel_sum<NL>(y);
+      if (a.gate) y *= silu(z);
+    }
+    if (a.y && q == 0) ((T*)a.y)[at] = y;
+  }
+  if (a.last) store_states<T, NS>(a.last, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, h);
+}
+
 // Backward, tile by tile from the chunk's last. From the state kept before the tile, its decays e
 // and the decayed states p = e h[t - 1] are formed again, then with G = dL/dh[t] carried back:
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
@@ -797,8 +868,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
       if (t < p.n)
 #pragma unroll
         for (int v = 0; v < WAVES; v++) sum += red[v][r][from];
-      const uint64_t rows = (uint64_t)a.batch * a.length * a.groups * a.states;
-      to[p.tile * rows + (((uint64_t)p.b * a.length + t) * a.groups + p.group) * a.states + k] = sum;
+      const uint64_t rows = (uint64_t)a.batch * a.length * a.map_stride * a.states;
+      to[p.tile * rows + (((uint64_t)p.b * a.length + t) * a.map_stride + p.group) * a.states + k] = sum;
     }
     __syncthreads();
   }
@@ -862,6 +933,10 @@ void launch_scan(hipStream_t s, ScanArgs a) {
     constexpr int NL = decltype(nl)::value, NS = decltype(ns)::value, EPT = ScanShape<T, NL, NS>::EPT;
     const bool vec = a.width % EPT == 0 && (a.width / a.groups) % EPT == 0;
     const uint32_t blocks = a.batch * a.groups * cut.tiles;
+    if (!GRAD && a.length <= SCAN_FEW && !a.marks) {
+      hipLaunchKernelGGL((k_scan_few<T, NL, NS>), dim3(blocks), dim3(TPB), 0, s, a, cut.tiles);
+      return;
+    }
     if (cut.chunks > 1) {
       const uint32_t joins = (a.batch * a.width * a.states + 63) / 64;
       hipLaunchKernelGGL((k_scan_ends<T, NL, NS, GRAD>), dim3(blocks * (cut.chunks - 1)), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
@@ -894,26 +969,55 @@ void selective_scan_grad(hipStream_t s, int dtype, const ScanArgs& a) {
 
 namespace {
 
-__device__ __forceinline__ void sin_cos_turns(double f, float* sn, float* cs) { sincospif(2.0f * (float)f, sn, cs); }
+// Sine and cosine of f turns, |f| <= 1/2: the nearest quarter taken off in 64 bits, then the Taylor
+// series of the remaining angle, at most pi / 4, whose next terms are below 2e-9.
+__device__ __forceinline__ void sin_cos_turns(double f, float* sn, float* cs) {
+  const double quarter = rint(4.0 * f);
+  const float t = (float)(fma(quarter, -0.25, f) * 6.283185307179586477), w = t * t;
+  const int q = (int)quarter;
+  float s = fma_(w, 2.7557319e-6f, -1.9841270e-4f);
+  s = fma_(w, s, 8.3333333e-3f);
+  s = fma_(w, s, -1.6666667e-1f);
+  s = fma_(t * w, s, t);
+  float c = fma_(w, -2.7557319e-7f, 2.4801587e-5f);
+  c = fma_(w, c, -1.3888889e-3f);
+  c = fma_(w, c, 4.1666667e-2f);
+  c = fma_(w, c, -0.5f);
+  c = fma_(w, c, 1.0f);
+  const float x = q & 1 ? c : s, y = q & 1 ? s : c;
+  *sn = q & 2 ? -x : x;
+  *cs = (q + 1) & 2 ? -y : y;
+}
 __device__ __forceinline__ void sin_cos_turns(double f, double* sn, double* cs) { sincospi(2.0 * f, sn, cs); }
 
+// The sum over the LG lanes of a group, in all of them (every lane of the wave takes part).
+template <int LG, class T>
+__device__ __forceinline__ T group_sum(T v) {
+  v = channel_sum<LG>(v);
+  if (LG >= 32) v = rows(v, v);
+  if (LG >= 64) v = halves(v, v);
+  return v;
+}
+
 // LG lanes share a head, each with UPL units of V pairs: both halves of a pair lie in one lane, so
-// the turn needs no exchange. A group of lanes keeps one head and walks the tokens.
+// the turn needs no exchange. A group of lanes keeps one head, its gain and its angles per position
+// in registers and walks the tokens. Bound by memory: 4 x 1024 x 24 heads of 64, the values' passing,
+// take 50 MB forward and 75 MB backward.
 template <class T, int V, int LG, int UPL, bool GRAD>
 __global__ void __launch_bounds__(TPB) k_rotary(RotaryArgs a) {
   constexpr int GROUPS = TPB / LG;
   const uint32_t group = blockIdx.x * GROUPS + threadIdx.x / LG, lane = threadIdx.x % LG;
-  const uint32_t all = gridDim.x * GROUPS, walkers = all / a.heads;
+  const uint32_t walkers = gridDim.x * GROUPS / a.heads, steps = (a.batch * a.length + walkers - 1) / walkers;
   const uint32_t head = group % a.heads, first = group / a.heads;
   const uint32_t half = a.turn / 2, rest = (a.head - a.turn) / 2, tokens = a.batch * a.length;
   uint32_t section = 0;
   while (section < a.sections && head >= a.last[section]) section++;
-  const bool on = first < walkers;
-  const bool used = section < a.sections;
+  const bool on = first < walkers, used = section < a.sections, normed = used && a.normed;
   // Where this lane's units lie in a head: their first and second halves.
   uint32_t lo[UPL], hi[UPL];
   bool has[UPL];
   Vec<T, V> g_lo[UPL], g_hi[UPL], d_lo[UPL], d_hi[UPL];
+  double2 turns[UPL][V];
 #pragma unroll
   for (int k = 0; k < UPL; k++) {
     const uint32_t u = (lane + k * LG) * V;
@@ -922,56 +1026,58 @@ __global__ void __launch_bounds__(TPB) k_rotary(RotaryArgs a) {
     hi[k] = lo[k] + (u < half ? half : rest);
     d_lo[k] = d_hi[k] = Vec<T, V>{};
 #pragma unroll
-    for (int v = 0; v < V; v++) g_lo[k].v[v] = g_hi[k].v[v] = T(1);
-    if (has[k] && used && a.normed) {
+    for (int v = 0; v < V; v++) {
+      g_lo[k].v[v] = g_hi[k].v[v] = T(1);
+      turns[k][v] = has[k] && used && u + v < half ? a.turns[u + v] : make_double2(0.0, 0.0);
+    }
+    if (has[k] && normed) {
       g_lo[k] = load<T, V>((const T*)a.gain + section * a.head + lo[k]);
       g_hi[k] = load<T, V>((const T*)a.gain + section * a.head + hi[k]);
     }
   }
-  for (uint32_t token = on ? first : tokens; token < tokens; token += walkers) {
+  for (uint32_t i = 0; i < steps; i++) {
+    const uint32_t token = first + i * walkers;
+    const bool valid = on && token < tokens;
     const uint64_t at = ((uint64_t)token * a.heads + head) * a.head;
-    const double pos = (double)a.positions[a.shared_positions ? token % a.length : token];
+    double pos = 0.0;
+    if (valid) {
+      const uint32_t b = token / a.length, t = token - b * a.length;
+      pos = a.positions_from ? (double)a.positions[b] + (double)t : (double)a.positions[a.shared_positions ? t : token];
+    }
     Vec<T, V> x_lo[UPL], x_hi[UPL], w_lo[UPL], w_hi[UPL];
     T ss = T(0);
 #pragma unroll
     for (int k = 0; k < UPL; k++) {
       x_lo[k] = x_hi[k] = w_lo[k] = w_hi[k] = Vec<T, V>{};
-      if (!has[k]) continue;
-      x_lo[k] = load<T, V>((const T*)a.x + at + lo[k]);
-      x_hi[k] = load<T, V>((const T*)a.x + at + hi[k]);
-      if (GRAD) {
-        w_lo[k] = load<T, V>((const T*)a.dy + at + lo[k]);
-        w_hi[k] = load<T, V>((const T*)a.dy + at + hi[k]);
+      if (valid && has[k]) {
+        x_lo[k] = load<T, V>((const T*)a.x + at + lo[k]);
+        x_hi[k] = load<T, V>((const T*)a.x + at + hi[k]);
+        if (GRAD) {
+          w_lo[k] = load<T, V>((const T*)a.dy + at + lo[k]);
+          w_hi[k] = load<T, V>((const T*)a.dy + at + hi[k]);
+        }
       }
 #pragma unroll
       for (int v = 0; v < V; v++) ss = fma_(x_lo[k].v[v], x_lo[k].v[v], fma_(x_hi[k].v[v], x_hi[k].v[v], ss));
     }
-    T r = T(1);
-    if (a.normed && used) {
-#pragma unroll
-      for (int m = 1; m < LG; m <<= 1) ss += __shfl_xor(ss, m);
-      r = T(1) / sqrt_(ss / T(a.head) + T(a.eps));
-    }
+    ss = group_sum<LG>(ss);
+    const T r = normed ? T(1) / sqrt_(ss / T(a.head) + T(a.eps)) : T(1);
     T mean = T(0);
 #pragma unroll
     for (int k = 0; k < UPL; k++) {
-      if (!has[k] || !used) continue;
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        T sn = T(0), cs = T(1);
-        if (lo[k] + v < half) {
-          const double2 turn = a.turns[lo[k] + v];
-          const double whole = rint(pos * turn.x);
-          sin_cos_turns(fma(pos, turn.y, fma(pos, turn.x, -whole)), &sn, &cs);
-        }
+        T sn, cs;
+        const double2 turn = turns[k][v];
+        sin_cos_turns(fma(pos, turn.y, fma(pos, turn.x, -rint(pos * turn.x))), &sn, &cs);
+        const T nf = x_lo[k].v[v] * r, ns = x_hi[k].v[v] * r;
         if (!GRAD) {
-          const T f = x_lo[k].v[v] * r * g_lo[k].v[v], s = x_hi[k].v[v] * r * g_hi[k].v[v];
-          w_lo[k].v[v] = fma_(f, cs, -(s * sn));
-          w_hi[k].v[v] = fma_(s, cs, f * sn);
-        } else {
+          const T f = nf * g_lo[k].v[v], s = ns * g_hi[k].v[v];
+          w_lo[k].v[v] = used ? fma_(f, cs, -(s * sn)) : x_lo[k].v[v];
+          w_hi[k].v[v] = used ? fma_(s, cs, f * sn) : x_hi[k].v[v];
+        } else if (used) {
           const T f = w_lo[k].v[v], s = w_hi[k].v[v];
           const T uf = fma_(f, cs, s * sn), us = fma_(s, cs, -(f * sn));
-          const T nf = x_lo[k].v[v] * r, ns = x_hi[k].v[v] * r;
           d_lo[k].v[v] = fma_(uf, nf, d_lo[k].v[v]);
           d_hi[k].v[v] = fma_(us, ns, d_hi[k].v[v]);
           w_lo[k].v[v] = uf * g_lo[k].v[v];
@@ -980,49 +1086,49 @@ __global__ void __launch_bounds__(TPB) k_rotary(RotaryArgs a) {
         }
       }
     }
-    if (GRAD && a.normed && used) {
+    if (GRAD) {
+      mean = group_sum<LG>(mean) / T(a.head);
+      if (normed)
 #pragma unroll
-      for (int m = 1; m < LG; m <<= 1) mean += __shfl_xor(mean, m);
-      mean /= T(a.head);
+        for (int k = 0; k < UPL; k++)
 #pragma unroll
-      for (int k = 0; k < UPL; k++)
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-          w_lo[k].v[v] = r * fma_(-(x_lo[k].v[v] * r), mean, w_lo[k].v[v]);
-          w_hi[k].v[v] = r * fma_(-(x_hi[k].v[v] * r), mean, w_hi[k].v[v]);
-        }
+          for (int v = 0; v < V; v++) {
+            w_lo[k].v[v] = r * fma_(-(x_lo[k].v[v] * r), mean, w_lo[k].v[v]);
+            w_hi[k].v[v] = r * fma_(-(x_hi[k].v[v] * r), mean, w_hi[k].v[v]);
+          }
     }
     T* out = (T*)(GRAD ? a.dx : a.y);
-    if (out)
+    if (out && valid)
 #pragma unroll
       for (int k = 0; k < UPL; k++) {
         if (!has[k]) continue;
-        const bool pass = !GRAD && !used;
-        store<T, V>(out + at + lo[k], pass ? x_lo[k] : w_lo[k]);
-        store<T, V>(out + at + hi[k], pass ? x_hi[k] : w_hi[k]);
+        store<T, V>(out + at + lo[k], w_lo[k]);
+        store<T, V>(out + at + hi[k], w_hi[k]);
       }
   }
-  if (!GRAD || !a.dgain_rows) return;
-  // One partial row a block: the groups of a section summed in order.
-  __shared__ T part[GROUPS][2 * LG * UPL * V];
-  __shared__ uint32_t of[GROUPS];
-  const uint32_t mine = threadIdx.x / LG;
-  if (lane == 0) of[mine] = on && used ? section : a.sections;
+  if constexpr (GRAD) {
+    if (!a.dgain_rows) return;
+    // One partial row a block: the groups of a section summed in order.
+    __shared__ T part[GROUPS][2 * LG * UPL * V];
+    __shared__ uint32_t of[GROUPS];
+    const uint32_t mine = threadIdx.x / LG;
+    if (lane == 0) of[mine] = on && used ? section : a.sections;
 #pragma unroll
-  for (int k = 0; k < UPL; k++)
-    if (has[k])
+    for (int k = 0; k < UPL; k++)
+      if (has[k])
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        part[mine][lo[k] + v] = d_lo[k].v[v];
-        part[mine][hi[k] + v] = d_hi[k].v[v];
-      }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < a.sections * a.head; i += TPB) {
-    const uint32_t s = i / a.head, k = i % a.head;
-    T sum = T(0);
-    for (int g = 0; g < GROUPS; g++)
-      if (of[g] == s) sum += part[g][k];
-    ((T*)a.dgain_rows)[(uint64_t)blockIdx.x * a.sections * a.head + i] = sum;
+        for (int v = 0; v < V; v++) {
+          part[mine][lo[k] + v] = d_lo[k].v[v];
+          part[mine][hi[k] + v] = d_hi[k].v[v];
+        }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.sections * a.head; i += TPB) {
+      const uint32_t s = i / a.head, k = i % a.head;
+      T sum = T(0);
+#pragma unroll 8
+      for (int g = 0; g < GROUPS; g++) sum += of[g] == s ? part[g][k] : T(0);
+      ((T*)a.dgain_rows)[(uint64_t)blockIdx.x * a.sections * a.head + i] = sum;
+    }
   }
 }
 
@@ -1044,18 +1150,22 @@ uint32_t rotary_unit(int dtype, const RotaryArgs& a) {
   return a.turn % (2 * v) == 0 && a.head % (2 * v) == 0 ? v : 1;
 }
 
-uint32_t rotary_blocks(int dtype, const RotaryArgs& a) {
+// Blocks: as many as there are heads of tokens for, up to eight a CU; backward two, each of which
+// leaves a partial row for the fold to sum (4 x 1024 x 24 heads of 64: 512 rows fold in 5 us, 1024 in 9).
+constexpr uint32_t ROTARY_BLOCKS = 2048, ROTARY_GRAD_BLOCKS = 512;
+
+uint32_t rotary_blocks(int dtype, const RotaryArgs& a, bool grad) {
   uint32_t blocks = 0;
   rotary_shape(a.head / 2 / rotary_unit(dtype, a), [&](auto lg, auto) {
     const uint64_t per = TPB / decltype(lg)::value, items = (uint64_t)a.batch * a.length * a.heads;
-    blocks = (uint32_t)std::max<uint64_t>(std::min<uint64_t>((items + per - 1) / per, 1024), (a.heads + per - 1) / per);
+    blocks = (uint32_t)std::max<uint64_t>(std::min<uint64_t>((items + per - 1) / per, grad ? ROTARY_GRAD_BLOCKS : ROTARY_BLOCKS), (a.heads + per - 1) / per);
   });
   return blocks;
 }
 
 template <class T, int V, bool GRAD>
 void launch_rotary(hipStream_t s, int dtype, const RotaryArgs& a) {
-  const uint32_t blocks = rotary_blocks(dtype, a);
+  const uint32_t blocks = rotary_blocks(dtype, a, GRAD);
   rotary_shape(a.head / 2 / V, [&](auto lg, auto upl) {
     hipLaunchKernelGGL((k_rotary<T, V, decltype(lg)::value, decltype(upl)::value, GRAD>), dim3(blocks), dim3(TPB), 0, s, a);
   });
@@ -1075,7 +1185,7 @@ void rotary(hipStream_t s, int dtype, const RotaryArgs& a) {
 
 }  // namespace
 
-uint32_t rotary_grad_rows(int dtype, const RotaryArgs& a) { return rotary_blocks(dtype, a); }
+uint32_t rotary_grad_rows(int dtype, const RotaryArgs& a) { return rotary_blocks(dtype, a, true); }
 void rotary_norm(hipStream_t s, int dtype, const RotaryArgs& a) { rotary<false>(s, dtype, a); }
 void rotary_norm_grad(hipStream_t s, int dtype, const RotaryArgs& a) { rotary<true>(s, dtype, a); }
 

@@ -355,11 +355,11 @@ class SelectiveSSM(Layer):
         u, conv = causal_conv(self.inward(params["in"], x), params["conv"]["w"], params["conv"]["b"], conv, lengths, "silu")
         maps = self.proj(params["proj"], u)
         dt = self.dt(params["dt"], maps[..., :self.rank])
-        positions = arange(t) if pos is None or not self.rotary else pos.reshape(b, 1) + arange(t)
+        positions = pos.reshape(b, 1) if self.rotary and pos is not None else None
         maps = rotary_norm(maps[..., self.rank:].reshape(b, t, 2 * self.groups, self.states), params["gain"], positions,
                            (self.groups, self.groups), None if self.rotary else 0, self.base)
-        y, scan = selective_scan(u, dt, -exp(params["a_log"]), maps[:, :, :self.groups], maps[:, :, self.groups:], params["d"],
-                                 self.gate(params["gate"], x), scan, lengths, softplus=True)
+        y, scan = selective_scan(u, dt, -exp(params["a_log"]), maps, None, params["d"], self.gate(params["gate"], x), scan, lengths,
+                                 softplus=True)
         read = t if lengths is None else lengths
         pos = zeros((b,), "int32") + read if pos is None else pos + read
         return self.out(params["out"], y), {"conv": conv, "scan": scan, "pos": pos}

@@ -13,7 +13,7 @@ from .tensor import TRACES, Tracer, caller_source, error, first_dtype, lift
 
 # The operand and variant flags of include/rg_plan.h.
 _CONV_BIAS, _CONV_STATE, _CONV_LENGTHS, _CONV_SILU = 1, 2, 4, 8
-_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS, _SCAN_SOFTPLUS = 1, 2, 4, 8, 16
+_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS, _SCAN_SOFTPLUS, _SCAN_JOINED = 1, 2, 4, 8, 16, 64
 _ROTARY_GAIN = 1
 
 
@@ -65,24 +65,26 @@ def causal_conv(x, w, bias=None, state=None, lengths=None, activation=None):
     return _with_results("causal_conv", operands, {"flags": flags | (_CONV_SILU if activation else 0)}, 2)
 
 
-def selective_scan(x, dt, a, b, c, d=None, z=None, state=None, lengths=None, softplus=False):
+def selective_scan(x, dt, a, b, c=None, d=None, z=None, state=None, lengths=None, softplus=False):
     """The selective state space scan: every channel of `x` (batch, length, width) drives `states`
     linear recurrences whose step `dt` (as `x`) and maps `b`, `c` change from position to position,
 
         h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t],   y[t] = (sum_n c[t] h[t] + d x[t]) silu(z[t]).
 
     `a` is (width, states), at most 64 of them; `b` and `c` are (batch, length, groups, states),
-    each group serving width / groups neighbouring channels, or (batch, length, states) for one.
+    each group serving width / groups neighbouring channels, or (batch, length, states) for one;
+    without `c`, `b` holds both, (batch, length, 2 * groups, states), as one projection makes them.
     `d` (width,) and the gate `z` (as `x`) may be left out. `state` (batch, width, states) is h
     before the first position (zeros without it). With `softplus`, `dt` is taken through
     log(1 + e^dt) first. Returns `(y, final state)`. With `lengths` (batch,), a padded batch: y is 0
     from lengths[b] on, nothing is read there, and the final state is that at lengths[b]."""
     if lengths is not None:
         lengths = _as_index(lengths)
-    if b.ndim == 3 and c.ndim == 3:
+    if c is not None and b.ndim == 3 and c.ndim == 3:
         b, c = (v.reshape(v.shape[0], v.shape[1], 1, v.shape[2]) for v in (b, c))
-    operands, flags = _present((x, dt, a, b, c), (d, z, state, lengths), (_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS))
-    return _with_results("selective_scan", operands, {"flags": flags | (_SCAN_SOFTPLUS if softplus else 0)}, 2)
+    maps, joined = ((b,), _SCAN_JOINED) if c is None else ((b, c), 0)
+    operands, flags = _present((x, dt, a, *maps), (d, z, state, lengths), (_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS))
+    return _with_results("selective_scan", operands, {"flags": flags | joined | (_SCAN_SOFTPLUS if softplus else 0)}, 2)
 
 
 def rotary_norm(x, gain=None, positions=None, sections=None, rotary_dims=None, base=10000.0, eps=1e-6):
@@ -93,8 +95,9 @@ def rotary_norm(x, gain=None, positions=None, sections=None, rotary_dims=None, b
     queries, keys and values of a fused projection are sections (heads, heads) of 3 * heads.
     Without `gain` heads are only rotated. The first `rotary_dims` values of a head (all of them by
     default, 0 for none) are turned in pairs (i, i + rotary_dims / 2) by the angle
-    position * base^(-2 i / rotary_dims), formed in 64 bits. `positions` is int32, (length,) or
-    (batch, length); 0, 1, ... without it."""
+    position * base^(-2 i / rotary_dims), formed in 64 bits. `positions` is int32: (length,), (batch,
+    length), or (batch, 1) for the first of each sequence, the others following it; 0, 1, ... without
+    it."""
     if x.ndim != 4:
         raise error("SHAPE_MISMATCH", {"input_shapes": [x.shape]}, "x_must_be_batch_length_heads_head")
     if gain is not None and gain.ndim == 1:

@@ -178,10 +178,10 @@ SCAN_CASES = [(1, 1, 1, 1, 1, ""), (2, 1, 8, 4, 1, "dzsp"), (1, 2, 64, 16, 1, "d
               (2, 17, 63, 8, 1, "zlp"), (1, 33, 6, 5, 3, "dsp"), (3, 40, 200, 8, 2, "dslp"), (1, 48, 130, 13, 2, "dzp"), (2, 31, 40, 24, 1, "dzslp"),
               (1, 20, 33, 33, 1, "dzs"), (2, 18, 36, 64, 4, "dzslp"), (1, 100, 16, 16, 1, "dzsp"), (2, 64, 4, 17, 2, "zp"), (1, 70, 132, 16, 1, "dzp"),
               (1, 300, 5, 16, 1, "dzsp"), (2, 523, 8, 4, 1, "dzslp")]
-# batch, length, sections, passing heads, head, rotary dims, flags: g gain, p own positions, t shared ones
+# batch, length, sections, passing heads, head, rotary dims, flags: g gain, p own positions, t shared ones, f first ones
 ROTARY_CASES = [(1, 1, (1,), 0, 2, 2, "g"), (2, 1, (4, 2), 2, 64, 64, "gp"), (1, 5, (3,), 1, 8, 8, ""), (2, 9, (6, 2), 2, 44, 22, "gp"),
                 (1, 33, (1, 1), 0, 16, 0, "g"), (2, 7, (2, 3), 0, 128, 128, "gt"), (1, 3, (5,), 0, 256, 256, "gp"), (1, 4, (2,), 1, 250, 250, "g"),
-                (3, 40, (8, 8), 8, 32, 32, "gp"), (1, 6, (1, 2, 3, 1), 0, 10, 6, "gp"), (2, 65, (7,), 0, 24, 8, "p")]
+                (3, 40, (8, 8), 8, 32, 32, "gp"), (1, 6, (1, 2, 3, 1), 0, 10, 6, "gp"), (2, 65, (7,), 0, 24, 8, "p"), (3, 17, (2, 1), 1, 32, 16, "gf")]
 
 
 def lengths_of(batch, length):
@@ -216,7 +216,9 @@ def rotary_inputs(case, dtype, seed=0):
     heads = sum(sections) + passing
     f = lambda *s: r.standard_normal(s).astype(dtype)  # noqa: E731
     pos = None
-    if "p" in flags:
+    if "f" in flags:
+        pos = r.integers(-5, 2000000, (b, 1)).astype(np.int32)
+    elif "p" in flags:
         pos = (r.integers(-5, 2000000, (b, 1)) + np.arange(t)).astype(np.int32)
     elif "t" in flags:
         pos = (700 + 3 * np.arange(t)).astype(np.int32)
@@ -263,7 +265,7 @@ def check_conv(case, dtype, device):
         agree(g, want["d" + name], size["d" + name], k, dtype, "d" + name)
 
 
-def check_scan(case, dtype, device, with_last=True):
+def check_scan(case, dtype, device, with_last=True, joined=False):
     v, lengths, soft = scan_inputs(case, dtype)
     dlast = v["dlast"] if with_last else None
     args = (v["x"], v["dt"], v["a"], v["b"], v["c"], v["d"], v["z"], v["state"], lengths, soft, v["dy"], dlast)
@@ -273,8 +275,12 @@ def check_scan(case, dtype, device, with_last=True):
         fill_outside(v, lengths, ["x", "dt", "b", "c", "z"])
     dy, dl = rg.tensor(v["dy"]), rg.tensor(v["dlast"])
 
+    if joined:
+        v["b"], v["c"] = np.concatenate([v["b"], v["c"]], 2), None
+        want["db"], size["db"] = (np.concatenate([w["db"], w["dc"]], 2) for w in (want, size))
+
     def fn(g):
-        y, last = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g.get("d"), g.get("z"), g.get("state"), lengths, soft)
+        y, last = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g.get("c"), g.get("d"), g.get("z"), g.get("state"), lengths, soft)
         return (y * dy).sum() + ((last * dl).sum() if with_last else 0.0), (y, last)
 
     (y, last), grads = _differentiated(fn, {n: v[n] for n in ("x", "dt", "a", "b", "c", "d", "z", "state")}, device)
@@ -287,7 +293,7 @@ def check_scan(case, dtype, device, with_last=True):
 def check_rotary(case, dtype, device):
     b, t, sections, passing, hd, turn, flags = case
     v, pos = rotary_inputs(case, dtype)
-    at = np.arange(t) if pos is None else pos
+    at = np.arange(t) if pos is None else pos + np.arange(t) if pos.shape == (b, 1) else pos
     args = (v["x"], v["gain"], at, sections, turn, 10000.0, 1e-6, v["dy"])
     want, size = rotary(*args), rotary(*args, mag=True)
     k = rotary_roundings(v["x"])

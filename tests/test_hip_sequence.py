@@ -31,6 +31,33 @@ def test_scan_whose_last_state_nobody_reads(case):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", [ref.SCAN_CASES[i] for i in (1, 3, 7, 11, 12, 16)], ids=str)
+def test_scan_of_maps_in_one_operand(case, dtype):
+    ref.check_scan(case, dtype, "hip", joined=True)
+
+
+FEW = [(1, 1, 1, 1, 1, ""), (3, 1, 70, 16, 1, "dzsp"), (2, 3, 130, 16, 2, "dzsp"), (5, 4, 33, 13, 1, "zslp"), (2, 2, 20, 64, 4, "dslp"), (2, 1, 9, 32, 1, "s"),
+       (5, 4, 40, 8, 2, "dzslp")]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", FEW, ids=str)
+def test_single_tokens_and_a_few(case, dtype):
+    """Without a gradient, up to four positions run on a kernel of their own."""
+    v, lengths, soft = ref.scan_inputs(case, dtype)
+    args = (v["x"], v["dt"], v["a"], v["b"], v["c"], v["d"], v["z"], v["state"], lengths, soft, v["dy"], None)
+    want, size, k = ref.scan(*args), ref.scan(*args, mag=True), ref.scan_roundings(v["x"], v["dt"], v["a"], soft)
+    if lengths is not None:
+        ref.fill_outside(v, lengths, ["x", "dt", "b", "c", "z"])
+    given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "d", "z", "state") if v[n] is not None}
+    program = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g.get("d"), g.get("z"), g.get("state"), lengths, soft), (given,),
+                         validate="none")
+    y, last = program(given)
+    ref.agree(y.numpy(), want["y"], size["y"], k, dtype, "y")
+    ref.agree(last.numpy(), want["last"], size["last"], k, dtype, "last")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
 @pytest.mark.parametrize("case", ref.ROTARY_CASES, ids=str)
 def test_rotary(case, dtype):
     ref.check_rotary(case, dtype, "hip")

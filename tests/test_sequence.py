@@ -27,6 +27,11 @@ def test_scan(case, dtype):
     ref.check_scan(case, dtype, "cpu")
 
 
+@pytest.mark.parametrize("case", [ref.SCAN_CASES[i] for i in (1, 3, 7, 11)], ids=str)
+def test_scan_of_maps_in_one_operand(case):
+    ref.check_scan(case, "float32", "cpu", joined=True)
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float64"])
 @pytest.mark.parametrize("case", ref.ROTARY_CASES, ids=str)
 def test_rotary(case, dtype):
@@ -119,6 +124,9 @@ def _scan(x=(2, 3, 4), dt=(2, 3, 4), a=(4, 5), b=(2, 3, 1, 5), c=(2, 3, 1, 5), *
     (lambda: _scan(a=(4, 65), b=(2, 3, 1, 65), c=(2, 3, 1, 65)), "SHAPE_MISMATCH", "a_must_be_width_by_at_most_64_states"),
     (lambda: _scan(b=(2, 3, 3, 5), c=(2, 3, 3, 5)), "SHAPE_MISMATCH", "b_must_be_batch_length_groups_states_with_groups_dividing_the_width"),
     (lambda: _scan(c=(2, 3, 2, 5)), "SHAPE_MISMATCH", "c_shape_differs_from_b"),
+    (lambda: rg.selective_scan(_t(2, 3, 4), _t(2, 3, 4), _t(4, 5), _t(2, 3, 3, 5)), "SHAPE_MISMATCH",
+     "b_must_be_batch_length_groups_states_with_groups_dividing_the_width"),
+    (lambda: rg.rotary_norm(_t(2, 3, 4, 6), positions=[[0], [1], [2]]), "SHAPE_MISMATCH", "positions_must_be_length_or_batch_length"),
     (lambda: _scan(d=_t(5)), "SHAPE_MISMATCH", "d_must_be_width"),
     (lambda: _scan(z=_t(2, 3, 5)), "SHAPE_MISMATCH", "z_shape_differs_from_x"),
     (lambda: _scan(state=_t(2, 5, 4)), "SHAPE_MISMATCH", "state_must_be_batch_width_states"),
