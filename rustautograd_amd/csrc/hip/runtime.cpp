@@ -577,6 +577,9 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     prog.fold_bytes += ((uint64_t)rows * k * esize(dtype) + 255) / 256 * 256;
     return (int64_t)off;
   };
+  auto check_blocks = [](uint64_t blocks) {
+    if (blocks >= rgk::SEQUENCE_BLOCKS) throw std::runtime_error("a sequence operator of " + std::to_string(blocks) + " blocks exceeds the launch limit");
+  };
   auto place = [pp](void* ws, int64_t off) { return off < 0 ? nullptr : (void*)((char*)ws + pp->fold_base() + off); };
   if (conv) {
     rgk::ConvArgs base{};
@@ -586,6 +589,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     base.taps = (uint32_t)q.taps;
     base.silu = (i.sequence.flags & RG_CONV_SILU) != 0;
     const bool grad = i.op == RG_OP_CAUSAL_CONV_GRAD;
+    check_blocks(rgk::conv_blocks(dtype, base));
     const uint32_t rows = rgk::conv_grad_rows(dtype, base);
     const int64_t dw = grad ? partial(1, rows, (uint64_t)q.taps * q.width) : -1, db = grad ? partial(2, rows, (uint64_t)q.width) : -1;
     return [=](hipStream_t s, void* const* sl, void* ws) {
@@ -667,6 +671,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
   base.map_stride = (uint32_t)(joined ? 2 * q.groups : q.groups);
   base.softplus = (i.sequence.flags & RG_SCAN_SOFTPLUS) != 0;
   const bool grad = i.op == RG_OP_SELECTIVE_SCAN_GRAD;
+  check_blocks(rgk::scan_blocks(dtype, base));
   const uint32_t tiles = rgk::scan_group_tiles(dtype, base), rows = rgk::scan_rows(dtype, base);
   prog.workspace_bytes = std::max(prog.workspace_bytes, rgk::scan_workspace(dtype, base));
   const uint64_t maps = (uint64_t)q.batch * q.length * base.map_stride * q.states;

@@ -11,6 +11,9 @@
 
 namespace rgk {
 
+// A launch's threads have to stay below 2^32: `*_blocks` of 256 below this.
+constexpr uint64_t SEQUENCE_BLOCKS = 1ull << 24;
+
 struct ConvArgs {
   uint32_t batch, length, width, taps;
   bool silu;
@@ -20,6 +23,7 @@ struct ConvArgs {
   const void *dy, *carry;       // backward
   void *dx, *dstate, *dw_rows, *db_rows;
 };
+uint64_t conv_blocks(int dtype, const ConvArgs& a);
 uint32_t conv_grad_rows(int dtype, const ConvArgs& a);
 void causal_conv(hipStream_t s, int dtype, const ConvArgs& a);
 void causal_conv_grad(hipStream_t s, int dtype, const ConvArgs& a);
@@ -42,6 +46,7 @@ struct ScanArgs {
   void *ends, *totals;
 };
 uint64_t scan_workspace(int dtype, const ScanArgs& a);
+uint64_t scan_blocks(int dtype, const ScanArgs& a);
 uint32_t scan_rows(int dtype, const ScanArgs& a);
 uint32_t scan_group_tiles(int dtype, const ScanArgs& a);
 void selective_scan(hipStream_t s, int dtype, const ScanArgs& a);

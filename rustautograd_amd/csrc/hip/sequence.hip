@@ -2,6 +2,7 @@
 #include "sequence.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace rgk {
 
@@ -294,6 +295,10 @@ void conv(hipStream_t s, int dtype, const ConvArgs& a) {
 
 }  // namespace
 
+uint64_t conv_blocks(int dtype, const ConvArgs& a) {
+  const ConvCut cut = conv_cut(dtype, a);
+  return (uint64_t)a.batch * conv_runs(a, cut.r) * ((a.width + 64 * cut.v - 1) / (64 * cut.v));
+}
 uint32_t conv_grad_rows(int dtype, const ConvArgs& a) { return a.batch * conv_runs(a, conv_cut(dtype, a).r); }
 
 void causal_conv(hipStream_t s, int dtype, const ConvArgs& a) {
@@ -603,6 +608,8 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
       total[j] = ((const T*)a.totals)[r];
       end[j] = ((const T*)a.ends)[r * a.states + k];
     }
+    // Backward the compiler would use each load as it comes (256 chunks 44 us, 28 so; forward 19, 27).
+    if (BACK) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (uint32_t j = 0; j < FLIGHT; j++) {
       if (c + j >= chunks) break;
@@ -899,10 +906,11 @@ void scan_shape(uint32_t states, F f) {
 }
 
 // Tiles of a group's channels, and the chunks a sequence is cut into: as many as bring the launch to
-// SCAN_BLOCKS blocks, two a CU, but no more than SCAN_CHUNKS. More and shorter chunks cost more
-// joining than they save (2 x 2048 x 512, 16 states, forward and backward: 32 chunks 112 us, 64 chunks
-// 123), fewer leave CUs idle (3 x 777 x 200, 8 states: 25 chunks 46 us, 13 chunks 62).
-constexpr uint32_t SCAN_BLOCKS = 512, SCAN_CHUNKS = 64;
+// SCAN_BLOCKS blocks, two a CU (3 x 777 x 200, 8 states: 25 chunks 46 us forward and backward, 13
+// chunks 62). Joining takes about 0.2 us a chunk and a tile of positions 6 us, both ways, so that few
+// channels are cut into no more than 4 sqrt(tiles) chunks (2 x 2048 x 512, 16 states: 32 chunks 112 us,
+// 64 chunks 123).
+constexpr uint32_t SCAN_BLOCKS = 512;
 
 struct ScanCut {
   uint32_t tiles = 1, chunk_tiles = 1, chunks = 1;
@@ -916,7 +924,7 @@ ScanCut scan_cut(const ScanArgs& a) {
   });
   const uint32_t marks = (a.length + TILE - 1) / TILE;
   const uint64_t blocks = (uint64_t)a.batch * a.groups * cut.tiles;
-  const uint32_t wanted = (uint32_t)std::min<uint64_t>((SCAN_BLOCKS + blocks - 1) / blocks, SCAN_CHUNKS);
+  const uint32_t wanted = (uint32_t)std::min<uint64_t>((SCAN_BLOCKS + blocks - 1) / blocks, (uint64_t)std::ceil(4.0 * std::sqrt((double)marks)));
   cut.chunk_tiles = (marks + wanted - 1) / wanted;
   cut.chunks = (marks + cut.chunk_tiles - 1) / cut.chunk_tiles;
   return cut;
@@ -949,6 +957,10 @@ void launch_scan(hipStream_t s, ScanArgs a) {
 
 }  // namespace
 
+uint64_t scan_blocks(int dtype, const ScanArgs& a) {
+  const ScanCut cut = scan_cut_of(dtype, a);
+  return (uint64_t)a.batch * a.groups * cut.tiles * cut.chunks;
+}
 uint32_t scan_rows(int dtype, const ScanArgs& a) { return a.batch * scan_cut_of(dtype, a).chunks; }
 uint32_t scan_group_tiles(int dtype, const ScanArgs& a) { return scan_cut_of(dtype, a).tiles; }
 uint64_t scan_workspace(int dtype, const ScanArgs& a) {

@@ -13,6 +13,7 @@ from . import random
 from .ops import (abs, arange, argmax, argsort, broadcast_to, concatenate, cumsum, equal, exp, eye, log, maximum, ones,
                   stop_gradient, swapaxes, take, take_along_axis, tanh, top_k, where, zeros)
 from .sequence import causal_conv, rotary_norm, selective_scan
+from .tensor import Value, tensor
 
 _GELU_C = math.sqrt(2.0 / math.pi)
 _MASKED = -1e9  # the score of a position a mask hides, and the logit of a filtered token
@@ -350,6 +351,9 @@ class SelectiveSSM(Layer):
         return self.extend(params, x)[0]
 
     def extend(self, params, x, state=None, lengths=None):
+        """`(y, state)` for the positions `x` of sequences in `state` (not yet begun without one)."""
+        if lengths is not None:
+            lengths = lengths if isinstance(lengths, Value) else tensor(lengths, "int32")
         b, t, _ = x.shape
         conv, scan, pos = (None, None, None) if state is None else (state["conv"], state["scan"], state["pos"])
         u, conv = causal_conv(self.inward(params["in"], x), params["conv"]["w"], params["conv"]["b"], conv, lengths, "silu")
@@ -360,7 +364,8 @@ class SelectiveSSM(Layer):
                            (self.groups, self.groups), None if self.rotary else 0, self.base)
         y, scan = selective_scan(u, dt, -exp(params["a_log"]), maps, None, params["d"], self.gate(params["gate"], x), scan, lengths,
                                  softplus=True)
-        read = t if lengths is None else lengths
+        # As many positions as the operators read: lengths within the batch's own.
+        read = t if lengths is None else where(lengths > t, t, where(lengths > 0, lengths, 0))
         pos = zeros((b,), "int32") + read if pos is None else pos + read
         return self.out(params["out"], y), {"conv": conv, "scan": scan, "pos": pos}
 
