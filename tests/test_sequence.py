@@ -182,6 +182,24 @@ def test_profile_prices_the_operators():
     assert "selective_scan" in str(c.profile(*args, repeats=1))
 
 
+@pytest.mark.parametrize("optimize", ["search", "search-linear", "standard", "none"])
+@pytest.mark.parametrize("device", ["cpu", "cpu_devplan"])
+def test_thorough_validation_and_every_optimizer(device, optimize):
+    """Differences on the float64 shadow graph, the optimizer's check, and plans with the operators in
+    the graph that the matrix search rewrites."""
+    layer, params = _ssm()
+    attn = nn.MultiHeadAttention(12, 2, qk_norm=True, rotary=100.0)
+    weights = attn.init(random.key(1))
+    x = rg.tensor(np.random.default_rng(0).standard_normal((2, 5, 12)).astype(F))
+    mask = rg.tril(5)
+
+    def step(p, v):
+        return rg.value_and_grad(lambda q: (layer(q["ssm"], v + attn(q["attn"], v, mask)) ** 2.0).mean())(p)
+
+    c = rg.compile(step, ({"ssm": params, "attn": weights}, x), validate="thorough", device=device, optimize=optimize)
+    assert c.report["status"] == "ok", c.report
+
+
 def _ssm(dtype="float32", **more):
     layer = nn.SelectiveSSM(12, states=6, taps=3, dt_rank=2, rotary=True, groups=2, dtype=dtype, **more)
     return layer, layer.init(random.key(3))
