@@ -23,7 +23,7 @@ __device__ __forceinline__ float exp_(float v) {
 __device__ __forceinline__ double exp_(double v) { return exp(v); }
 __device__ __forceinline__ float sqrt_(float v) { return sqrtf(v); }
 __device__ __forceinline__ double sqrt_(double v) { return sqrt(v); }
-// a / b for a positive, finite, normal b: the hardware's reciprocal and one step of Newton's method,
+// a / b for a finite a and a positive, finite, normal b: the hardware's reciprocal and one step of Newton's method,
 // within a unit in the last place or two (the full division, for every b, takes three times as long).
 __device__ __forceinline__ float over(float a, float b) {
   const float r = __builtin_amdgcn_rcpf(b), q = a * r;
@@ -36,7 +36,7 @@ __device__ __forceinline__ double logistic_base(double v) { return 1.0 + exp_(-v
 template <class T>
 __device__ __forceinline__ T sigmoid(T v) { return over(T(1), logistic_base(v)); }
 template <class T>
-__device__ __forceinline__ T silu(T v) { return over(v, logistic_base(v)); }
+__device__ __forceinline__ T silu(T v) { return v * sigmoid(v); }
 // silu'(v) from s = sigmoid(v).
 template <class T>
 __device__ __forceinline__ T silu_slope(T v, T s) { return s * fma_(v, T(1) - s, T(1)); }

@@ -88,6 +88,25 @@ def test_infinite_rates_and_values_stay_where_they_are():
     ref.agree(y[0, :, 1], want.astype(np.float64), size.astype(np.float64), 24, "float32", "forgetting channel")
 
 
+def test_activations_at_their_ends():
+    """SiLU and softplus far out: 0 and the value itself, infinities as the limits have them, NaN as NaN."""
+    far = np.array([-np.inf, -1e30, -200.0, -90.0, 0.0, 90.0, 1e30, np.inf, np.nan], F)
+    x = rg.tensor(far.reshape(1, 9, 1))
+    unit = rg.tensor(np.array([[0.0], [1.0]], F))
+    y = rg.compile(lambda v: rg.causal_conv(v, unit, activation="silu")[0], (x,), validate="none")(x).numpy().ravel()
+    # A product with the tap of 0 makes the infinite neighbours NaN; the finite positions stay.
+    assert np.abs(y[2:4]).max() <= 200.0 * 1e-37 and y[4] == 0.0 and y[5] == 90.0 and y[6] == F(1e30) and np.isnan(y[8])
+    one = rg.tensor(np.ones((1, 9, 1), F))
+    dt = rg.tensor(np.array([-np.inf, -1e30, -200.0, -30.0, 0.0, 30.0, 1e30, 3.0, -5.0], F).reshape(1, 9, 1))
+    run = rg.compile(lambda d: rg.selective_scan(one, d, rg.tensor(np.full((1, 1), -np.inf, F)), rg.ones((1, 9, 1)), rg.ones((1, 9, 1)), softplus=True)[0], (dt,),
+                     validate="none")
+    # With nothing kept, y is the step itself: log(1 + e^v), four roundings.
+    want = np.logaddexp(0.0, dt.numpy().ravel().astype(np.float64))
+    got = run(dt).numpy().ravel()
+    assert np.abs(got[:3]).max() <= 1e-40
+    ref.agree(got[3:], want[3:], want[3:], 8, "float32", "softplus")
+
+
 def _steps(program, state, data, n):
     """The state after n calls of `program`, one by one, and their scalars."""
     seen = []
