@@ -552,17 +552,24 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
     dt = mv.template load_from<T>(a.dt, at, in);
     u = mv.template load_from<T>(BACK ? a.dy : a.x, at, in);
     if (BACK && a.gate) z = mv.template load_from<T>(a.gate, at, in);
-    if (a.softplus && in)
-#pragma unroll
-      for (int j = 0; j < S::EPT; j++) dt.v[j] = softplus(dt.v[j]);
     map.read(a, p, BACK ? a.c : a.b, m);
   };
   read(0);
   for (uint32_t i = 0; i < count; i++) {
+    const bool in = mv.inside(p, BACK ? p.last - 1 - i : p.first + i);
+    if (a.softplus)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) {
+        const T soft = softplus(dt.v[j]);
+        dt.v[j] = in ? soft : T(0);
+      }
+    if (BACK && a.gate)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) u.v[j] *= silu(z.v[j]);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       sdt[mv.col + j][mv.row] = dt.v[j];
-      su[mv.col + j][mv.row] = BACK && a.gate ? u.v[j] * silu(z.v[j]) : u.v[j];
+      su[mv.col + j][mv.row] = u.v[j];
     }
     map.put(&smap[0][0]);
     __syncthreads();
@@ -654,10 +661,16 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   read(p.first);
   for (uint32_t m = p.first; m < p.last; m++) {
     const bool in = mv.inside(p, m);
+    if (a.softplus)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) {
+        const T soft = softplus(dt.v[j]);
+        dt.v[j] = in ? soft : T(0);
+      }
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       sx[mv.col + j][mv.row] = x.v[j];
-      sdt[mv.col + j][mv.row] = a.softplus && in ? softplus(dt.v[j]) : dt.v[j];
+      sdt[mv.col + j][mv.row] = dt.v[j];
     }
     bs.put(&sb[0][0]);
     cs.put(&sc[0][0]);
@@ -683,7 +696,10 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
     __syncthreads();
     Vec<T, S::EPT> y;
 #pragma unroll
-    for (int j = 0; j < S::EPT; j++) y.v[j] = !in ? T(0) : a.gate ? sx[mv.col + j][mv.row] * silu(gate.v[j]) : sx[mv.col + j][mv.row];
+    for (int j = 0; j < S::EPT; j++) y.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
+    if (a.gate)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) y.v[j] *= silu(gate.v[j]);
     mv.store_to(a.y, mv.at(a, p, m), y, m * TILE + mv.row < a.length);
     __syncthreads();
   }
@@ -736,7 +752,7 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
 // and the decayed states p = e h[t - 1] are formed again, then with G = dL/dh[t] carried back:
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
 // The sums over channels that db and dc take leave one partial row per tile of channels.
-template <class T, int NL, int NS>
+template <class T, int NL, int NS, bool GATE>
 __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_grad(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
   constexpr int WAVES = TPB / 64, COPIES = 16 / NL, M = 2 * NS;
@@ -770,7 +786,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     x = mv.template load_from<T>(a.x, at, in);
     raw = mv.template load_from<T>(a.dt, at, in);
     g = mv.template load_from<T>(a.dy, at, in);
-    if (a.gate) z = mv.template load_from<T>(a.gate, at, in);
+    if (GATE) z = mv.template load_from<T>(a.gate, at, in);
     bs.read(a, p, a.b, m);
     cs.read(a, p, a.c, m);
     if (on) start = load_states<T, NS>(a.marks, ((uint64_t)p.b * p.marks + m) * a.width + d, q * NS, a.states, whole);
@@ -779,19 +795,29 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   for (uint32_t m = p.last; m-- > p.first;) {
     const bool in = mv.inside(p, m);
     Vec<T, S::EPT> slope, gate_g;  // d dt / d raw; dy silu'(z)
+    Vec<T, S::EPT> step = raw, gy = g;
+    if (a.softplus) {
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) {
+        const T soft = softplus(raw.v[j], &slope.v[j]);
+        step.v[j] = in ? soft : T(0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) slope.v[j] = T(1);
+    }
+    if (GATE)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) {
+        const T s = sigmoid(z.v[j]);
+        gate_g.v[j] = g.v[j] * silu_slope(z.v[j], s);
+        gy.v[j] = g.v[j] * (z.v[j] * s);
+      }
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
-      T step = raw.v[j], gy = g.v[j];
-      slope.v[j] = T(1);
-      if (a.softplus && in) step = softplus(raw.v[j], &slope.v[j]);
-      if (a.gate) {
-        const T s = sigmoid(z.v[j]);
-        gate_g.v[j] = gy * silu_slope(z.v[j], s);
-        gy *= z.v[j] * s;
-      }
       sx[mv.col + j][mv.row] = x.v[j];
-      sdt[mv.col + j][mv.row] = step;
-      sg[mv.col + j][mv.row] = gy;
+      sdt[mv.col + j][mv.row] = step.v[j];
+      sg[mv.col + j][mv.row] = gy.v[j];
     }
     bs.put(&sb[0][0]);
     cs.put(&sc[0][0]);
@@ -813,7 +839,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
         h[j] = fma_(drive, sb[i][q * NS + j], kept[i][j]);
         y = fma_(sc[i][q * NS + j], h[j], y);
       }
-      if (a.gate) {
+      if (GATE) {
         y = channel_sum<NL>(y);
         if (i % NL == (int)q) mine = y;
         if (i % NL == NL - 1) sy[c][i - (NL - 1) + q] = mine;
@@ -858,13 +884,13 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     for (int j = 0; j < S::EPT; j++) {
       dx.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
       ddt.v[j] = in ? sdt[mv.col + j][mv.row] * slope.v[j] : T(0);
-      dz.v[j] = in && a.gate ? sy[mv.col + j][mv.row] * gate_g.v[j] : T(0);
+      dz.v[j] = in && GATE ? sy[mv.col + j][mv.row] * gate_g.v[j] : T(0);
     }
     const bool within = m * TILE + mv.row < a.length;
     const uint64_t at = mv.at(a, p, m);
     mv.store_to(a.dx, at, dx, within);
     mv.store_to(a.ddt, at, ddt, within);
-    mv.store_to(a.dz, at, dz, within);
+    if (GATE) mv.store_to(a.dz, at, dz, within);
     for (uint32_t i = threadIdx.x; i < TILE * 2 * S::NP; i += TPB) {
       // Value w NS + j of lane q is the gradient of b (w = 0) or c of state q NS + j.
       const uint32_t r = i / (2 * S::NP), w = i / S::NP % 2, k = i % S::NP, t = m * TILE + r;
@@ -950,8 +976,13 @@ void launch_scan(hipStream_t s, ScanArgs a) {
       hipLaunchKernelGGL((k_scan_ends<T, NL, NS, GRAD>), dim3(blocks * (cut.chunks - 1)), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
       hipLaunchKernelGGL((k_scan_join<T, GRAD>), dim3(joins), dim3(64), 0, s, a, cut.chunks);
     }
-    if constexpr (GRAD) hipLaunchKernelGGL((k_scan_grad<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
-    else hipLaunchKernelGGL((k_scan<T, NL, NS>), dim3(blocks * cut.chunks), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+    const dim3 grid(blocks * cut.chunks);
+    if constexpr (GRAD) {
+      if (a.gate) hipLaunchKernelGGL((k_scan_grad<T, NL, NS, true>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+      else hipLaunchKernelGGL((k_scan_grad<T, NL, NS, false>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+    } else {
+      hipLaunchKernelGGL((k_scan<T, NL, NS>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+    }
   });
 }
 
