@@ -465,6 +465,8 @@ inline void check_refs(const Plan& pl) {
           fail(at + " has a result of another size or dtype");
         for (const auto& o : in.outs) {
           if (o.first < 0 || (size_t)o.first >= q.results.size()) fail(at + " names a result it does not have");
+          for (const auto& other : in.outs)
+            if (&other != &o && other.first == o.first) fail(at + " names a result twice");
           fits(o.second, prod_of(q.results[(size_t)o.first]), (at + " result").c_str());
           if (pl.slots[(size_t)o.second].dtype != in.dtype) fail(at + " has a result of another dtype");
         }

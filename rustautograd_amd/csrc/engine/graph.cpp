@@ -704,6 +704,10 @@ void Graph::check_sequence(const Op& op, const std::vector<uint32_t>& inputs) co
 }
 
 uint32_t Graph::result(uint32_t node, size_t index) {
+  // A result has one reader, also where several gradients of the same node ask for it: a plan
+  // gives each reader a slot, and the operator writes each result once.
+  for (size_t i = node + 1; i < nodes.size(); i++)
+    if (nodes[i].op.kind == RG_OP_OUTPUT && nodes[i].inputs[0] == node && nodes[i].op.a == index) return (uint32_t)i;
   const Node& n = nodes[node];
   const rgplan::Sequence q = sequence(n.op, n.inputs);
   return output(node, index, Shape(q.results[index].begin(), q.results[index].end()), n.dtype);

@@ -629,6 +629,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     base.shared_positions = q.shared_positions;
     base.positions_from = q.positions_from;
     if ((uint64_t)q.batch * q.length >= (1ull << 31)) throw std::runtime_error("more than 2^31 positions in one rotation");
+    check_blocks((uint64_t)q.heads);  // a block takes one head or more
     if (base.turn > 0) {
       // Turns per position of each pair, its double and what that leaves out.
       std::vector<double> turns;

@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
   const bool on = c < p.chs;
   const bool whole = a.states % NS == 0;
   T rate[NS], h[NS], total = T(0);
-  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : p.ch0, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
     rate[j] = decay_rate(finite_rate(rates.v[j]));
@@ -596,7 +596,9 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
 
 // Chunks' ends into their starts, in place: the state carried from the sequence's start (backward:
 // the gradient from its end) to each chunk, a thread a state. Bound by the latency of its loads:
-// the operands of 32 chunks are in flight at a time.
+// the operands of 32 chunks are in flight at a time. Where states grow, the decay over a chunk may
+// overflow though its product with a small state does not: it is applied in two halves, and an empty
+// state stays empty.
 template <class T, bool BACK>
 __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
   const uint32_t i = blockIdx.x * 64 + threadIdx.x;
@@ -621,7 +623,8 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
     for (uint32_t j = 0; j < FLIGHT; j++) {
       if (c + j >= chunks) break;
       ((T*)a.ends)[row(c + j) * a.states + k] = h;
-      h = fma_(decay(total[j], rate), h, end[j]);
+      const T half = decay(T(0.5) * total[j], rate);
+      h = h == T(0) ? end[j] : fma_(half, half * h, end[j]);
     }
   }
 }
@@ -636,7 +639,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   const bool on = c < p.chs;
   const bool whole = a.states % NS == 0;
   T rate[NS], h[NS];
-  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : p.ch0, q * NS, a.states, whole);
   Vec<T, NS> from{};
   if (on && chunks > 1) from = load_states<T, NS>(a.ends, ((uint64_t)p.b * chunks + p.chunk) * a.width + d, q * NS, a.states, whole);
   else if (on && a.state) from = load_states<T, NS>(a.state, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
@@ -764,7 +767,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   const bool on = c < p.chs;
   const bool whole = a.states % NS == 0;
   T rate[NS], rate_e[NS], back[NS], da[NS], dd = T(0);
-  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : 0, q * NS, a.states, whole);
+  const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : p.ch0, q * NS, a.states, whole);
   Vec<T, NS> from{};
   if (on && chunks > 1) from = load_states<T, NS>(a.ends, ((uint64_t)p.b * chunks + p.chunk) * a.width + d, q * NS, a.states, whole);
   else if (on && a.carry) from = load_states<T, NS>(a.carry, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);

@@ -88,6 +88,73 @@ def test_infinite_rates_and_values_stay_where_they_are():
     ref.agree(y[0, :, 1], want.astype(np.float64), size.astype(np.float64), 24, "float32", "forgetting channel")
 
 
+def test_a_rate_that_is_nan_stays_in_its_channel_and_group():
+    """Channel 0's rate reaches its own results and the gradients of its group's maps, no others, also
+    where the last tile of channels is not full."""
+    v, _, _ = ref.scan_inputs((1, 40, 6, 4, 2, ""), "float32")
+    v["a"][0, 0] = np.nan
+    dy = rg.tensor(v["dy"])
+
+    def program(g):
+        return rg.grad(lambda g: (rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"])[0] * dy).sum())(g)
+
+    given = {k: rg.tensor(v[k]) for k in ("x", "dt", "a", "b", "c")}
+    grads = {k: g.numpy() for k, g in rg.compile(program, (given,), validate="none")(given).items()}
+    assert np.isfinite(grads["b"][:, :, 1]).all() and np.isfinite(grads["c"][:, :, 1]).all()
+    for k in ("x", "dt"):
+        assert np.isfinite(grads[k][..., 1:]).all() and not np.isfinite(grads[k][..., 0]).any()
+    assert np.isfinite(grads["a"][1:]).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+def test_states_that_grow_past_what_one_factor_holds(dtype):
+    """Growing states over many chunks. Channel 0 starts empty and its inputs begin late: it is 0 until
+    then. Channel 1 holds 1e-30 and grows by e^96 within a stretch of 32 positions (e^1200 from
+    1e-300 in 64 bits): more than one factor of its type holds, the state itself does not overflow."""
+    v, _, _ = ref.scan_inputs((1, 523, 2, 4, 1, "s"), dtype)
+    grow = 3.0 if dtype == "float32" else 37.5
+    v["a"][:] = 1.0
+    v["dt"][0, :, 0], v["x"][0, :, 0] = 1.0, 0.0
+    v["x"][0, 510:, 0] = 1.0
+    v["dt"][0, :, 1], v["dt"][0, 32:64, 1], v["x"][0, :, 1] = 0.0, grow, 0.0
+    v["state"][0, 0], v["state"][0, 1] = 0.0, 1e-30 if dtype == "float32" else 1e-300
+    v["dy"][:], v["dlast"][:] = 0.0, 0.0
+    v["dy"][0, 505:, 1] = 1e-30 if dtype == "float32" else 1e-300
+    args = (v["x"], v["dt"], v["a"], v["b"], v["c"], None, None, v["state"], None, False, v["dy"], None)
+    want, size = ref.scan(*args), ref.scan(*args, mag=True)
+    k = ref.scan_roundings(v["x"], v["dt"], v["a"], False)
+    dy = rg.tensor(v["dy"])
+
+    def program(g):
+        def loss(g):
+            y, last = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], state=g["state"])
+            return (y * dy).sum(), (y, last)
+        (_, results), grads = rg.value_and_grad(loss, has_aux=True)(g)
+        return results, grads["state"]
+
+    given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "state")}
+    (y, last), dstate = rg.compile(program, (given,), validate="none")(given)
+    assert (y.numpy()[0, :510, 0] == 0.0).all() and (dstate.numpy()[0, 0] == 0.0).all()
+    ref.agree(y.numpy(), want["y"], size["y"], k, dtype, "y")
+    ref.agree(last.numpy(), want["last"], size["last"], k, dtype, "last")
+    ref.agree(dstate.numpy(), want["dstate"], size["dstate"], k, dtype, "dstate")
+
+
+@pytest.mark.parametrize("optimize", ["none", "standard"])
+def test_gradients_asked_for_one_by_one(optimize):
+    """A scan differentiated once for each argument: as differentiated for both at once."""
+    v, _, _ = ref.scan_inputs((2, 40, 4, 3, 1, ""), "float32")
+    x, dt, a, b, c, dy = (rg.tensor(v[k]) for k in ("x", "dt", "a", "b", "c", "dy"))
+
+    def loss(x, dt):
+        return (rg.selective_scan(x, dt, a, b, c)[0] * dy).sum()
+
+    apart = rg.compile(lambda x, dt: rg.value_and_grad(loss, argnums=(0, 1))(x, dt)[1], (x, dt), validate="none", optimize=optimize)(x, dt)
+    both = rg.compile(lambda t: rg.grad(lambda t: loss(*t))(t), ((x, dt),), validate="none", optimize=optimize)((x, dt))
+    for one, other in zip(apart, both):
+        assert np.array_equal(one.numpy(), other.numpy())
+
+
 def test_activations_at_their_ends():
     """SiLU and softplus far out: 0 and the value itself, infinities as the limits have them, NaN as NaN."""
     far = np.array([-np.inf, -1e30, -200.0, -90.0, 0.0, 90.0, 1e30, np.inf, np.nan], F)

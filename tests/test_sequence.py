@@ -150,6 +150,17 @@ def test_refusals(call, code, cause):
     assert cause in str(e.value.diagnostic), e.value.diagnostic
 
 
+@pytest.mark.parametrize("optimize", ["none", "standard"])
+def test_gradients_asked_for_one_by_one_share_the_kept_states(optimize):
+    """One scan differentiated once for each argument: each of its results is in the plan once."""
+    v, _, _ = ref.scan_inputs((2, 40, 4, 3, 1, ""), "float32")
+    x, dt, a, b, c = (rg.tensor(v[k]) for k in ("x", "dt", "a", "b", "c"))
+    p = rg.compile(lambda x, dt: rg.value_and_grad(lambda *s: rg.selective_scan(*s, a, b, c)[0].sum(), argnums=(0, 1))(x, dt), (x, dt),
+                   validate="none", optimize=optimize)
+    (scan,) = [s for s in p.plan_summary() if s.get("op") == "selective_scan"]
+    assert [k for k, _ in scan["outs"]] == [0, 2]
+
+
 # ---- plans, validation, layers -----------------------------------------------------------------------
 
 def test_a_result_nobody_reads_has_no_slot():
