@@ -89,11 +89,13 @@
  *                  one) then x; 1: the K - 1 rows of past that end the sequence
  *       _GRAD      in the same, dy (, d of result 1); out dx, dw, dbias, dstate
  *     SELECTIVE_SCAN in x, dt[B,T,D], a[D,N], b, c[B,T,G,N] (, d[D]) (, z[B,T,D]) (, state[B,D,N])
- *                  (, lengths[B]) (with RG_SCAN_JOINED one b[B,T,2 G,N], b's groups then c's, and
- *                  no c); h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t];
+ *                  (, lengths[B]) (, dt bias[D], added to dt first) (with RG_SCAN_JOINED one
+ *                  b[B,T,2 G,N], b's groups then c's, and no c; with RG_SCAN_LOG a holds log(-a));
+ *                  h[t] = exp(dt[t] a) h[t-1] + dt[t] x[t] b[t];
  *                  out 0: (c[t] . h[t] + d x[t]) silu(z[t]); 1: the last h; 2: marks, h before
  *                  positions 0, RG_SCAN_MARK, 2 RG_SCAN_MARK, ..., for the gradient alone
- *       _GRAD      in the same, marks, dy (, d of result 1); out dx, ddt, da, db, dc, dd, dz, dstate
+ *       _GRAD      in the same, marks, dy (, d of result 1); out dx, ddt, da, db, dc, dd, dz, dstate,
+ *                  d of the dt bias
  *     ROTARY_NORM  in x[B,T,H,hd], positions[T], [B,T] or [B,1] (the first of each sequence)
  *                  (, gain[S,hd]); out x with the heads of
  *                  section s divided by their root mean square and scaled by gain[s], and their
@@ -144,7 +146,8 @@ enum rg_op {
 enum rg_conv_flags { RG_CONV_BIAS = 1, RG_CONV_STATE = 2, RG_CONV_LENGTHS = 4, RG_CONV_SILU = 8, RG_CONV_CARRY = 16 };
 enum rg_scan_flags {
   RG_SCAN_SKIP = 1, RG_SCAN_GATE = 2, RG_SCAN_STATE = 4, RG_SCAN_LENGTHS = 8, RG_SCAN_SOFTPLUS = 16, RG_SCAN_CARRY = 32,
-  RG_SCAN_JOINED = 64 /* b holds b and c: [B,T,2 G,N], and c is no operand */
+  RG_SCAN_JOINED = 64, /* b holds b and c: [B,T,2 G,N], and c is no operand */
+  RG_SCAN_BIAS = 128, RG_SCAN_LOG = 256 /* a holds the rates' logarithms: the rates are -e^a */
 };
 enum rg_rotary_flags { RG_ROTARY_GAIN = 1 };
 /* Taps of a causal convolution, states of a selective scan, and the length of a head. */
@@ -205,7 +208,7 @@ inline bool is_multi_result(int32_t op) { return is_sequence(op) && op != RG_OP_
 struct Sequence {
   int64_t batch = 0, length = 0, width = 0, taps = 0, states = 0, groups = 0, heads = 0, head = 0, used = 0;
   int x = 0, w = -1, bias = -1, dt = -1, a = -1, b = -1, c = -1, skip = -1, gate = -1, state = -1, lengths = -1, marks = -1, dy = -1,
-      carry = -1, positions = -1, gain = -1;
+      carry = -1, positions = -1, gain = -1, dt_bias = -1;
   bool shared_positions = false; /* positions of [length], the same for every sequence */
   bool positions_from = false;   /* positions of [batch, 1], the first of each sequence */
   std::vector<std::vector<int64_t>> results;
@@ -245,6 +248,7 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
     q.gate = take(f & RG_SCAN_GATE);
     q.state = take(f & RG_SCAN_STATE);
     q.lengths = take(f & RG_SCAN_LENGTHS);
+    q.dt_bias = take(f & RG_SCAN_BIAS);
     q.marks = take(grad);
     q.dy = take(grad);
     q.carry = take(grad && (f & RG_SCAN_CARRY));
@@ -323,10 +327,11 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
     if (q.c >= 0) dims(q.c, b, "c_shape_differs_from_b");
     if (q.skip >= 0) dims(q.skip, {q.width}, "d_must_be_width");
     if (q.gate >= 0) dims(q.gate, x, "z_shape_differs_from_x");
+    if (q.dt_bias >= 0) dims(q.dt_bias, {q.width}, "dt_bias_must_be_width");
     if (q.state >= 0) dims(q.state, state, "state_must_be_batch_width_states");
     if (q.carry >= 0) dims(q.carry, state, "state_cotangent_shape");
     if (q.marks >= 0) dims(q.marks, marks, "marks_shape");
-    if (grad) q.results = {x, x, a, b, b, {q.width}, x, state};
+    if (grad) q.results = {x, x, a, b, b, {q.width}, x, state, {q.width}};
     else q.results = {x, state, marks};
   }
   return q;

@@ -84,13 +84,15 @@ template <class T>
 void selective_scan(const Operands<T>& o) {
   const auto& q = o.q;
   const T *x = o.arg(q.x), *raw = o.arg(q.dt), *a = o.arg(q.a), *bm = o.arg(q.b), *cm = o.arg(q.c), *skip = o.arg(q.skip), *z = o.arg(q.gate),
-          *state = o.arg(q.state), *dy = o.arg(q.dy), *carry = o.arg(q.carry);
+          *state = o.arg(q.state), *dy = o.arg(q.dy), *carry = o.arg(q.carry), *bias = o.arg(q.dt_bias);
   const int64_t D = q.width, N = q.states, L = q.length, G = q.groups, per = D / G;
   const bool joined = q.c < 0;  // c's groups follow b's in one operand
   const int64_t GM = joined ? 2 * G : G, cg = joined ? G * N : 0;
   if (joined) cm = bm;
-  const bool grad = dy != nullptr, soft = o.has(RG_SCAN_SOFTPLUS);
-  std::vector<double> da((size_t)(D * N), 0.0), dd((size_t)D, 0.0);
+  const bool grad = dy != nullptr, soft = o.has(RG_SCAN_SOFTPLUS), logs = o.has(RG_SCAN_LOG);
+  auto rate = [&](int64_t k) { return logs ? -std::exp((double)a[k]) : (double)a[k]; };
+  auto given = [&](int64_t at, int64_t d) { return (double)raw[at] + (bias ? (double)bias[d] : 0.0); };
+  std::vector<double> da((size_t)(D * N), 0.0), dd((size_t)D, 0.0), dbias((size_t)D, 0.0);
   std::vector<double> db, dc;
   if (grad) {
     db.assign((size_t)(q.batch * L * GM * N), 0.0);
@@ -111,9 +113,9 @@ void selective_scan(const Operands<T>& o) {
       std::vector<double> y((size_t)n, 0.0);
       for (int64_t t = 0; t < n; t++) {
         const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * GM + g) * N;
-        const double dt = soft ? softplus((double)raw[at]) : (double)raw[at], u = (double)x[at];
+        const double given_dt = given(at, d), dt = soft ? softplus(given_dt) : given_dt, u = (double)x[at];
         for (int64_t s = 0; s < N; s++) {
-          const double v = std::exp(dt * (double)a[d * N + s]) * h[(size_t)(t * N + s)] + dt * u * (double)bm[row + s];
+          const double v = std::exp(dt * rate(d * N + s)) * h[(size_t)(t * N + s)] + dt * u * (double)bm[row + s];
           h[(size_t)((t + 1) * N + s)] = v;
           y[(size_t)t] += (double)cm[row + cg + s] * v;
         }
@@ -130,7 +132,7 @@ void selective_scan(const Operands<T>& o) {
         for (int64_t s = 0; s < N; s++) G_[(size_t)s] = (double)carry[(b * D + d) * N + s];
       for (int64_t t = n; t-- > 0;) {
         const int64_t at = (b * L + t) * D + d, row = ((b * L + t) * GM + g) * N;
-        const double dt = soft ? softplus((double)raw[at]) : (double)raw[at], u = (double)x[at];
+        const double given_dt = given(at, d), dt = soft ? softplus(given_dt) : given_dt, u = (double)x[at];
         double gy = (double)dy[at];
         if (z) {
           const double v = (double)z[at], s = sigmoid(v);
@@ -139,17 +141,19 @@ void selective_scan(const Operands<T>& o) {
         }
         double sb = 0, sa = 0;
         for (int64_t s = 0; s < N; s++) {
-          const double e = std::exp(dt * (double)a[d * N + s]), p = e * h[(size_t)(t * N + s)];
+          const double e = std::exp(dt * rate(d * N + s)), p = e * h[(size_t)(t * N + s)];
           const double gr = G_[(size_t)s] + gy * (double)cm[row + cg + s];
           (joined ? db : dc)[(size_t)(row + cg + s)] += gy * h[(size_t)((t + 1) * N + s)];
           db[(size_t)(row + s)] += gr * dt * u;
           sb += gr * (double)bm[row + s];
-          sa += gr * p * (double)a[d * N + s];
-          da[(size_t)(d * N + s)] += gr * p * dt;
+          sa += gr * p * rate(d * N + s);
+          da[(size_t)(d * N + s)] += gr * p * dt * (logs ? rate(d * N + s) : 1.0);
           G_[(size_t)s] = gr * e;
         }
         if (o.out[0]) o.out[0][at] = (T)(dt * sb + (skip ? gy * (double)skip[d] : 0.0));
-        if (o.out[1]) o.out[1][at] = (T)((u * sb + sa) * (soft ? sigmoid((double)raw[at]) : 1.0));
+        const double ddt = (u * sb + sa) * (soft ? sigmoid(given_dt) : 1.0);
+        if (o.out[1]) o.out[1][at] = (T)ddt;
+        dbias[(size_t)d] += ddt;
         dd[(size_t)d] += gy * u;
       }
       if (o.out[7])
@@ -165,6 +169,7 @@ void selective_scan(const Operands<T>& o) {
     store(3, db);
     if (!joined) store(4, dc);
     store(5, dd);
+    store(8, dbias);
   }
 }
 

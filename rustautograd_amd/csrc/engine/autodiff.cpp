@@ -541,7 +541,7 @@ std::vector<std::pair<uint32_t, uint32_t>> vjp_sequence(Graph& g, size_t i, cons
   const uint32_t grads = g.add(o, ins);
   std::vector<std::pair<uint32_t, uint32_t>> out;
   const std::vector<int> operands = conv ? std::vector<int>{q.x, q.w, q.bias, q.state}
-                                         : std::vector<int>{q.x, q.dt, q.a, q.b, q.c, q.skip, q.gate, q.state};
+                                         : std::vector<int>{q.x, q.dt, q.a, q.b, q.c, q.skip, q.gate, q.state, q.dt_bias};
   for (size_t k = 0; k < operands.size(); k++)
     if (operands[k] >= 0 && rel[node.inputs[(size_t)operands[k]]]) out.push_back({node.inputs[(size_t)operands[k]], g.result(grads, k)});
   return out;

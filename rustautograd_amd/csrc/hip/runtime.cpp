@@ -671,6 +671,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
   const bool joined = q.c < 0;
   base.map_stride = (uint32_t)(joined ? 2 * q.groups : q.groups);
   base.softplus = (i.sequence.flags & RG_SCAN_SOFTPLUS) != 0;
+  base.logs = (i.sequence.flags & RG_SCAN_LOG) != 0;
   const bool grad = i.op == RG_OP_SELECTIVE_SCAN_GRAD;
   check_blocks(rgk::scan_blocks(dtype, base));
   const uint32_t tiles = rgk::scan_group_tiles(dtype, base), rows = rgk::scan_rows(dtype, base);
@@ -683,10 +684,12 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
   const int64_t db = grad && !direct ? partial(3, tiles, maps) : -1, dc = grad && !direct && !joined ? partial(4, tiles, maps) : -1;
   const int64_t da = grad ? partial(2, rows, (uint64_t)q.width * q.states) : -1;
   const int64_t dd = grad && q.skip >= 0 ? partial(5, rows, (uint64_t)q.width) : -1;
+  const int64_t dbias = grad && q.dt_bias >= 0 ? partial(8, rows, (uint64_t)q.width) : -1;
   return [=](hipStream_t s, void* const* sl, void* ws) {
     rgk::ScanArgs a = base;
     a.x = arg(sl, q.x);
     a.dt = arg(sl, q.dt);
+    a.dt_bias = arg(sl, q.dt_bias);
     a.a = arg(sl, q.a);
     a.b = arg(sl, q.b);
     a.c = joined ? (const void*)((const char*)a.b + after) : arg(sl, q.c);
@@ -711,6 +714,7 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     a.dc_rows = joined ? (a.db_rows ? (char*)a.db_rows + after : nullptr) : direct ? slot(sl, outs[4]) : place(ws, dc);
     a.da_rows = place(ws, da);
     a.dd_rows = place(ws, dd);
+    a.dt_bias_rows = place(ws, dbias);
     a.dz = slot(sl, outs[6]);
     a.dstate = slot(sl, outs[7]);
     rgk::selective_scan_grad(s, dtype, a);

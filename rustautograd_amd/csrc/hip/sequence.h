@@ -31,15 +31,15 @@ void causal_conv_grad(hipStream_t s, int dtype, const ConvArgs& a);
 struct ScanArgs {
   uint32_t batch, length, width, states, groups;
   uint32_t map_stride;          // rows of states from one position to the next, in b and in c
-  bool softplus;
-  const void *x, *dt, *a, *b, *c, *skip, *gate, *state;
+  bool softplus, logs;          // logs: `a` holds the rates' logarithms
+  const void *x, *dt, *dt_bias, *a, *b, *c, *skip, *gate, *state;
   const int32_t* lengths;
   void *y, *last, *marks;       // forward; `marks` is read by the backward
   const void *dy, *carry;       // backward
   void *dx, *ddt, *dz, *dstate;
   // Partial rows: of b and c one per tile of a group's channels, each [batch, length, map_stride,
-  // states]; of a ([width, states]) and the skip ([width]) scan_rows of them.
-  void *db_rows, *dc_rows, *da_rows, *dd_rows;
+  // states]; of a ([width, states]), the skip and the dt bias ([width]) scan_rows of them.
+  void *db_rows, *dc_rows, *da_rows, *dd_rows, *dt_bias_rows;
   void* workspace;              // scan_workspace bytes
   // Set by the launchers: tiles of positions a chunk, and the chunks' ends and sums of steps.
   uint32_t chunk_tiles;

@@ -427,6 +427,12 @@ __device__ __forceinline__ void hold(int position) {
 __device__ __forceinline__ float finite_rate(float a) { return a > 2e38f ? 2e38f : a < -2e38f ? -2e38f : a; }
 __device__ __forceinline__ double finite_rate(double a) { return a > 1e308 ? 1e308 : a < -1e308 ? -1e308 : a; }
 
+// The rate of a decay from the operand's value: itself, or minus its exponential.
+template <class T>
+__device__ __forceinline__ T rate_of(T v, bool logs) {
+  return finite_rate(logs ? -exp_(sizeof(T) == 4 && v > T(88) ? T(88) : v) : v);
+}
+
 template <int C>
 __device__ __forceinline__ float dpp(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), C, 0xf, 0xf, false));
@@ -538,7 +544,7 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
   const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : p.ch0, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    rate[j] = decay_rate(finite_rate(rates.v[j]));
+    rate[j] = decay_rate(rate_of(rates.v[j], a.logs));
     h[j] = T(0);
   }
   const ScanMover<S> mv(p, vec);
@@ -554,15 +560,19 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
     if (BACK && a.gate) z = mv.template load_from<T>(a.gate, at, in);
     map.read(a, p, BACK ? a.c : a.b, m);
   };
+  const Vec<T, S::EPT> bias = mv.template load_from<T>(a.dt_bias, p.ch0 + mv.col, a.dt_bias && mv.left > 0);
   read(0);
   for (uint32_t i = 0; i < count; i++) {
     const bool in = mv.inside(p, BACK ? p.last - 1 - i : p.first + i);
     if (a.softplus)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) {
-        const T soft = softplus(dt.v[j]);
+        const T soft = softplus(dt.v[j] + bias.v[j]);
         dt.v[j] = in ? soft : T(0);
       }
+    else
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
     if (BACK && a.gate)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) u.v[j] *= silu(z.v[j]);
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
   const uint32_t i = blockIdx.x * 64 + threadIdx.x;
   if (i >= a.batch * a.width * a.states) return;
   const uint32_t k = i % a.states, d = i / a.states % a.width, b = i / a.states / a.width;
-  const T rate = decay_rate(finite_rate(((const T*)a.a)[(uint64_t)d * a.states + k]));
+  const T rate = decay_rate(rate_of(((const T*)a.a)[(uint64_t)d * a.states + k], a.logs));
   const T* given = (const T*)(BACK ? a.carry : a.state);
   T h = given ? given[i] : T(0);
   constexpr uint32_t FLIGHT = 32;
@@ -645,7 +655,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   else if (on && a.state) from = load_states<T, NS>(a.state, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    rate[j] = decay_rate(finite_rate(rates.v[j]));
+    rate[j] = decay_rate(rate_of(rates.v[j], a.logs));
     h[j] = from.v[j];
   }
   const T skip = on && q == 0 && a.skip ? ((const T*)a.skip)[d] : T(0);
@@ -661,15 +671,19 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
     bs.read(a, p, a.b, m);
     cs.read(a, p, a.c, m);
   };
+  const Vec<T, S::EPT> bias = mv.template load_from<T>(a.dt_bias, p.ch0 + mv.col, a.dt_bias && mv.left > 0);
   read(p.first);
   for (uint32_t m = p.first; m < p.last; m++) {
     const bool in = mv.inside(p, m);
     if (a.softplus)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) {
-        const T soft = softplus(dt.v[j]);
+        const T soft = softplus(dt.v[j] + bias.v[j]);
         dt.v[j] = in ? soft : T(0);
       }
+    else
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       sx[mv.col + j][mv.row] = x.v[j];
@@ -724,9 +738,13 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
   Vec<T, NS> from{};
   if (a.state) from = load_states<T, NS>(a.state, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
   const T skip = q == 0 && a.skip ? ((const T*)a.skip)[d] : T(0);
-  T h[NS];
+  const T bias = a.dt_bias ? ((const T*)a.dt_bias)[d] : T(0);
+  T rate[NS], h[NS];
 #pragma unroll
-  for (int j = 0; j < NS; j++) h[j] = from.v[j];
+  for (int j = 0; j < NS; j++) {
+    rate[j] = decay_rate(rate_of(rates.v[j], a.logs));
+    h[j] = from.v[j];
+  }
   for (uint32_t t = 0; t < a.length; t++) {
     const uint64_t at = ((uint64_t)p.b * a.length + t) * a.width + d, row = ((uint64_t)p.b * a.length + t) * a.map_stride + p.group;
     T y = T(0);
@@ -735,12 +753,13 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
       T step = ((const T*)a.dt)[at], z = T(0);
       if (a.gate) z = ((const T*)a.gate)[at];
       const Vec<T, NS> b = load_states<T, NS>(a.b, row, q * NS, a.states, whole), m = load_states<T, NS>(a.c, row, q * NS, a.states, whole);
+      step += bias;
       if (a.softplus) step = softplus(step);
       const T drive = step * u;
       y = skip * u;
 #pragma unroll
       for (int j = 0; j < NS; j++) {
-        h[j] = fma_(decay(step, decay_rate(finite_rate(rates.v[j]))), h[j], drive * b.v[j]);
+        h[j] = fma_(decay(step, rate[j]), h[j], drive * b.v[j]);
         y = fma_(m.v[j], h[j], y);
       }
       y = channel_sum<NL>(y);
@@ -761,6 +780,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   constexpr int WAVES = TPB / 64, COPIES = 16 / NL, M = 2 * NS;
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sg[S::CH][S::LD], sy[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
   __shared__ T red[WAVES][TILE][2 * S::NP];
+  __shared__ __align__(16) T sbias[S::CH], sdbias[TILE][S::CH];  // the steps' bias, and each thread's sums for its gradient
   const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c, wave = threadIdx.x / 64;
   const int copy = threadIdx.x % 16 / NL;
@@ -773,7 +793,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   else if (on && a.carry) from = load_states<T, NS>(a.carry, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    rate[j] = finite_rate(rates.v[j]);
+    rate[j] = rate_of(rates.v[j], a.logs);
     rate_e[j] = decay_rate(rate[j]);
     back[j] = from.v[j];
     da[j] = T(0);
@@ -795,8 +815,18 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     if (on) start = load_states<T, NS>(a.marks, ((uint64_t)p.b * p.marks + m) * a.width + d, q * NS, a.states, whole);
   };
   read(p.last - 1);
+  if (a.dt_bias) {
+    if (threadIdx.x < S::CH) sbias[threadIdx.x] = threadIdx.x < p.chs ? ((const T*)a.dt_bias)[p.ch0 + threadIdx.x] : T(0);
+    store<T, S::EPT>(&sdbias[mv.row][mv.col], Vec<T, S::EPT>{});
+    __syncthreads();
+  }
   for (uint32_t m = p.last; m-- > p.first;) {
     const bool in = mv.inside(p, m);
+    if (a.dt_bias) {
+      const Vec<T, S::EPT> bias = load<T, S::EPT>(&sbias[mv.col]);
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) raw.v[j] = in ? raw.v[j] + bias.v[j] : T(0);
+    }
     Vec<T, S::EPT> slope, gate_g;  // d dt / d raw; dy silu'(z)
     Vec<T, S::EPT> step = raw, gy = g;
     if (a.softplus) {
@@ -889,6 +919,12 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
       ddt.v[j] = in ? sdt[mv.col + j][mv.row] * slope.v[j] : T(0);
       dz.v[j] = in && GATE ? sy[mv.col + j][mv.row] * gate_g.v[j] : T(0);
     }
+    if (a.dt_bias) {
+      Vec<T, S::EPT> sum = load<T, S::EPT>(&sdbias[mv.row][mv.col]);
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) sum.v[j] += ddt.v[j];
+      store<T, S::EPT>(&sdbias[mv.row][mv.col], sum);
+    }
     const bool within = m * TILE + mv.row < a.length;
     const uint64_t at = mv.at(a, p, m);
     mv.store_to(a.dx, at, dx, within);
@@ -909,8 +945,17 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     }
     __syncthreads();
   }
-  if (!on) return;
   const uint64_t row = (uint64_t)p.b * chunks + p.chunk;
+  if (a.dt_bias_rows && threadIdx.x < p.chs) {  // after the last tile's barrier
+    T sum = T(0);
+#pragma unroll
+    for (int t = 0; t < TILE; t++) sum += sdbias[t][threadIdx.x];
+    ((T*)a.dt_bias_rows)[row * a.width + p.ch0 + threadIdx.x] = sum;
+  }
+  if (!on) return;
+  if (a.logs)
+#pragma unroll
+    for (int j = 0; j < NS; j++) da[j] *= rate[j];
   if (a.da_rows) store_states<T, NS>(a.da_rows, row * a.width + d, q * NS, a.states, whole, da);
   if (a.dstate && p.chunk == 0) store_states<T, NS>(a.dstate, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, back);
   if (a.dd_rows && q == 0) ((T*)a.dd_rows)[row * a.width + d] = dd;

@@ -358,12 +358,12 @@ class SelectiveSSM(Layer):
         conv, scan, pos = (None, None, None) if state is None else (state["conv"], state["scan"], state["pos"])
         u, conv = causal_conv(self.inward(params["in"], x), params["conv"]["w"], params["conv"]["b"], conv, lengths, "silu")
         maps = self.proj(params["proj"], u)
-        dt = self.dt(params["dt"], maps[..., :self.rank])
+        dt = maps[..., :self.rank] @ params["dt"]["w"]
         positions = pos.reshape(b, 1) if self.rotary and pos is not None else None
         maps = rotary_norm(maps[..., self.rank:].reshape(b, t, 2 * self.groups, self.states), params["gain"], positions,
                            (self.groups, self.groups), None if self.rotary else 0, self.base)
-        y, scan = selective_scan(u, dt, -exp(params["a_log"]), maps, None, params["d"], self.gate(params["gate"], x), scan, lengths,
-                                 softplus=True)
+        y, scan = selective_scan(u, dt, params["a_log"], maps, None, params["d"], self.gate(params["gate"], x), scan, lengths, softplus=True,
+                                 dt_bias=params["dt"]["b"], log_rates=True)
         # As many positions as the operators read: lengths within the batch's own.
         read = t if lengths is None else where(lengths > t, t, where(lengths > 0, lengths, 0))
         pos = zeros((b,), "int32") + read if pos is None else pos + read

@@ -13,7 +13,7 @@ from .tensor import TRACES, Tracer, caller_source, error, first_dtype, lift
 
 # The operand and variant flags of include/rg_plan.h.
 _CONV_BIAS, _CONV_STATE, _CONV_LENGTHS, _CONV_SILU = 1, 2, 4, 8
-_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS, _SCAN_SOFTPLUS, _SCAN_JOINED = 1, 2, 4, 8, 16, 64
+_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS, _SCAN_SOFTPLUS, _SCAN_JOINED, _SCAN_BIAS, _SCAN_LOG = 1, 2, 4, 8, 16, 64, 128, 256
 _ROTARY_GAIN = 1
 
 
@@ -65,7 +65,7 @@ def causal_conv(x, w, bias=None, state=None, lengths=None, activation=None):
     return _with_results("causal_conv", operands, {"flags": flags | (_CONV_SILU if activation else 0)}, 2)
 
 
-def selective_scan(x, dt, a, b, c=None, d=None, z=None, state=None, lengths=None, softplus=False):
+def selective_scan(x, dt, a, b, c=None, d=None, z=None, state=None, lengths=None, softplus=False, dt_bias=None, log_rates=False):
     """The selective state space scan: every channel of `x` (batch, length, width) drives `states`
     linear recurrences whose step `dt` (as `x`) and maps `b`, `c` change from position to position,
 
@@ -75,16 +75,19 @@ def selective_scan(x, dt, a, b, c=None, d=None, z=None, state=None, lengths=None
     each group serving width / groups neighbouring channels, or (batch, length, states) for one;
     without `c`, `b` holds both, (batch, length, 2 * groups, states), as one projection makes them.
     `d` (width,) and the gate `z` (as `x`) may be left out. `state` (batch, width, states) is h
-    before the first position (zeros without it). With `softplus`, `dt` is taken through
-    log(1 + e^dt) first. Returns `(y, final state)`. With `lengths` (batch,), a padded batch: y is 0
+    before the first position (zeros without it). `dt_bias` (width,) is added to `dt`, and with
+    `softplus` the sum taken through log(1 + e^dt) first. With `log_rates`, `a` holds the logarithms
+    of the rates at which states decay: -e^a takes its place. Returns `(y, final state)`. With `lengths` (batch,), a padded batch: y is 0
     from lengths[b] on, nothing is read there, and the final state is that at lengths[b]."""
     if lengths is not None:
         lengths = _as_index(lengths)
     if c is not None and b.ndim == 3 and c.ndim == 3:
         b, c = (v.reshape(v.shape[0], v.shape[1], 1, v.shape[2]) for v in (b, c))
     maps, joined = ((b,), _SCAN_JOINED) if c is None else ((b, c), 0)
-    operands, flags = _present((x, dt, a, *maps), (d, z, state, lengths), (_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS))
-    return _with_results("selective_scan", operands, {"flags": flags | joined | (_SCAN_SOFTPLUS if softplus else 0)}, 2)
+    operands, flags = _present((x, dt, a, *maps), (d, z, state, lengths, dt_bias),
+                               (_SCAN_SKIP, _SCAN_GATE, _SCAN_STATE, _SCAN_LENGTHS, _SCAN_BIAS))
+    flags |= joined | (_SCAN_SOFTPLUS if softplus else 0) | (_SCAN_LOG if log_rates else 0)
+    return _with_results("selective_scan", operands, {"flags": flags}, 2)
 
 
 def rotary_norm(x, gain=None, positions=None, sections=None, rotary_dims=None, base=10000.0, eps=1e-6):

@@ -290,6 +290,47 @@ def check_scan(case, dtype, device, with_last=True, joined=False):
         agree(g, want["d" + name], size["d" + name], k, dtype, "d" + name)
 
 
+def log_inputs(case, dtype):
+    """Inputs of a scan whose rates are given as logarithms and whose steps have a bias, and what the
+    formulas then take: the steps before the softplus, and the rates. The sum of a step is off by a
+    rounding of |dt| + |bias|, which moves the step by up to that times its value (without a softplus
+    all are positive), and a rate by the four units of its exponential: every position's error grows
+    by less than (|dt| + |bias| + 4) / 6 of that which scan_roundings counts."""
+    v, lengths, soft = scan_inputs(case, dtype)
+    r = np.random.default_rng(1)
+    bias = (r.standard_normal(case[2]) if soft else r.uniform(0.0, 0.1, case[2])).astype(dtype)
+    if soft:
+        v["dt"] = v["dt"] - bias
+    v["dt_bias"], v["a"] = bias, np.log(-v["a"])
+    raw, rates = v["dt"].astype(np.float64) + bias, -np.exp(v["a"].astype(np.float64))
+    grown = 1.0 + (float((np.abs(v["dt"]) + np.abs(bias)).max()) + 4.0) / 6.0
+    return v, lengths, soft, raw, rates, grown * scan_roundings(v["x"], raw, rates, soft)
+
+
+def check_scan_of_logs(case, dtype, device, joined=False):
+    v, lengths, soft, raw, rates, k = log_inputs(case, dtype)
+    args = (v["x"], raw, rates, v["b"], v["c"], v["d"], v["z"], v["state"], lengths, soft, v["dy"], v["dlast"])
+    want, size = scan(*args), scan(*args, mag=True)
+    for w, sign in ((want, 1.0), (size, -1.0)):
+        w["da"], w["ddt_bias"] = sign * w["da"] * rates, w["ddt"].sum((0, 1))
+    if lengths is not None:
+        fill_outside(v, lengths, ["x", "dt", "b", "c", "z"])
+    dy, dl = rg.tensor(v["dy"]), rg.tensor(v["dlast"])
+    if joined:
+        v["b"], v["c"] = np.concatenate([v["b"], v["c"]], 2), None
+        want["db"], size["db"] = (np.concatenate([w["db"], w["dc"]], 2) for w in (want, size))
+
+    def fn(g):
+        y, last = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g.get("c"), g.get("d"), g.get("z"), g.get("state"), lengths, soft, g["dt_bias"], True)
+        return (y * dy).sum() + (last * dl).sum(), (y, last)
+
+    (y, last), grads = _differentiated(fn, {n: v[n] for n in ("x", "dt", "a", "b", "c", "d", "z", "state", "dt_bias")}, device)
+    agree(y, want["y"], size["y"], k, dtype, "y")
+    agree(last, want["last"], size["last"], k, dtype, "last")
+    for name, g in grads.items():
+        agree(g, want["d" + name], size["d" + name], k, dtype, "d" + name)
+
+
 def check_rotary(case, dtype, device):
     b, t, sections, passing, hd, turn, flags = case
     v, pos = rotary_inputs(case, dtype)

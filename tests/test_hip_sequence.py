@@ -36,6 +36,23 @@ def test_scan_of_maps_in_one_operand(case, dtype):
     ref.check_scan(case, dtype, "hip", joined=True)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", ref.SCAN_CASES, ids=str)
+def test_scan_of_logarithms_with_a_bias(case, dtype):
+    ref.check_scan_of_logs(case, dtype, "hip", joined=case[1] % 2 == 0)
+
+
+def test_rates_of_logarithms_at_their_ends():
+    """A logarithm of minus infinity keeps the state, one past the type's exponential forgets it at once."""
+    a = np.array([[-np.inf], [200.0], [np.inf]], F)
+    state = np.array([[[0.5], [0.5], [0.5]]], F)
+    for length in (3, 40):  # a few positions, and tiles
+        x, dt, b = np.zeros((1, length, 3), F), np.full((1, length, 3), 0.25, F), np.ones((1, length, 1, 1), F)
+        y, last = rg.selective_scan(*(rg.tensor(v) for v in (x, dt, a, b, b)), state=rg.tensor(state), log_rates=True)
+        assert np.array_equal(y.numpy()[0], np.tile(np.array([0.5, 0.0, 0.0], F), (length, 1)))
+        assert last.numpy().ravel().tolist() == [0.5, 0.0, 0.0]
+
+
 FEW = [(1, 1, 1, 1, 1, ""), (3, 1, 70, 16, 1, "dzsp"), (2, 3, 130, 16, 2, "dzsp"), (5, 4, 33, 13, 1, "zslp"), (2, 2, 20, 64, 4, "dslp"), (2, 1, 9, 32, 1, "s"),
        (5, 4, 40, 8, 2, "dzslp")]
 
@@ -52,6 +69,22 @@ def test_single_tokens_and_a_few(case, dtype):
     given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "d", "z", "state") if v[n] is not None}
     program = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g.get("d"), g.get("z"), g.get("state"), lengths, soft), (given,),
                          validate="none")
+    y, last = program(given)
+    ref.agree(y.numpy(), want["y"], size["y"], k, dtype, "y")
+    ref.agree(last.numpy(), want["last"], size["last"], k, dtype, "last")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", FEW, ids=str)
+def test_a_few_positions_of_logarithms_with_a_bias(case, dtype):
+    v, lengths, soft, raw, rates, k = ref.log_inputs(case, dtype)
+    args = (v["x"], raw, rates, v["b"], v["c"], v["d"], v["z"], v["state"], lengths, soft, v["dy"], None)
+    want, size = ref.scan(*args), ref.scan(*args, mag=True)
+    if lengths is not None:
+        ref.fill_outside(v, lengths, ["x", "dt", "b", "c", "z"])
+    given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "d", "z", "state", "dt_bias") if v[n] is not None}
+    program = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g.get("d"), g.get("z"), g.get("state"), lengths, soft,
+                                                     g["dt_bias"], True), (given,), validate="none")
     y, last = program(given)
     ref.agree(y.numpy(), want["y"], size["y"], k, dtype, "y")
     ref.agree(last.numpy(), want["last"], size["last"], k, dtype, "last")

@@ -33,6 +33,12 @@ def test_scan_of_maps_in_one_operand(case):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", [ref.SCAN_CASES[i] for i in (0, 1, 3, 7, 9, 12)], ids=str)
+def test_scan_of_logarithms_with_a_bias(case, dtype):
+    ref.check_scan_of_logs(case, dtype, "cpu")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
 @pytest.mark.parametrize("case", ref.ROTARY_CASES, ids=str)
 def test_rotary(case, dtype):
     ref.check_rotary(case, dtype, "cpu")
@@ -42,6 +48,7 @@ def test_device_plans_run_the_same_operators():
     ref.check_conv(ref.CONV_CASES[4], "float32", "cpu_devplan")
     ref.check_scan(ref.SCAN_CASES[3], "float32", "cpu_devplan")
     ref.check_scan(ref.SCAN_CASES[7], "float32", "cpu_devplan", with_last=False)
+    ref.check_scan_of_logs(ref.SCAN_CASES[3], "float32", "cpu_devplan", joined=True)
     ref.check_rotary(ref.ROTARY_CASES[3], "float32", "cpu_devplan")
 
 
@@ -75,6 +82,12 @@ def test_scan_gradients_are_the_differences():
     v, n, _ = ref.scan_inputs((3, 9, 4, 3, 2, "dzslp"), "float64")
     _by_differences(lambda x, dt, a, b, c, d, z, s: sum((o * o).sum() for o in rg.selective_scan(x, dt, a, b, c, d, z, s, n, softplus=True)),
                     [v[k] for k in ("x", "dt", "a", "b", "c", "d", "z", "state")])
+
+
+def test_scan_of_logarithms_gradients_are_the_differences():
+    v, n, _, _, _, _ = ref.log_inputs((3, 9, 4, 3, 2, "dzslp"), "float64")
+    _by_differences(lambda x, dt, a, b, c, e: sum((o * o).sum() for o in rg.selective_scan(x, dt, a, b, c, lengths=n, softplus=True, dt_bias=e, log_rates=True)),
+                    [v[k] for k in ("x", "dt", "a", "b", "c", "dt_bias")])
 
 
 def test_rotary_gradients_are_the_differences():
@@ -129,6 +142,7 @@ def _scan(x=(2, 3, 4), dt=(2, 3, 4), a=(4, 5), b=(2, 3, 1, 5), c=(2, 3, 1, 5), *
     (lambda: rg.rotary_norm(_t(2, 3, 4, 6), positions=[[0], [1], [2]]), "SHAPE_MISMATCH", "positions_must_be_length_or_batch_length"),
     (lambda: _scan(d=_t(5)), "SHAPE_MISMATCH", "d_must_be_width"),
     (lambda: _scan(z=_t(2, 3, 5)), "SHAPE_MISMATCH", "z_shape_differs_from_x"),
+    (lambda: _scan(dt_bias=_t(5)), "SHAPE_MISMATCH", "dt_bias_must_be_width"),
     (lambda: _scan(state=_t(2, 5, 4)), "SHAPE_MISMATCH", "state_must_be_batch_width_states"),
     (lambda: rg.rotary_norm(_t(2, 3, 4)), "SHAPE_MISMATCH", "x_must_be_batch_length_heads_head"),
     (lambda: rg.rotary_norm(_t(2, 3, 4, 5), rotary_dims=4), "SHAPE_MISMATCH", "head_must_be_even_and_at_most_256"),
