@@ -564,15 +564,15 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
   read(0);
   for (uint32_t i = 0; i < count; i++) {
     const bool in = mv.inside(p, BACK ? p.last - 1 - i : p.first + i);
+    if (a.dt_bias)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
     if (a.softplus)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) {
-        const T soft = softplus(dt.v[j] + bias.v[j]);
+        const T soft = softplus(dt.v[j]);
         dt.v[j] = in ? soft : T(0);
       }
-    else
-#pragma unroll
-      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
     if (BACK && a.gate)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) u.v[j] *= silu(z.v[j]);
@@ -675,15 +675,15 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
   read(p.first);
   for (uint32_t m = p.first; m < p.last; m++) {
     const bool in = mv.inside(p, m);
+    if (a.dt_bias)
+#pragma unroll
+      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
     if (a.softplus)
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) {
-        const T soft = softplus(dt.v[j] + bias.v[j]);
+        const T soft = softplus(dt.v[j]);
         dt.v[j] = in ? soft : T(0);
       }
-    else
-#pragma unroll
-      for (int j = 0; j < S::EPT; j++) dt.v[j] = in ? dt.v[j] + bias.v[j] : T(0);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       sx[mv.col + j][mv.row] = x.v[j];
