@@ -41,8 +41,9 @@ struct ScanArgs {
   // states]; of a ([width, states]), the skip and the dt bias ([width]) scan_rows of them.
   void *db_rows, *dc_rows, *da_rows, *dd_rows, *dt_bias_rows;
   void* workspace;              // scan_workspace bytes
-  // Set by the launchers: tiles of positions a chunk, and the chunks' ends and sums of steps.
-  uint32_t chunk_tiles;
+  // Set by the launchers: tiles of positions a chunk, chunks a sequence and a block of the gradient,
+  // and the chunks' ends and sums of steps.
+  uint32_t chunk_tiles, chunks, split;
   void *ends, *totals;
 };
 uint64_t scan_workspace(int dtype, const ScanArgs& a);

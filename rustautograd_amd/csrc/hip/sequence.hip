@@ -334,7 +334,7 @@ struct ScanPlace {
   uint32_t n, marks;        // positions of the sequence; tiles of the padded one
 };
 template <class S>
-__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tiles, uint32_t first_chunk, uint32_t chunks) {
+__device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tiles, uint32_t first_chunk, uint32_t chunks, uint32_t chunk_tiles) {
   ScanPlace p;
   const uint32_t per = a.width / a.groups;
   uint32_t at = blockIdx.x;
@@ -348,8 +348,8 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tile
   p.chs = min((uint32_t)S::CH, per - p.tile * S::CH);
   p.n = end_of(a.lengths, p.b, a.length);
   p.marks = (a.length + TILE - 1) / TILE;
-  p.first = p.chunk * a.chunk_tiles;
-  p.last = min(p.marks, p.first + a.chunk_tiles);
+  p.first = p.chunk * chunk_tiles;
+  p.last = min(p.marks, p.first + chunk_tiles);
   return p;
 }
 
@@ -536,7 +536,7 @@ template <class T, int NL, int NS, bool BACK>
 __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
   __shared__ __align__(16) T sdt[S::CH][S::LD], su[S::CH][S::LD], smap[TILE][S::NP];
-  const ScanPlace p = scan_place<S>(a, tiles, BACK ? 1 : 0, chunks - 1);
+  const ScanPlace p = scan_place<S>(a, tiles, BACK ? 1 : 0, chunks - 1, a.chunk_tiles);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
   const bool whole = a.states % NS == 0;
@@ -644,7 +644,7 @@ template <class T, int NL, int NS>
 __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
-  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
+  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks, a.chunk_tiles);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
   const bool whole = a.states % NS == 0;
@@ -730,7 +730,7 @@ constexpr uint32_t SCAN_FEW = 4;
 template <class T, int NL, int NS>
 __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
   using S = ScanShape<T, NL, NS>;
-  const ScanPlace p = scan_place<S>(a, tiles, 0, 1);
+  const ScanPlace p = scan_place<S>(a, tiles, 0, 1, a.chunk_tiles);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   if (c >= p.chs) return;  // whole channels: the lanes that sum stay together
   const bool whole = a.states % NS == 0;
@@ -770,7 +770,7 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
   if (a.last) store_states<T, NS>(a.last, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, h);
 }
 
-// Backward, tile by tile from the chunk's last. From the state kept before the tile, its decays e
+// Backward, tile by tile from the last of `split` chunks. From the state kept before the tile, its decays e
 // and the decayed states p = e h[t - 1] are formed again, then with G = dL/dh[t] carried back:
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
 // The sums over channels that db and dc take leave one partial row per tile of channels.
@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sg[S::CH][S::LD], sy[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
   __shared__ T red[WAVES][TILE][2 * S::NP];
   __shared__ __align__(16) T sbias[S::CH], sdbias[TILE][S::CH];  // the steps' bias, and each thread's sums for its gradient
-  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks);
+  const ScanPlace p = scan_place<S>(a, tiles, 0, chunks, a.chunk_tiles * a.split);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c, wave = threadIdx.x / 64;
   const int copy = threadIdx.x % 16 / NL;
   const bool on = c < p.chs;
@@ -789,7 +789,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   T rate[NS], rate_e[NS], back[NS], da[NS], dd = T(0);
   const Vec<T, NS> rates = load_states<T, NS>(a.a, on ? d : p.ch0, q * NS, a.states, whole);
   Vec<T, NS> from{};
-  if (on && chunks > 1) from = load_states<T, NS>(a.ends, ((uint64_t)p.b * chunks + p.chunk) * a.width + d, q * NS, a.states, whole);
+  if (on && a.chunks > 1)
+    from = load_states<T, NS>(a.ends, ((uint64_t)p.b * a.chunks + min((p.chunk + 1) * a.split, a.chunks) - 1) * a.width + d, q * NS, a.states, whole);
   else if (on && a.carry) from = load_states<T, NS>(a.carry, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
@@ -983,32 +984,40 @@ void scan_shape(uint32_t states, F f) {
 // SCAN_BLOCKS blocks, two a CU (3 x 777 x 200, 8 states: 25 chunks 46 us forward and backward, 13
 // chunks 62). Joining takes about 0.2 us a chunk and a tile of positions 6 us, both ways, so that few
 // channels are cut into no more than 4 sqrt(tiles) chunks (2 x 2048 x 512, 16 states: 32 chunks 112 us,
-// 64 chunks 123).
-constexpr uint32_t SCAN_BLOCKS = 512;
+// 64 chunks 123). Chunks of four tiles or more are cut further, to eight blocks a CU, whose waves
+// cover each other's latency (4 x 2048 x 2048, 16 states: 16 chunks 169 us forward, 4 chunks 209; 2 x
+// 2048 x 512, 64 states 87 and 100). k_scan_grad has registers for two blocks a CU and takes `split` of
+// those chunks a block.
+constexpr uint32_t SCAN_BLOCKS = 512, SCAN_MOST_BLOCKS = 2048;
 
 struct ScanCut {
-  uint32_t tiles = 1, chunk_tiles = 1, chunks = 1;
+  uint32_t tiles = 1, chunk_tiles = 1, chunks = 1, split = 1, runs = 1;
 };
 template <class T>
-ScanCut scan_cut(const ScanArgs& a) {
+ScanCut scan_cut(const ScanArgs& a, bool grad) {
   ScanCut cut;
   scan_shape<T>(a.states, [&](auto nl, auto) {
     const uint32_t ch = TPB / decltype(nl)::value;
     cut.tiles = (a.width / a.groups + ch - 1) / ch;
   });
   const uint32_t marks = (a.length + TILE - 1) / TILE;
-  const uint64_t blocks = (uint64_t)a.batch * a.groups * cut.tiles;
-  const uint32_t wanted = (uint32_t)std::min<uint64_t>((SCAN_BLOCKS + blocks - 1) / blocks, (uint64_t)std::ceil(4.0 * std::sqrt((double)marks)));
-  cut.chunk_tiles = (marks + wanted - 1) / wanted;
+  const uint64_t blocks = (uint64_t)a.batch * a.groups * cut.tiles, most = (uint64_t)std::ceil(4.0 * std::sqrt((double)marks));
+  auto filling = [&](uint64_t n) { return std::min((n + blocks - 1) / blocks, most); };
+  const uint64_t few = filling(SCAN_BLOCKS), wanted = std::max(few, std::min<uint64_t>(filling(SCAN_MOST_BLOCKS), marks / 4));
+  cut.chunk_tiles = (uint32_t)((marks + wanted - 1) / wanted);
   cut.chunks = (marks + cut.chunk_tiles - 1) / cut.chunk_tiles;
+  if (grad) cut.split = (uint32_t)((cut.chunks + few - 1) / few);
+  cut.runs = (cut.chunks + cut.split - 1) / cut.split;
   return cut;
 }
-ScanCut scan_cut_of(int dtype, const ScanArgs& a) { return dtype == RG_F32 ? scan_cut<float>(a) : scan_cut<double>(a); }
+ScanCut scan_cut_of(int dtype, const ScanArgs& a, bool grad) { return dtype == RG_F32 ? scan_cut<float>(a, grad) : scan_cut<double>(a, grad); }
 
 template <class T, bool GRAD>
 void launch_scan(hipStream_t s, ScanArgs a) {
-  const ScanCut cut = scan_cut<T>(a);
+  const ScanCut cut = scan_cut<T>(a, GRAD);
   a.chunk_tiles = cut.chunk_tiles;
+  a.chunks = cut.chunks;
+  a.split = cut.split;
   a.ends = a.workspace;
   a.totals = (T*)a.workspace + (uint64_t)a.batch * cut.chunks * a.width * a.states;
   scan_shape<T>(a.states, [&](auto nl, auto ns) {
@@ -1024,12 +1033,12 @@ void launch_scan(hipStream_t s, ScanArgs a) {
       hipLaunchKernelGGL((k_scan_ends<T, NL, NS, GRAD>), dim3(blocks * (cut.chunks - 1)), dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
       hipLaunchKernelGGL((k_scan_join<T, GRAD>), dim3(joins), dim3(64), 0, s, a, cut.chunks);
     }
-    const dim3 grid(blocks * cut.chunks);
+    const dim3 grid(blocks * cut.runs);
     if constexpr (GRAD) {
-      if (a.gate) hipLaunchKernelGGL((k_scan_grad<T, NL, NS, true>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
-      else hipLaunchKernelGGL((k_scan_grad<T, NL, NS, false>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+      if (a.gate) hipLaunchKernelGGL((k_scan_grad<T, NL, NS, true>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.runs, vec);
+      else hipLaunchKernelGGL((k_scan_grad<T, NL, NS, false>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.runs, vec);
     } else {
-      hipLaunchKernelGGL((k_scan<T, NL, NS>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.chunks, vec);
+      hipLaunchKernelGGL((k_scan<T, NL, NS>), grid, dim3(TPB), 0, s, a, cut.tiles, cut.runs, vec);
     }
   });
 }
@@ -1037,13 +1046,13 @@ void launch_scan(hipStream_t s, ScanArgs a) {
 }  // namespace
 
 uint64_t scan_blocks(int dtype, const ScanArgs& a) {
-  const ScanCut cut = scan_cut_of(dtype, a);
+  const ScanCut cut = scan_cut_of(dtype, a, false);
   return (uint64_t)a.batch * a.groups * cut.tiles * cut.chunks;
 }
-uint32_t scan_rows(int dtype, const ScanArgs& a) { return a.batch * scan_cut_of(dtype, a).chunks; }
-uint32_t scan_group_tiles(int dtype, const ScanArgs& a) { return scan_cut_of(dtype, a).tiles; }
+uint32_t scan_rows(int dtype, const ScanArgs& a) { return a.batch * scan_cut_of(dtype, a, true).runs; }
+uint32_t scan_group_tiles(int dtype, const ScanArgs& a) { return scan_cut_of(dtype, a, true).tiles; }
 uint64_t scan_workspace(int dtype, const ScanArgs& a) {
-  const uint32_t chunks = scan_cut_of(dtype, a).chunks;
+  const uint32_t chunks = scan_cut_of(dtype, a, true).chunks;
   return chunks > 1 ? (uint64_t)a.batch * chunks * a.width * (a.states + 1) * (dtype == RG_F64 ? 8 : 4) : 0;
 }
 

@@ -25,6 +25,14 @@ def test_scan(case, dtype):
     ref.check_scan(case, dtype, "hip")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("with_last", [True, False])
+def test_scan_of_many_groups_over_long_sequences(dtype, with_last):
+    """Enough channels and positions that a block of the gradient takes two chunks of the forward pass, and
+    the last block one."""
+    ref.check_scan((4, 523, 32, 3, 32, "dzslp"), dtype, "hip", with_last=with_last)
+
+
 @pytest.mark.parametrize("case", [ref.SCAN_CASES[i] for i in (2, 7, 12, 16)], ids=str)
 def test_scan_whose_last_state_nobody_reads(case):
     ref.check_scan(case, "float32", "hip", with_last=False)
