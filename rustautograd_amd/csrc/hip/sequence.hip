@@ -40,17 +40,20 @@ __device__ __forceinline__ T silu(T v) { return v * sigmoid(v); }
 // silu'(v) from s = sigmoid(v).
 template <class T>
 __device__ __forceinline__ T silu_slope(T v, T s) { return s * fma_(v, T(1) - s, T(1)); }
-// log(1 + u), 0 <= u <= 1, to full relative precision: 2 artanh(s) = 2 s (1 + s^2/3 + s^4/5 + ...)
-// at s = u / (2 + u) <= 1/3, whose terms past s^12/13 add up to less than 2e-8, a quarter of a rounding.
+// log(1 + u), 0 <= u <= 1, to full relative precision: u + u^2 p(u), where 1 + u p(u) is the least
+// squares fit of degree 9 to log(1 + u) / u in Chebyshev polynomials of [0, 1]; with its roundings
+// 2.05 x 2^-24 off at most (over 5e5 values from 1e-30 on).
 __device__ __forceinline__ float log1p_(float u) {
-  const float s = over(u, 2.0f + u), w = s * s;
-  float p = 1.0f / 13.0f;
-  p = fma_(p, w, 1.0f / 11.0f);
-  p = fma_(p, w, 1.0f / 9.0f);
-  p = fma_(p, w, 1.0f / 7.0f);
-  p = fma_(p, w, 1.0f / 5.0f);
-  p = fma_(p, w, 1.0f / 3.0f);
-  return fma_(2.0f * s, p * w, 2.0f * s);
+  float p = -0.00325637846f;
+  p = fma_(p, u, 0.0199071616f);
+  p = fma_(p, u, -0.0570642017f);
+  p = fma_(p, u, 0.106142648f);
+  p = fma_(p, u, -0.153118625f);
+  p = fma_(p, u, 0.196781173f);
+  p = fma_(p, u, -0.249545589f);
+  p = fma_(p, u, 0.333300054f);
+  p = fma_(p, u, -0.499999046f);
+  return fma_(u * p, u, u);
 }
 __device__ __forceinline__ double log1p_(double u) { return log1p(u); }
 // log(1 + e^v) without overflow, small steps to full relative precision.
