@@ -784,6 +784,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sg[S::CH][S::LD], sy[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
   __shared__ T red[WAVES][TILE][2 * S::NP];
   __shared__ __align__(16) T sbias[S::CH], sdbias[TILE][S::CH];  // the steps' bias, and each thread's sums for its gradient
+  // A thread's d dt / d raw and dy silu'(z), kept here while a tile's states fill the registers.
+  __shared__ __align__(16) T sslope[TILE][S::CH], sgate[TILE][S::CH];
   const ScanPlace p = scan_place<S>(a, tiles, 0, chunks, a.chunk_tiles * a.split);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c, wave = threadIdx.x / 64;
   const int copy = threadIdx.x % 16 / NL;
@@ -831,7 +833,7 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) raw.v[j] = in ? raw.v[j] + bias.v[j] : T(0);
     }
-    Vec<T, S::EPT> slope, gate_g;  // d dt / d raw; dy silu'(z)
+    Vec<T, S::EPT> slope, gate_g;
     Vec<T, S::EPT> step = raw, gy = g;
     if (a.softplus) {
 #pragma unroll
@@ -850,6 +852,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
         gate_g.v[j] = g.v[j] * silu_slope(z.v[j], s);
         gy.v[j] = g.v[j] * (z.v[j] * s);
       }
+    store<T, S::EPT>(&sslope[mv.row][mv.col], slope);
+    if (GATE) store<T, S::EPT>(&sgate[mv.row][mv.col], gate_g);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       sx[mv.col + j][mv.row] = x.v[j];
@@ -917,6 +921,8 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
     }
     __syncthreads();
     Vec<T, S::EPT> dx, ddt, dz;
+    slope = load<T, S::EPT>(&sslope[mv.row][mv.col]);
+    if (GATE) gate_g = load<T, S::EPT>(&sgate[mv.row][mv.col]);
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) {
       dx.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
