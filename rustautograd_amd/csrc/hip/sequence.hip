@@ -360,12 +360,14 @@ __device__ __forceinline__ ScanPlace scan_place(const ScanArgs& a, uint32_t tile
   return p;
 }
 
-// The part of a tile that a thread moves: EPT neighbouring channels of one position.
+// The part of a tile that a thread moves: EPT neighbouring channels of one position. A wave moves the
+// channels that its own lanes compute, so that what passes through LDS needs no barrier; and no two of
+// its lanes use a bank (four channels and four floats between them: rows of 20) at once.
 template <class S>
 struct ScanMover {
   uint32_t row, col, left;
   bool vec;
-  __device__ __forceinline__ ScanMover(const ScanPlace& p, bool v) : row(threadIdx.x / 16), col(threadIdx.x % 16 * S::EPT), vec(v) {
+  __device__ __forceinline__ ScanMover(const ScanPlace& p, bool v) : row(threadIdx.x % 64 / 4), col((threadIdx.x / 64 * 4 + threadIdx.x % 4) * S::EPT), vec(v) {
     left = col < p.chs ? p.chs - col : 0;
   }
   __device__ __forceinline__ uint64_t at(const ScanArgs& a, const ScanPlace& p, uint32_t m) const {
@@ -424,6 +426,11 @@ __device__ __forceinline__ float decay(float dt, float a) { return __builtin_amd
 __device__ __forceinline__ double decay(double dt, double a) { return exp(dt * a); }
 __device__ __forceinline__ float decay_rate(float a) { return a * 1.44269504088896341f; }
 __device__ __forceinline__ double decay_rate(double a) { return a; }
+// LDS written by lanes of this wave is read by others of it after this.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 // Keeps the scheduler from bringing in the operands of later positions of an unrolled tile early,
 // which costs more registers than a wave has.
 __device__ __forceinline__ void hold(int position) {
@@ -545,7 +552,7 @@ __device__ __forceinline__ void store_states(void* dst, uint64_t row, uint32_t k
 template <class T, int NL, int NS, bool BACK>
 __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
-  __shared__ __align__(16) T sdt[S::CH][S::LD], su[S::CH][S::LD], smap[TILE][S::NP];
+  __shared__ __align__(16) T sdt[S::CH][S::LD], su[S::CH][S::LD], smaps[2][TILE][S::NP];  // maps of every other tile: one barrier a tile
   const ScanPlace p = scan_place<S>(a, tiles, BACK ? 1 : 0, chunks - 1, a.chunk_tiles);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
@@ -591,6 +598,7 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
       sdt[mv.col + j][mv.row] = dt.v[j];
       su[mv.col + j][mv.row] = u.v[j];
     }
+    auto& smap = smaps[i % 2];
     map.put(&smap[0][0]);
     __syncthreads();
     if (i + 1 < count) read(i + 1);
@@ -606,7 +614,7 @@ __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, u
         h[j] = BACK ? e * fma_(v, w, h[j]) : fma_(e, h[j], step * v * w);
       }
     }
-    __syncthreads();
+    wave_sync();
   }
   if (!on) return;
   const uint64_t at = ((uint64_t)p.b * chunks + p.chunk) * a.width + d;
@@ -658,7 +666,7 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
 template <class T, int NL, int NS>
 __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
-  __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sb[TILE][S::NP], sc[TILE][S::NP];
+  __shared__ __align__(16) T sx[S::CH][S::LD], sdt[S::CH][S::LD], sbs[2][TILE][S::NP], scs[2][TILE][S::NP];
   const ScanPlace p = scan_place<S>(a, tiles, 0, chunks, a.chunk_tiles);
   const uint32_t c = threadIdx.x / NL, q = threadIdx.x % NL, d = p.ch0 + c;
   const bool on = c < p.chs;
@@ -704,6 +712,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
       sx[mv.col + j][mv.row] = x.v[j];
       sdt[mv.col + j][mv.row] = dt.v[j];
     }
+    auto &sb = sbs[m % 2], &sc = scs[m % 2];
     bs.put(&sb[0][0]);
     cs.put(&sc[0][0]);
     const Vec<T, S::EPT> gate = z;
@@ -725,7 +734,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
       if (i % NL == (int)q) mine = y;
       if (i % NL == NL - 1) sx[c][i - (NL - 1) + q] = mine;
     }
-    __syncthreads();
+    wave_sync();
     Vec<T, S::EPT> y;
 #pragma unroll
     for (int j = 0; j < S::EPT; j++) y.v[j] = in ? sx[mv.col + j][mv.row] : T(0);
@@ -733,7 +742,7 @@ __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32
 #pragma unroll
       for (int j = 0; j < S::EPT; j++) y.v[j] *= silu(gate.v[j]);
     mv.store_to(a.y, mv.at(a, p, m), y, m * TILE + mv.row < a.length);
-    __syncthreads();
+    wave_sync();
   }
   if (a.last && on && p.last == p.marks) store_states<T, NS>(a.last, (uint64_t)p.b * a.width + d, q * NS, a.states, whole, h);
 }
@@ -969,10 +978,11 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
       const uint64_t rows = (uint64_t)a.batch * a.length * a.map_stride * a.states;
       to[p.tile * rows + (((uint64_t)p.b * a.length + t) * a.map_stride + p.group) * a.states + k] = sum;
     }
-    __syncthreads();
+    wave_sync();
   }
+  if (a.dt_bias) __syncthreads();
   const uint64_t row = (uint64_t)p.b * chunks + p.chunk;
-  if (a.dt_bias_rows && threadIdx.x < p.chs) {  // after the last tile's barrier
+  if (a.dt_bias_rows && threadIdx.x < p.chs) {
     T sum = T(0);
 #pragma unroll
     for (int t = 0; t < TILE; t++) sum += sdbias[t][threadIdx.x];
