@@ -88,7 +88,7 @@ __device__ __forceinline__ void store(T* p, const Vec<T, V>& v) { *(Vec<T, V>*)p
 // A wave takes 64 V neighbouring channels over a run of R positions and keeps the last K inputs
 // in registers, so that x is read once but for the K - 1 positions before a run. Bound by memory:
 // 8 x 4096 x 2048, four taps 88 us, 6.1 TB/s; below some 20 MB by the latency of a block's loads,
-// all of which are in flight at once (4 x 1024 x 512 5.1 us, 3.3 at the rate of a copy).
+// all of which are in flight at once (4 x 1024 x 512 5.4 us, 3.3 at the rate of a copy).
 template <class T, int K, int V, int R>
 __global__ void __launch_bounds__(TPB) k_conv(ConvArgs a, uint32_t nx, uint32_t runs) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -547,8 +547,8 @@ __device__ __forceinline__ void store_states(void* dst, uint64_t row, uint32_t k
 //   forward:  end[c]  = state after the chunk's last position, from zero before its first
 //   backward: end[c]  = gradient carried out of the chunk's first position, from zero after its last
 // Bound by vector instructions, an exponential and four others a state of 29 in all a position and
-// lane: 4 x 2048 x 2048, 16 states 61 us forward and 70 backward; with one or two waves a SIMD by their
-// latency (2 x 2048 x 512 13.4 and 14.1 us).
+// lane: 4 x 2048 x 2048, 16 states 61 us forward and 68 backward; 2 x 2048 x 512 12.2 and
+// 13.4 us, three quarters of the slots taken by two waves a SIMD.
 template <class T, int NL, int NS, bool BACK>
 __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
@@ -658,11 +658,11 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
 }
 
 // Forward: h[t] = e^(dt a) h[t - 1] + dt x b, y = c . h + d x, gated. Each lane's states stay in
-// registers, x, dt, z and y pass once (2 x 2048 x 512 moves 34 MB, 6.5 us of the 18.8 it takes); bound by
+// registers, x, dt, z and y pass once (2 x 2048 x 512 moves 34 MB, 6.5 us of the 18.0 it takes); bound by
 // vector instructions, of which an exponential and four others a state are the recurrence, and what a
 // lane does for its channel (its part of a softplus and a gate, the sum over the lanes, five reads of
-// LDS) is spread over four states: 4 x 2048 x 2048, 16 states 95 us. Two states a lane take 23.8 us
-// where four take 19, eight 31.5 (twice the chunks for as many waves).
+// LDS) is spread over four states: 4 x 2048 x 2048, 16 states 93 us. Two states a lane took 23.8 us
+// where four took 19, eight 31.5 (twice the chunks for as many waves).
 template <class T, int NL, int NS>
 __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
@@ -799,9 +799,9 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
 // The sums over channels that db and dc take leave one partial row per tile of channels.
 // Bound by vector instructions, 120 a position and lane of which 56 are the formulas' own: 2 x 2048 x
-// 512, 16 states 46 us, 76 % of the slots taken by two waves a SIMD; 4 x 2048 x 2048 340 us. A tile's
+// 512, 16 states 46 us, 80 % of the slots taken by two waves a SIMD; 4 x 2048 x 2048 332 us. A tile's
 // decays and decayed states fill 128 registers; two states a lane would leave room for three waves but
-// share what is done for a channel among fewer, 57.6 us.
+// share what is done for a channel among fewer (57.6 us, 48 then).
 template <class T, int NL, int NS, bool GATE>
 __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_grad(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
   using S = ScanShape<T, NL, NS>;
@@ -1020,7 +1020,7 @@ void scan_shape(uint32_t states, F f) {
 // chunks 62). Joining takes about 0.2 us a chunk and a tile of positions 6 us, both ways, so that few
 // channels are cut into no more than 4 sqrt(tiles) chunks (2 x 2048 x 512, 16 states: 64 chunks take a
 // tenth longer than 32). Chunks of four tiles or more are cut further, to eight blocks a CU, whose waves
-// cover each other's latency (4 x 2048 x 2048, 16 states: 16 chunks 169 us forward, 4 chunks 209; 2 x
+// cover each other's latency (4 x 2048 x 2048, 16 states: 16 chunks 169 us forward, 4 chunks 209 then; 2 x
 // 2048 x 512, 64 states 87 and 100). k_scan_grad has registers for two blocks a CU and takes `split` of
 // those chunks a block.
 constexpr uint32_t SCAN_BLOCKS = 512, SCAN_MOST_BLOCKS = 2048;
