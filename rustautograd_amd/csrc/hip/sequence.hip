@@ -1197,7 +1197,8 @@ __global__ void __launch_bounds__(TPB) k_rotary(RotaryArgs a) {
       for (int v = 0; v < V; v++) ss = fma_(x_lo[k].v[v], x_lo[k].v[v], fma_(x_hi[k].v[v], x_hi[k].v[v], ss));
     }
     ss = group_sum<LG>(ss);
-    const T r = normed ? T(1) / sqrt_(ss / T(a.head) + T(a.eps)) : T(1);
+    // A group without a token adds nothing: 1, as eps may be 0 and 0 / 0 would reach the gain's sums.
+    const T r = normed && valid ? T(1) / sqrt_(ss / T(a.head) + T(a.eps)) : T(1);
     T mean = T(0);
 #pragma unroll
     for (int k = 0; k < UPL; k++) {

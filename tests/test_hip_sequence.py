@@ -340,3 +340,40 @@ def test_the_oracle_agrees_at_standard_validation():
     x = rg.tensor(np.random.default_rng(7).standard_normal((2, 19, 16)).astype(F))
     c = rg.compile(lambda p, v: rg.value_and_grad(lambda q: (layer(q, v) ** 2.0).sum())(p), (params, x))
     assert c.report.ok, c.report
+
+
+# Batch, length, sections, passing heads, head, rotary dims. The walkers do not divide the tokens: some
+# have none in the last round, in the second of three or more walks or in the only one.
+WALKS = [(1, 5, (2, 1), 0, 8, 8), (2, 9, (3,), 2, 4, 2), (3, 701, (3,), 2, 256, 2), (3, 5001, (4, 3), 3, 8, 8), (3, 5001, (4, 3), 3, 8, 2)]
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", WALKS, ids=str)
+def test_rotary_without_eps_over_many_tokens(case, dtype):
+    """Heads of +1 and -1 have a root mean square of 1, without `eps` exactly; whole numbers for the rest,
+    and a position of 0, keep every sum exact (below 2^24): results and gradients are equal, not near."""
+    b, t, sections, passing, hd, turn = case
+    r = np.random.default_rng(11)
+    used = sum(sections)
+    x = (2 * r.integers(0, 2, (b, t, used + passing, hd)) - 1).astype(dtype)
+    dy, gain = (r.integers(-2, 3, s).astype(dtype) for s in (x.shape, (len(sections), hd)))
+    start, weight = rg.tensor(np.zeros(t, np.int32)), rg.tensor(dy)
+
+    def program(given):
+        def loss(g):
+            y = rg.rotary_norm(g["x"], g["gain"], start, sections, turn, eps=0.0)
+            return (y * weight).sum(), y
+        (_, y), grads = rg.value_and_grad(loss, has_aux=True)(given)
+        return y, grads
+
+    given = {"x": rg.tensor(x), "gain": rg.tensor(gain)}
+    y, grads = rg.compile(program, (given,), validate="none")(given)
+    rows = np.concatenate([np.repeat(gain, sections, 0), np.ones((passing, hd), dtype)])
+    assert np.array_equal(y.numpy(), x * rows)
+    u = dy * rows
+    mean = (u * x).sum(-1, keepdims=True) / hd
+    mean[:, :, used:] = 0.0
+    assert np.array_equal(grads["x"].numpy(), u - x * mean)
+    ends = np.cumsum(sections)
+    want = np.stack([(dy * x)[:, :, e - n:e].sum((0, 1, 2), dtype=np.float64) for n, e in zip(sections, ends)])
+    assert np.array_equal(grads["gain"].numpy(), want.astype(dtype))
