@@ -13,10 +13,10 @@ constexpr int TPB = 256;
 __device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
 // e^v for -infinity <= v <= 88: the hardware's power of two of v log2 e, times what the rounding of
-// that product leaves out (half the instructions of the full range). Below -103 it is 0 or next to it.
+// that product leaves out (half the instructions of the full range). Below -104 it is 0.
 __device__ __forceinline__ float exp_(float v) {
   constexpr float L = 1.44269504088896341f, REST = 1.92596303e-8f, LN2 = 0.693147180559945309f;  // log2 e = L + REST
-  v = v < -103.0f ? -103.0f : v;
+  v = v < -200.0f ? -200.0f : v;
   const float t = v * L, r = fma_(v, REST, fma_(v, L, -t)), e = __builtin_amdgcn_exp2f(t);
   return fma_(e, r * LN2, e);
 }
@@ -30,11 +30,15 @@ __device__ __forceinline__ float over(float a, float b) {
   return fma_(fma_(-b, q, a), r, q);
 }
 __device__ __forceinline__ double over(double a, double b) { return a / b; }
-// 1 + e^-v, kept finite: past the bound sigmoid is below 1e-37 (1e-300) either way.
-__device__ __forceinline__ float logistic_base(float v) { return 1.0f + exp_(-v > 86.0f ? 86.0f : -v); }
-__device__ __forceinline__ double logistic_base(double v) { return 1.0 + exp_(-v > 700.0 ? 700.0 : -v); }
+__device__ __forceinline__ float abs_(float v) { return __builtin_fabsf(v); }
+__device__ __forceinline__ double abs_(double v) { return __builtin_fabs(v); }
+// 1 / (1 + e^-v), below zero as e^v / (1 + e^v): it goes to 0 as the exponential does, so that v times it is 0
+// for the lowest values of the type, as masks have them.
 template <class T>
-__device__ __forceinline__ T sigmoid(T v) { return over(T(1), logistic_base(v)); }
+__device__ __forceinline__ T sigmoid(T v) {
+  const T u = exp_(-abs_(v));
+  return over(v > T(0) ? T(1) : u, T(1) + u);
+}
 template <class T>
 __device__ __forceinline__ T silu(T v) { return v * sigmoid(v); }
 // silu'(v) from s = sigmoid(v).

@@ -377,3 +377,75 @@ def test_rotary_without_eps_over_many_tokens(case, dtype):
     ends = np.cumsum(sections)
     want = np.stack([(dy * x)[:, :, e - n:e].sum((0, 1, 2), dtype=np.float64) for n, e in zip(sections, ends)])
     assert np.array_equal(grads["gain"].numpy(), want.astype(dtype))
+
+
+def _far_below(dtype):
+    """Values whose exponential is 0 in the type: SiLU and its slope are 0 there."""
+    return np.array([-110.0 if dtype == "float32" else -750.0, -1e4, -1e30, -1e37, np.finfo(dtype).min], dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+def test_silu_of_a_convolution_far_below_zero(dtype):
+    far = _far_below(dtype)
+    x = np.ones((1, 12, 3), dtype)
+    x[0, 2:7, 1] = far[::-1]  # the one before the next ordinary position, which its product with a slope keeps finite, last
+    weight = rg.tensor(np.full(x.shape, 2.0, dtype))
+    w = np.concatenate([np.zeros((1, 3)), np.ones((1, 3))]).astype(dtype)
+
+    def program(given):
+        def loss(g):
+            y = rg.causal_conv(g["x"], g["w"], g["b"], activation="silu")[0]
+            return (y * weight).sum(), y
+        (_, y), grads = rg.value_and_grad(loss, has_aux=True)(given)
+        return y, grads
+
+    given = {"x": rg.tensor(x), "w": rg.tensor(w), "b": rg.zeros(3, dtype)}
+    y, grads = rg.compile(program, (given,), validate="none")(given)
+    s = ref.sigmoid(1.0)
+    want, slope = np.full(x.shape, s), np.full(x.shape, 2.0 * s * (2.0 - s))
+    want[0, 2:7, 1] = slope[0, 2:7, 1] = 0.0
+    ref.agree(y.numpy(), want, np.abs(want), 24, dtype, "y")
+    ref.agree(grads["x"].numpy(), slope, np.abs(slope), 40, dtype, "dx")
+    # Sums of twelve terms of up to 40 roundings.
+    ref.agree(grads["b"].numpy(), slope.sum((0, 1)), slope.sum((0, 1)), 60, dtype, "db")
+    assert (y.numpy()[0, 2:7, 1] == 0.0).all() and (grads["x"].numpy()[0, 2:7, 1] == 0.0).all()
+    want_w = np.stack([(slope[0, 1:] * x[0, :-1]).sum(0), (slope[0] * x[0]).sum(0)])
+    assert np.isfinite(grads["w"].numpy()).all()
+    keep = np.array([True, False, True])
+    ref.agree(grads["w"].numpy()[:, keep], want_w[:, keep], want_w[:, keep], 60, dtype, "dw")
+    ref.agree(grads["w"].numpy()[1, 1], want_w[1, 1], want_w[1, 1], 60, dtype, "dw of the far channel")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("length", [8, 40])
+def test_a_gate_closed_with_the_lowest_values(length, dtype):
+    """A gate far below zero closes: its positions give 0 and pass no gradient, others are as ever."""
+    far = _far_below(dtype)
+    v, _, _ = ref.scan_inputs((2, length, 6, 4, 1, "dzp"), dtype)
+    v["z"][1, 2:7, 3] = far
+    v["z"][0, 1:6, 0] = far
+    shut = v["z"] <= far.max()
+    args = (v["x"], v["dt"], v["a"], v["b"], v["c"], v["d"], v["z"], None, None, True, v["dy"], None)
+    with np.errstate(over="ignore"):
+        want, size, k = ref.scan(*args), ref.scan(*args, mag=True), ref.scan_roundings(v["x"], v["dt"], v["a"], True)
+    weight = rg.tensor(v["dy"])
+
+    def fn(g):
+        y = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g["d"], g["z"], softplus=True)[0]
+        return (y * weight).sum(), (y,)
+
+    (y,), grads = ref._differentiated(fn, {n: v[n] for n in ("x", "dt", "a", "b", "c", "d", "z")}, "hip")
+    ref.agree(y, want["y"], size["y"], k, dtype, "y")
+    assert (y[shut] == 0.0).all() and (grads["z"][shut] == 0.0).all()
+    for n, g in grads.items():
+        ref.agree(g, want["d" + n], size["d" + n], k, dtype, "d" + n)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+def test_a_token_s_gate_closed_with_the_lowest_values(dtype):
+    far = _far_below(dtype)
+    v, _, _ = ref.scan_inputs((1, 1, 7, 4, 1, "dz"), dtype)
+    v["z"][0, 0, 1:6] = far
+    given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "d", "z")}
+    y = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g["d"], g["z"])[0], (given,), validate="none")(given).numpy()
+    assert (y[0, 0, 1:6] == 0.0).all() and np.isfinite(y).all() and (y[0, 0, [0, 6]] != 0.0).all()
