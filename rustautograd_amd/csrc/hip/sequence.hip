@@ -828,7 +828,9 @@ __global__ void __launch_bounds__(TPB, sizeof(T) == 8 && NS > 1 ? 1 : 2) k_scan_
   else if (on && a.carry) from = load_states<T, NS>(a.carry, (uint64_t)p.b * a.width + d, q * NS, a.states, whole);
 #pragma unroll
   for (int j = 0; j < NS; j++) {
-    rate[j] = rate_of(rates.v[j], a.logs);
+    // A lane without a channel may have a step (softplus of 0): with a rate of 0 its decays are 1, where a
+    // growing rate's overflow would reach the sums over channels as infinity times 0.
+    rate[j] = on ? rate_of(rates.v[j], a.logs) : T(0);
     rate_e[j] = decay_rate(rate[j]);
     back[j] = from.v[j];
     da[j] = T(0);

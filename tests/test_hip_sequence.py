@@ -449,3 +449,27 @@ def test_a_token_s_gate_closed_with_the_lowest_values(dtype):
     given = {n: rg.tensor(v[n]) for n in ("x", "dt", "a", "b", "c", "d", "z")}
     y = rg.compile(lambda g: rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], g["d"], g["z"])[0], (given,), validate="none")(given).numpy()
     assert (y[0, 0, 1:6] == 0.0).all() and np.isfinite(y).all() and (y[0, 0, [0, 6]] != 0.0).all()
+
+
+@pytest.mark.parametrize("dtype, width, rate, step", [("float32", 66, 200.0, 1e-3), ("float32", 65, 150.0, 1e-3), ("float64", 33, 1200.0, 1e-4)])
+def test_channels_that_do_not_fill_a_vector_beside_a_growing_one(dtype, width, rate, step):
+    """The last tile's first channel grows, by little in each of its small steps; the lanes past the last
+    channel, which have no step, leave the gradients of the maps alone."""
+    case = (2, 40, width, 4, 1, "zp")
+    v, _, _ = ref.scan_inputs(case, dtype)
+    last = 64 if dtype == "float32" else 32
+    v["a"][last] = rate
+    v["dt"][:, :, last] = np.log(np.expm1(step))
+    args = (v["x"], v["dt"], v["a"], v["b"], v["c"], None, v["z"], None, None, True, v["dy"], None)
+    want, size = ref.scan(*args), ref.scan(*args, mag=True)
+    k = ref.scan_roundings(v["x"], v["dt"], v["a"], True)
+    weight = rg.tensor(v["dy"])
+
+    def fn(g):
+        y = rg.selective_scan(g["x"], g["dt"], g["a"], g["b"], g["c"], z=g["z"], softplus=True)[0]
+        return (y * weight).sum(), (y,)
+
+    (y,), grads = ref._differentiated(fn, {n: v[n] for n in ("x", "dt", "a", "b", "c", "z")}, "hip")
+    ref.agree(y, want["y"], size["y"], k, dtype, "y")
+    for n, g in grads.items():
+        ref.agree(g, want["d" + n], size["d" + n], k, dtype, "d" + n)
