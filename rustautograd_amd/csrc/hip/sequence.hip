@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(TPB) k_conv(ConvArgs a, uint32_t nx, uint32_t 
 
 // The gradient: with gp[t] = dy[t] act'(pre[t]) (0 outside the sequence), the gradient of past[i]
 // is sum_k w[k] gp[i - k], and dw[k] sums gp[t] past[t + k]. A run forms the gp of the K - 1
-// positions after it again rather than exchange them. Bound as the forward pass is: 8 x 4096 x 2048
+// positions after it again rather than exchange them. Positions outside the sequence are left out rather
+// than multiplied by 0, which an infinite input or weight would make NaN. Bound as the forward pass is: 8 x 4096 x 2048
 // 144 us, 5.6 TB/s, 4 x 1024 x 512 9.4 us. The sums for w and the bias stay in a lane's registers over
 // its run, meet once in LDS and leave a row a block, of four runs.
 template <class T, int K, int V, int R>
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(TPB) k_conv_grad(ConvArgs a, uint32_t nx, uint
     const T* dy = (const T*)a.dy + (uint64_t)b * a.length * a.width + d;
     const T* state = a.state ? (const T*)a.state + (uint64_t)b * (K - 1) * a.width + d : nullptr;
     const T* carry = a.carry ? (const T*)a.carry + (uint64_t)b * (K - 1) * a.width + d : nullptr;
+    const uint32_t live = __builtin_amdgcn_readfirstlane(n > t0 ? n - t0 : 0u);  // positions from t0 on; a wave has one t0
     Vec<T, V> w[K], bias{}, in[R + 2 * (K - 1)], g[R + K - 1];
 #pragma unroll
     for (int k = 0; k < K; k++) w[k] = load<T, V>((const T*)a.w + (uint64_t)k * a.width + d);
@@ -180,13 +182,14 @@ __global__ void __launch_bounds__(TPB) k_conv_grad(ConvArgs a, uint32_t nx, uint
 #pragma unroll
     for (int i = 0; i < R + K - 1; i++) {
       g[i] = Vec<T, V>{};
-      if (t0 + i < n) g[i] = load<T, V>(dy + (uint64_t)(t0 + i) * a.width);
+      if ((uint32_t)i < live) g[i] = load<T, V>(dy + (uint64_t)(t0 + i) * a.width);
     }
 #pragma unroll
     for (int i = 0; i < R + K - 1; i++)
 #pragma unroll
       for (int v = 0; v < V; v++) {
-        if (a.silu && t0 + i < n) {
+        if ((uint32_t)i >= live) continue;
+        if (a.silu) {
           T pre = bias.v[v];
 #pragma unroll
           for (int k = 0; k < K; k++) pre = fma_(w[k].v[v], in[i + k].v[v], pre);
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(TPB) k_conv_grad(ConvArgs a, uint32_t nx, uint
       Vec<T, V> out{};
 #pragma unroll
       for (int k = 0; k < K; k++)
-        if (i >= k)
+        if (i >= k && (uint32_t)(i - k) < live)
 #pragma unroll
           for (int v = 0; v < V; v++) out.v[v] = fma_(w[k].v[v], g[i - k].v[v], out.v[v]);
       if (carry && p >= n && p < n + (K - 1)) {

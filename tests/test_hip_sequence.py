@@ -473,3 +473,35 @@ def test_channels_that_do_not_fill_a_vector_beside_a_growing_one(dtype, width, r
     ref.agree(y, want["y"], size["y"], k, dtype, "y")
     for n, g in grads.items():
         ref.agree(g, want["d" + n], size["d" + n], k, dtype, "d" + n)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("length, width, padded", [(5, 6, False), (37, 8, False), (37, 5, True)])
+def test_infinities_at_the_end_of_a_convolution(dtype, length, width, padded):
+    """The last input meets the last tap alone and the first tap the positions up to the last: gradients that
+    no formula multiplies with an infinite value are finite, and exact for whole numbers."""
+    r = np.random.default_rng(3)
+    x, w, dy = (r.integers(-3, 4, s).astype(dtype) for s in ((2, length, width), (3, width), (2, length, width)))
+    lengths = np.array([length, length - 2], np.int32) if padded else None
+    weight = rg.tensor(dy)
+    ends = [length, length - 2] if padded else [length, length]
+
+    def grads(x, w):
+        given = {"x": rg.tensor(x), "w": rg.tensor(w)}
+        program = rg.compile(lambda g: rg.grad(lambda g: (rg.causal_conv(g["x"], g["w"], lengths=lengths)[0] * weight).sum())(g), (given,), validate="none")
+        return {n: g.numpy() for n, g in program(given).items()}
+
+    clean = grads(x, w)
+    for i, n in enumerate(ends):
+        far = x.copy()
+        far[i, n - 1, 0] = np.inf
+        got = grads(far, w)
+        assert np.array_equal(got["w"][:2], clean["w"][:2]) and np.array_equal(got["w"][:, 1:], clean["w"][:, 1:])
+        assert np.array_equal(got["x"], clean["x"])
+    wide = w.copy()
+    wide[0, 1] = np.inf
+    got = grads(x, wide)
+    for i, n in enumerate(ends):
+        # The last two inputs before a sequence's end meet the first tap at no position; padded ones none.
+        assert np.array_equal(got["x"][i, n - 2:], clean["x"][i, n - 2:])
+        assert np.array_equal(got["x"][i, :, [0, *range(2, width)]], clean["x"][i, :, [0, *range(2, width)]])
