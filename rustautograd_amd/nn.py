@@ -232,7 +232,8 @@ class MultiHeadAttention(Layer):
     """Self-attention over `heads` heads of `d // heads`. `mask` broadcasts to (T, T); nonzero
     means visible. With `key` and a dropout rate, the weights and the output are dropped out.
     `qk_norm` divides each head's queries and keys by their root mean square, with a learned gain;
-    `rotary` turns them by position with that base (`positions` as in `rotary_norm`)."""
+    `rotary` turns them by position with that base, True with the usual 10000 (`positions` as in
+    `rotary_norm`)."""
 
     def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
         if d % heads != 0:
@@ -241,7 +242,7 @@ class MultiHeadAttention(Layer):
         self.heads = heads
         self.rate = dropout_rate
         self.qk_norm = qk_norm
-        self.rotary = rotary
+        self.rotary = 10000.0 if rotary is True else rotary
         self.qkv = Linear(d, 3 * d, bias, init, dtype)
         self.out = Linear(d, d, bias, init, dtype)
 

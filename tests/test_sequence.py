@@ -303,3 +303,16 @@ def test_attention_options_keep_the_fused_attention():
     assert sum("attn" in k or "attention" in k for k in kinds) == 2, kinds
     block = nn.TransformerBlock(64, 2, qk_norm=True, rotary=100.0)
     assert block(block.init(random.key(0)), x, mask).shape == x.shape
+
+
+def test_attention_turned_by_the_usual_base():
+    """`rotary=True` is the base that `rotary_norm` has by default, not a base of 1."""
+    x = rg.tensor(np.random.default_rng(4).standard_normal((1, 5, 8)).astype(F))
+    layers = [nn.MultiHeadAttention(8, 2, rotary=r) for r in (True, 10000.0, 1.0, False, None)]
+    params = layers[0].init(random.key(0))
+    usual, same, other, off, none = (layer(params, x).numpy() for layer in layers)
+    assert np.array_equal(usual, same) and not np.array_equal(usual, other)
+    assert np.array_equal(off, none) and not np.array_equal(usual, off)
+    block = [nn.TransformerBlock(8, 2, rotary=r) for r in (True, 10000.0)]
+    params = block[0].init(random.key(1))
+    assert np.array_equal(block[0](params, x).numpy(), block[1](params, x).numpy())
