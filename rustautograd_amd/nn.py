@@ -233,11 +233,13 @@ class MultiHeadAttention(Layer):
     means visible. With `key` and a dropout rate, the weights and the output are dropped out.
     `qk_norm` divides each head's queries and keys by their root mean square, with a learned gain;
     `rotary` turns them by position with that base, True with the usual 10000 (`positions` as in
-    `rotary_norm`)."""
+    `rotary_norm`). Heads that are normed or turned have an even number of values, at most 256."""
 
     def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
         if d % heads != 0:
             raise ValueError(f"{heads} heads cannot split a model dimension of {d}")
+        if (qk_norm or rotary) and (d // heads % 2 != 0 or d // heads > 256):
+            raise ValueError(f"heads of {d // heads} values cannot be normed or turned: an even number, at most 256")
         self.d = d
         self.heads = heads
         self.rate = dropout_rate
@@ -303,10 +305,11 @@ class TransformerBlock(Layer):
 
 class SelectiveSSM(Layer):
     """A selective state space layer, the linear-time counterpart of attention: a projection to
-    `width` channels (2 d by default), a short causal convolution with SiLU, step sizes and the
-    maps into and out of `states` states per channel computed from its result, the scan, a SiLU
-    gate and a projection back. The maps, one pair for each of `groups` groups of channels, are
-    normed like an attention's queries and keys, and turned by position with `rotary`.
+    `width` channels (2 d by default), a short causal convolution with SiLU over `taps` positions (2
+    to 8), step sizes and the maps into and out of `states` states per channel (an even number, at
+    most 64) computed from its result, the scan, a SiLU gate and a projection back. The maps, one
+    pair for each of `groups` groups of channels, are normed like an attention's queries and keys,
+    and turned by position with `rotary`.
 
     `layer(params, x)` reads whole sequences from an empty state. `layer.extend(params, x, state,
     lengths)` returns `(y, state)` for prompts, padded ones too, and for single tokens: the state
@@ -317,8 +320,12 @@ class SelectiveSSM(Layer):
         self.width = 2 * d if width is None else width
         if self.width % groups != 0:
             raise ValueError(f"{groups} groups cannot split {self.width} channels")
-        if rotary and states % 2 != 0:
-            raise ValueError(f"an odd number of states ({states}) cannot be turned in pairs")
+        if states % 2 != 0:
+            raise ValueError(f"an odd number of states ({states}) cannot be normed or turned in pairs")
+        if not 2 <= states <= 64:
+            raise ValueError(f"{states} states: a channel has 2 to 64")
+        if not 2 <= taps <= 8:
+            raise ValueError(f"{taps} taps: a convolution has 2 to 8")
         self.states = states
         self.taps = taps
         self.groups = groups

@@ -316,3 +316,19 @@ def test_attention_turned_by_the_usual_base():
     block = [nn.TransformerBlock(8, 2, rotary=r) for r in (True, 10000.0)]
     params = block[0].init(random.key(1))
     assert np.array_equal(block[0](params, x).numpy(), block[1](params, x).numpy())
+
+
+def test_layers_refuse_sizes_that_their_operators_do():
+    """When they are made, not at their first call."""
+    for states in (1, 5, 66, 0):
+        with pytest.raises(ValueError, match="states"):
+            nn.SelectiveSSM(8, states=states)
+    for taps in (1, 9):
+        with pytest.raises(ValueError, match="taps"):
+            nn.SelectiveSSM(8, taps=taps)
+    for options in ({"qk_norm": True}, {"rotary": 100.0}):
+        for d, heads in ((6, 2), (516, 2)):
+            with pytest.raises(ValueError, match="head"):
+                nn.MultiHeadAttention(d, heads, **options)
+    nn.MultiHeadAttention(6, 2)
+    nn.MultiHeadAttention(512, 2, qk_norm=True, rotary=True)
