@@ -701,6 +701,8 @@ void Graph::check_sequence(const Op& op, const std::vector<uint32_t>& inputs) co
   const bool rotary = op.kind == RG_OP_ROTARY_NORM || op.kind == RG_OP_ROTARY_NORM_GRAD;
   if (rotary && (!(op.base > 0) || !std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)))
     fail("INVALID_ARGUMENT", "base_must_be_positive_and_eps_not_negative");
+  // As 0 it would make the norm of a head of zeros NaN, which it is there to prevent.
+  if (rotary && q.gain >= 0 && d == DType::F32 && op.eps > 0 && (float)op.eps == 0.0f) fail("INVALID_ARGUMENT", "eps_rounds_to_zero_in_the_dtype");
 }
 
 uint32_t Graph::result(uint32_t node, size_t index) {

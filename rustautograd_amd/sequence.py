@@ -94,13 +94,13 @@ def rotary_norm(x, gain=None, positions=None, sections=None, rotary_dims=None, b
     """The norm of each head and its rotation by position in one pass over `x` (batch, length,
     heads, head). `sections` counts the heads of each section, in order (one of all heads without
     it); the heads of section s are divided by their root mean square (over the head, `eps` added
-    to the mean square) and multiplied by `gain[s]`, and heads past the sections pass unchanged:
-    queries, keys and values of a fused projection are sections (heads, heads) of 3 * heads.
-    Without `gain` heads are only rotated. The first `rotary_dims` values of a head (all of them by
-    default, 0 for none) are turned in pairs (i, i + rotary_dims / 2) by the angle
-    position * base^(-2 i / rotary_dims), formed in 64 bits. `positions` is int32: (length,), (batch,
-    length), or (batch, 1) for the first of each sequence, the others following it; 0, 1, ... without
-    it."""
+    to the mean square: 0 or a number that the dtype holds) and multiplied by `gain[s]`, and heads
+    past the sections pass unchanged: queries, keys and values of a fused projection are sections
+    (heads, heads) of 3 * heads. Without `gain` heads are only rotated. The first `rotary_dims`
+    values of a head (all of them by default, 0 for none) are turned in pairs (i, i + rotary_dims /
+    2) by the angle position * base^(-2 i / rotary_dims), formed in 64 bits. `positions` is int32:
+    (length,), (batch, length), or (batch, 1) for the first of each sequence, the others following
+    it; 0, 1, ... without it."""
     if x.ndim != 4:
         raise error("SHAPE_MISMATCH", {"input_shapes": [x.shape]}, "x_must_be_batch_length_heads_head")
     if gain is not None and gain.ndim == 1:

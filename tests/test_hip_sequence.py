@@ -505,3 +505,22 @@ def test_infinities_at_the_end_of_a_convolution(dtype, length, width, padded):
         # The last two inputs before a sequence's end meet the first tap at no position; padded ones none.
         assert np.array_equal(got["x"][i, n - 2:], clean["x"][i, n - 2:])
         assert np.array_equal(got["x"][i, :, [0, *range(2, width)]], clean["x"][i, :, [0, *range(2, width)]])
+
+
+@pytest.mark.parametrize("dtype, eps", [("float32", 1e-40), ("float32", 2e-38), ("float64", 1e-300)])
+def test_heads_of_zeros_under_the_smallest_eps(dtype, eps):
+    """They stay zeros, and their gradient is the cotangent over the root of `eps`."""
+    dy = np.random.default_rng(0).integers(-3, 4, (2, 3, 2, 4)).astype(dtype)
+    x, gain, weight = rg.zeros((2, 3, 2, 4), dtype), rg.ones((1, 4), dtype), rg.tensor(dy)
+
+    def program(given):
+        def loss(g):
+            y = rg.rotary_norm(g["x"], g["gain"], rotary_dims=0, eps=eps)
+            return (y * weight).sum(), y
+        (_, y), grads = rg.value_and_grad(loss, has_aux=True)(given)
+        return y, grads
+
+    y, grads = rg.compile(program, ({"x": x, "gain": gain},), validate="none")({"x": x, "gain": gain})
+    assert (y.numpy() == 0.0).all() and (grads["gain"].numpy() == 0.0).all()
+    want = dy.astype(np.float64) / np.sqrt(np.float64(np.dtype(dtype).type(eps)))
+    ref.agree(grads["x"].numpy(), want, np.abs(want), 8, dtype, "dx")

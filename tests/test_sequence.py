@@ -332,3 +332,14 @@ def test_layers_refuse_sizes_that_their_operators_do():
                 nn.MultiHeadAttention(d, heads, **options)
     nn.MultiHeadAttention(6, 2)
     nn.MultiHeadAttention(512, 2, qk_norm=True, rotary=True)
+
+
+def test_an_eps_that_float32_does_not_hold_is_refused():
+    """It would be 0 there, and the norm of a head of zeros NaN."""
+    zeros, gain = np.zeros((1, 2, 1, 4)), np.ones((1, 4))
+    with pytest.raises(rg.DiagnosticError, match="eps_rounds_to_zero_in_the_dtype"):
+        rg.rotary_norm(rg.tensor(zeros.astype(F)), rg.tensor(gain.astype(F)), eps=1e-50)
+    for dtype, eps in (("float32", 1e-40), ("float64", 1e-50)):
+        assert (rg.rotary_norm(rg.tensor(zeros.astype(dtype)), rg.tensor(gain.astype(dtype)), eps=eps).numpy() == 0.0).all()
+    # Heads that are only turned have no norm, and no use for it.
+    assert (rg.rotary_norm(rg.tensor(zeros.astype(F)), eps=1e-50).numpy() == 0.0).all()
