@@ -46,7 +46,7 @@ template <class T>
 __device__ __forceinline__ T silu_slope(T v, T s) { return s * fma_(v, T(1) - s, T(1)); }
 // log(1 + u), 0 <= u <= 1, to full relative precision: u + u^2 p(u), where 1 + u p(u) is the least
 // squares fit of degree 9 to log(1 + u) / u in Chebyshev polynomials of [0, 1]; with its roundings
-// 2.05 x 2^-24 off at most (over 5e5 values from 1e-30 on).
+// 2.31 x 2^-24 off at most (every float from 1/4 on, every seventh below).
 __device__ __forceinline__ float log1p_(float u) {
   float p = -0.00325637846f;
   p = fma_(p, u, 0.0199071616f);
