@@ -91,8 +91,8 @@ __device__ __forceinline__ void store(T* p, const Vec<T, V>& v) { *(Vec<T, V>*)p
 
 // A wave takes 64 V neighbouring channels over a run of R positions and keeps the last K inputs
 // in registers, so that x is read once but for the K - 1 positions before a run. Bound by memory:
-// 8 x 4096 x 2048, four taps 88 us, 6.1 TB/s; below some 20 MB by the latency of a block's loads,
-// all of which are in flight at once (4 x 1024 x 512 5.4 us, 3.3 at the rate of a copy).
+// 8 x 4096 x 2048, four taps 90 us, 6.0 TB/s; below some 20 MB by the latency of a block's loads,
+// all of which are in flight at once (4 x 1024 x 512 5.3 us, 3.3 at the rate of a copy).
 template <class T, int K, int V, int R>
 __global__ void __launch_bounds__(TPB) k_conv(ConvArgs a, uint32_t nx, uint32_t runs) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -144,10 +144,10 @@ __global__ void __launch_bounds__(TPB) k_conv(ConvArgs a, uint32_t nx, uint32_t 
 
 // The gradient: with gp[t] = dy[t] act'(pre[t]) (0 outside the sequence), the gradient of past[i]
 // is sum_k w[k] gp[i - k], and dw[k] sums gp[t] past[t + k]. A run forms the gp of the K - 1
-// positions after it again rather than exchange them. Positions outside the sequence are left out rather
-// than multiplied by 0, which an infinite input or weight would make NaN. Bound as the forward pass is: 8 x 4096 x 2048
-// 144 us, 5.6 TB/s, 4 x 1024 x 512 9.4 us. The sums for w and the bias stay in a lane's registers over
-// its run, meet once in LDS and leave a row a block, of four runs.
+// positions after it again rather than exchange them. Positions outside the sequence are left out
+// rather than multiplied by 0, which an infinite input or weight would make NaN. Bound as the forward
+// pass is: 8 x 4096 x 2048 146 us, 5.5 TB/s, 4 x 1024 x 512 9.2 us. The sums for w and the bias stay
+// in a lane's registers over its run, meet once in LDS and leave a row a block, of four runs.
 template <class T, int K, int V, int R>
 __global__ void __launch_bounds__(TPB) k_conv_grad(ConvArgs a, uint32_t nx, uint32_t runs) {
   __shared__ T part[TPB / 64][K + 1][64 * V];
@@ -264,9 +264,9 @@ void conv_taps(uint32_t taps, F launch) {
 }
 
 // Channels a lane takes (wide accesses) and the positions of a run (fewer of them read twice), as far
-// as that leaves eight waves a SIMD, or of runs two: 8 x 4096 x 2048 takes 88 us forward and 144
-// backward with four channels (6.1 and 5.6 TB/s; 95 and 162 with one), 4 x 1024 x 512 5.4 and 9.6 us
-// with one (7.1 and 11.6 with four), 5 x 333 x 77 backward 4.7 us in runs of four, 5.6 in runs of eight.
+// as that leaves eight waves a SIMD, or of runs two: 8 x 4096 x 2048 takes 90 us forward and 146
+// backward with four channels (6.0 and 5.5 TB/s; 95 and 162 with one), 4 x 1024 x 512 5.3 and 9.2 us
+// with one (7.1 and 11.6 with four), 5 x 333 x 77 backward 4.6 us in runs of four, 5.6 in runs of eight.
 struct ConvCut {
   uint32_t v, r;
 };
@@ -554,7 +554,7 @@ __device__ __forceinline__ void store_states(void* dst, uint64_t row, uint32_t k
 //   forward:  end[c]  = state after the chunk's last position, from zero before its first
 //   backward: end[c]  = gradient carried out of the chunk's first position, from zero after its last
 // Bound by vector instructions, an exponential and four others a state of 29 in all a position and
-// lane: 4 x 2048 x 2048, 16 states 61 us forward and 68 backward; 2 x 2048 x 512 12.2 and
+// lane: 4 x 2048 x 2048, 16 states 59 us forward and 69 backward; 2 x 2048 x 512 12.0 and
 // 13.4 us, three quarters of the slots taken by two waves a SIMD.
 template <class T, int NL, int NS, bool BACK>
 __global__ void __launch_bounds__(TPB) k_scan_ends(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
@@ -665,10 +665,10 @@ __global__ void __launch_bounds__(64) k_scan_join(ScanArgs a, uint32_t chunks) {
 }
 
 // Forward: h[t] = e^(dt a) h[t - 1] + dt x b, y = c . h + d x, gated. Each lane's states stay in
-// registers, x, dt, z and y pass once (2 x 2048 x 512 moves 34 MB, 6.5 us of the 18.0 it takes); bound by
+// registers, x, dt, z and y pass once (2 x 2048 x 512 moves 34 MB, 6.5 us of the 18.2 it takes); bound by
 // vector instructions, of which an exponential and four others a state are the recurrence, and what a
 // lane does for its channel (its part of a softplus and a gate, the sum over the lanes, five reads of
-// LDS) is spread over four states: 4 x 2048 x 2048, 16 states 93 us. Two states a lane took 23.8 us
+// LDS) is spread over four states: 4 x 2048 x 2048, 16 states 94 us. Two states a lane took 23.8 us
 // where four took 19, eight 31.5 (twice the chunks for as many waves).
 template <class T, int NL, int NS>
 __global__ void __launch_bounds__(TPB) k_scan(ScanArgs a, uint32_t tiles, uint32_t chunks, bool vec) {
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(TPB) k_scan_few(ScanArgs a, uint32_t tiles) {
 //   dx = dt sum G b + d gy, ddt = x sum G b + sum G p a, da += dt G p, db = G dt x, dc = gy h.
 // The sums over channels that db and dc take leave one partial row per tile of channels.
 // Bound by vector instructions, 120 a position and lane of which 56 are the formulas' own: 2 x 2048 x
-// 512, 16 states 46 us, 80 % of the slots taken by two waves a SIMD; 4 x 2048 x 2048 332 us. A tile's
+// 512, 16 states 46 us, 78 % of the slots taken by two waves a SIMD; 4 x 2048 x 2048 332 us. A tile's
 // decays and decayed states fill 128 registers; two states a lane would leave room for three waves but
 // share what is done for a channel among fewer (57.6 us, 48 then).
 template <class T, int NL, int NS, bool GATE>
@@ -1146,8 +1146,8 @@ __device__ __forceinline__ T group_sum(T v) {
 // LG lanes share a head, each with UPL units of V pairs: both halves of a pair lie in one lane, so
 // the turn needs no exchange. A group of lanes keeps one head, its gain and its angles per position
 // in registers and walks the tokens. Bound by memory: 4 x 1024 x 24 heads of 64, the values' passing,
-// are 50 MB forward, 11 us or 4.5 TB/s, and 75 MB backward, 18 us or 4.2 TB/s; 8 x 4096 x 48 heads of 128
-// 336 and 491 us, 4.8 and 4.9.
+// are 50 MB forward, 11 us or 4.7 TB/s, and 75 MB backward, 18 us or 4.2 TB/s; 8 x 4096 x 48 heads of 128
+// 337 and 507 us, 4.8 both.
 template <class T, int V, int LG, int UPL, bool GRAD>
 __global__ void __launch_bounds__(TPB) k_rotary(RotaryArgs a) {
   constexpr int GROUPS = TPB / LG;
