@@ -551,6 +551,9 @@ StepFn lower_instr(Program& prog, const Instr& i) {
   }
 }
 
+// Blocks of a fold's launch, whose threads have to stay below 2^32: of 1024 (fold_rows, fold_jobs) and of 256 (fold_wide).
+constexpr uint32_t FOLD_TILES = 1u << 22, FOLD_BLOCKS = 1u << 24;
+
 // A sequence operator (sequence.hip). Results that nothing reads have no slot and are not written;
 // sums over the batch and its positions leave partial rows in the fold area, folded with the other
 // deferred folds.
@@ -573,6 +576,8 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     const uint64_t off = prog.fold_bytes;
     Program::Fold fd{off, outs[r], rows, (uint32_t)k, RG_REDUCE_SUM, dtype};
     fd.wide = dtype == RG_F32 && k % 4 == 0 && rows <= 16;
+    if (!fd.wide && (k + 63) / 64 >= FOLD_TILES)
+      throw std::runtime_error("a gradient of " + std::to_string(k) + " values from " + std::to_string(rows) + " partial rows exceeds the launch limit");
     prog.folds.push_back(fd);
     prog.fold_bytes += ((uint64_t)rows * k * esize(dtype) + 255) / 256 * 256;
     return (int64_t)off;
@@ -1635,7 +1640,8 @@ bool latch(Exec* e, hipError_t err, const char* what) {
   return true;
 }
 
-// Runs the folds due before steps first..last: f32 ones together, FOLD_JOBS per launch.
+// Runs the folds due before steps first..last: f32 ones together, FOLD_JOBS per launch, as far as its
+// threads stay below 2^32.
 void flush_folds(const Program& p, hipStream_t s, void* const* slots, void* ws, size_t first, size_t last) {
   if (p.folds.empty()) return;
   rgk::FoldJobs jobs;
@@ -1649,8 +1655,14 @@ void flush_folds(const Program& p, hipStream_t s, void* const* slots, void* ws, 
     for (size_t f : p.folds_due[k]) {
       const auto& fd = p.folds[f];
       if (fd.wide) {
+        const uint32_t more = (uint32_t)(((uint64_t)fd.k + 1023) / 1024);
+        if (wide.n > 0 && blocks + more >= FOLD_BLOCKS) {
+          rgk::fold_wide(s, wide, blocks);
+          wide.n = 0;
+          blocks = 0;
+        }
         wide.job[wide.n++] = {(const float*)(base + fd.offset), (float*)slots[fd.out_slot], fd.k, fd.rows, blocks};
-        blocks += (fd.k + 1023) / 1024;
+        blocks += more;
         if (wide.n == rgk::FOLD_JOBS) {
           rgk::fold_wide(s, wide, blocks);
           wide.n = 0;
@@ -1662,8 +1674,14 @@ void flush_folds(const Program& p, hipStream_t s, void* const* slots, void* ws, 
         rgk::fold_rows(s, fd.dtype, fd.kind, base + fd.offset, slots[fd.out_slot], fd.rows, fd.k);
         continue;
       }
+      const uint32_t more = (uint32_t)(((uint64_t)fd.k + 63) / 64);
+      if (jobs.n > 0 && tiles + more >= FOLD_TILES) {
+        rgk::fold_jobs(s, jobs, tiles);
+        jobs.n = 0;
+        tiles = 0;
+      }
       jobs.job[jobs.n++] = {(const float*)(base + fd.offset), (float*)slots[fd.out_slot], fd.rows, fd.k, (uint32_t)fd.kind, tiles};
-      tiles += (fd.k + 63) / 64;
+      tiles += more;
       if (jobs.n == rgk::FOLD_JOBS) {
         rgk::fold_jobs(s, jobs, tiles);
         jobs.n = 0;

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import rustautograd_amd as rg
+from rustautograd_amd import random
 import sequence_reference as ref
 import sequence_sizes as sizes
 
@@ -98,3 +99,40 @@ def test_a_scan_of_many_chunks_inside_control_flow():
         assert np.array_equal(got, want)
     for k in inputs:
         assert np.array_equal(one[1][k], other[1][k]), k
+
+
+def _long_maps(joined):
+    """Gradients of the maps of a scan of 2137153 positions, 17 channels (two tiles, each a partial row) and
+    63 states, less those that the formulas give. Rates of minus infinity and whole numbers keep every
+    value exact: db = c sum dy x, dc = b sum dy x. Made and compared on the device."""
+    length, width, states = 2 ** 21 + 40001, 17, 63
+
+    def whole(key, shape):
+        return rg.floor(random.uniform(key, shape) * 5.0) - 2.0
+
+    def program(key):
+        keys = random.split(key, 4)
+        x, dy = (whole(k, (1, length, width)) for k in keys[:2])
+        b, c = (whole(k, (1, length, 1, states)) for k in keys[2:])
+        dt, rates = rg.broadcast_to(rg.ones((1,)), x.shape), rg.tensor(np.full((width, states), -np.inf, np.float32))
+        maps = (rg.concatenate([b, c], 2), None) if joined else (b, c)
+        given = {k: m for k, m in zip("bc", maps) if m is not None}
+        grads = rg.grad(lambda g: (rg.selective_scan(x, dt, rates, g["b"], g.get("c"))[0] * dy).sum())(given)
+        sums = (x * dy).sum(-1).reshape(1, length, 1, 1)
+        wants = (rg.concatenate([c, b], 2) * sums,) if joined else (c * sums, b * sums)
+        return [rg.abs(g - w).max() for g, w in zip((grads[k] for k in sorted(grads)), wants)], rg.abs(grads["b"]).max()
+
+    key = random.key(0)
+    return rg.compile(program, (key,), validate="none")(key)
+
+
+def test_folds_that_do_not_fit_one_launch():
+    """Two gradients of 1.35e8 values each: the threads that fold both are more than a launch may have."""
+    off, most = _long_maps(joined=False)
+    assert [float(v) for v in off] == [0.0, 0.0] and float(most) > 20.0
+
+
+def test_a_fold_that_no_launch_holds_is_refused():
+    """One gradient of 2.7e8 values, an odd multiple of two."""
+    with pytest.raises(rg.DiagnosticError, match="exceeds the launch limit"):
+        _long_maps(joined=True)
