@@ -79,7 +79,7 @@
  *                  whose constants lie in the same blob (scan: body; while: condition, body;
  *                  cond: then, else)
  *   CAUSAL_CONV, CAUSAL_CONV_GRAD, SELECTIVE_SCAN, SELECTIVE_SCAN_GRAD, ROTARY_NORM,
- *   ROTARY_NORM_GRAD
+ *   ROTARY_NORM_GRAD, ATTENTION, ATTENTION_GRAD, PAGED_ATTENTION, JOINT_NORM
  *                  flags, rotary dims, base (f64 bits), eps (f64 bits), n_sections, sections...,
  *                  n_results, per result the program reads: result index, slot
  *   Sequence operators (no reference counterpart; `sequence_of` says which operands follow which
@@ -101,6 +101,22 @@
  *                  section s divided by their root mean square and scaled by gain[s], and their
  *                  pairs (i, i + R / 2), i < R / 2, turned by position * base^(-2 i / R)
  *       _GRAD      in the same, dy; out dx, dgain
+ *     ATTENTION    in q[B,T,H,hd], k, v[B,T,G,hd] (with RG_ATTEND_JOINED one x[B,T,H + 2 G,hd], the
+ *                  heads of q, k and v in order) (, slopes[H]) (, documents[B,T]) (, prefix[B])
+ *                  (, lengths[B]); base is the scale, eps the cap (0: none), sections H, G;
+ *                  s = cap tanh(scale q.k / cap) - slope |i - j|; key j is seen by query i when
+ *                  (j <= i, or not RG_ATTEND_CAUSAL, or j < prefix) and both have the same document,
+ *                  not negative; query head h reads head h G / H of k and v;
+ *                  out 0: y[B,T,H,hd], the softmax of s over the keys seen, times v (0 where none is);
+ *                  1: the logarithm to base 2 of the softmax's sum, [B,H,T], for the gradient alone
+ *       _GRAD      in the same, y, result 1, dy; out dq (joined: dx), dk, dv, dslopes
+ *     PAGED_ATTENTION in q, k, v or x as above, k and v pages[P,page,G,hd], table[B,N], first[B]
+ *                  (, slopes[H]) (, lengths[B]); position p of sequence b lies in row p % page of
+ *                  page table[b, p / page]; the T new positions follow the first[b] that the pages
+ *                  hold, and see those and each other in causal order; out y and the pages with the
+ *                  new rows of k and v. Positions whose page is not one of the P are not there: not
+ *                  read, not written
+ *     JOINT_NORM   in tensors; out 0: the square root of the sum of all their squares
  *   With lengths, positions from lengths[b] on (clamped to 0..T) are outside sequence b: their
  *   results and gradients are 0, their inputs are not read into any other value.
  *   Control flow (plan.rs:737-831): the step's `dst` is -1 and its results go to the listed
@@ -139,6 +155,7 @@ enum rg_op {
   RG_OP_KEY_SPLIT, RG_OP_ARG_TOP_K, RG_OP_CUMSUM, RG_OP_SCAN, RG_OP_WHILE, RG_OP_COND,
   RG_OP_OUTPUT, RG_OP_PLACEHOLDER, RG_OP_CUSTOM, RG_OP_CAUSAL_CONV, RG_OP_CAUSAL_CONV_GRAD,
   RG_OP_SELECTIVE_SCAN, RG_OP_SELECTIVE_SCAN_GRAD, RG_OP_ROTARY_NORM, RG_OP_ROTARY_NORM_GRAD,
+  RG_OP_ATTENTION, RG_OP_ATTENTION_GRAD, RG_OP_PAGED_ATTENTION, RG_OP_JOINT_NORM,
   RG_OP_COUNT
 };
 
@@ -150,6 +167,11 @@ enum rg_scan_flags {
   RG_SCAN_BIAS = 128, RG_SCAN_LOG = 256 /* a holds the rates' logarithms: the rates are -e^a */
 };
 enum rg_rotary_flags { RG_ROTARY_GAIN = 1 };
+enum rg_attend_flags {
+  RG_ATTEND_JOINED = 1, RG_ATTEND_SLOPES = 2, RG_ATTEND_DOCUMENTS = 4, RG_ATTEND_PREFIX = 8, RG_ATTEND_LENGTHS = 16, RG_ATTEND_CAUSAL = 32
+};
+/* The longest head of an attention operator. */
+#define RG_ATTEND_MAX_HEAD 256
 /* Taps of a causal convolution, states of a selective scan, and the length of a head. */
 #define RG_CONV_MAX_TAPS 8
 #define RG_SCAN_MAX_STATES 64
@@ -199,21 +221,118 @@ struct Instr {
   std::vector<std::pair<int64_t, int64_t>> outs; /* theirs: (result index, slot) */
 };
 
-inline bool is_sequence(int32_t op) { return op >= RG_OP_CAUSAL_CONV && op <= RG_OP_ROTARY_NORM_GRAD; }
+inline bool is_sequence(int32_t op) { return op >= RG_OP_CAUSAL_CONV && op <= RG_OP_JOINT_NORM; }
 /* Those whose results are numbered; ROTARY_NORM has one, in `dst`. */
 inline bool is_multi_result(int32_t op) { return is_sequence(op) && op != RG_OP_ROTARY_NORM; }
 
 /* A sequence operator's sizes, where its operands are among the arguments (-1: absent), and the
  * shapes of its results. The one definition that the engine, the backend and the parser share. */
 struct Sequence {
-  int64_t batch = 0, length = 0, width = 0, taps = 0, states = 0, groups = 0, heads = 0, head = 0, used = 0;
+  int64_t batch = 0, length = 0, width = 0, taps = 0, states = 0, groups = 0, heads = 0, head = 0, used = 0, keys = 0, pages = 0, page = 0,
+          table_pages = 0;
   int x = 0, w = -1, bias = -1, dt = -1, a = -1, b = -1, c = -1, skip = -1, gate = -1, state = -1, lengths = -1, marks = -1, dy = -1,
-      carry = -1, positions = -1, gain = -1, dt_bias = -1;
+      carry = -1, positions = -1, gain = -1, dt_bias = -1, k = -1, v = -1, slopes = -1, documents = -1, prefix = -1, k_pages = -1, v_pages = -1,
+      table = -1, first = -1, y = -1, sums = -1;
   bool shared_positions = false; /* positions of [length], the same for every sequence */
   bool positions_from = false;   /* positions of [batch, 1], the first of each sequence */
   std::vector<std::vector<int64_t>> results;
   std::string wrong; /* empty when the operands fit */
+  /* Operands of whole numbers (int32). */
+  bool is_index(int operand) const {
+    for (int at : {lengths, positions, documents, prefix, table, first})
+      if (at >= 0 && at == operand) return true;
+    return false;
+  }
 };
+
+/* Attention and its paged form, whose sections are the heads of q and of k and v. */
+inline Sequence attention_of(int32_t op, const SequenceAttr& at, const std::vector<std::vector<int64_t>>& s) {
+  Sequence q;
+  auto fail = [&](const char* what) {
+    if (q.wrong.empty()) q.wrong = what;
+  };
+  const int64_t f = at.flags;
+  const bool joined = (f & RG_ATTEND_JOINED) != 0, paged = op == RG_OP_PAGED_ATTENTION, grad = op == RG_OP_ATTENTION_GRAD;
+  int next = 1;
+  auto take = [&](bool present) { return present ? next++ : -1; };
+  q.k = take(!joined);
+  q.v = take(!joined);
+  q.k_pages = take(paged);
+  q.v_pages = take(paged);
+  q.table = take(paged);
+  q.first = take(paged);
+  q.slopes = take((f & RG_ATTEND_SLOPES) != 0);
+  q.documents = take((f & RG_ATTEND_DOCUMENTS) != 0);
+  q.prefix = take((f & RG_ATTEND_PREFIX) != 0);
+  q.lengths = take((f & RG_ATTEND_LENGTHS) != 0);
+  q.y = take(grad);
+  q.sums = take(grad);
+  q.dy = take(grad);
+  if ((int)s.size() != next || (paged && (f & (RG_ATTEND_DOCUMENTS | RG_ATTEND_PREFIX)))) {
+    fail("operand_count_does_not_match_the_flags");
+    return q;
+  }
+  for (const auto& v : s)
+    for (int64_t d : v)
+      if (d < 1) {
+        fail("empty_operand");
+        return q;
+      }
+  if (at.sections.size() != 2 || at.sections[0] < 1 || at.sections[1] < 1 || at.sections[0] % at.sections[1] != 0) {
+    fail("heads_must_be_a_multiple_of_the_key_heads");
+    return q;
+  }
+  q.heads = at.sections[0];
+  q.keys = at.sections[1];
+  const std::vector<int64_t>& x = s[0];
+  if (x.size() != 4 || x[2] != q.heads + (joined ? 2 * q.keys : 0)) {
+    fail(joined ? "x_must_be_batch_length_heads_and_twice_the_key_heads_head" : "q_must_be_batch_length_heads_head");
+    return q;
+  }
+  q.batch = x[0];
+  q.length = x[1];
+  q.head = x[3];
+  if (q.head > RG_ATTEND_MAX_HEAD) fail("head_must_be_at_most_256");
+  auto dims = [&](int k, const std::vector<int64_t>& want, const char* what) {
+    if (k >= 0 && s[(size_t)k] != want) fail(what);
+  };
+  const std::vector<int64_t> keys = {q.batch, q.length, q.keys, q.head}, out = {q.batch, q.length, q.heads, q.head};
+  const std::vector<int64_t> sums = {q.batch, q.heads, q.length};
+  dims(q.k, keys, "k_must_be_batch_length_key_heads_head");
+  dims(q.v, keys, "v_must_be_batch_length_key_heads_head");
+  dims(q.slopes, {q.heads}, "slopes_must_be_one_per_head");
+  dims(q.documents, {q.batch, q.length}, "documents_must_be_batch_length");
+  dims(q.prefix, {q.batch}, "prefix_must_be_one_per_sequence");
+  dims(q.lengths, {q.batch}, "lengths_must_be_one_per_sequence");
+  dims(q.first, {q.batch}, "first_must_be_one_per_sequence");
+  dims(q.y, out, "result_shape");
+  dims(q.sums, sums, "sums_shape");
+  dims(q.dy, out, "cotangent_shape_differs_from_the_result");
+  if (paged) {
+    const std::vector<int64_t>&p = s[(size_t)q.k_pages], &t = s[(size_t)q.table];
+    if (p.size() != 4 || p[2] != q.keys || p[3] != q.head) {
+      fail("pages_must_be_pages_page_key_heads_head");
+      return q;
+    }
+    dims(q.v_pages, p, "pages_of_k_and_v_differ");
+    if (t.size() != 2 || t[0] != q.batch) {
+      fail("table_must_be_batch_by_pages");
+      return q;
+    }
+    q.pages = p[0];
+    q.page = p[1];
+    q.table_pages = t[1];
+    if (q.page > (1ll << 30) / t[1] || q.length > (1ll << 30)) fail("more_than_2_to_the_30_positions");
+    q.results = {out, p, p};
+  } else if (grad) {
+    if (joined) q.results = {x, keys, keys, {q.heads}};
+    else q.results = {out, keys, keys, {q.heads}};
+  } else {
+    if (q.length > (1ll << 30)) fail("more_than_2_to_the_30_positions");
+    q.results = {out, sums};
+  }
+  return q;
+}
 
 inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vector<std::vector<int64_t>>& s) {
   Sequence q;
@@ -223,6 +342,15 @@ inline Sequence sequence_of(int32_t op, const SequenceAttr& at, const std::vecto
   auto dims = [&](int k, const std::vector<int64_t>& want, const char* what) {
     if (s[(size_t)k] != want) fail(what);
   };
+  if (op == RG_OP_ATTENTION || op == RG_OP_ATTENTION_GRAD || op == RG_OP_PAGED_ATTENTION) return attention_of(op, at, s);
+  if (op == RG_OP_JOINT_NORM) {
+    if (s.empty()) fail("operand_count_does_not_match_the_flags");
+    for (const auto& v : s)
+      for (int64_t d : v)
+        if (d < 1) fail("empty_operand");
+    q.results = {{}};
+    return q;
+  }
   const int64_t f = at.flags;
   int next = 1;
   auto take = [&](bool present) { return present ? next++ : -1; };
@@ -463,7 +591,7 @@ inline void check_refs(const Plan& pl) {
         if (!q.wrong.empty()) fail(at + ": " + q.wrong);
         if (in.dtype != RG_F32 && in.dtype != RG_F64) fail(at + " is not of a floating-point dtype");
         for (size_t j = 0; j < in.args.size(); j++) {
-          const int32_t want = (int)j == q.lengths || (int)j == q.positions ? (int32_t)RG_I32 : in.dtype;
+          const int32_t want = q.is_index((int)j) ? (int32_t)RG_I32 : in.dtype;
           if (in.args[j].slot < 0 || pl.slots[(size_t)in.args[j].slot].dtype != want) fail(at + " has an argument of another dtype");
         }
         if (!is_multi_result(in.op) && (in.dst < 0 || in.n != prod_of(q.results[0]) || pl.slots[(size_t)in.dst].dtype != in.dtype))

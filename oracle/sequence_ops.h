@@ -2,6 +2,7 @@
 // formulas, one position after another, and rounded once to the operator's dtype when stored. The
 // angles of a rotation, whose error grows with the position, are formed in extended precision.
 #pragma once
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <vector>
@@ -231,6 +232,189 @@ void rotary_norm(const Operands<T>& o) {
     for (size_t k = 0; k < dgain.size(); k++) o.out[1][k] = (T)dgain[k];
 }
 
+// The rows of a query, key or value operand: `heads` of them from `at` on in rows of `stride` values.
+template <class T>
+struct Rows {
+  const T* p;
+  int64_t stride, head;
+  const T* operator()(int64_t position, int64_t h) const { return p + position * stride + h * head; }
+};
+
+template <class T>
+void attention(const Operands<T>& o) {
+  const auto& q = o.q;
+  const int64_t L = q.length, H = q.heads, G = q.keys, hd = q.head, per = H / G, row = q.k < 0 ? (H + 2 * G) * hd : H * hd;
+  const bool joined = q.k < 0, grad = q.dy >= 0, causal = o.has(RG_ATTEND_CAUSAL);
+  const Rows<T> qs{o.arg(q.x), row, hd}, ks{joined ? o.arg(q.x) + H * hd : o.arg(q.k), joined ? row : G * hd, hd},
+      vs{joined ? o.arg(q.x) + (H + G) * hd : o.arg(q.v), joined ? row : G * hd, hd};
+  const T *slopes = o.arg(q.slopes), *dy = o.arg(q.dy);
+  const int32_t* docs = q.documents < 0 ? nullptr : (const int32_t*)o.slot[(size_t)q.documents];
+  const int32_t* prefix = q.prefix < 0 ? nullptr : (const int32_t*)o.slot[(size_t)q.prefix];
+  const double scale = o.in.sequence.base, cap = o.in.sequence.eps;
+  std::vector<double> dq, dk, dv, dslope((size_t)(q.batch * H), 0.0);
+  if (grad) {
+    dq.assign((size_t)(q.batch * L * H * hd), 0.0);
+    dk.assign((size_t)(q.batch * L * G * hd), 0.0);
+    dv.assign(dk.size(), 0.0);
+  }
+#pragma omp parallel for
+  for (int64_t bg = 0; bg < q.batch * G; bg++) {
+    const int64_t b = bg / G, g = bg % G, n = o.end(b);
+    std::vector<double> s((size_t)L), slope_of(s.size());
+    for (int64_t h = g * per; h < (g + 1) * per; h++)
+      for (int64_t i = 0; i < L; i++) {
+        const T* qi = qs(b * L + i, h);
+        std::vector<int64_t> seen;
+        const bool in = i < n && (!docs || docs[b * L + i] >= 0);
+        for (int64_t j = 0; in && j < n; j++)
+          if ((!causal || j <= i || (prefix && j < prefix[b])) && (!docs || docs[b * L + j] == docs[b * L + i])) seen.push_back(j);
+        double top = -INFINITY, sum = 0.0;
+        for (int64_t j : seen) {
+          double u = 0.0;
+          const T* kj = ks(b * L + j, g);
+          for (int64_t d = 0; d < hd; d++) u += (double)qi[d] * (double)kj[d];
+          u *= scale;
+          slope_of[(size_t)j] = 1.0;
+          if (cap > 0) {
+            const double t = std::tanh(u / cap);
+            u = cap * t;
+            slope_of[(size_t)j] = 1.0 - t * t;
+          }
+          if (slopes) u -= (double)slopes[h] * (double)std::llabs(i - j);
+          s[(size_t)j] = u;
+          top = u > top || std::isnan(u) ? u : top;
+        }
+        for (int64_t j : seen) sum += s[(size_t)j] = std::exp(s[(size_t)j] - top);
+        for (int64_t j : seen) s[(size_t)j] /= sum;
+        if (!grad) {
+          if (o.out[0])
+            for (int64_t d = 0; d < hd; d++) {
+              double y = 0.0;
+              for (int64_t j : seen) y += s[(size_t)j] * (double)vs(b * L + j, g)[d];
+              o.out[0][((b * L + i) * H + h) * hd + d] = (T)y;
+            }
+          if (o.out[1]) o.out[1][(b * H + h) * L + i] = seen.empty() ? (T)INFINITY : (T)((top + std::log(sum)) / std::log(2.0));
+          continue;
+        }
+        const T* gi = dy + ((b * L + i) * H + h) * hd;
+        double dot = 0.0;
+        std::vector<double> dp(seen.size(), 0.0);
+        for (size_t c = 0; c < seen.size(); c++) {
+          for (int64_t d = 0; d < hd; d++) dp[c] += (double)gi[d] * (double)vs(b * L + seen[c], g)[d];
+          dot += s[(size_t)seen[c]] * dp[c];
+        }
+        for (size_t c = 0; c < seen.size(); c++) {
+          const int64_t j = seen[c];
+          const double p = s[(size_t)j], ds = p * (dp[c] - dot), du = ds * slope_of[(size_t)j] * scale;
+          const T* kj = ks(b * L + j, g);
+          for (int64_t d = 0; d < hd; d++) {
+            dv[(size_t)(((b * L + j) * G + g) * hd + d)] += p * (double)gi[d];
+            dq[(size_t)(((b * L + i) * H + h) * hd + d)] += du * (double)kj[d];
+            dk[(size_t)(((b * L + j) * G + g) * hd + d)] += du * (double)qi[d];
+          }
+          dslope[(size_t)(b * H + h)] -= ds * (double)std::llabs(i - j);
+        }
+      }
+  }
+  if (!grad) return;
+  auto put = [&](size_t r, const std::vector<double>& v, int64_t heads, int64_t stride, int64_t at) {
+    if (!o.out[r]) return;
+    for (int64_t t = 0; t < q.batch * L; t++)
+      for (int64_t d = 0; d < heads * hd; d++) o.out[r][t * stride + at + d] = (T)v[(size_t)(t * heads * hd + d)];
+  };
+  put(0, dq, H, row, 0);
+  put(joined ? 0 : 1, dk, G, joined ? row : G * hd, joined ? H * hd : 0);
+  put(joined ? 0 : 2, dv, G, joined ? row : G * hd, joined ? (H + G) * hd : 0);
+  if (o.out[3])
+    for (int64_t h = 0; h < H; h++) {
+      double sum = 0.0;
+      for (int64_t b = 0; b < q.batch; b++) sum += dslope[(size_t)(b * H + h)];
+      o.out[3][h] = (T)sum;
+    }
+}
+
+template <class T>
+void paged_attention(const Operands<T>& o) {
+  const auto& q = o.q;
+  const int64_t L = q.length, H = q.heads, G = q.keys, hd = q.head, per = H / G, row = q.k < 0 ? (H + 2 * G) * hd : H * hd;
+  const bool joined = q.k < 0;
+  const Rows<T> qs{o.arg(q.x), row, hd}, ks{joined ? o.arg(q.x) + H * hd : o.arg(q.k), joined ? row : G * hd, hd},
+      vs{joined ? o.arg(q.x) + (H + G) * hd : o.arg(q.v), joined ? row : G * hd, hd};
+  const T *slopes = o.arg(q.slopes), *kp = o.arg(q.k_pages), *vp = o.arg(q.v_pages);
+  const int32_t *table = (const int32_t*)o.slot[(size_t)q.table], *first = (const int32_t*)o.slot[(size_t)q.first];
+  const double scale = o.in.sequence.base, cap = o.in.sequence.eps;
+  const int64_t room = q.table_pages * q.page;
+  // The first value of position p's row among the pages, or -1 where it has none.
+  auto place = [&](int64_t b, int64_t p) -> int64_t {
+    if (p < 0 || p >= room) return -1;
+    const int64_t page = table[b * q.table_pages + p / q.page];
+    return page < 0 || page >= q.pages ? -1 : (page * q.page + p % q.page) * G * hd;
+  };
+  auto begin_of = [&](int64_t b) { return std::min<int64_t>(std::max<int64_t>(0, first[b]), 1ll << 30); };
+  for (int64_t b = 0; b < q.batch; b++) {
+    const int64_t n = o.end(b), begin = begin_of(b);
+    for (int64_t i = 0; i < L; i++)
+      for (int64_t h = 0; h < H && o.out[0]; h++) {
+        T* y = o.out[0] + ((b * L + i) * H + h) * hd;
+        std::fill(y, y + hd, (T)0);
+        if (i >= n) continue;
+        const int64_t g = h / per;
+        std::vector<double> s;
+        std::vector<const T*> value;
+        double top = -INFINITY, sum = 0.0;
+        auto add = [&](const T* k, const T* v, int64_t distance) {
+          double u = 0.0;
+          for (int64_t d = 0; d < hd; d++) u += (double)qs(b * L + i, h)[d] * (double)k[d];
+          u *= scale;
+          if (cap > 0) u = cap * std::tanh(u / cap);
+          if (slopes) u -= (double)slopes[h] * (double)distance;
+          s.push_back(u);
+          value.push_back(v);
+          top = u > top || std::isnan(u) ? u : top;
+        };
+        for (int64_t p = 0; p < std::min(begin, room); p++) {
+          const int64_t at = place(b, p);
+          if (at >= 0) add(kp + at + g * hd, vp + at + g * hd, begin + i - p);
+        }
+        for (int64_t j = 0; j <= i; j++) add(ks(b * L + j, g), vs(b * L + j, g), i - j);
+        for (double& u : s) sum += u = std::exp(u - top);
+        for (int64_t d = 0; d < hd; d++) {
+          double v = 0.0;
+          for (size_t c = 0; c < s.size(); c++) v += s[c] / sum * (double)value[c][d];
+          y[d] = (T)v;
+        }
+      }
+  }
+  const int64_t all = q.pages * q.page * G * hd;
+  for (int r : {1, 2}) {
+    T* out = o.out[(size_t)r];
+    if (!out) continue;
+    const T* from = r == 1 ? kp : vp;
+    if (out != from) std::copy(from, from + all, out);
+    for (int64_t b = 0; b < q.batch; b++)
+      for (int64_t i = 0; i < o.end(b); i++) {
+        const int64_t at = place(b, begin_of(b) + i);
+        if (at < 0) continue;
+        for (int64_t g = 0; g < G; g++) {
+          const T* src = (r == 1 ? ks : vs)(b * L + i, g);
+          std::copy(src, src + hd, out + at + g * hd);
+        }
+      }
+  }
+}
+
+template <class T, class Slot>
+void joint_norm(const rgplan::Instr& in, const Operands<T>& o, Slot slot_bytes) {
+  long double sum = 0.0L;
+  for (auto& a : in.args) {
+    int64_t n = 1;
+    for (int64_t d : a.shape) n *= d;
+    const T* x = (const T*)slot_bytes(a.slot);
+    for (int64_t k = 0; k < n; k++) sum += (long double)x[k] * (long double)x[k];
+  }
+  if (o.out[0]) o.out[0][0] = (T)std::sqrt(sum);
+}
+
 template <class T, class Slot>
 void run(const rgplan::Instr& in, Slot slot_bytes) {
   Operands<T> o{in, rgplan::sequence_of(in), {}, {}};
@@ -239,6 +423,9 @@ void run(const rgplan::Instr& in, Slot slot_bytes) {
   if (!rgplan::is_multi_result(in.op)) o.out[0] = (T*)slot_bytes(in.dst);
   for (auto& r : in.outs) o.out[(size_t)r.first] = (T*)slot_bytes(r.second);
   if (in.op == RG_OP_CAUSAL_CONV || in.op == RG_OP_CAUSAL_CONV_GRAD) causal_conv(o);
+  else if (in.op == RG_OP_ATTENTION || in.op == RG_OP_ATTENTION_GRAD) attention(o);
+  else if (in.op == RG_OP_PAGED_ATTENTION) paged_attention(o);
+  else if (in.op == RG_OP_JOINT_NORM) joint_norm(in, o, slot_bytes);
   else if (in.op == RG_OP_SELECTIVE_SCAN || in.op == RG_OP_SELECTIVE_SCAN_GRAD) selective_scan(o);
   else rotary_norm(o);
 }

@@ -522,6 +522,33 @@ std::vector<std::pair<uint32_t, uint32_t>> vjp_sequence(Graph& g, size_t i, cons
                                                         const std::vector<bool>& rel) {
   const Node node = g.nodes[i];
   const bool conv = node.op.kind == RG_OP_CAUSAL_CONV;
+  if (node.op.kind == RG_OP_ATTENTION) {
+    Op o = node.op;
+    o.kind = RG_OP_ATTENTION_GRAD;
+    std::vector<uint32_t> ins = node.inputs;
+    auto dy = cots.find(0);
+    if (dy == cots.end()) return {};
+    for (uint32_t x : {g.result((uint32_t)i, 0), g.result((uint32_t)i, 1), dy->second}) ins.push_back(x);
+    const rgplan::Sequence q = g.sequence(node.op, node.inputs);
+    const uint32_t grads = g.add(o, ins);
+    std::vector<std::pair<uint32_t, uint32_t>> out;
+    const std::vector<int> operands = {q.x, q.k, q.v, q.slopes};
+    for (size_t k = 0; k < operands.size(); k++)
+      if (operands[k] >= 0 && rel[node.inputs[(size_t)operands[k]]]) out.push_back({node.inputs[(size_t)operands[k]], g.result(grads, k)});
+    return out;
+  }
+  if (node.op.kind == RG_OP_JOINT_NORM) {
+    // x / norm, and 0 where the norm is 0.
+    auto dn = cots.find(0);
+    if (dn == cots.end()) return {};
+    const uint32_t norm = g.result((uint32_t)i, 0), one = g.constant(Tensor::full(node.dtype, {}, 1.0)), none = zeros(g, {}, node.dtype);
+    const uint32_t safe = g.add(Op::make(RG_OP_WHERE), {bin(g, RG_OP_GT, norm, none), norm, one});
+    const uint32_t factor = bin(g, RG_OP_DIV, dn->second, safe);
+    std::vector<std::pair<uint32_t, uint32_t>> out;
+    for (uint32_t x : node.inputs)
+      if (rel[x]) out.push_back({x, bin(g, RG_OP_MUL, x, factor)});
+    return out;
+  }
   if (!conv && node.op.kind != RG_OP_SELECTIVE_SCAN) {
     Json obs = Json::obj();
     obs["operation"] = node.op.name();

@@ -72,6 +72,10 @@ const char* Op::name() const {
     case RG_OP_SELECTIVE_SCAN_GRAD: return "selective_scan_grad";
     case RG_OP_ROTARY_NORM: return "rotary_norm";
     case RG_OP_ROTARY_NORM_GRAD: return "rotary_norm_grad";
+    case RG_OP_ATTENTION: return "attention";
+    case RG_OP_ATTENTION_GRAD: return "attention_grad";
+    case RG_OP_PAGED_ATTENTION: return "paged_attention";
+    case RG_OP_JOINT_NORM: return "joint_norm";
     default: return "unknown";
   }
 }
@@ -694,9 +698,15 @@ void Graph::check_sequence(const Op& op, const std::vector<uint32_t>& inputs) co
   const DType d = dtype(inputs[0]);
   if (d == DType::I32) fail("UNSUPPORTED_DTYPE", "operation_is_float_only_cast_first");
   for (size_t k = 0; k < inputs.size(); k++) {
-    const bool index = (int)k == q.lengths || (int)k == q.positions;
+    const bool index = q.is_index((int)k);
     if (index && dtype(inputs[k]) != DType::I32) fail("DTYPE_MISMATCH", "lengths_and_positions_must_be_int32");
     if (!index && dtype(inputs[k]) != d) fail("DTYPE_MISMATCH", "implicit_promotion_not_allowed");
+  }
+  if (q.keys > 0) {
+    if (!std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)) fail("INVALID_ARGUMENT", "scale_must_be_finite_and_cap_positive");
+    // Scores are divided by the cap and multiplied by it in the dtype.
+    if (d == DType::F32 && op.eps > 0 && !(op.eps >= 1e-30 && op.eps <= 1e30)) fail("INVALID_ARGUMENT", "cap_out_of_the_dtypes_range");
+    if (d == DType::F32 && std::fabs(op.base) > 1e30) fail("INVALID_ARGUMENT", "scale_out_of_the_dtypes_range");
   }
   const bool rotary = op.kind == RG_OP_ROTARY_NORM || op.kind == RG_OP_ROTARY_NORM_GRAD;
   if (rotary && (!(op.base > 0) || !std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)))

@@ -157,6 +157,14 @@ Op parse_op(const std::string& name, const py::object& a) {
     o.turn = attr<size_t>(a, "rotary_dims");
     o.base = attr<double>(a, "base");
     o.eps = attr<double>(a, "eps");
+  } else if (name == "attention" || name == "paged_attention") {
+    o.kind = name == "attention" ? RG_OP_ATTENTION : RG_OP_PAGED_ATTENTION;
+    o.a = attr<size_t>(a, "flags");
+    o.v = attr<Shape>(a, "heads");
+    o.base = attr<double>(a, "scale");
+    o.eps = attr<double>(a, "cap");
+  } else if (name == "joint_norm") {
+    o.kind = RG_OP_JOINT_NORM;
   } else {
     throw py::value_error("unknown op " + name);
   }

@@ -1145,7 +1145,9 @@ Plan build_with(const Graph& g, const std::vector<uint32_t>& outputs, bool reuse
       for (size_t o = i + 1; o < total; o++) {
         const Node& on = g.nodes[o];
         if (keep[o] && on.op.kind == RG_OP_OUTPUT && on.inputs[0] == i) {
-          const size_t sl = a.alloc(on.dtype, on.n(), exact[o]);
+          // Pages with new rows get a buffer of their own, so that a step loop that carries them can
+          // write the rows into the pages where they are.
+          const size_t sl = a.alloc(on.dtype, on.n(), exact[o] || (node.op.kind == RG_OP_PAGED_ATTENTION && on.op.a > 0));
           value_slot[o] = sl;
           in.outs.push_back({on.op.a, sl});
           p.naive_bytes += on.n() * dsize(on.dtype);
@@ -1363,6 +1365,26 @@ StepWork step_work(const Step& s, const PriceFn& price) {
       w.bytes = elems * ds;
       return w;
     }
+    case RG_OP_ATTENTION: case RG_OP_ATTENTION_GRAD: {
+      // Products over the pairs that the order leaves, two forward and five backward; what lengths,
+      // documents and prefixes leave is not known here.
+      std::vector<std::vector<int64_t>> shapes;
+      for (auto& a : i.arg_shapes) shapes.emplace_back(a.begin(), a.end());
+      const rgplan::Sequence q = rgplan::sequence_of(i.op.kind, i.op.sequence_attr(), shapes);
+      const double t = (double)q.length, pairs = (i.op.a & RG_ATTEND_CAUSAL) ? t * (t + 1) / 2 : t * t;
+      w.flops = (i.op.kind == RG_OP_ATTENTION ? 4.0 : 10.0) * (double)(q.batch * q.heads * q.head) * pairs;
+      w.executed_flops = w.flops;
+      w.bytes = in_elems * ds;
+      w.compute = true;
+      return w;
+    }
+    case RG_OP_PAGED_ATTENTION:
+      // The pages once, and the new tokens' operands and results.
+      w.bytes = (in_elems + (double)i.arg_shapes[0][0] * i.arg_shapes[0][1] * i.op.v[0] * i.arg_shapes[0][3]) * ds;
+      return w;
+    case RG_OP_JOINT_NORM:
+      w.bytes = in_elems * ds;
+      return w;
     case RG_OP_ROTARY_NORM_GRAD:
       w.bytes = (in_elems + (double)numel(i.arg_shapes[0])) * ds;
       return w;

@@ -24,6 +24,7 @@
 #include "jit.h"
 #include "kernels.h"
 #include "noalloc.h"
+#include "attend.h"
 #include "sequence.h"
 
 using namespace rgplan;
@@ -723,6 +724,117 @@ StepFn lower_sequence(Program& prog, const Instr& i) {
     a.dz = slot(sl, outs[6]);
     a.dstate = slot(sl, outs[7]);
     rgk::selective_scan_grad(s, dtype, a);
+  };
+}
+
+// An attention operator (attend.hip): with shaped scores, its gradient, or over a paged cache.
+StepFn lower_attend(Program& prog, const Instr& i) {
+  const Sequence q = sequence_of(i);
+  const int dtype = i.dtype;
+  std::vector<int64_t> args, outs(q.results.size(), -1);
+  for (auto& a : i.args) args.push_back(a.slot);
+  for (auto& o : i.outs) outs[(size_t)o.first] = o.second;
+  auto arg = [args](void* const* sl, int k) { return k < 0 ? nullptr : sl[args[(size_t)k]]; };
+  auto out = [outs](void* const* sl, size_t r) { return outs[r] < 0 ? nullptr : sl[outs[r]]; };
+  const bool paged = i.op == RG_OP_PAGED_ATTENTION, grad = i.op == RG_OP_ATTENTION_GRAD;
+  rgk::AttendArgs base{};
+  base.joined = q.k < 0;
+  const uint64_t positions = (uint64_t)q.batch * q.length, stride = (uint64_t)q.heads + (base.joined ? 2 * q.keys : 0);
+  if (positions >= (1ull << 31) || stride * q.head >= (1ull << 31) || (uint64_t)q.pages * q.page >= (1ull << 31))
+    throw std::runtime_error("an attention of 2^31 positions or values a position exceeds the index range");
+  base.batch = (uint32_t)q.batch;
+  base.length = (uint32_t)q.length;
+  base.heads = (uint32_t)q.heads;
+  base.keys = (uint32_t)q.keys;
+  base.head = (uint32_t)q.head;
+  base.causal = (i.sequence.flags & RG_ATTEND_CAUSAL) != 0;
+  base.scale = i.sequence.base;
+  base.cap = i.sequence.eps;
+  base.pages = (uint32_t)q.pages;
+  base.page = (uint32_t)q.page;
+  base.table_pages = (uint32_t)q.table_pages;
+  const uint64_t blocks = paged ? rgk::paged_blocks(dtype, base) : rgk::attend_blocks(dtype, base);
+  if (blocks >= rgk::ATTEND_BLOCKS) throw std::runtime_error("an attention of " + std::to_string(blocks) + " blocks exceeds the launch limit");
+  if (paged) prog.workspace_bytes = std::max(prog.workspace_bytes, rgk::paged_workspace(dtype, base));
+  if (grad) prog.workspace_bytes = std::max(prog.workspace_bytes, rgk::attend_workspace(dtype, base));
+  int64_t slopes = -1;
+  if (grad && outs[3] >= 0) {
+    slopes = (int64_t)prog.fold_bytes;
+    Program::Fold fd{prog.fold_bytes, outs[3], rgk::attend_slope_rows(dtype, base), base.heads, RG_REDUCE_SUM, dtype};
+    prog.folds.push_back(fd);
+    prog.fold_bytes += ((uint64_t)fd.rows * fd.k * esize(dtype) + 255) / 256 * 256;
+  }
+  const Program* pp = &prog;
+  const uint64_t after_q = (uint64_t)q.heads * q.head * esize(dtype), after_k = after_q + (uint64_t)q.keys * q.head * esize(dtype);
+  return [=](hipStream_t s, void* const* sl, void* ws) {
+    rgk::AttendArgs a = base;
+    a.q = arg(sl, q.x);
+    a.k = base.joined ? (const char*)a.q + after_q : arg(sl, q.k);
+    a.v = base.joined ? (const char*)a.q + after_k : arg(sl, q.v);
+    a.slopes = arg(sl, q.slopes);
+    a.documents = (const int32_t*)arg(sl, q.documents);
+    a.prefix = (const int32_t*)arg(sl, q.prefix);
+    a.lengths = (const int32_t*)arg(sl, q.lengths);
+    a.workspace = ws;
+    if (paged) {
+      a.k_pages = arg(sl, q.k_pages);
+      a.v_pages = arg(sl, q.v_pages);
+      a.table = (const int32_t*)arg(sl, q.table);
+      a.first = (const int32_t*)arg(sl, q.first);
+      a.y = out(sl, 0);
+      a.k_out = out(sl, 1);
+      a.v_out = out(sl, 2);
+      rgk::paged_attend(s, dtype, a);
+      return;
+    }
+    if (!grad) {
+      a.y = out(sl, 0);
+      a.sums = out(sl, 1);
+      rgk::attend(s, dtype, a);
+      return;
+    }
+    a.y_in = arg(sl, q.y);
+    a.sums_in = arg(sl, q.sums);
+    a.dy = arg(sl, q.dy);
+    a.dq = out(sl, 0);
+    a.dk = base.joined ? (a.dq ? (char*)a.dq + after_q : nullptr) : out(sl, 1);
+    a.dv = base.joined ? (a.dq ? (char*)a.dq + after_k : nullptr) : out(sl, 2);
+    a.dslopes_rows = slopes < 0 ? nullptr : (char*)ws + pp->fold_base() + slopes;
+    rgk::attend_grad(s, dtype, a);
+  };
+}
+
+// The joint norm of many tensors (attend.hip): each launch sums the squares of up to NORM_TENSORS.
+StepFn lower_norm(Program& prog, const Instr& i) {
+  const int dtype = i.dtype;
+  struct Launch {
+    rgk::NormTensors t;
+    std::vector<int64_t> slots;
+    uint32_t blocks, from;
+  };
+  std::vector<Launch> launches;
+  uint64_t all = 0;
+  for (const auto& a : i.args) {
+    if (launches.empty() || launches.back().t.count == rgk::NORM_TENSORS) launches.push_back({{}, {}, 0, (uint32_t)all});
+    Launch& l = launches.back();
+    const uint64_t n = prod(a.shape), blocks = rgk::norm_blocks(n);
+    all += blocks;
+    if (all >= rgk::ATTEND_BLOCKS) throw std::runtime_error("a norm of " + std::to_string(all) + " blocks exceeds the launch limit");
+    l.t.n[l.t.count] = n;
+    l.t.first_block[l.t.count++] = l.blocks;
+    l.slots.push_back(a.slot);
+    l.blocks += (uint32_t)blocks;
+  }
+  prog.workspace_bytes = std::max(prog.workspace_bytes, all * 8);
+  const int64_t dst = i.outs.empty() ? -1 : i.outs[0].second;
+  return [=](hipStream_t s, void* const* sl, void* ws) {
+    if (dst < 0) return;
+    for (const Launch& l : launches) {
+      rgk::NormTensors t = l.t;
+      for (uint32_t k = 0; k < t.count; k++) t.x[k] = sl[l.slots[k]];
+      rgk::norm_squares(s, dtype, t, l.blocks, (double*)ws + l.from);
+    }
+    rgk::norm_root(s, dtype, (const double*)ws, (uint32_t)all, sl[dst]);
   };
 }
 
@@ -1537,6 +1649,10 @@ void build_program(Program& prog) {
         const bool ta = in.op == RG_OP_MATMUL_T && in.attr[0] != 0, tb = in.op == RG_OP_MATMUL_T && in.attr[1] != 0;
         gemm_fills[k] = gemm_fill(prog, in, ta, tb, &gemm_base[k]);
         prog.steps.push_back(gemm_step(gemm_fills[k]));
+      } else if (in.op == RG_OP_JOINT_NORM) {
+        prog.steps.push_back(lower_norm(prog, in));
+      } else if (in.op == RG_OP_ATTENTION || in.op == RG_OP_ATTENTION_GRAD || in.op == RG_OP_PAGED_ATTENTION) {
+        prog.steps.push_back(lower_attend(prog, in));
       } else if (is_sequence(in.op)) {
         prog.steps.push_back(lower_sequence(prog, in));
       } else {

@@ -11,6 +11,7 @@ import typing
 
 from . import tree
 from .ops import cos, full, maximum, minimum, where, zeros_like
+from .sequence import _with_results
 
 
 class Optimizer(typing.NamedTuple):
@@ -52,6 +53,26 @@ def clip_by_global_norm(grads, max_norm):
     total = tree.global_norm(grads)
     factor = max_norm / where(total >= max_norm, total, max_norm)
     return tree.map(lambda g: g * factor, grads)
+
+
+def gradient_norm(grads):
+    """The joint L2 norm of all leaves of `grads`, of one floating-point dtype: one operator over all
+    of them, whose squares are summed in 64 bits. Its gradient is 0 where the norm is."""
+    values = tree.leaves(grads)
+    if not values:
+        raise ValueError("a tree without leaves has no norm")
+    return _with_results("joint_norm", values, {}, 1)[0]
+
+
+def clip_gradients(grads, max_norm):
+    """`(clipped, norm)`: `grads` scaled so that their joint L2 norm is at most `max_norm`, and the norm
+    they had, to be watched. They pass unchanged where it is smaller. Where it
+    is infinite, finite gradients become 0 and infinite ones NaN; where it is NaN all do."""
+    if isinstance(max_norm, (int, float)) and not max_norm > 0:
+        raise ValueError(f"a norm of at most {max_norm}: it must be positive")
+    norm = gradient_norm(grads)
+    factor = max_norm / maximum(norm, max_norm)
+    return tree.map(lambda g: g * factor, grads), norm
 
 
 def _prepare(grads, max_grad_norm):
