@@ -10,8 +10,9 @@
 // No score is kept: the forward walks the keys once with a running maximum and sum, and leaves the
 // logarithm of each query's sum, from which the backward forms p again.
 //
-// A block of four waves takes 64 rows (queries, or keys where the gradients of k and v are formed),
-// a wave 16 of them, and the other side passes through LDS in tiles of 32. Products run on the
+// A block takes 64 rows (queries, or keys where the gradients of k and v are formed), a wave 16 of
+// them, and the other side passes through LDS, 32 rows at a time for each set of four waves: with
+// two sets a block walks two such tiles at once and joins its halves at the end. Products run on the
 // 16x16x4 matrix instructions of the type. A score tile is formed so that a lane holds one of its
 // wave's rows and four of the other side's, and feeds the next product from where it lies: that
 // product's four steps each take, from every lane, the value of one register, and the other
@@ -48,16 +49,26 @@ struct Type<float> {
   static __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
   static __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
   static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
-  // Below 0.7 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 + ...)), off
-  // by 2e-9 of it there; from there on (e^2x - 1) / (e^2x + 1). One division for either.
-  static __device__ __forceinline__ float tanh_of(float x) {
-    const float a = fminf(fabsf(x), 16.0f), z = a * a;
-    const float e = __builtin_amdgcn_exp2f(2.8853900817779268f * a);
-    const bool low = a < 0.7f;
-    const float num = low ? a * fmaf(z, z + 105.0f, 945.0f) : e - 1.0f, den = low ? fmaf(z, fmaf(15.0f, z, 420.0f), 945.0f) : e + 1.0f;
-    const float r = __builtin_amdgcn_rcpf(den), q = num * r;
-    return x != x ? x : copysignf(fmaf(fmaf(-den, q, num), r, q), x);
+  // tanh of up to 1 in size: x + x^3 q(x^2), q the polynomial whose largest relative error over
+  // that range is least (4e-9, 1.6 units of 2^-24 with the roundings).
+  static __device__ __forceinline__ float tanh_low(float x) {
+    const float z = x * x;
+    float q = -3.5334553103893995e-4f;
+    q = fmaf(q, z, 2.282229484990239e-3f);
+    q = fmaf(q, z, -7.917444221675396e-3f);
+    q = fmaf(q, z, 2.1464820951223373e-2f);
+    q = fmaf(q, z, -5.387091264128685e-2f);
+    q = fmaf(q, z, 1.333215981721878e-1f);
+    q = fmaf(q, z, -3.333327770233154e-1f);
+    return fmaf(q, x * z, x);
   }
+  // Of any size: past 1, (e^2x - 1) / (e^2x + 1).
+  static __device__ __forceinline__ float tanh_of(float x) {
+    const float a = fminf(fabsf(x), 16.0f), e = __builtin_amdgcn_exp2f(2.8853900817779268f * a), num = e - 1.0f, den = e + 1.0f;
+    const float r = __builtin_amdgcn_rcpf(den), q = num * r, t = fmaf(fmaf(-den, q, num), r, q);
+    return fabsf(x) > 1.0f ? copysignf(t, x) : tanh_low(x);
+  }
+  static constexpr bool LOW = true;
 };
 template <>
 struct Type<double> {
@@ -69,7 +80,9 @@ struct Type<double> {
   static __device__ __forceinline__ double exp2_of(double x) { return exp2(x); }
   static __device__ __forceinline__ double log2_of(double x) { return log2(x); }
   static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+  static __device__ __forceinline__ double tanh_low(double x) { return tanh(x); }
   static __device__ __forceinline__ double tanh_of(double x) { return tanh(x); }
+  static constexpr bool LOW = false;
 };
 
 // Over the four lanes that hold one row (l, l + 16, l + 32, l + 48), the same in all of them.
@@ -88,7 +101,17 @@ __device__ __forceinline__ T row_sum(T x) {
   return a + b;
 }
 
-constexpr int ROWS = 64, TILE = 32, NT = 256;  // rows of a block, rows of a tile, threads
+constexpr int ROWS = 64, TILE = 32;  // rows of a block, rows of a wave's tile
+
+// Sets of four waves in a block, and rows of the other side that they stage at once. Two sets where
+// their registers (256 a lane) hold the fragments and results; one for wider heads.
+template <class T, int HD>
+struct Geo {
+  static constexpr int SETS = (int)sizeof(T) * HD <= 512 ? 2 : 1, NT = 256 * SETS, STAGE = TILE * SETS;
+  // Waves a SIMD that the registers are to leave room for.
+  static constexpr int WAVES = (int)sizeof(T) * HD <= 256 && sizeof(T) == 4 ? 4 : (int)sizeof(T) * HD <= 512 ? 2 : 1;
+  static constexpr int GRAD_WAVES = (int)sizeof(T) * HD <= 128 ? 4 : (int)sizeof(T) * HD <= 512 ? 2 : 1;
+};
 
 // Rows of HD values in LDS lie 16 bytes further apart than that: 16 lanes reading 16 bytes of 16
 // rows each reach every bank once.
@@ -177,43 +200,83 @@ __device__ __forceinline__ void weigh(const T* lds, int l16, int g, const typena
     }
 }
 
-// The lane's share of its row of a result, times `by`.
+// The lane's share of its row of a result, times `by`; 0 where there is none.
 template <class T, int HD>
-__device__ __forceinline__ void put_row(T* row, int g, uint32_t head, const typename Type<T>::acc* acc, T by) {
+__device__ __forceinline__ void put_row(T* row, int g, uint32_t head, const typename Type<T>::acc* acc, T by, bool none) {
   constexpr int ND = HD / 16;
 #pragma unroll
   for (int r = 0; r < 4; r++)
 #pragma unroll
     for (int n = 0; n < ND; n++) {
       const uint32_t d = (uint32_t)(Type<T>::row_of(r, g) * ND + n);
-      if (d < head) row[d] = acc[n][r] * by;
+      if (d < head) row[d] = none ? (T)0 : acc[n][r] * by;
     }
+}
+
+// Positions from 0 of the tile rows that a lane's scores [t][r] belong to.
+template <class T>
+__device__ __forceinline__ constexpr int tile_row(int t, int r) {
+  return 16 * t + Type<T>::row_of(r, 0);
 }
 
 // The scores of one head, to base 2: cap log2(e) tanh(dot mul) or dot mul, less slope log2(e) times
 // the distance.
 template <class T>
 struct Scorer {
+  typedef typename Type<T>::acc acc;
   T mul, cap, slope;  // cap and slope times log2(e)
-  bool capped;
+  bool capped, sloped;
   __device__ __forceinline__ Scorer(const AttendArgs& a, uint32_t h) {
     constexpr double LOG2E = 1.4426950408889634;
     capped = a.cap > 0;
+    sloped = a.slopes != nullptr;
     mul = (T)(capped ? a.scale / a.cap : a.scale * LOG2E);
     cap = (T)(a.cap * LOG2E);
-    slope = a.slopes ? (T)((double)((const T*)a.slopes)[h] * LOG2E) : (T)0;
+    slope = sloped ? (T)((double)((const T*)a.slopes)[h] * LOG2E) : (T)0;
   }
-  // The score, and the slope of the cap there (1 without one).
-  __device__ __forceinline__ T operator()(T dot, int distance, T* bend) const {
-    T s = dot * mul;
-    *bend = 1;
+  // Makes scores of dot products, and leaves the tanh of each (0 without a cap) where asked to.
+  // `apart` is the signed distance between the lane's row and row row_of(0, g) of the tile.
+  template <bool TANH>
+  __device__ __forceinline__ void operator()(acc* s, acc* bent, int apart) const {
+#pragma unroll
+    for (int t = 0; t < 2; t++) s[t] *= mul;
     if (capped) {
-      const T t = Type<T>::tanh_of(s);
-      *bend = 1 - t * t;
-      s = cap * t;
+      // Scores far below the cap, as most are, take the short form.
+      bool high = !Type<T>::LOW;
+      if constexpr (Type<T>::LOW) {
+        T most = 0;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) most = Type<T>::max_of(most, s[t][r] < 0 ? -s[t][r] : s[t][r]);
+        high = __ballot(most > 1) != 0;
+      }
+      if (high) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[t][r] = Type<T>::tanh_of(s[t][r]);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[t][r] = Type<T>::tanh_low(s[t][r]);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        if (TANH) bent[t] = s[t];
+        s[t] *= cap;
+      }
     }
-    return s - slope * (T)distance;
+    if (sloped) {
+      const T d = (T)apart;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[t][r] -= slope * abs_of(d - (T)tile_row<T>(t, r));
+    }
   }
+  static __device__ __forceinline__ T abs_of(T x) { return x < 0 ? -x : x; }
 };
 
 // The sequence of a batch that a block works in: its positions, which of them belong to it, and
@@ -231,88 +294,176 @@ struct Sight {
   __device__ __forceinline__ int document(int i) const { return i >= length ? -1 : documents ? documents[i] : 0; }
   // With the documents of both at hand; those of no sequence are negative.
   __device__ __forceinline__ bool sees(int i, int di, int j, int dj) const { return di >= 0 && di == dj && (!causal || j <= i || j < prefix); }
+  // Whether every query from i on that there is sees every key of [j, end).
+  __device__ __forceinline__ bool all_see(int i, int end) const { return !documents && end <= length && (!causal || end - 1 <= i || end <= prefix); }
   // Keys [0, this) hold every one that a query before `end` sees.
   __device__ __forceinline__ int keys_to(int end) const { return min(causal ? max(end, prefix) : length, length); }
   // Queries [this, length) hold every one that sees a key from j on.
   __device__ __forceinline__ int queries_from(int j) const { return causal && j >= prefix ? j : 0; }
 };
 
-// One tile of `TILE` rows of two operands on its way to LDS: 16 bytes a thread and step.
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) x = min(x, __shfl_xor(x, o));
+  return x;
+}
+
+// The stages of the other side, [from, end) of them, that may hold a position of the documents of a
+// block's rows; all of them without documents. Every thread of the block calls it alike.
+template <int STAGE, int NT>
+struct Stages {
+  const Sight& sight;
+  int low, high;  // documents of the rows
+  int from, end;
+  int chunk = -1;  // of 64 stages
+  uint64_t live = 0;
+  uint64_t* shared;
+  static constexpr int WAVES = NT / 64;
+  __device__ __forceinline__ Stages(const Sight& s, int rows, int from_, int end_, uint64_t* shared_) : sight(s), from(from_), end(end_), shared(shared_) {
+    if (!sight.documents) return;
+    const int d = sight.document(rows + (int)(threadIdx.x & 63));
+    low = wave_min(d < 0 ? 0x7fffffff : d);
+    high = -wave_min(-max(d, -1));
+  }
+  // Each wave looks at every WAVES-th stage of the chunk; a wave's lanes take its positions.
+  __device__ __forceinline__ void look(int c) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint64_t mine = 0;
+    for (int k = wave; k < 64; k += WAVES) {
+      const int first = (c * 64 + k) * STAGE;
+      if (c * 64 + k < from || c * 64 + k >= end) continue;
+      int least = 0x7fffffff, most = -1;
+      for (int p = lane; p < STAGE; p += 64) {
+        const int d = sight.document(first + p);
+        least = min(least, d < 0 ? 0x7fffffff : d);
+        most = max(most, d);
+      }
+      if (wave_min(least) <= high && -wave_min(-most) >= low) mine |= 1ull << k;
+    }
+    __syncthreads();
+    if (lane == 0) shared[wave] = mine;
+    __syncthreads();
+    live = 0;
+    for (int w = 0; w < WAVES; w++) live |= shared[w];
+    chunk = c;
+  }
+  // The first live stage from k on, or `end`.
+  __device__ __forceinline__ int at(int k) {
+    if (!sight.documents) return min(k, end);
+    while (k < end) {
+      if (k / 64 != chunk) look(k / 64);
+      const uint64_t left = live >> (k % 64);
+      if (left) return k + __builtin_ctzll(left);
+      k = (k / 64 + 1) * 64;
+    }
+    return end;
+  }
+};
+
+// Rows of the other side on their way to LDS, of two operands, 16 bytes a thread and step. Loads
+// are of rows and columns that there are; what does not belong is made 0 as it is stored.
 template <class T, int HD>
 struct Staged {
-  static constexpr int PER = TILE * HD / Type<T>::V / NT > 0 ? TILE * HD / Type<T>::V / NT : 1;
-  static constexpr bool ALL = TILE * HD / Type<T>::V >= NT;
+  static constexpr int V = Type<T>::V, NT = Geo<T, HD>::NT, PER = Geo<T, HD>::STAGE * HD / V / NT;
+  static_assert(PER * NT * V == Geo<T, HD>::STAGE * HD, "whole steps");
   typedef typename Type<T>::vec vec;
   vec x[PER], y[PER];
-  // `rows(r)` gives the pointers of row r of the two operands, null where there is none.
+  uint32_t off;  // bit i: step i is not there
+  static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * NT) / (HD / V); }
+  static __device__ __forceinline__ uint32_t column(int i) { return (uint32_t)(((int)threadIdx.x + i * NT) % (HD / V)) * V; }
+  // `rows(r)` gives row r's place in both operands and whether it is there; the places of rows that
+  // are not may be any that can be read.
   template <class R>
-  __device__ __forceinline__ void load(const R& rows, uint32_t head, bool whole) {
+  __device__ __forceinline__ void load(const T* xs, const T* ys, const R& rows, uint32_t head, bool whole) {
+    off = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const int at = (int)threadIdx.x + i * NT;
-      if (!ALL && at >= TILE * HD / Type<T>::V) continue;
-      const auto p = rows(at / (HD / Type<T>::V));
-      const uint32_t d = (uint32_t)(at % (HD / Type<T>::V)) * Type<T>::V;
-      x[i] = row_vec(p.x, d, head, whole);
-      y[i] = row_vec(p.y, d, head, whole);
+      const auto p = rows(row(i));
+      const uint32_t c = column(i);
+      if (whole) {
+        const uint32_t d = c < head ? c : 0;
+        x[i] = *(const vec*)(xs + p.x + d);
+        y[i] = *(const vec*)(ys + p.y + d);
+        if (!p.there || c >= head) off |= 1u << i;
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++) {
+          const uint32_t d = c + j < head ? c + j : 0;
+          const T u = xs[p.x + d], v = ys[p.y + d];
+          x[i][j] = c + j < head ? u : (T)0;
+          y[i][j] = c + j < head ? v : (T)0;
+        }
+        if (!p.there) off |= 1u << i;
+      }
     }
   }
   __device__ __forceinline__ void store(T* xs, T* ys) const {
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const int at = (int)threadIdx.x + i * NT;
-      if (!ALL && at >= TILE * HD / Type<T>::V) continue;
-      const int o = at / (HD / Type<T>::V) * PITCH<T, HD> + at % (HD / Type<T>::V) * Type<T>::V;
-      *(vec*)(xs + o) = x[i];
-      *(vec*)(ys + o) = y[i];
+      const int o = row(i) * PITCH<T, HD> + (int)column(i);
+      const bool none = off >> i & 1;
+      vec u = x[i], v = y[i];
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        u[j] = none ? (T)0 : u[j];
+        v[j] = none ? (T)0 : v[j];
+      }
+      *(vec*)(xs + o) = u;
+      *(vec*)(ys + o) = v;
     }
   }
 };
-template <class T>
-struct RowPair {
-  const T *x, *y;
+struct RowAt {
+  int64_t x, y;
+  bool there;
 };
 
-// Block `blockIdx.x`'s head and tile of rows: the heads of a batch next to each other, so that blocks
-// of one head meet in the same L2 where their number is a multiple of the eight dies, and the tiles
-// with the most work under a causal order first (`last_first`).
+// A block's head and tile of rows: the heads of a batch next to each other, so that blocks of one
+// head meet in the same L2 where their number is a multiple of the eight dies, and the tiles with the
+// most work under a causal order first (`last_first`).
 struct Place {
   uint32_t b, h, tile;
-  __device__ __forceinline__ Place(uint32_t batch, uint32_t heads, uint32_t tiles, bool last_first) {
-    const uint32_t bh = blockIdx.x % (batch * heads), at = blockIdx.x / (batch * heads);
+  __device__ __forceinline__ Place(uint32_t at, uint32_t batch, uint32_t heads, uint32_t tiles, bool last_first) {
+    const uint32_t bh = at % (batch * heads), n = at / (batch * heads);
     b = bh / heads;
     h = bh % heads;
-    tile = last_first ? tiles - 1 - at : at;
+    tile = last_first ? tiles - 1 - n : n;
   }
 };
 
-// The running softmax of a row over its keys: maximum, sum (of the lane's own keys until the end)
-// and weighed values.
+// The running softmax of a row over its keys: a bound that its scores stay near, the sum (of the
+// lane's own keys until the end) and the weighed values. The bound is the largest score when it was
+// last moved; it moves once a score is more than 2^8 times as heavy, and then what there is is scaled.
 template <class T, int HD>
 struct Running {
-  typename Type<T>::acc out[HD / 16];
+  typedef typename Type<T>::acc acc;
+  acc out[HD / 16];
   T top = -(T)__builtin_huge_val(), sum = 0;
   __device__ __forceinline__ Running() {
 #pragma unroll
-    for (int n = 0; n < HD / 16; n++) out[n] = typename Type<T>::acc{0, 0, 0, 0};
+    for (int n = 0; n < HD / 16; n++) out[n] = acc{0, 0, 0, 0};
   }
+  __device__ __forceinline__ void scale(T by) {
+    sum *= by;
+#pragma unroll
+    for (int n = 0; n < HD / 16; n++) out[n] *= by;
+  }
+  // What the bound is to scores: a row that has seen nothing keeps weights of 0.
+  static __device__ __forceinline__ T base(T top) { return top == -(T)__builtin_huge_val() ? (T)0 : top; }
   // Takes in two tiles of scores, minus infinity where a key is not seen, and leaves their weights.
-  __device__ __forceinline__ void add(typename Type<T>::acc* s) {
-    T high = s[0][0];
+  __device__ __forceinline__ void add(acc* s) {
+    T most = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) high = Type<T>::max_of(high, s[t][r]);
-    const T next = Type<T>::max_of(top, row_max(high));
-    // A row that has seen nothing keeps weights of 0.
-    const T at = next == -(T)__builtin_huge_val() ? (T)0 : next;
-    if (__ballot(next != top) != 0) {
-      const T by = Type<T>::exp2_of(top - at);
-      sum *= by;
-#pragma unroll
-      for (int n = 0; n < HD / 16; n++) out[n] *= by;
+      for (int r = 0; r < 4; r++) most = Type<T>::max_of(most, s[t][r]);
+    most = row_max(most);
+    if (__ballot(most > top + 8) != 0) {
+      const T next = Type<T>::max_of(top, most);
+      scale(Type<T>::exp2_of(top - base(next)));
       top = next;
     }
+    const T at = base(top);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -323,209 +474,357 @@ struct Running {
   }
 };
 
+// Set 1's share of a lane's results, added to set 0's through LDS; `buffer` holds 64 HD values.
 template <class T, int HD>
-__global__ void __launch_bounds__(NT) k_attend(AttendArgs a) {
-  __shared__ __align__(16) T ks[TILE * PITCH<T, HD>];
-  __shared__ __align__(16) T vs[TILE * PITCH<T, HD>];
-  __shared__ int docs[TILE];
-  const Place at(a.batch, a.heads, a.tiles, a.causal);
+__device__ __forceinline__ void join(typename Type<T>::acc* out, T* buffer, int set) {
+  const int at = (int)threadIdx.x & 255;
+  __syncthreads();
+  if (set == 1)
+#pragma unroll
+    for (int n = 0; n < HD / 16; n++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) buffer[(n * 4 + r) * 256 + at] = out[n][r];
+  __syncthreads();
+  if (set == 0)
+#pragma unroll
+    for (int n = 0; n < HD / 16; n++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) out[n][r] += buffer[(n * 4 + r) * 256 + at];
+}
+// The same of running softmaxes: afterwards set 0 has the whole.
+template <class T, int HD>
+__device__ __forceinline__ void join(Running<T, HD>& run, T* buffer, T* tops, T* sums, int set) {
+  tops[threadIdx.x] = run.top;
+  sums[threadIdx.x] = run.sum;
+  __syncthreads();
+  const T other = tops[threadIdx.x ^ 256], top = Type<T>::max_of(run.top, other), base = Running<T, HD>::base(top);
+  run.scale(Type<T>::exp2_of(run.top - base));
+  run.sum += sums[threadIdx.x ^ 256] * Type<T>::exp2_of(other - base);
+  run.top = top;
+  join<T, HD>(run.out, buffer, set);
+}
+
+// A query's share in its 64: set, row and the wave's first row.
+struct Lane {
+  int l16, g, set, row, first;
+  __device__ __forceinline__ Lane() {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    l16 = lane & 15;
+    g = lane >> 4;
+    set = wave >> 2;
+    first = (wave & 3) * 16;
+    row = first + l16;
+  }
+};
+
+template <class T, int HD>
+__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_attend(AttendArgs a) {
+  typedef typename Type<T>::acc acc;
+  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) int docs[STAGE];
+  __shared__ T tops[SETS == 2 ? 512 : 1], sums[SETS == 2 ? 512 : 1];
+  __shared__ uint64_t found[NT / 64];
+  T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
+  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal);
   const Sight sight(a, at.b);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int begin = (int)at.tile * ROWS, i = begin + (int)(threadIdx.x >> 6) * 16 + l16;
+  const Lane l;
+  const int begin = (int)at.tile * ROWS, i = begin + l.row, i0 = begin + l.first;
   const uint32_t kh = at.h / (a.heads / a.keys);
   const bool whole = a.head % Type<T>::V == 0;
   const Scorer<T> scorer(a, at.h);
   const int di = sight.document(i);
   T frag[HD / 4];
-  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, g, a.head, whole, frag);
+  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, l.g, a.head, whole, frag);
   const T *kb = (const T*)a.k + (int64_t)at.b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)at.b * a.length * a.k_row + kh * a.head;
   const int end = begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
+  const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
+  Stages<STAGE, NT> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
   Running<T, HD> run;
   Staged<T, HD> next;
-  auto load = [&](int first) {
-    next.load([&](int r) {
-      const bool in = sight.document(first + r) >= 0;
-      const int64_t o = (int64_t)(first + r) * a.k_row;
-      return RowPair<T>{in ? kb + o : nullptr, in ? vb + o : nullptr};
+  int doc = 0;
+  auto load = [&](int stage) {
+    const int first = stage * STAGE;
+    next.load(kb, vb, [&](int r) {
+      const int j = min(first + r, sight.length - 1);
+      const bool in = first + r < sight.length && (!sight.documents || sight.documents[j] >= 0);
+      return RowAt{j * a.k_row, j * a.k_row, in};
     }, a.head, whole);
+    if (threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
   };
-  if (end > 0) load(0);
-  for (int first = 0; first < end; first += TILE) {
+  int k = stages.at(0);
+  if (k < stages.end) load(k);
+  while (k < stages.end) {
     __syncthreads();
     next.store(ks, vs);
-    if (threadIdx.x < TILE) docs[threadIdx.x] = sight.document(first + (int)threadIdx.x);
+    if (threadIdx.x < STAGE) docs[threadIdx.x] = doc;
     __syncthreads();
-    if (first + TILE < end) load(first + TILE);
-    typename Type<T>::acc s[2];
-    score<T, HD>(ks, l16, g, frag, s);
+    const int here = k, first = here * STAGE + l.set * TILE;
+    k = stages.at(here + 1);
+    if (k < stages.end) load(k);
+    if (first >= seen_to) continue;
+    acc s[2];
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    scorer.template operator()<false>(s, nullptr, i - (first + Type<T>::row_of(0, l.g)));
+    if (!sight.all_see(i0, first + TILE)) {
 #pragma unroll
-    for (int t = 0; t < 2; t++)
+      for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int row = t * 16 + Type<T>::row_of(r, g), j = first + row;
-        T bend;
-        const T v = scorer(s[t][r], abs(i - j), &bend);
-        s[t][r] = sight.sees(i, di, j, docs[row]) ? v : -(T)__builtin_huge_val();
-      }
+        for (int r = 0; r < 4; r++) {
+          const int row = 16 * t + Type<T>::row_of(r, l.g);
+          s[t][r] = sight.sees(i, di, first + row, docs[l.set * TILE + row]) ? s[t][r] : -(T)__builtin_huge_val();
+        }
+    }
     run.add(s);
-    weigh<T, HD>(vs, l16, g, s, run.out);
+    weigh<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, run.out);
   }
-  const T sum = row_sum(run.sum);
-  if (i >= (int)a.length) return;
+  run.sum = row_sum(run.sum);
+  if constexpr (SETS == 2) join(run, smem, tops, sums, l.set);
+  if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h;
-  const bool none = sum == 0;
-  if (a.y) put_row<T, HD>((T*)a.y + row * a.head, g, a.head, run.out, none ? (T)0 : 1 / sum);
+  const bool none = run.sum == 0 || di < 0;
+  if (a.y) put_row<T, HD>((T*)a.y + row * a.head, l.g, a.head, run.out, 1 / run.sum, none);
   // Of a query that sees nothing infinity, so that the backward forms weights of 0.
-  if (a.sums && g == 0) ((T*)a.sums)[((uint64_t)at.b * a.heads + at.h) * a.length + i] = none ? (T)__builtin_huge_val() : run.top + Type<T>::log2_of(sum);
+  if (a.sums && l.g == 0)
+    ((T*)a.sums)[((uint64_t)at.b * a.heads + at.h) * a.length + i] = none ? (T)__builtin_huge_val() : run.top + Type<T>::log2_of(run.sum);
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others.
 template <class T, int HD>
-__global__ void __launch_bounds__(NT) k_attend_dq(AttendArgs a) {
-  __shared__ __align__(16) T ks[TILE * PITCH<T, HD>];
-  __shared__ __align__(16) T vs[TILE * PITCH<T, HD>];
-  __shared__ int docs[TILE];
+__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_attend_dq(AttendArgs a) {
+  typedef typename Type<T>::acc acc;
+  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) int docs[STAGE];
   __shared__ T waves[NT / 64];
-  const Place at(a.batch, a.heads, a.tiles, a.causal);
+  __shared__ uint64_t found[NT / 64];
+  T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
+  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal);
   const Sight sight(a, at.b);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int begin = (int)at.tile * ROWS, i = begin + (int)(threadIdx.x >> 6) * 16 + l16;
+  const Lane l;
+  const int begin = (int)at.tile * ROWS, i = begin + l.row, i0 = begin + l.first;
   const uint32_t kh = at.h / (a.heads / a.keys);
   const bool whole = a.head % Type<T>::V == 0;
   const Scorer<T> scorer(a, at.h);
   const int di = sight.document(i);
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h, stat = ((uint64_t)at.b * a.heads + at.h) * a.length + i;
   T frag[HD / 4], grad[HD / 4];
-  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, g, a.head, whole, frag);
-  row_frag<T, HD>(di >= 0 ? (const T*)a.dy + row * a.head : nullptr, g, a.head, whole, grad);
+  row_frag<T, HD>(di >= 0 ? (const T*)a.dy + row * a.head : nullptr, l.g, a.head, whole, grad);
   T dot = 0;
   {
     T y[HD / 4];
-    row_frag<T, HD>(di >= 0 ? (const T*)a.y_in + row * a.head : nullptr, g, a.head, whole, y);
+    row_frag<T, HD>(di >= 0 ? (const T*)a.y_in + row * a.head : nullptr, l.g, a.head, whole, y);
 #pragma unroll
     for (int n = 0; n < HD / 4; n++) dot += y[n] * grad[n];
   }
+  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, l.g, a.head, whole, frag);
   dot = row_sum(dot);
   const T sums = di >= 0 ? ((const T*)a.sums_in)[stat] : (T)__builtin_huge_val();
-  if (g == 0 && i < (int)a.length) ((T*)a.workspace)[stat] = dot;
+  if (l.set == 0 && l.g == 0 && i < (int)a.length) ((T*)a.workspace)[stat] = dot;
   const T *kb = (const T*)a.k + (int64_t)at.b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)at.b * a.length * a.k_row + kh * a.head;
-  const int end = begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
-  typename Type<T>::acc out[HD / 16];
+  const int end = (a.dq || a.dslopes_rows) && begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
+  const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
+  Stages<STAGE, NT> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
+  acc out[HD / 16];
 #pragma unroll
-  for (int n = 0; n < HD / 16; n++) out[n] = typename Type<T>::acc{0, 0, 0, 0};
+  for (int n = 0; n < HD / 16; n++) out[n] = acc{0, 0, 0, 0};
   T dslope = 0;
   Staged<T, HD> next;
-  auto load = [&](int first) {
-    next.load([&](int r) {
-      const bool in = sight.document(first + r) >= 0;
-      const int64_t o = (int64_t)(first + r) * a.k_row;
-      return RowPair<T>{in ? kb + o : nullptr, in ? vb + o : nullptr};
+  int doc = 0;
+  auto load = [&](int stage) {
+    const int first = stage * STAGE;
+    next.load(kb, vb, [&](int r) {
+      const int j = min(first + r, sight.length - 1);
+      const bool in = first + r < sight.length && (!sight.documents || sight.documents[j] >= 0);
+      return RowAt{j * a.k_row, j * a.k_row, in};
     }, a.head, whole);
+    if (threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
   };
-  if (end > 0) load(0);
-  for (int first = 0; first < end; first += TILE) {
+  int k = stages.at(0);
+  if (k < stages.end) load(k);
+  while (k < stages.end) {
     __syncthreads();
     next.store(ks, vs);
-    if (threadIdx.x < TILE) docs[threadIdx.x] = sight.document(first + (int)threadIdx.x);
+    if (threadIdx.x < STAGE) docs[threadIdx.x] = doc;
     __syncthreads();
-    if (first + TILE < end) load(first + TILE);
-    typename Type<T>::acc s[2], dp[2];
-    score<T, HD>(ks, l16, g, frag, s);
-    score<T, HD>(vs, l16, g, grad, dp);
+    const int here = k, first = here * STAGE + l.set * TILE;
+    k = stages.at(here + 1);
+    if (k < stages.end) load(k);
+    if (first >= seen_to) continue;
+    acc s[2], dp[2], bent[2];
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    score<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, grad, dp);
+    const int apart = i - (first + Type<T>::row_of(0, l.g));
+    scorer.template operator()<true>(s, bent, apart);
+    if (!sight.all_see(i0, first + TILE)) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int row_in = 16 * t + Type<T>::row_of(r, l.g);
+          const bool sees = sight.sees(i, di, first + row_in, docs[l.set * TILE + row_in]);
+          s[t][r] = sees ? s[t][r] : -(T)__builtin_huge_val();
+          dp[t][r] = sees ? dp[t][r] : dot;
+          if (scorer.capped) bent[t][r] = sees ? bent[t][r] : (T)0;
+        }
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int row_in = t * 16 + Type<T>::row_of(r, g), j = first + row_in, distance = abs(i - j);
-        T bend;
-        const T v = scorer(s[t][r], distance, &bend);
-        const bool seen = sight.sees(i, di, j, docs[row_in]);
-        const T ds = seen ? Type<T>::exp2_of(v - sums) * (dp[t][r] - dot) : (T)0;
-        dslope -= ds * (T)distance;
-        s[t][r] = ds * bend;
-      }
-    weigh<T, HD>(ks, l16, g, s, out);
+      for (int r = 0; r < 4; r++) s[t][r] = Type<T>::exp2_of(s[t][r] - sums) * (dp[t][r] - dot);
+    if (scorer.sloped) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) dslope -= s[t][r] * Scorer<T>::abs_of((T)apart - (T)tile_row<T>(t, r));
+    }
+    if (scorer.capped) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) s[t] -= s[t] * (bent[t] * bent[t]);
+    }
+    weigh<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, out);
   }
-  if (a.dq && i < (int)a.length) put_row<T, HD>((T*)a.dq + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head, g, a.head, out, (T)a.scale);
+  if constexpr (SETS == 2) join<T, HD>(out, smem, l.set);
+  if (a.dq && l.set == 0 && i < (int)a.length)
+    put_row<T, HD>((T*)a.dq + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head, l.g, a.head, out, (T)a.scale, di < 0);
   if (a.dslopes_rows) {
-    dslope = rg_wave_sum(dslope);
-    if (lane == 0) waves[threadIdx.x >> 6] = dslope;
+    dslope = rg_wave_sum(di < 0 ? (T)0 : dslope);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = dslope;
     __syncthreads();
-    if (threadIdx.x == 0)
-      ((T*)a.dslopes_rows)[((uint64_t)at.b * a.tiles + at.tile) * a.heads + at.h] = ((waves[0] + waves[1]) + waves[2]) + waves[3];
+    if (threadIdx.x == 0) {
+      dslope = waves[0];
+      for (int w = 1; w < NT / 64; w++) dslope += waves[w];
+      ((T*)a.dslopes_rows)[((uint64_t)at.b * a.tiles + at.tile) * a.heads + at.h] = dslope;
+    }
   }
 }
 
-// The gradients of k and v: a block's 64 keys against the queries of every head that reads them.
+// The gradients of k and v: a block's 64 keys against the queries of the heads that read them, all
+// of a group's or, where that leaves too few blocks, a part of them, whose sums k_attend_parts adds up.
 template <class T, int HD>
-__global__ void __launch_bounds__(NT) k_attend_dkv(AttendArgs a) {
-  __shared__ __align__(16) T qs[TILE * PITCH<T, HD>];
-  __shared__ __align__(16) T gs[TILE * PITCH<T, HD>];
-  __shared__ int docs[TILE];
-  __shared__ T sums[TILE], dots[TILE];
-  const Place at(a.batch, a.keys, a.tiles, false);
+__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_attend_dkv(AttendArgs a) {
+  typedef typename Type<T>::acc acc;
+  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) int docs[STAGE];
+  __shared__ __align__(16) T sums[STAGE];
+  __shared__ __align__(16) T dots[STAGE];
+  __shared__ uint64_t found[NT / 64];
+  T *qs = smem, *gs = smem + STAGE * PITCH<T, HD>;
+  const Place at(blockIdx.x, a.batch, a.keys * a.parts, a.tiles, false);
+  const uint32_t kh = at.h / a.parts, part = at.h % a.parts, group = a.heads / a.keys, per_part = group / a.parts;
   const Sight sight(a, at.b);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int begin = (int)at.tile * ROWS, j = begin + (int)(threadIdx.x >> 6) * 16 + l16;
-  const uint32_t group = a.heads / a.keys;
+  const Lane l;
+  const int begin = (int)at.tile * ROWS, j = begin + l.row, j0 = begin + l.first;
   const bool whole = a.head % Type<T>::V == 0;
   const int dj = sight.document(j);
-  const int64_t key = ((int64_t)at.b * a.length + j) * a.k_row + at.h * a.head;
+  const int64_t key = ((int64_t)at.b * a.length + j) * a.k_row + kh * a.head;
   T frag[HD / 4], value[HD / 4];
-  row_frag<T, HD>(dj >= 0 ? (const T*)a.k + key : nullptr, g, a.head, whole, frag);
-  row_frag<T, HD>(dj >= 0 ? (const T*)a.v + key : nullptr, g, a.head, whole, value);
-  typename Type<T>::acc dk[HD / 16], dv[HD / 16];
+  row_frag<T, HD>(dj >= 0 ? (const T*)a.k + key : nullptr, l.g, a.head, whole, frag);
+  row_frag<T, HD>(dj >= 0 ? (const T*)a.v + key : nullptr, l.g, a.head, whole, value);
+  acc dk[HD / 16], dv[HD / 16];
 #pragma unroll
-  for (int n = 0; n < HD / 16; n++) dk[n] = dv[n] = typename Type<T>::acc{0, 0, 0, 0};
-  const int from = sight.queries_from(begin) / TILE * TILE, end = begin < sight.length ? sight.length : 0;
-  const uint32_t per_head = end > from ? (uint32_t)(end - from + TILE - 1) / TILE : 0, steps = per_head * group;
+  for (int n = 0; n < HD / 16; n++) dk[n] = dv[n] = acc{0, 0, 0, 0};
+  const int end = begin < sight.length ? (sight.length + STAGE - 1) / STAGE : 0;
+  Stages<STAGE, NT> stages(sight, begin, min(sight.queries_from(begin) / STAGE, end), end, found);
+  // The wave's keys are seen by no query before this.
+  const int seen_from = sight.queries_from(j0);
+  uint32_t h = kh * group + part * per_part;
+  const uint32_t last = h + per_part;
   Staged<T, HD> next;
-  auto load = [&](uint32_t step) {
-    const uint32_t h = at.h * group + step / per_head;
-    const int first = from + (int)(step % per_head) * TILE;
-    next.load([&](int r) {
-      const bool in = sight.document(first + r) >= 0;
-      const int64_t t = (int64_t)at.b * a.length + first + r;
-      return RowPair<T>{in ? (const T*)a.q + t * a.q_row + h * a.head : nullptr, in ? (const T*)a.dy + (t * a.heads + h) * a.head : nullptr};
+  int doc = 0;
+  T sum = 0, dot = 0;
+  auto load = [&](uint32_t of, int stage) {
+    const int first = stage * STAGE;
+    const int64_t t = (int64_t)at.b * a.length;
+    next.load((const T*)a.q + t * a.q_row + of * a.head, (const T*)a.dy + (t * a.heads + of) * a.head, [&](int r) {
+      const int i = min(first + r, sight.length - 1);
+      const bool in = first + r < sight.length && (!sight.documents || sight.documents[i] >= 0);
+      return RowAt{i * a.q_row, (int64_t)i * a.heads * a.head, in};
     }, a.head, whole);
+    if (threadIdx.x < STAGE) {
+      const int i = first + (int)threadIdx.x;
+      doc = sight.document(i);
+      const uint64_t stat = ((uint64_t)at.b * a.heads + of) * a.length + min(i, sight.length - 1);
+      sum = ((const T*)a.sums_in)[stat];
+      dot = ((const T*)a.workspace)[stat];
+    }
   };
-  if (steps > 0) load(0);
-  for (uint32_t step = 0; step < steps; step++) {
-    const uint32_t h = at.h * group + step / per_head;
-    const int first = from + (int)(step % per_head) * TILE;
-    const Scorer<T> scorer(a, h);
+  int k = stages.at(stages.from);
+  const bool some = k < stages.end;
+  if (some) load(h, k);
+  while (some && h < last) {
     __syncthreads();
     next.store(qs, gs);
-    if (threadIdx.x < TILE) {
-      const int i = first + (int)threadIdx.x, di = sight.document(i);
-      const uint64_t stat = ((uint64_t)at.b * a.heads + h) * a.length + i;
-      docs[threadIdx.x] = di;
-      sums[threadIdx.x] = di >= 0 ? ((const T*)a.sums_in)[stat] : (T)__builtin_huge_val();
-      dots[threadIdx.x] = di >= 0 ? ((const T*)a.workspace)[stat] : (T)0;
+    if (threadIdx.x < STAGE) {
+      docs[threadIdx.x] = doc;
+      sums[threadIdx.x] = doc < 0 ? (T)__builtin_huge_val() : sum;  // weights of 0
+      dots[threadIdx.x] = doc < 0 ? (T)0 : dot;
     }
     __syncthreads();
-    if (step + 1 < steps) load(step + 1);
-    typename Type<T>::acc s[2], dp[2];
-    score<T, HD>(qs, l16, g, frag, s);
-    score<T, HD>(gs, l16, g, value, dp);
+    const int here = k, first = here * STAGE + l.set * TILE;
+    const Scorer<T> scorer(a, h);
+    k = stages.at(here + 1);
+    if (k >= stages.end) {
+      h++;
+      if (h < last) k = stages.at(stages.from);
+    }
+    if (h < last) load(h, k);
+    if (first + TILE <= seen_from || first >= sight.length) continue;
+    acc s[2], dp[2], bent[2];
+    score<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    score<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, value, dp);
+    scorer.template operator()<true>(s, bent, j - (first + Type<T>::row_of(0, l.g)));
+    const bool all = !sight.documents && (!sight.causal || j0 + 15 <= first || j0 + 15 < sight.prefix);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int row = t * 16 + Type<T>::row_of(r, g), i = first + row;
-        T bend;
-        const T v = scorer(s[t][r], abs(i - j), &bend);
-        const bool seen = sight.sees(i, docs[row], j, dj);
-        const T p = seen ? Type<T>::exp2_of(v - sums[row]) : (T)0;
-        s[t][r] = p;
-        dp[t][r] = seen ? p * (dp[t][r] - dots[row]) * bend : (T)0;
+        const int row = l.set * TILE + 16 * t + Type<T>::row_of(r, l.g);
+        if (!all && !sight.sees(here * STAGE + row, docs[row], j, dj)) {
+          s[t][r] = -(T)__builtin_huge_val();
+          dp[t][r] = 0;
+          if (scorer.capped) bent[t][r] = 0;
+        }
+        s[t][r] = Type<T>::exp2_of(s[t][r] - sums[row]);
+        dp[t][r] = s[t][r] * (dp[t][r] - dots[row]);
       }
-    weigh<T, HD>(gs, l16, g, s, dv);
-    weigh<T, HD>(qs, l16, g, dp, dk);
+    if (scorer.capped) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) dp[t] -= dp[t] * (bent[t] * bent[t]);
+    }
+    weigh<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, dv);
+    weigh<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, dp, dk);
   }
-  if (j >= (int)a.length) return;
-  if (a.dk) put_row<T, HD>((T*)a.dk + key, g, a.head, dk, (T)a.scale);
-  if (a.dv) put_row<T, HD>((T*)a.dv + key, g, a.head, dv, (T)1);
+  if constexpr (SETS == 2) {
+    join<T, HD>(dk, smem, l.set);
+    join<T, HD>(dv, smem, l.set);
+  }
+  if (l.set != 0 || j >= (int)a.length) return;
+  const bool none = dj < 0;
+  if (a.parts == 1) {
+    if (a.dk) put_row<T, HD>((T*)a.dk + key, l.g, a.head, dk, (T)a.scale, none);
+    if (a.dv) put_row<T, HD>((T*)a.dv + key, l.g, a.head, dv, (T)1, none);
+    return;
+  }
+  // A part's rows: [parts][batch, length, keys, head] of k, then of v.
+  const uint64_t all_rows = (uint64_t)a.batch * a.length * a.keys, at_row = ((uint64_t)at.b * a.length + j) * a.keys + kh;
+  put_row<T, HD>((T*)a.partial + (part * all_rows + at_row) * a.head, l.g, a.head, dk, (T)a.scale, none);
+  put_row<T, HD>((T*)a.partial + ((a.parts + part) * all_rows + at_row) * a.head, l.g, a.head, dv, (T)1, none);
+}
+
+// Adds up the parts of the gradients of k and v, in order.
+template <class T>
+__global__ void __launch_bounds__(256) k_attend_parts(AttendArgs a) {
+  const uint64_t n = (uint64_t)a.batch * a.length * a.keys * a.head, per = a.keys * a.head;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (uint64_t)gridDim.x * 256) {
+    const uint64_t at = i < n ? i : i - n;
+    const T* from = (const T*)a.partial + (i < n ? 0 : a.parts * n) + at;
+    T sum = from[0];
+    for (uint32_t p = 1; p < a.parts; p++) sum += from[p * n];
+    T* into = (T*)(i < n ? a.dk : a.dv);
+    if (into) into[at / per * a.k_row + at % per] = sum;
+  }
 }
 
 // ---- over a paged cache ----------------------------------------------------------------------------
@@ -554,83 +853,100 @@ struct Cache {
   }
 };
 
-// Rows of a sequence's queries: the heads of one key head side by side, token after token.
+// Rows of a sequence's queries: the heads of one key head side by side, token after token. A block
+// takes 64 of them and a split of the keys.
 template <class T, int HD>
-__global__ void __launch_bounds__(NT) k_paged(AttendArgs a) {
-  __shared__ __align__(16) T ks[TILE * PITCH<T, HD>];
-  __shared__ __align__(16) T vs[TILE * PITCH<T, HD>];
-  __shared__ int there[TILE];
+__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged(AttendArgs a) {
+  typedef typename Type<T>::acc acc;
+  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS;
+  __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) int there[STAGE];
+  __shared__ T tops[SETS == 2 ? 512 : 1], sums[SETS == 2 ? 512 : 1];
+  T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
   const uint32_t split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
-  const uint32_t bh = rest % (a.batch * a.keys), tile = rest / (a.batch * a.keys), b = bh / a.keys, kh = bh % a.keys, group = a.heads / a.keys;
+  const Place at(rest, a.batch, a.keys, a.tiles, true);
+  const uint32_t b = at.b, kh = at.h, group = a.heads / a.keys;
   const Cache cache(a, b);
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const uint32_t begin = tile * ROWS, r0 = begin + (threadIdx.x >> 6) * 16 + l16;
+  const Lane l;
+  const uint32_t begin = at.tile * ROWS, r0 = begin + l.row;
   const int i = (int)(r0 / group);
   const uint32_t h = kh * group + r0 % group;
   const bool whole = a.head % Type<T>::V == 0, in = i < cache.count;
   const Scorer<T> scorer(a, h);
   T frag[HD / 4];
-  row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, g, a.head, whole, frag);
+  row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, l.g, a.head, whole, frag);
   // Keys in order: `past` of the pages, then the new tokens up to the last query of the tile.
-  const int last = min((int)((begin + ROWS - 1) / group), cache.count - 1);
+  const int last = min((int)((begin + ROWS - 1) / group), cache.count - 1), least = (int)((begin + l.first) / group);
   const int all = (int)(begin / group) < cache.count ? cache.past + last + 1 : 0;
   const int from = (int)min((uint64_t)split * a.split_keys, (uint64_t)all), end = (int)min((uint64_t)(split + 1) * a.split_keys, (uint64_t)all);
-  const T *kb = (const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head;
+  // New rows as places in the pages' operands: their distance from those.
+  const int64_t kn = (const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.k_pages;
+  const int64_t vn = (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.v_pages;
   Running<T, HD> run;
   Staged<T, HD> next;
-  auto load = [&](int at) {
-    next.load([&](int r) {
-      const int c = at + r;
-      if (c >= end) return RowPair<T>{nullptr, nullptr};
-      if (c >= cache.past) {
-        const int64_t o = (int64_t)(c - cache.past) * a.k_row;
-        return RowPair<T>{kb + o, vb + o};
-      }
-      const int64_t row = cache.row((uint32_t)c);
-      if (row < 0) return RowPair<T>{nullptr, nullptr};
-      const int64_t o = (row * a.keys + kh) * a.head;
-      return RowPair<T>{(const T*)a.k_pages + o, (const T*)a.v_pages + o};
+  int has = 0;
+  auto load = [&](int first) {
+    next.load((const T*)a.k_pages, (const T*)a.v_pages, [&](int r) {
+      const int c = min(first + r, end - 1);
+      if (c >= cache.past) return RowAt{kn + (int64_t)(c - cache.past) * a.k_row, vn + (int64_t)(c - cache.past) * a.k_row, first + r < end};
+      const int64_t row = cache.row((uint32_t)c), o = (max(row, (int64_t)0) * a.keys + kh) * a.head;
+      return RowAt{o, o, row >= 0 && first + r < end};
     }, a.head, whole);
+    if (threadIdx.x < STAGE) {
+      const int c = first + (int)threadIdx.x;
+      has = c < end && (c >= cache.past || cache.row((uint32_t)c) >= 0);
+    }
   };
   if (from < end) load(from);
-  for (int at = from; at < end; at += TILE) {
+  for (int stage = from; stage < end; stage += STAGE) {
     __syncthreads();
     next.store(ks, vs);
-    if (threadIdx.x < TILE) {
-      const int c = at + (int)threadIdx.x;
-      there[threadIdx.x] = c < end && (c >= cache.past || cache.row((uint32_t)c) >= 0);
-    }
+    if (threadIdx.x < STAGE) there[threadIdx.x] = has;
     __syncthreads();
-    if (at + TILE < end) load(at + TILE);
-    typename Type<T>::acc s[2];
-    score<T, HD>(ks, l16, g, frag, s);
+    if (stage + STAGE < end) load(stage + STAGE);
+    const int first = stage + l.set * TILE;
+    if (first >= end || least >= cache.count) continue;
+    acc s[2];
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    // Positions of old keys run on to the new ones' unless the table ends before them.
+    const int apart = i + (first >= cache.past ? cache.past : cache.first) - first - Type<T>::row_of(0, l.g);
+    const bool one = first + TILE <= cache.past || first >= cache.past || cache.first == cache.past;
+    scorer.template operator()<false>(s, nullptr, apart);
+    if (!one && scorer.sloped) {
+      // A tile with keys on both sides of a gap: the new ones are nearer than their place says.
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int c = first + 16 * t + Type<T>::row_of(r, l.g);
+          if (c >= cache.past)
+            s[t][r] += scorer.slope * (Scorer<T>::abs_of((T)apart - (T)tile_row<T>(t, r)) - Scorer<T>::abs_of((T)(i - (c - cache.past))));
+        }
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const int row = t * 16 + Type<T>::row_of(r, g), c = at + row;
-        const bool old = c < cache.past;
-        const int distance = old ? cache.first + i - c : i - (c - cache.past);
-        T bend;
-        const T v = scorer(s[t][r], distance, &bend);
-        s[t][r] = in && there[row] && distance >= 0 ? v : -(T)__builtin_huge_val();
+        const int row = 16 * t + Type<T>::row_of(r, l.g), c = first + row;
+        s[t][r] = in && there[l.set * TILE + row] && c - cache.past <= i ? s[t][r] : -(T)__builtin_huge_val();
       }
     run.add(s);
-    weigh<T, HD>(vs, l16, g, s, run.out);
+    weigh<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, run.out);
   }
-  const T sum = row_sum(run.sum);
-  if (i >= (int)a.length) return;
+  run.sum = row_sum(run.sum);
+  if constexpr (SETS == 2) join(run, smem, tops, sums, l.set);
+  if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)b * a.length + i) * a.heads + h;
   if (a.splits == 1) {
-    if (a.y) put_row<T, HD>((T*)a.y + row * a.head, g, a.head, run.out, sum == 0 ? (T)0 : 1 / sum);
+    if (a.y) put_row<T, HD>((T*)a.y + row * a.head, l.g, a.head, run.out, 1 / run.sum, run.sum == 0);
     return;
   }
-  // A split's maximum, sum and weighed values: [rows][splits] of 2 + head.
+  // A split's bound, sum and weighed values: [rows][splits] of 2 + head.
   T* part = (T*)a.partial + (row * a.splits + split) * (a.head + 2);
-  put_row<T, HD>(part + 2, g, a.head, run.out, (T)1);
-  if (g == 0) {
+  put_row<T, HD>(part + 2, l.g, a.head, run.out, (T)1, false);
+  if (l.g == 0) {
     part[0] = run.top;
-    part[1] = sum;
+    part[1] = run.sum;
   }
 }
 
@@ -638,10 +954,10 @@ __global__ void __launch_bounds__(NT) k_paged(AttendArgs a) {
 // tokens' keys and values into their pages, a wave a token and key head. Rows that a later sequence
 // writes too are left to it, so that the result does not depend on which comes first.
 template <class T>
-__global__ void __launch_bounds__(NT) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
+__global__ void __launch_bounds__(256) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
   const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < join_blocks) {
-    const uint64_t row = (uint64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    const uint64_t row = (uint64_t)blockIdx.x * (256 / 64) + (threadIdx.x >> 6);
     if (row >= (uint64_t)a.batch * a.length * a.heads) return;
     const T* part = (const T*)a.partial + row * a.splits * (a.head + 2);
     T top = -(T)__builtin_huge_val();
@@ -658,7 +974,7 @@ __global__ void __launch_bounds__(NT) k_paged_finish(AttendArgs a, uint32_t join
     }
     return;
   }
-  const uint64_t item = (uint64_t)(blockIdx.x - join_blocks) * (NT / 64) + (threadIdx.x >> 6);
+  const uint64_t item = (uint64_t)(blockIdx.x - join_blocks) * (256 / 64) + (threadIdx.x >> 6);
   if (item >= (uint64_t)a.batch * a.length * a.keys) return;
   const uint32_t kh = (uint32_t)(item % a.keys), i = (uint32_t)(item / a.keys % a.length), b = (uint32_t)(item / a.keys / a.length);
   const Cache cache(a, b);
@@ -689,17 +1005,17 @@ __global__ void __launch_bounds__(NT) k_paged_finish(AttendArgs a, uint32_t join
 constexpr uint64_t NORM_PER_BLOCK = 16384;
 
 template <class T>
-__global__ void __launch_bounds__(NT) k_norm_squares(NormTensors t, double* partial) {
+__global__ void __launch_bounds__(256) k_norm_squares(NormTensors t, double* partial) {
   uint32_t k = 0;
   while (k + 1 < t.count && blockIdx.x >= t.first_block[k + 1]) k++;
   const uint64_t begin = (uint64_t)(blockIdx.x - t.first_block[k]) * NORM_PER_BLOCK, end = min(begin + NORM_PER_BLOCK, t.n[k]);
   const T* x = (const T*)t.x[k];
   double sum = 0;
-  for (uint64_t i = begin + threadIdx.x; i < end; i += NT) {
+  for (uint64_t i = begin + threadIdx.x; i < end; i += 256) {
     const double v = (double)x[i];
     sum += v * v;
   }
-  __shared__ double waves[NT / 64];
+  __shared__ double waves[256 / 64];
   sum = rg_wave_sum(sum);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -759,32 +1075,56 @@ void set_splits(AttendArgs& a) {
 
 }  // namespace
 
-uint64_t attend_blocks(int, const AttendArgs& a) { return (uint64_t)a.batch * a.heads * ((a.length + ROWS - 1) / ROWS); }
-uint64_t attend_workspace(int dtype, const AttendArgs& a) { return (uint64_t)a.batch * a.heads * a.length * size_of(dtype); }
+uint64_t attend_blocks(int, const AttendArgs& a) { return (uint64_t)a.batch * a.heads * ((a.length + ROWS - 1) / ROWS) * 2; }
+
+// A gradient's workspace: dy.y of every query, then the parts of dk and dv.
+static uint64_t dots_bytes(int dtype, const AttendArgs& a) { return ((uint64_t)a.batch * a.heads * a.length * size_of(dtype) + 255) / 256 * 256; }
+// Parts of a group's heads: as few as leave two blocks for every CU.
+static uint32_t parts_of(const AttendArgs& a) {
+  const uint32_t group = a.heads / a.keys;
+  const uint64_t blocks = (uint64_t)a.batch * a.keys * ((a.length + ROWS - 1) / ROWS);
+  for (uint32_t p = 1; p < group; p++)
+    if (group % p == 0 && blocks * p >= 512) return p;
+  return group;
+}
+uint64_t attend_workspace(int dtype, const AttendArgs& a) {
+  const uint32_t parts = parts_of(a);
+  return dots_bytes(dtype, a) + (parts > 1 ? 2 * (uint64_t)parts * a.batch * a.length * a.keys * a.head * size_of(dtype) : 0);
+}
 uint32_t attend_slope_rows(int, const AttendArgs& a) { return a.batch * ((a.length + ROWS - 1) / ROWS); }
 
 void attend(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
   set_rows(a);
   by_head(dtype, a.head, [&](auto t, auto hd) {
-    k_attend<decltype(t), decltype(hd)::value><<<a.tiles * a.batch * a.heads, NT, 0, s>>>(a);
+    typedef decltype(t) T;
+    constexpr int HD = decltype(hd)::value;
+    k_attend<T, HD><<<a.tiles * a.batch * a.heads, Geo<T, HD>::NT, 0, s>>>(a);
   });
 }
 
 void attend_grad(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
   set_rows(a);
+  a.parts = parts_of(a);
+  a.partial = (char*)a.workspace + dots_bytes(dtype, a);
   by_head(dtype, a.head, [&](auto t, auto hd) {
-    k_attend_dq<decltype(t), decltype(hd)::value><<<a.tiles * a.batch * a.heads, NT, 0, s>>>(a);
-    if (a.dk || a.dv) k_attend_dkv<decltype(t), decltype(hd)::value><<<a.tiles * a.batch * a.keys, NT, 0, s>>>(a);
+    typedef decltype(t) T;
+    constexpr int HD = decltype(hd)::value;
+    k_attend_dq<T, HD><<<a.tiles * a.batch * a.heads, Geo<T, HD>::NT, 0, s>>>(a);
+    if (!a.dk && !a.dv) return;
+    k_attend_dkv<T, HD><<<a.tiles * a.batch * a.keys * a.parts, Geo<T, HD>::NT, 0, s>>>(a);
+    if (a.parts == 1) return;
+    const uint64_t n = 2 * (uint64_t)a.batch * a.length * a.keys * a.head;
+    k_attend_parts<T><<<(uint32_t)std::min<uint64_t>((n + 255) / 256, 8192), 256, 0, s>>>(a);
   });
 }
 
 uint64_t paged_blocks(int, const AttendArgs& args) {
   AttendArgs a = args;
   set_splits(a);
-  const uint64_t rows = (uint64_t)a.batch * a.length * (a.heads + a.keys) / (NT / 64) + 2;
-  return std::max((uint64_t)a.batch * a.keys * paged_tiles(a) * a.splits, rows);
+  const uint64_t rows = (uint64_t)a.batch * a.length * (a.heads + a.keys) / 4 + 2;
+  return std::max((uint64_t)a.batch * a.keys * paged_tiles(a) * a.splits * 2, rows);
 }
 
 uint64_t paged_workspace(int dtype, const AttendArgs& args) {
@@ -797,27 +1137,31 @@ void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
   set_rows(a);
   set_splits(a);
+  a.tiles = paged_tiles(a);
   a.partial = a.workspace;
   a.page_div = FastDiv(a.page);
   const uint64_t values = (uint64_t)a.pages * a.page * a.keys * a.head * size_of(dtype);
   if (a.k_out && a.k_out != a.k_pages) copy_bytes(s, a.k_out, a.k_pages, values);
   if (a.v_out && a.v_out != a.v_pages) copy_bytes(s, a.v_out, a.v_pages, values);
-  const uint32_t blocks = a.batch * a.keys * paged_tiles(a) * a.splits;
-  by_head(dtype, a.head, [&](auto t, auto hd) {
-    if (a.y) k_paged<decltype(t), decltype(hd)::value><<<blocks, NT, 0, s>>>(a);
-  });
-  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)(((uint64_t)a.batch * a.length * a.heads + NT / 64 - 1) / (NT / 64)) : 0;
-  const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + NT / 64 - 1) / (NT / 64)) : 0;
+  const uint32_t blocks = a.batch * a.keys * a.tiles * a.splits;
+  if (a.y)
+    by_head(dtype, a.head, [&](auto t, auto hd) {
+      typedef decltype(t) T;
+      constexpr int HD = decltype(hd)::value;
+      k_paged<T, HD><<<blocks, Geo<T, HD>::NT, 0, s>>>(a);
+    });
+  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)(((uint64_t)a.batch * a.length * a.heads + 3) / 4) : 0;
+  const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + 3) / 4) : 0;
   if (join + append == 0) return;
-  if (dtype == RG_F32) k_paged_finish<float><<<join + append, NT, 0, s>>>(a, join);
-  else k_paged_finish<double><<<join + append, NT, 0, s>>>(a, join);
+  if (dtype == RG_F32) k_paged_finish<float><<<join + append, 256, 0, s>>>(a, join);
+  else k_paged_finish<double><<<join + append, 256, 0, s>>>(a, join);
 }
 
 uint32_t norm_blocks(uint64_t n) { return (uint32_t)((n + NORM_PER_BLOCK - 1) / NORM_PER_BLOCK); }
 
 void norm_squares(hipStream_t s, int dtype, const NormTensors& t, uint32_t blocks, double* partial) {
-  if (dtype == RG_F32) k_norm_squares<float><<<blocks, NT, 0, s>>>(t, partial);
-  else k_norm_squares<double><<<blocks, NT, 0, s>>>(t, partial);
+  if (dtype == RG_F32) k_norm_squares<float><<<blocks, 256, 0, s>>>(t, partial);
+  else k_norm_squares<double><<<blocks, 256, 0, s>>>(t, partial);
 }
 
 void norm_root(hipStream_t s, int dtype, const double* partial, uint32_t blocks, void* out) {
