@@ -66,7 +66,10 @@ struct Type<float> {
   static __device__ __forceinline__ float tanh_of(float x) {
     const float a = fminf(fabsf(x), 16.0f), e = __builtin_amdgcn_exp2f(2.8853900817779268f * a), num = e - 1.0f, den = e + 1.0f;
     const float r = __builtin_amdgcn_rcpf(den), q = num * r, t = fmaf(fmaf(-den, q, num), r, q);
-    return fabsf(x) > 1.0f ? copysignf(t, x) : tanh_low(x);
+    // Both are formed: of a branch for each of a tile's scores the compiler makes eight.
+    float low = tanh_low(x);
+    asm volatile("" : "+v"(low));
+    return fabsf(x) > 1.0f ? copysignf(t, x) : low;
   }
   static constexpr bool LOW = true;
 };
@@ -829,6 +832,7 @@ __global__ void __launch_bounds__(256) k_attend_parts(AttendArgs a) {
 
 // ---- over a paged cache ----------------------------------------------------------------------------
 
+constexpr uint32_t PAGED_SPLITS = 2048;  // of a sequence's keys, at most
 constexpr int FIRST_MOST = 1 << 30;  // positions before the new tokens that are told apart
 
 // A sequence's keys in order: those that its pages hold, then the new tokens'.
@@ -950,31 +954,242 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged
   }
 }
 
-// Joins the splits of each row, a wave a row, and then (blocks from `join_blocks` on) puts the new
+// Rows that one wave's tile holds, of single tokens and a few: a wave of the block's four takes every
+// fourth step of the split's keys, straight from memory into the fragments of both products, while the
+// rows of its next step are looked up. A key's row is read by the four lanes that hold it 16 bytes
+// apart, a value's by sixteen. Three waves a SIMD, with 16 KB on the way each, hide what they wait for;
+// a second step's fragments in registers left room for one (32 us against the 23 of the block's kernel).
+// WHOLE: heads of whole 16 bytes.
+template <class T, int HD>
+struct FewGeo {
+  static constexpr int TILES = (int)sizeof(T) * HD <= 256 ? 2 : 1, STEP = 16 * TILES;  // keys of a wave's step
+  static constexpr bool FITS = (int)sizeof(T) * HD <= 512;
+};
+constexpr int FEW_ROWS = 16;
+
+template <class T, int HD, bool WHOLE>
+__global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(AttendArgs a) {
+  typedef typename Type<T>::acc acc;
+  typedef typename Type<T>::vec vec;
+  constexpr int TILES = FewGeo<T, HD>::TILES, STEP = FewGeo<T, HD>::STEP, ND = HD / 16, V = Type<T>::V;
+  constexpr int KV = HD / 4 / V;  // vectors of a key's quarter
+  __shared__ T outs[4][16 * (HD + 1)], tops[4][16], sums[4][16];
+  const uint32_t split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits, b = rest / a.keys, kh = rest % a.keys, group = a.heads / a.keys;
+  const Cache cache(a, b);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g = lane >> 4;
+  const int i = l16 / (int)group;
+  const uint32_t h = kh * group + l16 % group;
+  const bool in = l16 < (int)(a.length * group) && i < cache.count;
+  const int from = (int)min((uint64_t)split * a.split_keys, (uint64_t)cache.past), end = (int)min((uint64_t)(split + 1) * a.split_keys, (uint64_t)cache.past);
+  // The new tokens' own keys go to the split that the old ones end in.
+  const bool own = cache.count > 0 && split == min((uint32_t)cache.past / a.split_keys, a.splits - 1);
+  const Scorer<T> scorer(a, in ? h : kh * group);
+  T frag[HD / 4];
+  row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, g, a.head, WHOLE, frag);
+  Running<T, HD> run;
+  struct Rows {
+    vec k[TILES][KV];
+    T v[TILES][4][ND];
+    uint64_t there[TILES];
+  };
+  // Rows of a step's keys, a lane's own of each tile: places in both operands or -1.
+  auto look = [&](int first, int64_t* row) {
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+      const int c = first + 16 * t + l16;
+      row[t] = c < end ? cache.row((uint32_t)c) : -1;
+    }
+  };
+  auto fetch = [&](const T* ks, const T* vs, int64_t pitch, const int64_t* row, Rows& x) {
+#pragma unroll
+    for (int t = 0; t < TILES; t++) {
+      x.there[t] = __ballot(row[t] >= 0);
+      const T* k = ks + max(row[t], (int64_t)0) * pitch;
+#pragma unroll
+      for (int n = 0; n < KV; n++) {
+        const uint32_t d = (uint32_t)(n * V / 4 * 16 + 4 * g + n * V % 4);
+        if constexpr (WHOLE) {
+          x.k[t][n] = *(const vec*)(k + (d < a.head ? d : 0));
+        } else {
+#pragma unroll
+          for (uint32_t j = 0; j < V; j++) x.k[t][n][j] = k[d + j < a.head ? d + j : 0];
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const T* v = vs + max((int64_t)__shfl(row[t], Type<T>::row_of(r, g)), (int64_t)0) * pitch;
+        const uint32_t d = (uint32_t)(l16 * ND);
+        constexpr int VN = !WHOLE ? 1 : ND % V == 0 ? V : 2;  // whole heads are a multiple of it
+#pragma unroll
+        for (int n = 0; n < ND; n += VN) {
+          const T* from = v + (d + n < a.head ? d + n : 0);
+          if constexpr (WHOLE) take<VN>(from, x.v[t][r] + n);
+          else x.v[t][r][n] = *from;
+        }
+      }
+  };
+  // Makes 0 what was loaded in the place of columns past the head and of rows that are not there; not
+  // as it is loaded, which would wait for it.
+  auto clear = [&](Rows& x) {
+    if (a.head < HD) {
+#pragma unroll
+      for (int t = 0; t < TILES; t++) {
+#pragma unroll
+        for (int n = 0; n < KV; n++)
+#pragma unroll
+          for (uint32_t j = 0; j < V; j++)
+            if ((uint32_t)(n * V / 4 * 16 + 4 * g + n * V % 4) + j >= a.head) x.k[t][n][j] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (uint32_t n = 0; n < ND; n++)
+            if ((uint32_t)(l16 * ND) + n >= a.head) x.v[t][r][n] = 0;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+      if (x.there[t] != ~0ull) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int n = 0; n < ND; n++)
+            if (!(x.there[t] >> Type<T>::row_of(r, g) & 1)) x.v[t][r][n] = 0;
+      }
+  };
+  // `apart`: the distance of the lane's row from the step's first key.
+  auto work = [&](Rows& x, int apart, bool ordered) {
+    clear(x);
+    acc s[2] = {acc{0, 0, 0, 0}, acc{0, 0, 0, 0}};
+#pragma unroll
+    for (int n = 0; n < KV; n++)
+#pragma unroll
+      for (int j = 0; j < V; j++)
+#pragma unroll
+        for (int t = 0; t < TILES; t++) s[t] = Type<T>::mfma(x.k[t][n][j], frag[n * V + j], s[t]);
+    scorer.template operator()<false>(s, nullptr, apart - Type<T>::row_of(0, g));
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int of = Type<T>::row_of(r, g);
+        const bool sees = t < TILES && in && (x.there[t < TILES ? t : 0] >> of & 1) && (!ordered || 16 * t + of <= apart);
+        s[t][r] = sees ? s[t][r] : -(T)__builtin_huge_val();
+      }
+    run.add(s);
+#pragma unroll
+    for (int t = 0; t < TILES; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int n = 0; n < ND; n++) run.out[n] = Type<T>::mfma(x.v[t][r][n], s[t][r], run.out[n]);
+  };
+  const T *kp = (const T*)a.k_pages + kh * a.head, *vp = (const T*)a.v_pages + kh * a.head;
+  const int64_t pitch = (int64_t)a.keys * a.head;
+  int64_t row[TILES];
+  Rows x;
+  int first = from + wave * STEP;
+  if (first < end) look(first, row);
+  for (; first < end; first += 4 * STEP) {
+    fetch(kp, vp, pitch, row, x);
+    look(first + 4 * STEP, row);
+    work(x, cache.first + i - first, false);
+  }
+  if (own && wave == 3) {
+#pragma unroll
+    for (int t = 0; t < TILES; t++) row[t] = t == 0 && l16 < cache.count ? l16 : -1;
+    fetch((const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head, (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head, a.k_row, row, x);
+    work(x, i, true);
+  }
+  // The four waves' results, joined in order.
+  const T sum = row_sum(run.sum);
+  if (g == 0) {
+    tops[wave][l16] = run.top;
+    sums[wave][l16] = sum;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int n = 0; n < ND; n++) outs[wave][l16 * (HD + 1) + Type<T>::row_of(r, g) * ND + n] = run.out[n][r];
+  __syncthreads();
+  const uint32_t rows = a.length * group;
+  for (uint32_t at = threadIdx.x; at < rows * HD; at += 256) {
+    const uint32_t r = at / HD, d = at % HD;
+    if (d >= a.head) continue;
+    T top = tops[0][r];
+#pragma unroll
+    for (int w = 1; w < 4; w++) top = Type<T>::max_of(top, tops[w][r]);
+    const T base = Running<T, HD>::base(top);
+    T all = 0, v = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const T by = Type<T>::exp2_of(tops[w][r] - base);
+      all += sums[w][r] * by;
+      v += outs[w][r * (HD + 1) + d] * by;
+    }
+    const uint64_t row = ((uint64_t)b * a.length + r / group) * a.heads + kh * group + r % group;
+    if (a.splits == 1) {
+      ((T*)a.y)[row * a.head + d] = all == 0 ? (T)0 : v / all;
+      continue;
+    }
+    T* part = (T*)a.partial + (row * a.splits + split) * (a.head + 2);
+    part[2 + d] = v;
+    if (d == 0) {
+      part[0] = top;
+      part[1] = all;
+    }
+  }
+}
+
+// Joins the splits of each row, a block a row, and then (blocks from `join_blocks` on) puts the new
 // tokens' keys and values into their pages, a wave a token and key head. Rows that a later sequence
-// writes too are left to it, so that the result does not depend on which comes first.
+// writes too are left to it, so that the result does not depend on which comes first. It comes after
+// every read of the pages, so that it may write into the ones that were read.
 template <class T>
-__global__ void __launch_bounds__(256) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
+__global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
   const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < join_blocks) {
-    const uint64_t row = (uint64_t)blockIdx.x * (256 / 64) + (threadIdx.x >> 6);
-    if (row >= (uint64_t)a.batch * a.length * a.heads) return;
-    const T* part = (const T*)a.partial + row * a.splits * (a.head + 2);
+    __shared__ T weights[PAGED_SPLITS], lanes[512], waves[16];
+    const uint64_t row = blockIdx.x;
+    const uint32_t pitch = a.head + 2;
+    const T* part = (const T*)a.partial + row * a.splits * pitch;
     T top = -(T)__builtin_huge_val();
-    for (uint32_t p = lane; p < a.splits; p += 64) top = Type<T>::max_of(top, part[(uint64_t)p * (a.head + 2)]);
+    for (uint32_t p = threadIdx.x; p < a.splits; p += 512) top = Type<T>::max_of(top, weights[p] = part[(uint64_t)p * pitch]);
     top = rg_wave_max(top);
-    if (top == -(T)__builtin_huge_val()) top = 0;
+    if (lane == 0) waves[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < 8; w++) top = Type<T>::max_of(top, waves[w]);
+    const T base = top == -(T)__builtin_huge_val() ? (T)0 : top;
     T sum = 0;
-    for (uint32_t p = lane; p < a.splits; p += 64) sum += part[(uint64_t)p * (a.head + 2) + 1] * Type<T>::exp2_of(part[(uint64_t)p * (a.head + 2)] - top);
-    sum = rg_wave_sum(sum);
-    for (uint32_t d = lane; d < a.head; d += 64) {
-      T v = 0;
-      for (uint32_t p = 0; p < a.splits; p++) v += part[(uint64_t)p * (a.head + 2) + 2 + d] * Type<T>::exp2_of(part[(uint64_t)p * (a.head + 2)] - top);
-      ((T*)a.y)[row * a.head + d] = sum == 0 ? (T)0 : v / sum;
+    for (uint32_t p = threadIdx.x; p < a.splits; p += 512) {
+      const T by = Type<T>::exp2_of(weights[p] - base);
+      weights[p] = by;
+      sum += part[(uint64_t)p * pitch + 1] * by;
     }
+    sum = rg_wave_sum(sum);
+    if (lane == 0) waves[8 + (threadIdx.x >> 6)] = sum;
+    __syncthreads();
+    sum = waves[8];
+    for (int w = 9; w < 16; w++) sum += waves[w];
+    // Threads side by side on the head, the rest of them on the splits.
+    uint32_t width = 1;
+    while (width < a.head) width *= 2;
+    const uint32_t d = threadIdx.x % width, first = threadIdx.x / width, step = 512 / width;
+    T v = 0;
+    if (d < a.head) {
+#pragma unroll 8
+      for (uint32_t p = first; p < a.splits; p += step) v += part[(uint64_t)p * pitch + 2 + d] * weights[p];
+    }
+    lanes[threadIdx.x] = v;
+    __syncthreads();
+    if (first != 0 || d >= a.head) return;
+    for (uint32_t k = 1; k < step; k++) v += lanes[k * width + d];
+    ((T*)a.y)[row * a.head + d] = sum == 0 ? (T)0 : v / sum;
     return;
   }
-  const uint64_t item = (uint64_t)(blockIdx.x - join_blocks) * (256 / 64) + (threadIdx.x >> 6);
+  const uint64_t item = (uint64_t)(blockIdx.x - join_blocks) * (512 / 64) + (threadIdx.x >> 6);
   if (item >= (uint64_t)a.batch * a.length * a.keys) return;
   const uint32_t kh = (uint32_t)(item % a.keys), i = (uint32_t)(item / a.keys % a.length), b = (uint32_t)(item / a.keys / a.length);
   const Cache cache(a, b);
@@ -1061,16 +1276,24 @@ void set_rows(AttendArgs& a) {
 
 uint64_t size_of(int dtype) { return dtype == RG_F32 ? 4 : 8; }
 
-// Tiles of a sequence's rows in the paged form, and over how many blocks their keys are split: as
-// many as leave each 256 keys and the device four blocks for every CU.
+// Tiles of a sequence's rows in the paged form.
 uint32_t paged_tiles(const AttendArgs& a) { return (uint32_t)(((uint64_t)a.length * (a.heads / a.keys) + ROWS - 1) / ROWS); }
-void set_splits(AttendArgs& a) {
-  const uint64_t keys = (uint64_t)a.table_pages * a.page + a.length, blocks = (uint64_t)a.batch * a.keys * paged_tiles(a);
-  const uint64_t most = (keys + 255) / 256, want = (1024 + blocks - 1) / blocks;
-  uint64_t n = std::max<uint64_t>(1, std::min(most, want));
-  const uint64_t per = ((keys + n - 1) / n + TILE - 1) / TILE * TILE;
-  a.splits = (uint32_t)((keys + per - 1) / per);
+// Whether the rows of a key head are few enough for one wave, and the heads for its registers.
+bool few_rows(int dtype, const AttendArgs& a) {
+  return (uint64_t)a.length * (a.heads / a.keys) <= FEW_ROWS && a.head <= (dtype == RG_F32 ? 128 : 64);
+}
+// Over how many blocks a sequence's keys are split, by the room of its table, since only the device
+// knows how much of it is used: three blocks of few rows for every CU, of whole tiles two, but no
+// fewer than 128 keys (a step of each wave) or 256 each.
+void set_splits(int dtype, AttendArgs& a) {
+  const bool few = few_rows(dtype, a);
+  const uint64_t keys = (uint64_t)a.table_pages * a.page + (few ? 0 : a.length), blocks = (uint64_t)a.batch * a.keys * (few ? 1 : paged_tiles(a));
+  const uint64_t least = few ? 128 : 256, want = std::max<uint64_t>(1, (few ? 768 : 512) / blocks);
+  uint64_t per = std::max(least, (keys + want - 1) / want);
+  per = std::max(per, (keys + PAGED_SPLITS - 1) / PAGED_SPLITS);
+  per = (per + least - 1) / least * least;
   a.split_keys = (uint32_t)per;
+  a.splits = (uint32_t)((keys + per - 1) / per);
 }
 
 }  // namespace
@@ -1120,41 +1343,49 @@ void attend_grad(hipStream_t s, int dtype, const AttendArgs& args) {
   });
 }
 
-uint64_t paged_blocks(int, const AttendArgs& args) {
+uint64_t paged_blocks(int dtype, const AttendArgs& args) {
   AttendArgs a = args;
-  set_splits(a);
-  const uint64_t rows = (uint64_t)a.batch * a.length * (a.heads + a.keys) / 4 + 2;
-  return std::max((uint64_t)a.batch * a.keys * paged_tiles(a) * a.splits * 2, rows);
+  set_splits(dtype, a);
+  const uint64_t rows = (uint64_t)a.batch * a.length * (a.heads + a.keys / 8 + 1) + 1;
+  return 2 * std::max((uint64_t)a.batch * a.keys * paged_tiles(a) * a.splits, rows);
 }
 
 uint64_t paged_workspace(int dtype, const AttendArgs& args) {
   AttendArgs a = args;
-  set_splits(a);
+  set_splits(dtype, a);
   return a.splits == 1 ? 0 : (uint64_t)a.batch * a.length * a.heads * a.splits * (a.head + 2) * size_of(dtype);
 }
 
 void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
   set_rows(a);
-  set_splits(a);
+  set_splits(dtype, a);
   a.tiles = paged_tiles(a);
   a.partial = a.workspace;
   a.page_div = FastDiv(a.page);
   const uint64_t values = (uint64_t)a.pages * a.page * a.keys * a.head * size_of(dtype);
   if (a.k_out && a.k_out != a.k_pages) copy_bytes(s, a.k_out, a.k_pages, values);
   if (a.v_out && a.v_out != a.v_pages) copy_bytes(s, a.v_out, a.v_pages, values);
-  const uint32_t blocks = a.batch * a.keys * a.tiles * a.splits;
+  const bool few = few_rows(dtype, a);
   if (a.y)
     by_head(dtype, a.head, [&](auto t, auto hd) {
       typedef decltype(t) T;
       constexpr int HD = decltype(hd)::value;
-      k_paged<T, HD><<<blocks, Geo<T, HD>::NT, 0, s>>>(a);
+      if constexpr (FewGeo<T, HD>::FITS) {
+        if (few) {
+          const uint32_t blocks = a.batch * a.keys * a.splits;
+          if (a.head % Type<T>::V == 0) k_paged_few<T, HD, true><<<blocks, 256, 0, s>>>(a);
+          else k_paged_few<T, HD, false><<<blocks, 256, 0, s>>>(a);
+          return;
+        }
+      }
+      k_paged<T, HD><<<a.batch * a.keys * a.tiles * a.splits, Geo<T, HD>::NT, 0, s>>>(a);
     });
-  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)(((uint64_t)a.batch * a.length * a.heads + 3) / 4) : 0;
-  const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + 3) / 4) : 0;
+  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)((uint64_t)a.batch * a.length * a.heads) : 0;
+  const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + 7) / 8) : 0;
   if (join + append == 0) return;
-  if (dtype == RG_F32) k_paged_finish<float><<<join + append, 256, 0, s>>>(a, join);
-  else k_paged_finish<double><<<join + append, 256, 0, s>>>(a, join);
+  if (dtype == RG_F32) k_paged_finish<float><<<join + append, 512, 0, s>>>(a, join);
+  else k_paged_finish<double><<<join + append, 512, 0, s>>>(a, join);
 }
 
 uint32_t norm_blocks(uint64_t n) { return (uint32_t)((n + NORM_PER_BLOCK - 1) / NORM_PER_BLOCK); }

@@ -70,7 +70,7 @@ struct RunBuffers {
 
 struct RunCache {
   std::vector<int64_t> key;
-  std::vector<void*> table[2];
+  std::vector<void*> table[2], steps[2];  // run_tables
   int n_graphs = 0;
   void* mem = nullptr;  // one allocation holding the run buffers and the snapshot
   uint64_t mem_bytes = 0;
@@ -2229,7 +2229,6 @@ void enqueue_run_step(const Program& p, hipStream_t s, void* ws, const rg_run_de
   rgk::counter_inc(s, b.counter);
 }
 
-// The two slot tables a run alternates between: `start`, and `start` with every swap applied.
 // Refuses a run description whose sizes or pointers do not fit this program before anything is
 // copied or launched: every slot index in range; swapped slots pairwise disjoint, of one dtype
 // and capacity; copies within both slots and of one dtype; data inputs within their slots, with
@@ -2297,10 +2296,65 @@ std::string check_run_desc(const Program& p, const rg_run_desc* d) {
   return "";
 }
 
-void run_tables(const std::vector<void*>& start, const rg_run_desc* d, std::vector<void*> out[2]) {
-  out[0] = start;
-  out[1] = start;
-  for (int64_t k = 0; k < d->n_swaps; k++) std::swap(out[1][(size_t)d->swaps[2 * k]], out[1][(size_t)d->swaps[2 * k + 1]]);
+// The swaps whose two slots may share one buffer while a loop runs: the pages of a paged attention,
+// which then writes its new rows where they are instead of copying the others. The step has to be the
+// only one that names either slot, once each, and neither may be anything else of the plan. Its
+// kernels read rows before the new ones alone, and write after every read.
+std::vector<char> swaps_in_place(const Program& p, const rg_run_desc* d) {
+  std::vector<char> in_place((size_t)d->n_swaps, 0);
+  for (int64_t k = 0; k < d->n_swaps; k++) {
+    const int64_t is = d->swaps[2 * k], os = d->swaps[2 * k + 1];
+    bool fits = false, other = false;
+    for (const auto& st : p.plan.steps) {
+      const auto reads = step_reads(st), writes = step_writes(st);
+      const auto named = [&](int64_t s) { return std::count(reads.begin(), reads.end(), s) + std::count(writes.begin(), writes.end(), s); };
+      const auto n_in = named(is), n_out = named(os);
+      if (n_in == 0 && n_out == 0) continue;
+      bool here = st.kind == RG_STEP_INSTR && st.instr.op == RG_OP_PAGED_ATTENTION && n_in == 1 && n_out == 1;
+      if (here) {
+        const Sequence q = sequence_of(st.instr);
+        here = false;
+        for (const auto& o : st.instr.outs)
+          if (o.second == os) here = (o.first == 1 && st.instr.args[(size_t)q.k_pages].slot == is) || (o.first == 2 && st.instr.args[(size_t)q.v_pages].slot == is);
+      }
+      if (here && !fits) fits = true;
+      else other = true;
+    }
+    for (const auto& c : p.control)
+      if (c)
+        for (const auto& r : c->attr.results) other = other || r.second == is || r.second == os;
+    for (const auto& c : p.plan.consts) other = other || c.slot == is || c.slot == os;
+    int64_t inputs = 0, outputs = 0;
+    for (const auto& in : p.plan.inputs) {
+      inputs += in.first == is;
+      other = other || in.first == os;
+    }
+    for (const auto& o : p.plan.outputs) {
+      outputs += o.slot == os;
+      other = other || o.slot == is;
+    }
+    for (int64_t c = 0; c < d->n_copies; c++)
+      for (int64_t s : {d->copies[3 * c], d->copies[3 * c + 1]}) other = other || s == is || s == os;
+    for (int64_t j = 0; j < d->n_data; j++) other = other || d->data_slots[j] == is || d->data_slots[j] == os;
+    for (int64_t h = 0; h < d->n_history; h++) other = other || d->history_slots[h] == is || d->history_slots[h] == os;
+    in_place[(size_t)k] = fits && !other && inputs == 1 && outputs == 1;
+  }
+  return in_place;
+}
+
+// The two slot tables a run alternates between: `start`, and `start` with every swap applied but
+// those made in place, whose state stays in the buffer that it started in; and the tables that the
+// steps run under, where both slots of a swap made in place name that buffer.
+void run_tables(const Program& p, const std::vector<void*>& start, const rg_run_desc* d, std::vector<void*> out[2], std::vector<void*> steps[2]) {
+  const std::vector<char> in_place = swaps_in_place(p, d);
+  for (int g = 0; g < 2; g++) {
+    out[g] = start;
+    for (int64_t k = 0; k < d->n_swaps && g == 1; k++)
+      if (!in_place[(size_t)k]) std::swap(out[g][(size_t)d->swaps[2 * k]], out[g][(size_t)d->swaps[2 * k + 1]]);
+    steps[g] = out[g];
+    for (int64_t k = 0; k < d->n_swaps; k++)
+      if (in_place[(size_t)k]) steps[g][(size_t)d->swaps[2 * k + 1]] = steps[g][(size_t)d->swaps[2 * k]];
+  }
 }
 
 }  // namespace
@@ -2731,7 +2785,7 @@ int rg_hip_exec_run(void* exec, const rg_run_desc* d, rg_run_result* out) {
     key.insert(key.end(), d->data_slots, d->data_slots + d->n_data);
     for (int64_t j = 0; j < d->n_data; j++) key.push_back((int64_t)d->data_bytes[j]);
     key.insert(key.end(), d->history_slots, d->history_slots + d->n_history);
-    auto tables_from = [&](const std::vector<void*>& start) { run_tables(start, d, rc.table); };
+    auto tables_from = [&](const std::vector<void*>& start) { run_tables(*p, start, d, rc.table, rc.steps); };
     if (rc.key != key) {
       rc.release();
       // One allocation: the run buffers, then the snapshot of the changing state slots.
@@ -2758,7 +2812,7 @@ int rg_hip_exec_run(void* exec, const rg_run_desc* d, rg_run_result* out) {
     }
     // Step k (counted from this run's start) runs under table (parity + k) % n_graphs.
     const int parity = f->slot == rc.table[0] ? 0 : 1;
-    auto enqueue_step = [&](int g) { enqueue_run_step(*p, f->stream, f->workspace, d, rc.buf, rc.table[g], rc.table[(g + 1) % n_graphs]); };
+    auto enqueue_step = [&](int g) { enqueue_run_step(*p, f->stream, f->workspace, d, rc.buf, rc.steps[g], rc.steps[(g + 1) % n_graphs]); };
     // Each slot table is captured once as a HIP graph and replayed; RG_HIP_GRAPHS=0 launches the
     // same kernels directly instead (for tools that do not follow graph launches).
     const char* env = getenv("RG_HIP_GRAPHS");
@@ -2903,8 +2957,8 @@ int rg_hip_exec_run_noalloc(void* exec, const rg_run_desc* d, rg_run_result* out
   }
   const RunBuffers b = lay.place(base);
   const int n_tables = d->n_swaps > 0 ? 2 : 1;
-  std::vector<void*> table[2];
-  run_tables(f->slot, d, table);
+  std::vector<void*> table[2], steps[2];
+  run_tables(*p, f->slot, d, table, steps);
   int result = 0;
   int64_t enqueued = 0, done = 0;
   try {
@@ -2919,7 +2973,7 @@ int rg_hip_exec_run_noalloc(void* exec, const rg_run_desc* d, rg_run_result* out
         result = -1;
         break;
       }
-      enqueue_run_step(*p, f->stream, f->workspace, d, b, table[k % n_tables], table[(k + 1) % n_tables]);
+      enqueue_run_step(*p, f->stream, f->workspace, d, b, steps[k % n_tables], steps[(k + 1) % n_tables]);
       if (latch(e, hipGetLastError(), "step launch")) {
         result = -1;
         break;

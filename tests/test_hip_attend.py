@@ -40,3 +40,165 @@ def test_norm(sizes, dtype):
     # Sums of squares in 64 bits: at most the number of terms in roundings of 2^-53, far below one of
     # float32; the root halves them.
     assert abs(got - want) <= (np.finfo(dtype).eps + sum(sizes) * 2.0 ** -53) * want
+
+
+# ---- step loops ---------------------------------------------------------------------------------------
+
+def _tokens(seed=0, batch=3, dtype="float32"):
+    """A cache, the tokens to go on from, and a step that reads and appends and makes the next tokens."""
+    r = np.random.default_rng(seed)
+    h, g, hd, page, n = 4, 2, 24, 7, 6
+    pages = r.permutation(batch * n + 1)[:batch * n].reshape(batch, n).astype(np.int32)
+    state = {"x": r.standard_normal((batch, 1, h + 2 * g, hd)), "k": r.standard_normal((batch * n + 1, page, g, hd)),
+             "v": r.standard_normal((batch * n + 1, page, g, hd)), "first": np.array([20, 0, 6][:batch], np.int32)}
+    state = {k: rg.tensor(v if v.dtype == np.int32 else v.astype(dtype)) for k, v in state.items()}
+    data = {"table": rg.tensor(pages), "drive": rg.tensor(r.standard_normal((batch, 1, h + 2 * g, hd)).astype(dtype))}
+
+    def step(s, data):
+        y, (k, v) = rg.paged_attention(s["x"], cache=(s["k"], s["v"]), table=data["table"], first=s["first"], heads=(h, g), cap=9.0)
+        x = rg.tanh(0.5 * rg.concatenate([y, y], axis=2) + data["drive"])
+        return {"x": x, "k": k, "v": v, "first": s["first"] + 1}
+
+    return state, data, step
+
+
+def _same(got, want):
+    for k in want:
+        assert np.array_equal(got[k].numpy(), want[k].numpy(), equal_nan=True), k
+
+
+def _one_by_one(step, state, data, steps):
+    program = rg.compile(step, (state, data), validate="none")
+    for _ in range(steps):
+        out = program(state, data)
+        state = out[0] if isinstance(out, tuple) else out
+    return state
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("kind", ["carried", "watched", "read twice"])
+def test_a_cache_carried_by_a_loop(kind, dtype, monkeypatch):
+    """The loop writes new rows where the pages are, unless something else reads them; either way it does
+    what single calls do, in one run and in several, also of an odd number of steps."""
+    state, data, plain = _tokens(dtype=dtype)
+    seen = {"carried": lambda s, new: new["x"].sum(), "watched": lambda s, new: (new["x"].sum() + s["k"].sum(), s["v"]),
+            "read twice": lambda s, new: (rg.paged_attention(s["x"], cache=(s["k"], s["k"]), table=data["table"], first=s["first"], heads=(4, 2))[0]).sum()}[kind]
+
+    def step(s, data):
+        new = plain(s, data)
+        return new, seen(s, new)
+
+    want = _one_by_one(step, state, data, 7)
+    program = rg.compile(step, (state, data), validate="none")
+    _same(rg.run(program, state, [data], steps=7).state, want)
+    now = state
+    for steps in (3, 1, 2, 1):
+        now = rg.run(program, now, [data], steps=steps).state
+        float(rg.ones(5).sum())  # the program's own work between
+    _same(now, want)
+    monkeypatch.setenv("RG_HIP_GRAPHS", "0")
+    _same(rg.run(program, state, [data], steps=7).state, want)
+
+
+def test_a_cache_in_a_loop_that_stops():
+    """A value that is not finite ends the run after its step; the pages are those of that step."""
+    state, data, plain = _tokens(1)
+
+    def step(s, data):
+        new = plain(s, data)
+        return new, 1.0 / (24 - new["first"][0]).cast("float32")
+
+    program = rg.compile(step, (state, data), validate="none")
+    r = rg.run(program, state, [data], steps=90)
+    assert len(r.history["aux"]) == 4
+    _same(r.state, _one_by_one(plain, state, data, 4))
+
+
+def test_cycled_tables_and_batches():
+    """A table for every step: rows go where the step's own table says."""
+    state, data, step = _tokens(2)
+    other = {**data, "table": rg.tensor(data["table"].numpy()[::-1].copy())}
+    program = rg.compile(step, (state, data), validate="none")
+    want = state
+    for k in range(5):
+        want = program(want, (data, other)[k % 2])
+    _same(rg.run(program, state, [data, other], steps=5).state, want)
+
+
+def test_rows_written_twice_keep_the_later_sequence():
+    for seed in range(3):
+        case = (6, 3, 2, 1, 16, 4, 3, "j", 0)
+
+        def share(v):
+            r = np.random.default_rng(seed)
+            v["table"][:] = r.integers(0, 5, v["table"].shape)
+            v["first"][:] = r.integers(0, 10, 6)
+
+        v = ref.paged_inputs(case, np.dtype("float32"))
+        share(v)
+        x = ref.paged_given(case, v)
+        _, (k, held) = rg.compile(lambda x: ref.paged_call(case, x), (x,), validate="none")(x)
+        _, _, want_k, want_v = ref.paged_expected(case, v, np.dtype("float32"))
+        assert np.array_equal(k.numpy(), want_k) and np.array_equal(held.numpy(), want_v)
+
+
+def test_training_loop_with_every_mask_and_the_clip():
+    """Captured and replayed steps against the same steps one by one."""
+    case = (3, 75, 4, 2, 40, "jcsdpl", 7.0)
+    v = ref.inputs(case, np.dtype("float32"))
+    x = {"x": rg.tensor(np.concatenate([v["q"], v["k"], v["v"]], axis=2)), "slopes": rg.tensor(v["slopes"])}
+    t = rg.tensor(v["dy"])
+
+    def step(s, t):
+        def loss(s):
+            off = ref.call(case, s, v) - t
+            return (off * off).sum()
+
+        value, grads = rg.value_and_grad(loss)(s)
+        grads, norm = optim.clip_gradients(grads, 3.0)
+        return {k: s[k] - 0.05 * grads[k] for k in s}, (value, norm)
+
+    program = rg.compile(step, (x, t), validate="none")
+    run = rg.run(program, x, [t], steps=6)
+    s, losses, norms = x, [], []
+    for _ in range(6):
+        s, (value, norm) = program(s, t)
+        losses.append(float(value))
+        norms.append(float(norm))
+    _same(run.state, s)
+    assert run.history["aux.0"] == losses and run.history["aux.1"] == norms
+    _same(rg.run(program, x, [t], steps=6).state, s)
+
+
+def test_attention_inside_a_scan_body():
+    case = (2, 37, 2, 1, 32, "jcd", 4.0)
+    v = ref.inputs(case, np.dtype("float32"))
+    x = rg.tensor(np.concatenate([v["q"], v["k"], v["v"]], axis=2))
+    body = lambda c, _: (rg.concatenate([ref.call(case, {"x": c}, v), c[:, :, 2:]], axis=2), c[:, :, :1].sum())
+    direct = x
+    for _ in range(3):
+        direct = rg.compile(lambda c: body(c, None)[0], (direct,), validate="none")(direct)
+    looped, _ = rg.compile(lambda c: rg.scan(body, c, rg.zeros(3)), (x,), validate="none")(x)
+    assert np.array_equal(looped.numpy(), direct.numpy())
+
+
+def test_tokens_continue_what_attention_reads_at_once():
+    """Prompt in a chunk, then token by token over the pages: the rows of one attention over all."""
+    r = np.random.default_rng(4)
+    b, t, h, g, hd, page = 2, 45, 4, 2, 32, 8
+    x = r.standard_normal((b, t, h + 2 * g, hd)).astype(F)
+    slopes = rg.tensor(np.array([0.5, 0.2, 0.1, 0.05], F))
+    whole = rg.attention(rg.tensor(x), heads=(h, g), cap=6.0, slopes=slopes).numpy()
+    cache = tuple(rg.zeros((b * 6, page, g, hd)) for _ in range(2))
+    table = rg.tensor(r.permutation(b * 6).reshape(b, 6).astype(np.int32))
+    out, at = [], 0
+    for n in (30, 1, 1, 5, 1, 7):
+        first = rg.tensor(np.full(b, at, np.int32))
+        y, cache = rg.paged_attention(rg.tensor(x[:, at:at + n].copy()), cache=cache, table=table, first=first, heads=(h, g), cap=6.0, slopes=slopes)
+        out.append(y.numpy())
+        at += n
+    case = (b, t, h, g, hd, "jcs", 6.0)
+    v = {"q": x[:, :, :h], "k": x[:, :, h:h + g], "v": x[:, :, h + g:], "slopes": slopes.numpy(), "documents": None, "prefix": None, "lengths": None}
+    want, off = ref.expected(case, v, np.dtype("float32"), False)
+    ref.agree(np.concatenate(out, axis=1), want["y"], off["y"], np.dtype("float32"), "y")
+    ref.agree(whole, want["y"], off["y"], np.dtype("float32"), "y")
