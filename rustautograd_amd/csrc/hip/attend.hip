@@ -62,14 +62,14 @@ struct Type<float> {
     q = fmaf(q, z, -3.333327770233154e-1f);
     return fmaf(q, x * z, x);
   }
-  // Of any size: past 1, (e^2x - 1) / (e^2x + 1).
+  // Of any size: below 0.7 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 +
+  // ...)), off by 2e-9 of it there, from there on (e^2x - 1) / (e^2x + 1), with one division.
   static __device__ __forceinline__ float tanh_of(float x) {
-    const float a = fminf(fabsf(x), 16.0f), e = __builtin_amdgcn_exp2f(2.8853900817779268f * a), num = e - 1.0f, den = e + 1.0f;
+    const float a = fminf(fabsf(x), 16.0f), z = a * a, e = __builtin_amdgcn_exp2f(2.8853900817779268f * a);
+    const bool low = a < 0.7f;
+    const float num = low ? a * fmaf(z, z + 105.0f, 945.0f) : e - 1.0f, den = low ? fmaf(z, fmaf(15.0f, z, 420.0f), 945.0f) : e + 1.0f;
     const float r = __builtin_amdgcn_rcpf(den), q = num * r, t = fmaf(fmaf(-den, q, num), r, q);
-    // Both are formed: of a branch for each of a tile's scores the compiler makes eight.
-    float low = tanh_low(x);
-    asm volatile("" : "+v"(low));
-    return fabsf(x) > 1.0f ? copysignf(t, x) : low;
+    return copysignf(x == x ? t : x, x);
   }
   static constexpr bool LOW = true;
 };
@@ -104,16 +104,21 @@ __device__ __forceinline__ T row_sum(T x) {
   return a + b;
 }
 
-constexpr int ROWS = 64, TILE = 32;  // rows of a block, rows of a wave's tile
+constexpr int TILE = 32;  // rows of the other side in a wave's tile
 
-// Sets of four waves in a block, and rows of the other side that they stage at once. Two sets where
-// their registers (256 a lane) hold the fragments and results; one for wider heads.
-template <class T, int HD>
+// A block's waves: RW of them take 16 rows each, in SETS sets, and each set has a tile of its own of the
+// STAGE rows staged at once. Eight waves where four fit a SIMD (two blocks a CU), else four, of which two
+// fit, in blocks of their own.
+template <class T, int HD, int RW_>
 struct Geo {
-  static constexpr int SETS = (int)sizeof(T) * HD <= 512 ? 2 : 1, NT = 256 * SETS, STAGE = TILE * SETS;
+  static constexpr int SIZE = (int)sizeof(T) * HD, RW = RW_;
+  static constexpr bool NARROW = SIZE <= 256;
+  static constexpr int WAVES = NARROW ? 8 : 4, SETS = WAVES / RW, NT = 64 * WAVES, ROWS = 16 * RW, STAGE = TILE * SETS;
   // Waves a SIMD that the registers are to leave room for.
-  static constexpr int WAVES = (int)sizeof(T) * HD <= 256 && sizeof(T) == 4 ? 4 : (int)sizeof(T) * HD <= 512 ? 2 : 1;
-  static constexpr int GRAD_WAVES = (int)sizeof(T) * HD <= 128 ? 4 : (int)sizeof(T) * HD <= 512 ? 2 : 1;
+  static constexpr int FORWARD = SIZE <= 256 && sizeof(T) == 4 ? 4 : SIZE <= 512 ? 2 : 1;
+  static constexpr int BACKWARD = SIZE <= 256 && sizeof(T) == 4 ? (SIZE == 256 && RW == 2 ? 2 : 4) : SIZE <= 512 && sizeof(T) == 4 ? 2 : SIZE <= 256 ? 2 : 1;
+  // The backward's own rows lie in LDS and not in registers.
+  static constexpr bool KEPT = NARROW && sizeof(T) == 4;
 };
 
 // Rows of HD values in LDS lie 16 bytes further apart than that: 16 lanes reading 16 bytes of 16
@@ -170,19 +175,36 @@ __device__ __forceinline__ void row_frag(const T* row, int g, uint32_t head, boo
     }
 }
 
-// Two score tiles (rows 0..15 and 16..31 of `lds` against the lane's row).
+// A lane's row as the fragments of a product over the head: in registers, or in LDS where the waves of
+// all sets share it.
 template <class T, int HD>
-__device__ __forceinline__ void score(const T* lds, int l16, int g, const T* frag, typename Type<T>::acc* s) {
+struct Registers {
+  T frag[HD / 4];
+  __device__ __forceinline__ void get(int n, T* out) const {
+#pragma unroll
+    for (int j = 0; j < 4; j++) out[j] = frag[4 * n + j];
+  }
+};
+template <class T, int HD>
+struct Kept {
+  const T* at;  // the row's place 4 g
+  __device__ __forceinline__ void get(int n, T* out) const { take<4>(at + n * 16, out); }
+};
+
+// Two score tiles (rows 0..15 and 16..31 of `lds` against the lane's row).
+template <class T, int HD, class F>
+__device__ __forceinline__ void score(const T* lds, int l16, int g, const F& own, typename Type<T>::acc* s) {
   s[0] = s[1] = typename Type<T>::acc{0, 0, 0, 0};
 #pragma unroll
   for (int n = 0; n < HD / 16; n++) {
-    T a[4], b[4];
+    T a[4], b[4], x[4];
     take<4>(lds + l16 * PITCH<T, HD> + n * 16 + 4 * g, a);
     take<4>(lds + (16 + l16) * PITCH<T, HD> + n * 16 + 4 * g, b);
+    own.get(n, x);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      s[0] = Type<T>::mfma(a[j], frag[4 * n + j], s[0]);
-      s[1] = Type<T>::mfma(b[j], frag[4 * n + j], s[1]);
+      s[0] = Type<T>::mfma(a[j], x[j], s[0]);
+      s[1] = Type<T>::mfma(b[j], x[j], s[1]);
     }
   }
 }
@@ -295,6 +317,8 @@ struct Sight {
     causal = a.causal;
   }
   __device__ __forceinline__ int document(int i) const { return i >= length ? -1 : documents ? documents[i] : 0; }
+  // Position i's document, of which `doc` is the one that LDS holds where there are documents.
+  __device__ __forceinline__ int in(int i, int doc) const { return documents ? doc : i < length ? 0 : -1; }
   // With the documents of both at hand; those of no sequence are negative.
   __device__ __forceinline__ bool sees(int i, int di, int j, int dj) const { return di >= 0 && di == dj && (!causal || j <= i || j < prefix); }
   // Whether every query from i on that there is sees every key of [j, end).
@@ -313,7 +337,7 @@ __device__ __forceinline__ int wave_min(int x) {
 
 // The stages of the other side, [from, end) of them, that may hold a position of the documents of a
 // block's rows; all of them without documents. Every thread of the block calls it alike.
-template <int STAGE, int NT>
+template <class G>
 struct Stages {
   const Sight& sight;
   int low, high;  // documents of the rows
@@ -321,10 +345,10 @@ struct Stages {
   int chunk = -1;  // of 64 stages
   uint64_t live = 0;
   uint64_t* shared;
-  static constexpr int WAVES = NT / 64;
+  static constexpr int STAGE = G::STAGE, WAVES = G::WAVES;
   __device__ __forceinline__ Stages(const Sight& s, int rows, int from_, int end_, uint64_t* shared_) : sight(s), from(from_), end(end_), shared(shared_) {
     if (!sight.documents) return;
-    const int d = sight.document(rows + (int)(threadIdx.x & 63));
+    const int d = sight.document(rows + (int)(threadIdx.x & 63) % G::ROWS);
     low = wave_min(d < 0 ? 0x7fffffff : d);
     high = -wave_min(-max(d, -1));
   }
@@ -363,12 +387,94 @@ struct Stages {
   }
 };
 
-// Rows of the other side on their way to LDS, of two operands, 16 bytes a thread and step. Loads
-// are of rows and columns that there are; what does not belong is made 0 as it is stored.
-template <class T, int HD>
+// Sixteen bytes of a buffer, and one value, 0 past its end. The whole place is the vector offset: a
+// scalar one past the end would be taken from the buffer's size without a check.
+template <class T>
+__device__ __forceinline__ typename Type<T>::vec buffer_vec(__amdgpu_buffer_rsrc_t from, uint32_t at) {
+  typedef uint32_t words __attribute__((ext_vector_type(4)));
+  const words w = __builtin_amdgcn_raw_buffer_load_b128(from, (int)at, 0, 0);
+  return __builtin_bit_cast(typename Type<T>::vec, w);
+}
+__device__ __forceinline__ float buffer_value(__amdgpu_buffer_rsrc_t from, uint32_t at, float) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(from, (int)at, 0, 0));
+}
+__device__ __forceinline__ double buffer_value(__amdgpu_buffer_rsrc_t from, uint32_t at, double) {
+  typedef uint32_t words __attribute__((ext_vector_type(2)));
+  const words w = __builtin_amdgcn_raw_buffer_load_b64(from, (int)at, 0, 0);
+  return __builtin_bit_cast(double, w);
+}
+
+// N rows of one operand on their way to LDS, 16 bytes a thread and step. They are read as a buffer that
+// ends with the sequence, and columns past the head from past its end, so that what does not belong
+// is 0 as it arrives, with no selection that would wait for it.
+template <class T, int HD, class G, int N = G::STAGE>
 struct Staged {
-  static constexpr int V = Type<T>::V, NT = Geo<T, HD>::NT, PER = Geo<T, HD>::STAGE * HD / V / NT;
-  static_assert(PER * NT * V == Geo<T, HD>::STAGE * HD, "whole steps");
+  static constexpr int V = Type<T>::V, NT = G::NT, LANES = HD / V, PER = N * LANES / NT;
+  // Where all of a thread's steps have one column, its place is held once.
+  static constexpr bool EVEN = NT % LANES == 0;
+  static_assert(PER * NT == N * LANES, "whole steps");
+  typedef typename Type<T>::vec vec;
+  static constexpr uint32_t OUTSIDE = 0x80000000u;  // past a stage's rows (lower_attend)
+  vec x[PER];
+  uint32_t at[EVEN ? 1 : PER], pitch;
+  static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * NT) / LANES; }
+  static __device__ __forceinline__ uint32_t column(int i) { return (uint32_t)(((int)threadIdx.x + i * NT) % LANES) * V; }
+  // `step` values from one row to the next.
+  __device__ __forceinline__ Staged(int64_t step, uint32_t head) : pitch((uint32_t)step * (uint32_t)sizeof(T)) {
+#pragma unroll
+    for (int i = 0; i < (EVEN ? 1 : PER); i++) at[i] = column(i) < head ? (uint32_t)row(i) * pitch + column(i) * (uint32_t)sizeof(T) : OUTSIDE;
+  }
+  // The rows from `p` on, of which `rows` are there.
+  __device__ __forceinline__ void load(const T* p, int rows, uint32_t head, bool whole) {
+    const uint64_t bytes = rows > 0 ? (uint64_t)(min(rows, N) - 1) * pitch + head * sizeof(T) : 0;
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const uint32_t place = EVEN ? at[0] + (uint32_t)(i * (NT / LANES)) * pitch : at[i];
+      if (whole) {
+        x[i] = buffer_vec<T>(from, place);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < V; j++)
+          x[i][j] = buffer_value(from, column(i) + j < head ? place + j * (uint32_t)sizeof(T) : OUTSIDE, (T)0);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* xs) const {
+#pragma unroll
+    for (int i = 0; i < PER; i++) *(vec*)(xs + row(i) * PITCH<T, HD> + (int)column(i)) = x[i];
+  }
+  // Makes 0, once they are there, the rows whose entry in `docs` is negative.
+  static __device__ __forceinline__ void clear(T* xs, const int* docs) {
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (docs[row(i)] < 0) *(vec*)(xs + row(i) * PITCH<T, HD> + (int)column(i)) = 0;
+  }
+};
+
+// The end of a stage's arrival in LDS, for the whole block: its documents, where there are any, go to
+// `docs`, and the rows of none are made 0.
+template <class T, int HD, class G>
+__device__ __forceinline__ void settle(const Sight& sight, int first, int doc, int* docs, T* xs, T* ys) {
+  if (!sight.documents) {
+    __syncthreads();
+    return;
+  }
+  const bool mine = threadIdx.x < G::STAGE;
+  if (mine) docs[threadIdx.x] = doc;
+  if (__syncthreads_or(mine && doc < 0 && first + (int)threadIdx.x < sight.length)) {
+    Staged<T, HD, G>::clear(xs, docs);
+    Staged<T, HD, G>::clear(ys, docs);
+    __syncthreads();
+  }
+}
+
+// Rows of two operands anywhere in memory on their way to LDS. Loads are of rows and columns that there
+// are; what does not belong is made 0 as it is stored.
+template <class T, int HD, class G>
+struct Gathered {
+  static constexpr int V = Type<T>::V, NT = G::NT, PER = G::STAGE * HD / V / NT;
+  static_assert(PER * NT * V == G::STAGE * HD && PER <= 32, "whole steps");
   typedef typename Type<T>::vec vec;
   vec x[PER], y[PER];
   uint32_t off;  // bit i: step i is not there
@@ -421,12 +527,17 @@ struct RowAt {
   bool there;
 };
 
-// A block's head and tile of rows: the heads of a batch next to each other, so that blocks of one
-// head meet in the same L2 where their number is a multiple of the eight dies, and the tiles with the
-// most work under a causal order first (`last_first`).
+// A block's head and tile of rows. Heads of a batch lie next to each other, so that blocks of one head
+// meet in the same L2 where their number is a multiple of the eight dies. Under a causal order the tiles
+// with the most work come first (`last_first`: the last), so that short ones fill up at the end; where
+// two blocks share a CU (`paired`), every second round of as many blocks as there are CUs runs the other
+// way, since they all start at once and a long and a short one are to meet.
+constexpr uint32_t CUS = 256;
 struct Place {
   uint32_t b, h, tile;
-  __device__ __forceinline__ Place(uint32_t at, uint32_t batch, uint32_t heads, uint32_t tiles, bool last_first) {
+  __device__ __forceinline__ Place(uint32_t at, uint32_t batch, uint32_t heads, uint32_t tiles, bool last_first, bool paired) {
+    const uint32_t blocks = batch * heads * tiles, round = at / CUS * CUS;
+    if (paired && round / CUS % 2 == 1) at = round + min(CUS, blocks - round) - 1 - (at - round);
     const uint32_t bh = at % (batch * heads), n = at / (batch * heads);
     b = bh / heads;
     h = bh % heads;
@@ -477,97 +588,132 @@ struct Running {
   }
 };
 
-// Set 1's share of a lane's results, added to set 0's through LDS; `buffer` holds 64 HD values.
-template <class T, int HD>
+// The sets' shares of a lane's results, added up in set 0 in the sets' order through LDS; `buffer`
+// holds G::ROWS * HD values.
+template <class T, int HD, class G>
 __device__ __forceinline__ void join(typename Type<T>::acc* out, T* buffer, int set) {
-  const int at = (int)threadIdx.x & 255;
-  __syncthreads();
-  if (set == 1)
+  constexpr int N = 64 * G::RW;
+  const int at = (int)threadIdx.x % N;
 #pragma unroll
-    for (int n = 0; n < HD / 16; n++)
+  for (int other = 1; other < G::SETS; other++) {
+    __syncthreads();
+    if (set == other)
 #pragma unroll
-      for (int r = 0; r < 4; r++) buffer[(n * 4 + r) * 256 + at] = out[n][r];
-  __syncthreads();
-  if (set == 0)
+      for (int n = 0; n < HD / 16; n++)
 #pragma unroll
-    for (int n = 0; n < HD / 16; n++)
+        for (int r = 0; r < 4; r++) buffer[(n * 4 + r) * N + at] = out[n][r];
+    __syncthreads();
+    if (set == 0)
 #pragma unroll
-      for (int r = 0; r < 4; r++) out[n][r] += buffer[(n * 4 + r) * 256 + at];
+      for (int n = 0; n < HD / 16; n++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) out[n][r] += buffer[(n * 4 + r) * N + at];
+  }
 }
 // The same of running softmaxes: afterwards set 0 has the whole.
-template <class T, int HD>
+template <class T, int HD, class G>
 __device__ __forceinline__ void join(Running<T, HD>& run, T* buffer, T* tops, T* sums, int set) {
+  constexpr int N = 64 * G::RW;
+  const int at = (int)threadIdx.x % N;
   tops[threadIdx.x] = run.top;
   sums[threadIdx.x] = run.sum;
   __syncthreads();
-  const T other = tops[threadIdx.x ^ 256], top = Type<T>::max_of(run.top, other), base = Running<T, HD>::base(top);
+  T top = tops[at];
+#pragma unroll
+  for (int other = 1; other < G::SETS; other++) top = Type<T>::max_of(top, tops[other * N + at]);
+  const T base = Running<T, HD>::base(top);
   run.scale(Type<T>::exp2_of(run.top - base));
-  run.sum += sums[threadIdx.x ^ 256] * Type<T>::exp2_of(other - base);
   run.top = top;
-  join<T, HD>(run.out, buffer, set);
+  run.sum = 0;
+#pragma unroll
+  for (int other = 0; other < G::SETS; other++) run.sum += sums[other * N + at] * Type<T>::exp2_of(tops[other * N + at] - base);
+  join<T, HD, G>(run.out, buffer, set);
 }
 
-// A query's share in its 64: set, row and the wave's first row.
+// A lane's set, its row among the block's and the wave's first row.
+template <int RW>
 struct Lane {
   int l16, g, set, row, first;
   __device__ __forceinline__ Lane() {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     l16 = lane & 15;
     g = lane >> 4;
-    set = wave >> 2;
-    first = (wave & 3) * 16;
+    set = wave / RW;
+    first = wave % RW * 16;
     row = first + l16;
   }
 };
 
-template <class T, int HD>
-__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_attend(AttendArgs a) {
+// A block's own rows, in registers or in LDS (Geo::KEPT).
+template <class T, int HD, class G>
+struct Own {
+  T* kept;
+  Registers<T, HD> held;
+  __device__ __forceinline__ Own(T* k) : kept(k) {}
+  __device__ __forceinline__ void set(const T* x, const Lane<G::RW>& l) {
+    if constexpr (G::KEPT) {
+      if (l.set == 0)
+#pragma unroll
+        for (int n = 0; n < HD / 16; n++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) kept[l.row * PITCH<T, HD> + n * 16 + 4 * l.g + j] = x[4 * n + j];
+    } else {
+#pragma unroll
+      for (int n = 0; n < HD / 4; n++) held.frag[n] = x[n];
+    }
+  }
+  __device__ __forceinline__ auto of(const Lane<G::RW>& l) const {
+    if constexpr (G::KEPT) return Kept<T, HD>{kept + l.row * PITCH<T, HD> + 4 * l.g};
+    else return held;
+  }
+};
+
+template <class T, int HD, int RW>
+__global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_attend(AttendArgs a) {
+  typedef Geo<T, HD, RW> G;
   typedef typename Type<T>::acc acc;
-  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  constexpr int STAGE = G::STAGE, SETS = G::SETS, NT = G::NT, ROWS = G::ROWS;
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
   __shared__ __align__(16) int docs[STAGE];
-  __shared__ T tops[SETS == 2 ? 512 : 1], sums[SETS == 2 ? 512 : 1];
+  __shared__ T tops[SETS > 1 ? NT : 1], sums[SETS > 1 ? NT : 1];
   __shared__ uint64_t found[NT / 64];
   T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
-  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal);
+  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal, G::FORWARD * 4 == 2 * G::WAVES);
   const Sight sight(a, at.b);
-  const Lane l;
+  const Lane<RW> l;
   const int begin = (int)at.tile * ROWS, i = begin + l.row, i0 = begin + l.first;
   const uint32_t kh = at.h / (a.heads / a.keys);
   const bool whole = a.head % Type<T>::V == 0;
   const Scorer<T> scorer(a, at.h);
   const int di = sight.document(i);
-  T frag[HD / 4];
-  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, l.g, a.head, whole, frag);
+  Registers<T, HD> own;
+  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, l.g, a.head, whole, own.frag);
   const T *kb = (const T*)a.k + (int64_t)at.b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)at.b * a.length * a.k_row + kh * a.head;
   const int end = begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
   const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
-  Stages<STAGE, NT> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
+  Stages<G> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
   Running<T, HD> run;
-  Staged<T, HD> next;
+  Staged<T, HD, G> next_k(a.k_row, a.head), next_v(a.k_row, a.head);
   int doc = 0;
   auto load = [&](int stage) {
     const int first = stage * STAGE;
-    next.load(kb, vb, [&](int r) {
-      const int j = min(first + r, sight.length - 1);
-      const bool in = first + r < sight.length && (!sight.documents || sight.documents[j] >= 0);
-      return RowAt{j * a.k_row, j * a.k_row, in};
-    }, a.head, whole);
-    if (threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
+    next_k.load(kb + first * a.k_row, sight.length - first, a.head, whole);
+    next_v.load(vb + first * a.k_row, sight.length - first, a.head, whole);
+    if (sight.documents && threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
   };
   int k = stages.at(0);
   if (k < stages.end) load(k);
   while (k < stages.end) {
     __syncthreads();
-    next.store(ks, vs);
-    if (threadIdx.x < STAGE) docs[threadIdx.x] = doc;
-    __syncthreads();
+    next_k.store(ks);
+    next_v.store(vs);
+    settle<T, HD, G>(sight, k * STAGE, doc, docs, ks, vs);
     const int here = k, first = here * STAGE + l.set * TILE;
     k = stages.at(here + 1);
     if (k < stages.end) load(k);
     if (first >= seen_to) continue;
     acc s[2];
-    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, own, s);
     scorer.template operator()<false>(s, nullptr, i - (first + Type<T>::row_of(0, l.g)));
     if (!sight.all_see(i0, first + TILE)) {
 #pragma unroll
@@ -575,14 +721,14 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_atten
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           const int row = 16 * t + Type<T>::row_of(r, l.g);
-          s[t][r] = sight.sees(i, di, first + row, docs[l.set * TILE + row]) ? s[t][r] : -(T)__builtin_huge_val();
+          s[t][r] = sight.sees(i, di, first + row, sight.in(first + row, docs[l.set * TILE + row])) ? s[t][r] : -(T)__builtin_huge_val();
         }
     }
     run.add(s);
     weigh<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, run.out);
   }
   run.sum = row_sum(run.sum);
-  if constexpr (SETS == 2) join(run, smem, tops, sums, l.set);
+  if constexpr (SETS > 1) join<T, HD, G>(run, smem, tops, sums, l.set);
   if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h;
   const bool none = run.sum == 0 || di < 0;
@@ -593,70 +739,74 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_atten
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others.
-template <class T, int HD>
-__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_attend_dq(AttendArgs a) {
+template <class T, int HD, int RW>
+__global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dq(AttendArgs a) {
+  typedef Geo<T, HD, RW> G;
   typedef typename Type<T>::acc acc;
-  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  constexpr int STAGE = G::STAGE, SETS = G::SETS, NT = G::NT, ROWS = G::ROWS;
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) T kept[G::KEPT ? 2 * ROWS * PITCH<T, HD> : 4];
   __shared__ __align__(16) int docs[STAGE];
   __shared__ T waves[NT / 64];
   __shared__ uint64_t found[NT / 64];
   T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
-  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal);
+  const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal, G::BACKWARD * 4 == 2 * G::WAVES);
   const Sight sight(a, at.b);
-  const Lane l;
+  const Lane<RW> l;
   const int begin = (int)at.tile * ROWS, i = begin + l.row, i0 = begin + l.first;
   const uint32_t kh = at.h / (a.heads / a.keys);
   const bool whole = a.head % Type<T>::V == 0;
   const Scorer<T> scorer(a, at.h);
   const int di = sight.document(i);
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h, stat = ((uint64_t)at.b * a.heads + at.h) * a.length + i;
-  T frag[HD / 4], grad[HD / 4];
-  row_frag<T, HD>(di >= 0 ? (const T*)a.dy + row * a.head : nullptr, l.g, a.head, whole, grad);
+  const T *qb = (const T*)a.q + (int64_t)at.b * a.length * a.q_row + at.h * a.head, *gb = (const T*)a.dy + ((int64_t)at.b * a.length * a.heads + at.h) * a.head;
+  const T* yb = (const T*)a.y_in + ((int64_t)at.b * a.length * a.heads + at.h) * a.head;
   T dot = 0;
+  Own<T, HD, G> own(kept), grad(kept + (G::KEPT ? ROWS * PITCH<T, HD> : 0));
   {
-    T y[HD / 4];
-    row_frag<T, HD>(di >= 0 ? (const T*)a.y_in + row * a.head : nullptr, l.g, a.head, whole, y);
+    // In registers for dy.y; the ones in LDS are there after the first stage's barriers.
+    T y[HD / 4], x[HD / 4];
+    row_frag<T, HD>(di >= 0 ? yb + (int64_t)i * a.heads * a.head : nullptr, l.g, a.head, whole, y);
+    row_frag<T, HD>(di >= 0 ? gb + (int64_t)i * a.heads * a.head : nullptr, l.g, a.head, whole, x);
 #pragma unroll
-    for (int n = 0; n < HD / 4; n++) dot += y[n] * grad[n];
+    for (int n = 0; n < HD / 4; n++) dot += y[n] * x[n];
+    grad.set(x, l);
+    row_frag<T, HD>(di >= 0 ? qb + (int64_t)i * a.q_row : nullptr, l.g, a.head, whole, x);
+    own.set(x, l);
   }
-  row_frag<T, HD>(di >= 0 ? (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head : nullptr, l.g, a.head, whole, frag);
   dot = row_sum(dot);
   const T sums = di >= 0 ? ((const T*)a.sums_in)[stat] : (T)__builtin_huge_val();
   if (l.set == 0 && l.g == 0 && i < (int)a.length) ((T*)a.workspace)[stat] = dot;
   const T *kb = (const T*)a.k + (int64_t)at.b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)at.b * a.length * a.k_row + kh * a.head;
   const int end = (a.dq || a.dslopes_rows) && begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
   const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
-  Stages<STAGE, NT> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
+  Stages<G> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
   acc out[HD / 16];
 #pragma unroll
   for (int n = 0; n < HD / 16; n++) out[n] = acc{0, 0, 0, 0};
   T dslope = 0;
-  Staged<T, HD> next;
+  Staged<T, HD, G> next_k(a.k_row, a.head), next_v(a.k_row, a.head);
   int doc = 0;
   auto load = [&](int stage) {
     const int first = stage * STAGE;
-    next.load(kb, vb, [&](int r) {
-      const int j = min(first + r, sight.length - 1);
-      const bool in = first + r < sight.length && (!sight.documents || sight.documents[j] >= 0);
-      return RowAt{j * a.k_row, j * a.k_row, in};
-    }, a.head, whole);
-    if (threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
+    next_k.load(kb + first * a.k_row, sight.length - first, a.head, whole);
+    next_v.load(vb + first * a.k_row, sight.length - first, a.head, whole);
+    if (sight.documents && threadIdx.x < STAGE) doc = sight.document(first + (int)threadIdx.x);
   };
   int k = stages.at(0);
   if (k < stages.end) load(k);
   while (k < stages.end) {
     __syncthreads();
-    next.store(ks, vs);
-    if (threadIdx.x < STAGE) docs[threadIdx.x] = doc;
-    __syncthreads();
+    next_k.store(ks);
+    next_v.store(vs);
+    settle<T, HD, G>(sight, k * STAGE, doc, docs, ks, vs);
     const int here = k, first = here * STAGE + l.set * TILE;
     k = stages.at(here + 1);
     if (k < stages.end) load(k);
     if (first >= seen_to) continue;
     acc s[2], dp[2], bent[2];
-    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
-    score<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, grad, dp);
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, own.of(l), s);
+    score<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, grad.of(l), dp);
     const int apart = i - (first + Type<T>::row_of(0, l.g));
     scorer.template operator()<true>(s, bent, apart);
     if (!sight.all_see(i0, first + TILE)) {
@@ -665,7 +815,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
 #pragma unroll
         for (int r = 0; r < 4; r++) {
           const int row_in = 16 * t + Type<T>::row_of(r, l.g);
-          const bool sees = sight.sees(i, di, first + row_in, docs[l.set * TILE + row_in]);
+          const bool sees = sight.sees(i, di, first + row_in, sight.in(first + row_in, docs[l.set * TILE + row_in]));
           s[t][r] = sees ? s[t][r] : -(T)__builtin_huge_val();
           dp[t][r] = sees ? dp[t][r] : dot;
           if (scorer.capped) bent[t][r] = sees ? bent[t][r] : (T)0;
@@ -687,7 +837,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
     }
     weigh<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, out);
   }
-  if constexpr (SETS == 2) join<T, HD>(out, smem, l.set);
+  if constexpr (SETS > 1) join<T, HD, G>(out, smem, l.set);
   if (a.dq && l.set == 0 && i < (int)a.length)
     put_row<T, HD>((T*)a.dq + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head, l.g, a.head, out, (T)a.scale, di < 0);
   if (a.dslopes_rows) {
@@ -704,47 +854,51 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
 
 // The gradients of k and v: a block's 64 keys against the queries of the heads that read them, all
 // of a group's or, where that leaves too few blocks, a part of them, whose sums k_attend_parts adds up.
-template <class T, int HD>
-__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_attend_dkv(AttendArgs a) {
+template <class T, int HD, int RW>
+__global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dkv(AttendArgs a) {
+  typedef Geo<T, HD, RW> G;
   typedef typename Type<T>::acc acc;
-  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS, NT = Geo<T, HD>::NT;
+  constexpr int STAGE = G::STAGE, SETS = G::SETS, NT = G::NT, ROWS = G::ROWS;
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
+  __shared__ __align__(16) T kept[G::KEPT ? 2 * ROWS * PITCH<T, HD> : 4];
   __shared__ __align__(16) int docs[STAGE];
   __shared__ __align__(16) T sums[STAGE];
   __shared__ __align__(16) T dots[STAGE];
   __shared__ uint64_t found[NT / 64];
   T *qs = smem, *gs = smem + STAGE * PITCH<T, HD>;
-  const Place at(blockIdx.x, a.batch, a.keys * a.parts, a.tiles, false);
+  const Place at(blockIdx.x, a.batch, a.keys * a.parts, a.tiles, false, G::BACKWARD * 4 == 2 * G::WAVES);
   const uint32_t kh = at.h / a.parts, part = at.h % a.parts, group = a.heads / a.keys, per_part = group / a.parts;
   const Sight sight(a, at.b);
-  const Lane l;
+  const Lane<RW> l;
   const int begin = (int)at.tile * ROWS, j = begin + l.row, j0 = begin + l.first;
   const bool whole = a.head % Type<T>::V == 0;
   const int dj = sight.document(j);
   const int64_t key = ((int64_t)at.b * a.length + j) * a.k_row + kh * a.head;
-  T frag[HD / 4], value[HD / 4];
-  row_frag<T, HD>(dj >= 0 ? (const T*)a.k + key : nullptr, l.g, a.head, whole, frag);
-  row_frag<T, HD>(dj >= 0 ? (const T*)a.v + key : nullptr, l.g, a.head, whole, value);
+  Own<T, HD, G> own(kept), value(kept + (G::KEPT ? ROWS * PITCH<T, HD> : 0));
+  {
+    T x[HD / 4];
+    row_frag<T, HD>(dj >= 0 ? (const T*)a.k + key : nullptr, l.g, a.head, whole, x);
+    own.set(x, l);
+    row_frag<T, HD>(dj >= 0 ? (const T*)a.v + key : nullptr, l.g, a.head, whole, x);
+    value.set(x, l);
+  }
   acc dk[HD / 16], dv[HD / 16];
 #pragma unroll
   for (int n = 0; n < HD / 16; n++) dk[n] = dv[n] = acc{0, 0, 0, 0};
   const int end = begin < sight.length ? (sight.length + STAGE - 1) / STAGE : 0;
-  Stages<STAGE, NT> stages(sight, begin, min(sight.queries_from(begin) / STAGE, end), end, found);
+  Stages<G> stages(sight, begin, min(sight.queries_from(begin) / STAGE, end), end, found);
   // The wave's keys are seen by no query before this.
   const int seen_from = sight.queries_from(j0);
   uint32_t h = kh * group + part * per_part;
   const uint32_t last = h + per_part;
-  Staged<T, HD> next;
+  Staged<T, HD, G> next_q(a.q_row, a.head), next_g((int64_t)a.heads * a.head, a.head);
   int doc = 0;
   T sum = 0, dot = 0;
   auto load = [&](uint32_t of, int stage) {
     const int first = stage * STAGE;
-    const int64_t t = (int64_t)at.b * a.length;
-    next.load((const T*)a.q + t * a.q_row + of * a.head, (const T*)a.dy + (t * a.heads + of) * a.head, [&](int r) {
-      const int i = min(first + r, sight.length - 1);
-      const bool in = first + r < sight.length && (!sight.documents || sight.documents[i] >= 0);
-      return RowAt{i * a.q_row, (int64_t)i * a.heads * a.head, in};
-    }, a.head, whole);
+    const int64_t t = (int64_t)at.b * a.length + first;
+    next_q.load((const T*)a.q + t * a.q_row + of * a.head, sight.length - first, a.head, whole);
+    next_g.load((const T*)a.dy + (t * a.heads + of) * a.head, sight.length - first, a.head, whole);
     if (threadIdx.x < STAGE) {
       const int i = first + (int)threadIdx.x;
       doc = sight.document(i);
@@ -758,13 +912,13 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
   if (some) load(h, k);
   while (some && h < last) {
     __syncthreads();
-    next.store(qs, gs);
+    next_q.store(qs);
+    next_g.store(gs);
     if (threadIdx.x < STAGE) {
-      docs[threadIdx.x] = doc;
       sums[threadIdx.x] = doc < 0 ? (T)__builtin_huge_val() : sum;  // weights of 0
       dots[threadIdx.x] = doc < 0 ? (T)0 : dot;
     }
-    __syncthreads();
+    settle<T, HD, G>(sight, k * STAGE, doc, docs, qs, gs);
     const int here = k, first = here * STAGE + l.set * TILE;
     const Scorer<T> scorer(a, h);
     k = stages.at(here + 1);
@@ -775,8 +929,8 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
     if (h < last) load(h, k);
     if (first + TILE <= seen_from || first >= sight.length) continue;
     acc s[2], dp[2], bent[2];
-    score<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
-    score<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, value, dp);
+    score<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, own.of(l), s);
+    score<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, value.of(l), dp);
     scorer.template operator()<true>(s, bent, j - (first + Type<T>::row_of(0, l.g)));
     const bool all = !sight.documents && (!sight.causal || j0 + 15 <= first || j0 + 15 < sight.prefix);
 #pragma unroll
@@ -784,7 +938,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int row = l.set * TILE + 16 * t + Type<T>::row_of(r, l.g);
-        if (!all && !sight.sees(here * STAGE + row, docs[row], j, dj)) {
+        if (!all && !sight.sees(here * STAGE + row, sight.in(here * STAGE + row, docs[row]), j, dj)) {
           s[t][r] = -(T)__builtin_huge_val();
           dp[t][r] = 0;
           if (scorer.capped) bent[t][r] = 0;
@@ -799,9 +953,9 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::GRAD_WAVES)) k_
     weigh<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, dv);
     weigh<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, dp, dk);
   }
-  if constexpr (SETS == 2) {
-    join<T, HD>(dk, smem, l.set);
-    join<T, HD>(dv, smem, l.set);
+  if constexpr (SETS > 1) {
+    join<T, HD, G>(dk, smem, l.set);
+    join<T, HD, G>(dv, smem, l.set);
   }
   if (l.set != 0 || j >= (int)a.length) return;
   const bool none = dj < 0;
@@ -832,7 +986,6 @@ __global__ void __launch_bounds__(256) k_attend_parts(AttendArgs a) {
 
 // ---- over a paged cache ----------------------------------------------------------------------------
 
-constexpr uint32_t PAGED_SPLITS = 2048;  // of a sequence's keys, at most
 constexpr int FIRST_MOST = 1 << 30;  // positions before the new tokens that are told apart
 
 // A sequence's keys in order: those that its pages hold, then the new tokens'.
@@ -859,26 +1012,27 @@ struct Cache {
 
 // Rows of a sequence's queries: the heads of one key head side by side, token after token. A block
 // takes 64 of them and a split of the keys.
-template <class T, int HD>
-__global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged(AttendArgs a) {
+template <class T, int HD, int RW>
+__global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_paged(AttendArgs a) {
+  typedef Geo<T, HD, RW> G;
   typedef typename Type<T>::acc acc;
-  constexpr int STAGE = Geo<T, HD>::STAGE, SETS = Geo<T, HD>::SETS;
+  constexpr int STAGE = G::STAGE, SETS = G::SETS, NT = G::NT, ROWS = G::ROWS;
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
   __shared__ __align__(16) int there[STAGE];
-  __shared__ T tops[SETS == 2 ? 512 : 1], sums[SETS == 2 ? 512 : 1];
+  __shared__ T tops[SETS > 1 ? NT : 1], sums[SETS > 1 ? NT : 1];
   T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
   const uint32_t split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
-  const Place at(rest, a.batch, a.keys, a.tiles, true);
+  const Place at(rest, a.batch, a.keys, a.tiles, true, false);
   const uint32_t b = at.b, kh = at.h, group = a.heads / a.keys;
   const Cache cache(a, b);
-  const Lane l;
+  const Lane<RW> l;
   const uint32_t begin = at.tile * ROWS, r0 = begin + l.row;
   const int i = (int)(r0 / group);
   const uint32_t h = kh * group + r0 % group;
   const bool whole = a.head % Type<T>::V == 0, in = i < cache.count;
   const Scorer<T> scorer(a, h);
-  T frag[HD / 4];
-  row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, l.g, a.head, whole, frag);
+  Registers<T, HD> own;
+  row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, l.g, a.head, whole, own.frag);
   // Keys in order: `past` of the pages, then the new tokens up to the last query of the tile.
   const int last = min((int)((begin + ROWS - 1) / group), cache.count - 1), least = (int)((begin + l.first) / group);
   const int all = (int)(begin / group) < cache.count ? cache.past + last + 1 : 0;
@@ -887,7 +1041,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged
   const int64_t kn = (const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.k_pages;
   const int64_t vn = (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.v_pages;
   Running<T, HD> run;
-  Staged<T, HD> next;
+  Gathered<T, HD, G> next;
   int has = 0;
   auto load = [&](int first) {
     next.load((const T*)a.k_pages, (const T*)a.v_pages, [&](int r) {
@@ -911,7 +1065,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged
     const int first = stage + l.set * TILE;
     if (first >= end || least >= cache.count) continue;
     acc s[2];
-    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, frag, s);
+    score<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, own, s);
     // Positions of old keys run on to the new ones' unless the table ends before them.
     const int apart = i + (first >= cache.past ? cache.past : cache.first) - first - Type<T>::row_of(0, l.g);
     const bool one = first + TILE <= cache.past || first >= cache.past || cache.first == cache.past;
@@ -938,7 +1092,7 @@ __global__ void __launch_bounds__((Geo<T, HD>::NT), (Geo<T, HD>::WAVES)) k_paged
     weigh<T, HD>(vs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, run.out);
   }
   run.sum = row_sum(run.sum);
-  if constexpr (SETS == 2) join(run, smem, tops, sums, l.set);
+  if constexpr (SETS > 1) join<T, HD, G>(run, smem, tops, sums, l.set);
   if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)b * a.length + i) * a.heads + h;
   if (a.splits == 1) {
@@ -1151,41 +1305,57 @@ template <class T>
 __global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
   const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < join_blocks) {
-    __shared__ T weights[PAGED_SPLITS], lanes[512], waves[16];
+    // Threads side by side on the head, the rest of them on the splits, each over its own with a
+    // maximum of its own, so that nothing waits for a first look at them all.
+    __shared__ T lanes[512], tops[512], sums[512];
     const uint64_t row = blockIdx.x;
     const uint32_t pitch = a.head + 2;
     const T* part = (const T*)a.partial + row * a.splits * pitch;
-    T top = -(T)__builtin_huge_val();
-    for (uint32_t p = threadIdx.x; p < a.splits; p += 512) top = Type<T>::max_of(top, weights[p] = part[(uint64_t)p * pitch]);
-    top = rg_wave_max(top);
-    if (lane == 0) waves[threadIdx.x >> 6] = top;
-    __syncthreads();
-    for (int w = 0; w < 8; w++) top = Type<T>::max_of(top, waves[w]);
-    const T base = top == -(T)__builtin_huge_val() ? (T)0 : top;
-    T sum = 0;
-    for (uint32_t p = threadIdx.x; p < a.splits; p += 512) {
-      const T by = Type<T>::exp2_of(weights[p] - base);
-      weights[p] = by;
-      sum += part[(uint64_t)p * pitch + 1] * by;
-    }
-    sum = rg_wave_sum(sum);
-    if (lane == 0) waves[8 + (threadIdx.x >> 6)] = sum;
-    __syncthreads();
-    sum = waves[8];
-    for (int w = 9; w < 16; w++) sum += waves[w];
-    // Threads side by side on the head, the rest of them on the splits.
     uint32_t width = 1;
     while (width < a.head) width *= 2;
-    const uint32_t d = threadIdx.x % width, first = threadIdx.x / width, step = 512 / width;
-    T v = 0;
-    if (d < a.head) {
-#pragma unroll 8
-      for (uint32_t p = first; p < a.splits; p += step) v += part[(uint64_t)p * pitch + 2 + d] * weights[p];
+    const uint32_t d = threadIdx.x % width, first = threadIdx.x / width, step = 512 / width, column = 2 + min(d, a.head - 1);
+    T top = -(T)__builtin_huge_val(), sum = 0, v = 0;
+    constexpr uint32_t N = 8;
+    for (uint32_t p = first; p < a.splits; p += N * step) {
+      T high[N], of[N], x[N];
+#pragma unroll
+      for (uint32_t k = 0; k < N; k++) {
+        const T* from = part + (uint64_t)min(p + k * step, a.splits - 1) * pitch;
+        high[k] = from[0];
+        of[k] = from[1];
+        x[k] = from[column];
+      }
+      T next = top;
+#pragma unroll
+      for (uint32_t k = 0; k < N; k++) {
+        if (p + k * step >= a.splits) high[k] = -(T)__builtin_huge_val();
+        next = Type<T>::max_of(next, high[k]);
+      }
+      const T base = next == -(T)__builtin_huge_val() ? (T)0 : next, by = Type<T>::exp2_of(top - base);
+      top = next;
+      sum *= by;
+      v *= by;
+#pragma unroll
+      for (uint32_t k = 0; k < N; k++) {
+        // A split that has seen nothing adds nothing.
+        const T w = Type<T>::exp2_of(high[k] - base);
+        sum += w == 0 ? (T)0 : of[k] * w;
+        v += w == 0 ? (T)0 : x[k] * w;
+      }
     }
     lanes[threadIdx.x] = v;
+    tops[threadIdx.x] = top;
+    sums[threadIdx.x] = sum;
     __syncthreads();
     if (first != 0 || d >= a.head) return;
-    for (uint32_t k = 1; k < step; k++) v += lanes[k * width + d];
+    for (uint32_t k = 1; k < step; k++) top = Type<T>::max_of(top, tops[k * width + d]);
+    const T base = top == -(T)__builtin_huge_val() ? (T)0 : top;
+    sum = v = 0;
+    for (uint32_t k = 0; k < step; k++) {
+      const T w = Type<T>::exp2_of(tops[k * width + d] - base);
+      sum += sums[k * width + d] * w;
+      v += lanes[k * width + d] * w;
+    }
     ((T*)a.y)[row * a.head + d] = sum == 0 ? (T)0 : v / sum;
     return;
   }
@@ -1254,89 +1424,106 @@ __global__ void __launch_bounds__(1024) k_norm_root(const double* partial, uint3
 
 // ---- launchers -------------------------------------------------------------------------------------
 
-// Calls f with the type and the padded head as constants.
+// Calls f with the type, the padded head and the row waves as constants.
 template <class F>
-void by_head(int dtype, uint32_t head, const F& f) {
+void by_head(int dtype, uint32_t head, uint32_t rows, const F& f) {
   auto of = [&](auto t) {
-    if (head <= 32) f(t, std::integral_constant<int, 32>{});
-    else if (head <= 64) f(t, std::integral_constant<int, 64>{});
-    else if (head <= 96) f(t, std::integral_constant<int, 96>{});
-    else if (head <= 128) f(t, std::integral_constant<int, 128>{});
-    else f(t, std::integral_constant<int, 256>{});
+    auto by_rows = [&](auto hd) {
+      constexpr int SIZE = (int)sizeof(t) * decltype(hd)::value;
+      if constexpr (SIZE <= 512)
+        if (rows == 32) return f(t, hd, std::integral_constant<int, 2>{});
+      if constexpr (SIZE <= 256 || SIZE > 512) f(t, hd, std::integral_constant<int, 4>{});
+    };
+    if (head <= 32) by_rows(std::integral_constant<int, 32>{});
+    else if (head <= 64) by_rows(std::integral_constant<int, 64>{});
+    else if (head <= 96) by_rows(std::integral_constant<int, 96>{});
+    else if (head <= 128) by_rows(std::integral_constant<int, 128>{});
+    else by_rows(std::integral_constant<int, 256>{});
   };
   if (dtype == RG_F32) of(float{});
   else of(double{});
 }
 
-void set_rows(AttendArgs& a) {
+// Heads of more than 256 and of more than 512 bytes.
+bool wide_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 64u : 32u); }
+bool widest_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 128u : 64u); }
+// Rows of a block: 64, or 32 where those leave fewer than two blocks for every CU, and for heads whose
+// blocks have four waves.
+uint32_t rows_of(int dtype, const AttendArgs& a) {
+  if (widest_head(dtype, a.head)) return 64;
+  return wide_head(dtype, a.head) || (uint64_t)a.batch * a.heads * ((a.length + 63) / 64) < 2 * CUS ? 32 : 64;
+}
+uint32_t tiles_of(int dtype, const AttendArgs& a) { return (a.length + rows_of(dtype, a) - 1) / rows_of(dtype, a); }
+
+void set_rows(int dtype, AttendArgs& a) {
   a.q_row = (int64_t)(a.joined ? a.heads + 2 * a.keys : a.heads) * a.head;
   a.k_row = a.joined ? a.q_row : (int64_t)a.keys * a.head;
-  a.tiles = (a.length + ROWS - 1) / ROWS;
+  a.tiles = tiles_of(dtype, a);
 }
 
 uint64_t size_of(int dtype) { return dtype == RG_F32 ? 4 : 8; }
 
-// Tiles of a sequence's rows in the paged form.
-uint32_t paged_tiles(const AttendArgs& a) { return (uint32_t)(((uint64_t)a.length * (a.heads / a.keys) + ROWS - 1) / ROWS); }
 // Whether the rows of a key head are few enough for one wave, and the heads for its registers.
-bool few_rows(int dtype, const AttendArgs& a) {
-  return (uint64_t)a.length * (a.heads / a.keys) <= FEW_ROWS && a.head <= (dtype == RG_F32 ? 128 : 64);
+bool few_rows(int dtype, const AttendArgs& a) { return (uint64_t)a.length * (a.heads / a.keys) <= FEW_ROWS && !widest_head(dtype, a.head); }
+// Rows of a block in the paged form, and tiles of a sequence's rows.
+uint32_t paged_rows(int dtype, const AttendArgs& a) { return wide_head(dtype, a.head) && !widest_head(dtype, a.head) ? 32 : 64; }
+uint32_t paged_tiles(int dtype, const AttendArgs& a) {
+  return (uint32_t)(((uint64_t)a.length * (a.heads / a.keys) + paged_rows(dtype, a) - 1) / paged_rows(dtype, a));
 }
 // Over how many blocks a sequence's keys are split, by the room of its table, since only the device
 // knows how much of it is used: three blocks of few rows for every CU, of whole tiles two, but no
 // fewer than 128 keys (a step of each wave) or 256 each.
 void set_splits(int dtype, AttendArgs& a) {
   const bool few = few_rows(dtype, a);
-  const uint64_t keys = (uint64_t)a.table_pages * a.page + (few ? 0 : a.length), blocks = (uint64_t)a.batch * a.keys * (few ? 1 : paged_tiles(a));
-  const uint64_t least = few ? 128 : 256, want = std::max<uint64_t>(1, (few ? 768 : 512) / blocks);
+  const uint64_t keys = (uint64_t)a.table_pages * a.page + (few ? 0 : a.length), blocks = (uint64_t)a.batch * a.keys * (few ? 1 : paged_tiles(dtype, a));
+  const uint64_t least = few ? 128 : 256, want = std::max<uint64_t>(1, (few ? 3 * CUS : 2 * CUS) / blocks);
   uint64_t per = std::max(least, (keys + want - 1) / want);
-  per = std::max(per, (keys + PAGED_SPLITS - 1) / PAGED_SPLITS);
   per = (per + least - 1) / least * least;
   a.split_keys = (uint32_t)per;
   a.splits = (uint32_t)((keys + per - 1) / per);
 }
 
-}  // namespace
-
-uint64_t attend_blocks(int, const AttendArgs& a) { return (uint64_t)a.batch * a.heads * ((a.length + ROWS - 1) / ROWS) * 2; }
-
 // A gradient's workspace: dy.y of every query, then the parts of dk and dv.
-static uint64_t dots_bytes(int dtype, const AttendArgs& a) { return ((uint64_t)a.batch * a.heads * a.length * size_of(dtype) + 255) / 256 * 256; }
+uint64_t dots_bytes(int dtype, const AttendArgs& a) { return ((uint64_t)a.batch * a.heads * a.length * size_of(dtype) + 255) / 256 * 256; }
 // Parts of a group's heads: as few as leave two blocks for every CU.
-static uint32_t parts_of(const AttendArgs& a) {
+uint32_t parts_of(int dtype, const AttendArgs& a) {
   const uint32_t group = a.heads / a.keys;
-  const uint64_t blocks = (uint64_t)a.batch * a.keys * ((a.length + ROWS - 1) / ROWS);
+  const uint64_t blocks = (uint64_t)a.batch * a.keys * tiles_of(dtype, a);
   for (uint32_t p = 1; p < group; p++)
-    if (group % p == 0 && blocks * p >= 512) return p;
+    if (group % p == 0 && blocks * p >= 2 * CUS) return p;
   return group;
 }
+
+}  // namespace
+
+uint64_t attend_blocks(int dtype, const AttendArgs& a) { return 2 * (uint64_t)a.batch * a.heads * tiles_of(dtype, a); }
 uint64_t attend_workspace(int dtype, const AttendArgs& a) {
-  const uint32_t parts = parts_of(a);
+  const uint32_t parts = parts_of(dtype, a);
   return dots_bytes(dtype, a) + (parts > 1 ? 2 * (uint64_t)parts * a.batch * a.length * a.keys * a.head * size_of(dtype) : 0);
 }
-uint32_t attend_slope_rows(int, const AttendArgs& a) { return a.batch * ((a.length + ROWS - 1) / ROWS); }
+uint32_t attend_slope_rows(int dtype, const AttendArgs& a) { return a.batch * tiles_of(dtype, a); }
 
 void attend(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
-  set_rows(a);
-  by_head(dtype, a.head, [&](auto t, auto hd) {
+  set_rows(dtype, a);
+  by_head(dtype, a.head, rows_of(dtype, a), [&](auto t, auto hd, auto rw) {
     typedef decltype(t) T;
-    constexpr int HD = decltype(hd)::value;
-    k_attend<T, HD><<<a.tiles * a.batch * a.heads, Geo<T, HD>::NT, 0, s>>>(a);
+    constexpr int HD = decltype(hd)::value, RW = decltype(rw)::value;
+    k_attend<T, HD, RW><<<a.tiles * a.batch * a.heads, Geo<T, HD, RW>::NT, 0, s>>>(a);
   });
 }
 
 void attend_grad(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
-  set_rows(a);
-  a.parts = parts_of(a);
+  set_rows(dtype, a);
+  a.parts = parts_of(dtype, a);
   a.partial = (char*)a.workspace + dots_bytes(dtype, a);
-  by_head(dtype, a.head, [&](auto t, auto hd) {
+  by_head(dtype, a.head, rows_of(dtype, a), [&](auto t, auto hd, auto rw) {
     typedef decltype(t) T;
-    constexpr int HD = decltype(hd)::value;
-    k_attend_dq<T, HD><<<a.tiles * a.batch * a.heads, Geo<T, HD>::NT, 0, s>>>(a);
+    constexpr int HD = decltype(hd)::value, RW = decltype(rw)::value;
+    k_attend_dq<T, HD, RW><<<a.tiles * a.batch * a.heads, Geo<T, HD, RW>::NT, 0, s>>>(a);
     if (!a.dk && !a.dv) return;
-    k_attend_dkv<T, HD><<<a.tiles * a.batch * a.keys * a.parts, Geo<T, HD>::NT, 0, s>>>(a);
+    k_attend_dkv<T, HD, RW><<<a.tiles * a.batch * a.keys * a.parts, Geo<T, HD, RW>::NT, 0, s>>>(a);
     if (a.parts == 1) return;
     const uint64_t n = 2 * (uint64_t)a.batch * a.length * a.keys * a.head;
     k_attend_parts<T><<<(uint32_t)std::min<uint64_t>((n + 255) / 256, 8192), 256, 0, s>>>(a);
@@ -1347,7 +1534,7 @@ uint64_t paged_blocks(int dtype, const AttendArgs& args) {
   AttendArgs a = args;
   set_splits(dtype, a);
   const uint64_t rows = (uint64_t)a.batch * a.length * (a.heads + a.keys / 8 + 1) + 1;
-  return 2 * std::max((uint64_t)a.batch * a.keys * paged_tiles(a) * a.splits, rows);
+  return 2 * std::max((uint64_t)a.batch * a.keys * paged_tiles(dtype, a) * a.splits, rows);
 }
 
 uint64_t paged_workspace(int dtype, const AttendArgs& args) {
@@ -1358,9 +1545,9 @@ uint64_t paged_workspace(int dtype, const AttendArgs& args) {
 
 void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
   AttendArgs a = args;
-  set_rows(a);
+  set_rows(dtype, a);
   set_splits(dtype, a);
-  a.tiles = paged_tiles(a);
+  a.tiles = paged_tiles(dtype, a);
   a.partial = a.workspace;
   a.page_div = FastDiv(a.page);
   const uint64_t values = (uint64_t)a.pages * a.page * a.keys * a.head * size_of(dtype);
@@ -1368,9 +1555,9 @@ void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
   if (a.v_out && a.v_out != a.v_pages) copy_bytes(s, a.v_out, a.v_pages, values);
   const bool few = few_rows(dtype, a);
   if (a.y)
-    by_head(dtype, a.head, [&](auto t, auto hd) {
+    by_head(dtype, a.head, paged_rows(dtype, a), [&](auto t, auto hd, auto rw) {
       typedef decltype(t) T;
-      constexpr int HD = decltype(hd)::value;
+      constexpr int HD = decltype(hd)::value, RW = decltype(rw)::value;
       if constexpr (FewGeo<T, HD>::FITS) {
         if (few) {
           const uint32_t blocks = a.batch * a.keys * a.splits;
@@ -1379,7 +1566,8 @@ void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
           return;
         }
       }
-      k_paged<T, HD><<<a.batch * a.keys * a.tiles * a.splits, Geo<T, HD>::NT, 0, s>>>(a);
+      if constexpr ((RW == 2) == ((int)sizeof(T) * HD > 256 && (int)sizeof(T) * HD <= 512))
+        k_paged<T, HD, RW><<<a.batch * a.keys * a.tiles * a.splits, Geo<T, HD, RW>::NT, 0, s>>>(a);
     });
   const uint32_t join = a.y && a.splits > 1 ? (uint32_t)((uint64_t)a.batch * a.length * a.heads) : 0;
   const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + 7) / 8) : 0;
