@@ -32,7 +32,7 @@ struct AttendArgs {
   void *k_out, *v_out;          // the pages with the new rows; may be k_pages and v_pages
   // Set by the launchers.
   int64_t q_row, k_row;         // values from one position to the next, of q and of k and v
-  uint32_t tiles, splits, split_keys, parts;
+  uint32_t tiles, splits, parts;
   void *partial;
   FastDiv page_div;
 };

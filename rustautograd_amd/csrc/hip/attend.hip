@@ -469,8 +469,9 @@ __device__ __forceinline__ void settle(const Sight& sight, int first, int doc, i
   }
 }
 
-// Rows of two operands anywhere in memory on their way to LDS. Loads are of rows and columns that there
-// are; what does not belong is made 0 as it is stored.
+// Rows of two operands anywhere in memory on their way to LDS; their places in both, and whether they are
+// there, lie in LDS. Loads are of rows and columns that there are, so the places of rows that are not may
+// be any that can be read; what does not belong is made 0 as it is stored.
 template <class T, int HD, class G>
 struct Gathered {
   static constexpr int V = Type<T>::V, NT = G::NT, PER = G::STAGE * HD / V / NT;
@@ -480,29 +481,25 @@ struct Gathered {
   uint32_t off;  // bit i: step i is not there
   static __device__ __forceinline__ int row(int i) { return ((int)threadIdx.x + i * NT) / (HD / V); }
   static __device__ __forceinline__ uint32_t column(int i) { return (uint32_t)(((int)threadIdx.x + i * NT) % (HD / V)) * V; }
-  // `rows(r)` gives row r's place in both operands and whether it is there; the places of rows that
-  // are not may be any that can be read.
-  template <class R>
-  __device__ __forceinline__ void load(const T* xs, const T* ys, const R& rows, uint32_t head, bool whole) {
+  __device__ __forceinline__ void load(const T* xs, const T* ys, const int64_t* x_at, const int64_t* y_at, const int* there, uint32_t head, bool whole) {
     off = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const auto p = rows(row(i));
+      const T *u_row = xs + x_at[row(i)], *v_row = ys + y_at[row(i)];
       const uint32_t c = column(i);
+      off |= there[row(i)] && c < head ? 0u : 1u << i;
       if (whole) {
         const uint32_t d = c < head ? c : 0;
-        x[i] = *(const vec*)(xs + p.x + d);
-        y[i] = *(const vec*)(ys + p.y + d);
-        if (!p.there || c >= head) off |= 1u << i;
+        x[i] = *(const vec*)(u_row + d);
+        y[i] = *(const vec*)(v_row + d);
       } else {
 #pragma unroll
         for (uint32_t j = 0; j < V; j++) {
           const uint32_t d = c + j < head ? c + j : 0;
-          const T u = xs[p.x + d], v = ys[p.y + d];
+          const T u = u_row[d], v = v_row[d];
           x[i][j] = c + j < head ? u : (T)0;
           y[i][j] = c + j < head ? v : (T)0;
         }
-        if (!p.there) off |= 1u << i;
       }
     }
   }
@@ -521,10 +518,6 @@ struct Gathered {
       *(vec*)(ys + o) = v;
     }
   }
-};
-struct RowAt {
-  int64_t x, y;
-  bool there;
 };
 
 // A block's head and tile of rows. Heads of a batch lie next to each other, so that blocks of one head
@@ -909,8 +902,9 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   };
   int k = stages.at(stages.from);
   const bool some = k < stages.end;
-  if (some) load(h, k);
+  if (G::NARROW && some) load(h, k);
   while (some && h < last) {
+    if (!G::NARROW) load(h, k);  // its registers are the accumulators' while it computes
     __syncthreads();
     next_q.store(qs);
     next_g.store(gs);
@@ -926,7 +920,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
       h++;
       if (h < last) k = stages.at(stages.from);
     }
-    if (h < last) load(h, k);
+    if (G::NARROW && h < last) load(h, k);
     if (first + TILE <= seen_from || first >= sight.length) continue;
     acc s[2], dp[2], bent[2];
     score<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, own.of(l), s);
@@ -1019,6 +1013,8 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   constexpr int STAGE = G::STAGE, SETS = G::SETS, NT = G::NT, ROWS = G::ROWS;
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
   __shared__ __align__(16) int there[STAGE];
+  __shared__ int coming[STAGE];
+  __shared__ int64_t k_at[STAGE], v_at[STAGE];
   __shared__ T tops[SETS > 1 ? NT : 1], sums[SETS > 1 ? NT : 1];
   T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
   const uint32_t split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits;
@@ -1036,32 +1032,56 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   // Keys in order: `past` of the pages, then the new tokens up to the last query of the tile.
   const int last = min((int)((begin + ROWS - 1) / group), cache.count - 1), least = (int)((begin + l.first) / group);
   const int all = (int)(begin / group) < cache.count ? cache.past + last + 1 : 0;
-  const int from = (int)min((uint64_t)split * a.split_keys, (uint64_t)all), end = (int)min((uint64_t)(split + 1) * a.split_keys, (uint64_t)all);
+  // Split evenly, in whole stages.
+  const int per = ((all + (int)a.splits - 1) / (int)a.splits + STAGE - 1) / STAGE * STAGE;
+  const int from = (int)min((int64_t)split * per, (int64_t)all), end = min(from + per, all);
   // New rows as places in the pages' operands: their distance from those.
   const int64_t kn = (const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.k_pages;
   const int64_t vn = (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.v_pages;
   Running<T, HD> run;
   Gathered<T, HD, G> next;
+  // Where a stage's rows lie is looked up by its first threads a stage before it is loaded, two before
+  // it is used, so that no load waits for the table.
+  const bool looks = threadIdx.x < STAGE;
+  int64_t k_mine = 0, v_mine = 0;
   int has = 0;
-  auto load = [&](int first) {
-    next.load((const T*)a.k_pages, (const T*)a.v_pages, [&](int r) {
-      const int c = min(first + r, end - 1);
-      if (c >= cache.past) return RowAt{kn + (int64_t)(c - cache.past) * a.k_row, vn + (int64_t)(c - cache.past) * a.k_row, first + r < end};
-      const int64_t row = cache.row((uint32_t)c), o = (max(row, (int64_t)0) * a.keys + kh) * a.head;
-      return RowAt{o, o, row >= 0 && first + r < end};
-    }, a.head, whole);
-    if (threadIdx.x < STAGE) {
-      const int c = first + (int)threadIdx.x;
-      has = c < end && (c >= cache.past || cache.row((uint32_t)c) >= 0);
+  auto look = [&](int first) {
+    const int c = first + (int)threadIdx.x;
+    has = looks && c < end;
+    if (!has) return;
+    if (c >= cache.past) {
+      k_mine = kn + (int64_t)(c - cache.past) * a.k_row;
+      v_mine = vn + (int64_t)(c - cache.past) * a.k_row;
+    } else {
+      const int64_t row = cache.row((uint32_t)c);
+      has = row >= 0;
+      k_mine = v_mine = (max(row, (int64_t)0) * a.keys + kh) * a.head;
     }
   };
-  if (from < end) load(from);
+  auto leave = [&] {
+    if (!looks) return;
+    k_at[threadIdx.x] = has ? k_mine : 0;
+    v_at[threadIdx.x] = has ? v_mine : 0;
+    coming[threadIdx.x] = has;
+  };
+  auto load = [&] { next.load((const T*)a.k_pages, (const T*)a.v_pages, k_at, v_at, coming, a.head, whole); };
+  if (from < end) {
+    look(from);
+    leave();
+    __syncthreads();
+    load();
+    look(from + STAGE);
+  }
   for (int stage = from; stage < end; stage += STAGE) {
     __syncthreads();
     next.store(ks, vs);
-    if (threadIdx.x < STAGE) there[threadIdx.x] = has;
+    if (looks) there[threadIdx.x] = coming[threadIdx.x];
+    leave();
     __syncthreads();
-    if (stage + STAGE < end) load(stage + STAGE);
+    if (stage + STAGE < end) {
+      load();
+      look(stage + 2 * STAGE);
+    }
     const int first = stage + l.set * TILE;
     if (first >= end || least >= cache.count) continue;
     acc s[2];
@@ -1134,9 +1154,10 @@ __global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(A
   const int i = l16 / (int)group;
   const uint32_t h = kh * group + l16 % group;
   const bool in = l16 < (int)(a.length * group) && i < cache.count;
-  const int from = (int)min((uint64_t)split * a.split_keys, (uint64_t)cache.past), end = (int)min((uint64_t)(split + 1) * a.split_keys, (uint64_t)cache.past);
-  // The new tokens' own keys go to the split that the old ones end in.
-  const bool own = cache.count > 0 && split == min((uint32_t)cache.past / a.split_keys, a.splits - 1);
+  // The old keys split evenly, in whole rounds of the four waves; the new ones go to the last split.
+  const int per = ((cache.past + (int)a.splits - 1) / (int)a.splits + 4 * STEP - 1) / (4 * STEP) * (4 * STEP);
+  const int from = (int)min((int64_t)split * per, (int64_t)cache.past), end = min(from + per, cache.past);
+  const bool own = cache.count > 0 && split == a.splits - 1;
   const Scorer<T> scorer(a, in ? h : kh * group);
   T frag[HD / 4];
   row_frag<T, HD>(in ? (const T*)a.q + ((int64_t)b * a.length + i) * a.q_row + h * a.head : nullptr, g, a.head, WHOLE, frag);
@@ -1438,7 +1459,7 @@ void by_head(int dtype, uint32_t head, uint32_t rows, const F& f) {
     else if (head <= 64) by_rows(std::integral_constant<int, 64>{});
     else if (head <= 96) by_rows(std::integral_constant<int, 96>{});
     else if (head <= 128) by_rows(std::integral_constant<int, 128>{});
-    else by_rows(std::integral_constant<int, 256>{});
+    else if constexpr (sizeof(t) == 4) by_rows(std::integral_constant<int, 256>{});
   };
   if (dtype == RG_F32) of(float{});
   else of(double{});
@@ -1471,15 +1492,14 @@ uint32_t paged_tiles(int dtype, const AttendArgs& a) {
   return (uint32_t)(((uint64_t)a.length * (a.heads / a.keys) + paged_rows(dtype, a) - 1) / paged_rows(dtype, a));
 }
 // Over how many blocks a sequence's keys are split, by the room of its table, since only the device
-// knows how much of it is used: three blocks of few rows for every CU, of whole tiles two, but no
-// fewer than 128 keys (a step of each wave) or 256 each.
+// knows how much of it is used: three blocks of few rows for every CU, of whole tiles two, but not so
+// many that a full table leaves one fewer than 128 keys (a step of each wave) or 256.
 void set_splits(int dtype, AttendArgs& a) {
   const bool few = few_rows(dtype, a);
   const uint64_t keys = (uint64_t)a.table_pages * a.page + (few ? 0 : a.length), blocks = (uint64_t)a.batch * a.keys * (few ? 1 : paged_tiles(dtype, a));
   const uint64_t least = few ? 128 : 256, want = std::max<uint64_t>(1, (few ? 3 * CUS : 2 * CUS) / blocks);
   uint64_t per = std::max(least, (keys + want - 1) / want);
   per = (per + least - 1) / least * least;
-  a.split_keys = (uint32_t)per;
   a.splits = (uint32_t)((keys + per - 1) / per);
 }
 

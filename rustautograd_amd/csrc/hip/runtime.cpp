@@ -742,6 +742,8 @@ StepFn lower_attend(Program& prog, const Instr& i) {
   const uint64_t positions = (uint64_t)q.batch * q.length, stride = (uint64_t)q.heads + (base.joined ? 2 * q.keys : 0);
   if (positions >= (1ull << 31) || stride * q.head >= (1ull << 31) || (uint64_t)q.pages * q.page >= (1ull << 31))
     throw std::runtime_error("an attention of 2^31 positions or values a position exceeds the index range");
+  // Wider ones do not fit the registers: four of the backward's operands and results are a row each.
+  if (dtype == RG_F64 && q.head > 128) throw std::runtime_error("an attention of float64 heads of " + std::to_string(q.head) + " values: at most 128");
   // The rows that a block stages at once lie within 2^31 bytes.
   if (stride * q.head * (uint64_t)esize(dtype) >= (1ull << 31) / 129) throw std::runtime_error("an attention of more than 2^24 bytes a position exceeds the index range");
   base.batch = (uint32_t)q.batch;
