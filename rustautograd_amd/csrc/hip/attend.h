@@ -32,7 +32,7 @@ struct AttendArgs {
   void *k_out, *v_out;          // the pages with the new rows; may be k_pages and v_pages
   // Set by the launchers.
   int64_t q_row, k_row;         // values from one position to the next, of q and of k and v
-  uint32_t tiles, splits, parts;
+  uint32_t tiles, splits, parts, join_width, join_step;
   void *partial;
   FastDiv page_div;
 };
@@ -47,14 +47,14 @@ uint64_t paged_workspace(int dtype, const AttendArgs& a);
 void paged_attend(hipStream_t s, int dtype, const AttendArgs& a);
 
 // The norm's tensors, NORM_TENSORS a launch: `first_block` is the block that begins each.
-constexpr int NORM_TENSORS = 48;
+constexpr int NORM_TENSORS = 128;
 struct NormTensors {
   const void* x[NORM_TENSORS];
   uint64_t n[NORM_TENSORS];
   uint32_t first_block[NORM_TENSORS];
   uint32_t count;
 };
-uint32_t norm_blocks(uint64_t n);
+uint32_t norm_blocks(uint64_t n);  // x is 16 bytes aligned
 // The blocks' sums of squares in `partial` (64 bits, from `first_partial` on), then their root.
 void norm_squares(hipStream_t s, int dtype, const NormTensors& t, uint32_t blocks, double* partial);
 void norm_root(hipStream_t s, int dtype, const double* partial, uint32_t blocks, void* out);

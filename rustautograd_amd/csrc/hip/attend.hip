@@ -1318,7 +1318,7 @@ __global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(A
   }
 }
 
-// Joins the splits of each row, a block a row, and then (blocks from `join_blocks` on) puts the new
+// Joins the splits of each row, and then (blocks from `join_blocks` on) puts the new
 // tokens' keys and values into their pages, a wave a token and key head. Rows that a later sequence
 // writes too are left to it, so that the result does not depend on which comes first. It comes after
 // every read of the pages, so that it may write into the ones that were read.
@@ -1326,15 +1326,15 @@ template <class T>
 __global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t join_blocks) {
   const uint32_t lane = threadIdx.x & 63;
   if (blockIdx.x < join_blocks) {
-    // Threads side by side on the head, the rest of them on the splits, each over its own with a
-    // maximum of its own, so that nothing waits for a first look at them all.
+    // Threads side by side on the head, `join_step` such rows of them on the splits, each over its own
+    // with a maximum of its own, so that nothing waits for a first look at them all; the rest of the
+    // block on other rows.
     __shared__ T lanes[512], tops[512], sums[512];
-    const uint64_t row = blockIdx.x;
-    const uint32_t pitch = a.head + 2;
+    const uint32_t width = a.join_width, step = a.join_step, pitch = a.head + 2;
+    const uint64_t rows = (uint64_t)a.batch * a.length * a.heads, mine = (uint64_t)blockIdx.x * (512 / (width * step)) + threadIdx.x / (width * step);
+    const uint64_t row = min(mine, rows - 1);
     const T* part = (const T*)a.partial + row * a.splits * pitch;
-    uint32_t width = 1;
-    while (width < a.head) width *= 2;
-    const uint32_t d = threadIdx.x % width, first = threadIdx.x / width, step = 512 / width, column = 2 + min(d, a.head - 1);
+    const uint32_t d = threadIdx.x % width, first = threadIdx.x / width % step, column = 2 + min(d, a.head - 1);
     T top = -(T)__builtin_huge_val(), sum = 0, v = 0;
     constexpr uint32_t N = 8;
     for (uint32_t p = first; p < a.splits; p += N * step) {
@@ -1368,14 +1368,14 @@ __global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t joi
     tops[threadIdx.x] = top;
     sums[threadIdx.x] = sum;
     __syncthreads();
-    if (first != 0 || d >= a.head) return;
-    for (uint32_t k = 1; k < step; k++) top = Type<T>::max_of(top, tops[k * width + d]);
+    if (first != 0 || d >= a.head || mine >= rows) return;
+    for (uint32_t k = 1; k < step; k++) top = Type<T>::max_of(top, tops[threadIdx.x + k * width]);
     const T base = top == -(T)__builtin_huge_val() ? (T)0 : top;
     sum = v = 0;
     for (uint32_t k = 0; k < step; k++) {
-      const T w = Type<T>::exp2_of(tops[k * width + d] - base);
-      sum += sums[k * width + d] * w;
-      v += lanes[k * width + d] * w;
+      const T w = Type<T>::exp2_of(tops[threadIdx.x + k * width] - base);
+      sum += sums[threadIdx.x + k * width] * w;
+      v += lanes[threadIdx.x + k * width] * w;
     }
     ((T*)a.y)[row * a.head + d] = sum == 0 ? (T)0 : v / sum;
     return;
@@ -1408,20 +1408,33 @@ __global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t joi
 
 // ---- the joint norm --------------------------------------------------------------------------------
 
-constexpr uint64_t NORM_PER_BLOCK = 16384;
+// Values of a block: four 16 bytes a thread of float32 on their way at once.
+constexpr uint64_t NORM_PER_BLOCK = 4096;
 
 template <class T>
 __global__ void __launch_bounds__(256) k_norm_squares(NormTensors t, double* partial) {
+  typedef typename Type<T>::vec vec;
+  constexpr int V = Type<T>::V, N = (int)(NORM_PER_BLOCK / (256 * V));
   uint32_t k = 0;
-  while (k + 1 < t.count && blockIdx.x >= t.first_block[k + 1]) k++;
-  const uint64_t begin = (uint64_t)(blockIdx.x - t.first_block[k]) * NORM_PER_BLOCK, end = min(begin + NORM_PER_BLOCK, t.n[k]);
-  const T* x = (const T*)t.x[k];
+#pragma unroll
+  for (uint32_t half = NORM_TENSORS / 2; half > 0; half /= 2)
+    if (k + half < t.count && blockIdx.x >= t.first_block[k + half]) k += half;
+  const uint64_t begin = (uint64_t)(blockIdx.x - t.first_block[k]) * NORM_PER_BLOCK;
+  const T* x = (const T*)t.x[k] + begin;
+  const uint32_t n = (uint32_t)min(NORM_PER_BLOCK, t.n[k] - begin);
   double sum = 0;
-  for (uint64_t i = begin + threadIdx.x; i < end; i += 256) {
-    const double v = (double)x[i];
-    sum += v * v;
+  if (n == NORM_PER_BLOCK) {
+    vec v[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = *(const vec*)(x + (i * 256 + threadIdx.x) * V);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int j = 0; j < V; j++) sum = fma((double)v[i][j], (double)v[i][j], sum);
+  } else {
+    for (uint32_t i = threadIdx.x; i < n; i += 256) sum = fma((double)x[i], (double)x[i], sum);
   }
-  __shared__ double waves[256 / 64];
+  __shared__ double waves[4];
   sum = rg_wave_sum(sum);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
   __syncthreads();
@@ -1432,6 +1445,7 @@ template <class T>
 __global__ void __launch_bounds__(1024) k_norm_root(const double* partial, uint32_t blocks, T* out) {
   __shared__ double waves[16];
   double sum = 0;
+#pragma unroll 4
   for (uint32_t i = threadIdx.x; i < blocks; i += 1024) sum += partial[i];
   sum = rg_wave_sum(sum);
   if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
@@ -1589,7 +1603,12 @@ void paged_attend(hipStream_t s, int dtype, const AttendArgs& args) {
       if constexpr ((RW == 2) == ((int)sizeof(T) * HD > 256 && (int)sizeof(T) * HD <= 512))
         k_paged<T, HD, RW><<<a.batch * a.keys * a.tiles * a.splits, Geo<T, HD, RW>::NT, 0, s>>>(a);
     });
-  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)((uint64_t)a.batch * a.length * a.heads) : 0;
+  // A thread of the join takes eight splits in one round of loads, and a block as many rows as that leaves.
+  a.join_width = a.join_step = 1;
+  while (a.join_width < a.head) a.join_width *= 2;
+  while (a.join_step * 8 < a.splits && a.join_step * 2 * a.join_width <= 512) a.join_step *= 2;
+  const uint64_t rows = (uint64_t)a.batch * a.length * a.heads, per_block = 512 / (a.join_width * a.join_step);
+  const uint32_t join = a.y && a.splits > 1 ? (uint32_t)((rows + per_block - 1) / per_block) : 0;
   const uint32_t append = a.k_out || a.v_out ? (uint32_t)(((uint64_t)a.batch * a.length * a.keys + 7) / 8) : 0;
   if (join + append == 0) return;
   if (dtype == RG_F32) k_paged_finish<float><<<join + append, 512, 0, s>>>(a, join);
