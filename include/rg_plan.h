@@ -108,7 +108,8 @@
  *                  (j <= i, or not RG_ATTEND_CAUSAL, or j < prefix) and both have the same document,
  *                  not negative; query head h reads head h G / H of k and v;
  *                  out 0: y[B,T,H,hd], the softmax of s over the keys seen, times v (0 where none is);
- *                  1: the logarithm to base 2 of the softmax's sum, [B,H,T], for the gradient alone
+ *                  1: the logarithm to base 2 of the softmax's sum, [B,H,T], or the dtype's largest
+ *                  value where no key is seen, for the gradient alone
  *       _GRAD      in the same, y, result 1, dy; out dq (joined: dx), dk, dv, dslopes
  *     PAGED_ATTENTION in q, k, v or x as above, k and v pages[P,page,G,hd], table[B,N], first[B]
  *                  (, slopes[H]) (, lengths[B]); position p of sequence b lies in row p % page of

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <limits>
 #include <vector>
 
 #include "../include/rg_plan.h"
@@ -293,7 +294,7 @@ void attention(const Operands<T>& o) {
               for (int64_t j : seen) y += s[(size_t)j] * (double)vs(b * L + j, g)[d];
               o.out[0][((b * L + i) * H + h) * hd + d] = (T)y;
             }
-          if (o.out[1]) o.out[1][(b * H + h) * L + i] = seen.empty() ? (T)INFINITY : (T)((top + std::log(sum)) / std::log(2.0));
+          if (o.out[1]) o.out[1][(b * H + h) * L + i] = seen.empty() ? std::numeric_limits<T>::max() : (T)((top + std::log(sum)) / std::log(2.0));
           continue;
         }
         const T* gi = dy + ((b * L + i) * H + h) * hd;

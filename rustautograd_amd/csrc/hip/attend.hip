@@ -43,6 +43,7 @@ struct Type<float> {
   typedef floatx4 acc;
   typedef floatx4 vec;  // 16 bytes
   static constexpr int V = 4;
+  static constexpr float MOST = __FLT_MAX__;
   static __device__ __forceinline__ acc mfma(float a, float b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
   // The tile row of register r in a lane of group g (its lane number over 16).
   static __device__ __forceinline__ int row_of(int r, int g) { return 4 * g + r; }
@@ -78,6 +79,7 @@ struct Type<double> {
   typedef doublex4 acc;
   typedef doublex2 vec;
   static constexpr int V = 2;
+  static constexpr double MOST = __DBL_MAX__;
   static __device__ __forceinline__ acc mfma(double a, double b, acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ int row_of(int r, int g) { return 4 * r + g; }
   static __device__ __forceinline__ double exp2_of(double x) { return exp2(x); }
@@ -726,9 +728,9 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h;
   const bool none = run.sum == 0 || di < 0;
   if (a.y) put_row<T, HD>((T*)a.y + row * a.head, l.g, a.head, run.out, 1 / run.sum, none);
-  // Of a query that sees nothing infinity, so that the backward forms weights of 0.
+  // Of a query that sees nothing the type's largest value, so that the backward forms weights of 0.
   if (a.sums && l.g == 0)
-    ((T*)a.sums)[((uint64_t)at.b * a.heads + at.h) * a.length + i] = none ? (T)__builtin_huge_val() : run.top + Type<T>::log2_of(run.sum);
+    ((T*)a.sums)[((uint64_t)at.b * a.heads + at.h) * a.length + i] = none ? Type<T>::MOST : run.top + Type<T>::log2_of(run.sum);
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others.

@@ -10,6 +10,7 @@ reference's python/rg/nn.py; the code is this package's own.
 import math
 
 from . import random
+from .attention import attention, paged_attention
 from .ops import (abs, arange, argmax, argsort, broadcast_to, concatenate, cumsum, equal, exp, eye, log, maximum, ones,
                   stop_gradient, swapaxes, take, take_along_axis, tanh, top_k, where, zeros)
 from .sequence import causal_conv, rotary_norm, selective_scan
@@ -233,11 +234,23 @@ class MultiHeadAttention(Layer):
     means visible. With `key` and a dropout rate, the weights and the output are dropped out.
     `qk_norm` divides each head's queries and keys by their root mean square, with a learned gain;
     `rotary` turns them by position with that base, True with the usual 10000 (`positions` as in
-    `rotary_norm`). Heads that are normed or turned have an even number of values, at most 256."""
+    `rotary_norm`). Heads that are normed or turned have an even number of values, at most 256.
 
-    def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
+    `kv_heads` heads of keys and values serve heads / kv_heads heads of queries each; `cap` caps the
+    scores, cap * tanh(score / cap); `distance` lowers them with the distance of query and key, by a
+    learned slope a head. With any of them, or with `documents`, `prefix` or `lengths` in the call, the
+    layer runs on `attention`, as which it is causal unless `causal` is False: it then takes no `mask`
+    and drops nothing out. `layer.extend(params, x, state, lengths)` returns `(y, state)` for the next
+    positions of sequences, prompts and single tokens, over the pages of `layer.state(batch, length)`."""
+
+    def __init__(self, d, heads, bias=True, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None, kv_heads=None, cap=None, distance=False,
+                 causal=True):
         if d % heads != 0:
             raise ValueError(f"{heads} heads cannot split a model dimension of {d}")
+        if kv_heads is not None and (kv_heads < 1 or heads % kv_heads != 0):
+            raise ValueError(f"{kv_heads} heads of keys cannot serve {heads} of queries")
+        if cap is not None and not cap > 0:
+            raise ValueError(f"scores cannot be capped at {cap}")
         if (qk_norm or rotary) and (d // heads % 2 != 0 or d // heads > 256):
             raise ValueError(f"heads of {d // heads} values cannot be normed or turned: an even number, at most 256")
         self.d = d
@@ -245,7 +258,12 @@ class MultiHeadAttention(Layer):
         self.rate = dropout_rate
         self.qk_norm = qk_norm
         self.rotary = 10000.0 if rotary is True else rotary
-        self.qkv = Linear(d, 3 * d, bias, init, dtype)
+        self.kv_heads = heads if kv_heads is None else kv_heads
+        self.cap = cap
+        self.distance = distance
+        self.causal = causal
+        self.shaped = kv_heads is not None or cap is not None or distance or not causal
+        self.qkv = Linear(d, d + 2 * self.kv_heads * (d // heads), bias, init, dtype)
         self.out = Linear(d, d, bias, init, dtype)
 
     def init(self, key):
@@ -253,16 +271,59 @@ class MultiHeadAttention(Layer):
         params = {"qkv": self.qkv.init(k_qkv), "out": self.out.init(k_out)}
         if self.qk_norm:
             params["gain"] = ones((2, self.d // self.heads), self.qkv.dtype)
+        if self.distance:
+            # From 1 / 2 down to 1 / 256, as logarithms, so that training keeps them positive.
+            params["slope_log"] = log(tensor([2.0 ** (-8.0 * (h + 1) / self.heads) for h in range(self.heads)], self.qkv.dtype))
         return params
 
-    def __call__(self, params, x, mask=None, key=None, positions=None):
+    def _projected(self, params, x, positions):
+        """Queries, keys and values (batch, length, heads + 2 kv_heads, head), normed and turned."""
         b, t, d = x.shape
         hd = d // self.heads
-        qkv = self.qkv(params["qkv"], x)
+        qkv = self.qkv(params["qkv"], x).reshape(b, t, self.heads + 2 * self.kv_heads, hd)
         if self.qk_norm or self.rotary:
             # Queries and keys in place in the fused projection; the values pass.
-            qkv = rotary_norm(qkv.reshape(b, t, 3 * self.heads, hd), params["gain"] if self.qk_norm else None, positions,
-                              (self.heads, self.heads), None if self.rotary else 0, self.rotary or 10000.0)
+            qkv = rotary_norm(qkv, params["gain"] if self.qk_norm else None, positions, (self.heads, self.kv_heads), None if self.rotary else 0,
+                              self.rotary or 10000.0)
+        return qkv
+
+    def _slopes(self, params):
+        return exp(params["slope_log"]) if self.distance else None
+
+    def state(self, batch, length, page=64):
+        """The state of `batch` sequences not yet begun, with pages for `length` positions of each."""
+        if batch < 1 or length < 1 or page < 1:
+            raise ValueError(f"a cache of {batch} sequences of {length} positions in pages of {page}")
+        each = -(-length // page)
+        pages = (batch * each, page, self.kv_heads, self.d // self.heads)
+        return {"k": zeros(pages, self.qkv.dtype), "v": zeros(pages, self.qkv.dtype), "table": arange(batch * each).reshape(batch, each),
+                "pos": zeros((batch,), "int32")}
+
+    def extend(self, params, x, state, lengths=None):
+        """`(y, state)` for the positions `x` that follow those in `state`; causal. Of a padded batch
+        `lengths` (batch,) counts the positions that are there: y is the output's bias at the others."""
+        if not self.causal:
+            raise ValueError("a layer that sees ahead cannot be extended")
+        if lengths is not None:
+            lengths = lengths if isinstance(lengths, Value) else tensor(lengths, "int32")
+        b, t, d = x.shape
+        qkv = self._projected(params, x, state["pos"].reshape(b, 1))
+        y, (k, v) = paged_attention(qkv, cache=(state["k"], state["v"]), table=state["table"], first=state["pos"], lengths=lengths,
+                                    heads=(self.heads, self.kv_heads), cap=self.cap, slopes=self._slopes(params))
+        # As many positions as were there: lengths within the batch's own.
+        read = t if lengths is None else where(lengths > t, t, where(lengths > 0, lengths, 0))
+        return self.out(params["out"], y.reshape(b, t, d)), {"k": k, "v": v, "table": state["table"], "pos": state["pos"] + read}
+
+    def __call__(self, params, x, mask=None, key=None, positions=None, documents=None, prefix=None, lengths=None):
+        b, t, d = x.shape
+        hd = d // self.heads
+        if self.shaped or documents is not None or prefix is not None or lengths is not None:
+            if mask is not None or (key is not None and self.rate > 0.0):
+                raise ValueError("attention with shaped scores takes no mask and drops nothing out")
+            y = attention(self._projected(params, x, positions), heads=(self.heads, self.kv_heads), causal=self.causal, cap=self.cap,
+                          slopes=self._slopes(params), documents=documents, prefix=prefix, lengths=lengths)
+            return self.out(params["out"], y.reshape(b, t, d))
+        qkv = self._projected(params, x, positions) if self.qk_norm or self.rotary else self.qkv(params["qkv"], x)
         # (b, t, 3d) -> (3, b, heads, t, hd): q, k and v for every head.
         qkv = qkv.reshape(b, t, 3, self.heads, hd).transpose(2, 0, 3, 1, 4)
         q, k, v = qkv[0], qkv[1], qkv[2]
@@ -281,13 +342,15 @@ class MultiHeadAttention(Layer):
 
 class TransformerBlock(Layer):
     """Pre-norm transformer block: x + attention(norm(x)), then x + mlp(norm(x)) with a GELU
-    MLP of `mlp_ratio * d` hidden units. `qk_norm` and `rotary` are the attention's."""
+    MLP of `mlp_ratio * d` hidden units. `qk_norm`, `rotary`, `kv_heads`, `cap`, `distance`, `causal`
+    and what a call masks are the attention's, and so are `state` and `extend`."""
 
-    def __init__(self, d, heads, mlp_ratio=4, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None):
+    def __init__(self, d, heads, mlp_ratio=4, dropout_rate=0.0, init=None, dtype="float32", qk_norm=False, rotary=None, kv_heads=None, cap=None, distance=False,
+                 causal=True):
         self.rate = dropout_rate
         self.norm1 = LayerNorm(d, dtype=dtype)
         self.norm2 = LayerNorm(d, dtype=dtype)
-        self.attn = MultiHeadAttention(d, heads, True, dropout_rate, init, dtype, qk_norm, rotary)
+        self.attn = MultiHeadAttention(d, heads, True, dropout_rate, init, dtype, qk_norm, rotary, kv_heads, cap, distance, causal)
         self.fc1 = Linear(d, mlp_ratio * d, True, init, dtype)
         self.fc2 = Linear(mlp_ratio * d, d, True, init, dtype)
 
@@ -296,11 +359,22 @@ class TransformerBlock(Layer):
         return {"norm1": self.norm1.init(), "attn": self.attn.init(k_attn), "norm2": self.norm2.init(),
                 "fc1": self.fc1.init(k_fc1), "fc2": self.fc2.init(k_fc2)}
 
-    def __call__(self, params, x, mask=None, key=None, positions=None):
+    def __call__(self, params, x, mask=None, key=None, positions=None, documents=None, prefix=None, lengths=None):
         k_attn, k_mlp = (None, None) if key is None else random.split(key)
-        x = x + self.attn(params["attn"], self.norm1(params["norm1"], x), mask, k_attn, positions)
-        hidden = self.fc2(params["fc2"], gelu(self.fc1(params["fc1"], self.norm2(params["norm2"], x))))
+        x = x + self.attn(params["attn"], self.norm1(params["norm1"], x), mask, k_attn, positions, documents, prefix, lengths)
+        hidden = self._mlp(params, x)
         return x + (dropout(k_mlp, hidden, self.rate) if key is not None else hidden)
+
+    def _mlp(self, params, x):
+        return self.fc2(params["fc2"], gelu(self.fc1(params["fc1"], self.norm2(params["norm2"], x))))
+
+    def state(self, batch, length, page=64):
+        return self.attn.state(batch, length, page)
+
+    def extend(self, params, x, state, lengths=None):
+        y, state = self.attn.extend(params["attn"], self.norm1(params["norm1"], x), state, lengths)
+        x = x + y
+        return x + self._mlp(params, x), state
 
 
 class SelectiveSSM(Layer):

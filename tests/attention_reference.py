@@ -25,8 +25,11 @@ CASES = [
 PAGED = [
     (1, 1, 1, 1, 1, 1, 3, "", 0), (2, 1, 4, 1, 16, 8, 5, "js", 0), (3, 1, 8, 2, 64, 24, 20, "jl", 10.0), (2, 3, 6, 3, 40, 7, 13, "sl", 4.0), (1, 17, 2, 1, 33, 16, 9, "j", 0),
     (4, 1, 16, 1, 64, 64, 12, "js", 20.0), (2, 70, 4, 2, 64, 64, 6, "jl", 0), (1, 1, 8, 2, 128, 100, 41, "s", 0), (2, 5, 3, 1, 96, 32, 11, "jsl", 7.0), (1, 2, 2, 2, 256, 5, 60, "j", 0),
-    (1, 1, 2, 1, 64, 256, 24, "js", 0), (3, 40, 1, 1, 130, 10, 9, "l", 3.0),
+    (1, 1, 2, 1, 64, 256, 24, "js", 0), (3, 40, 1, 1, 130, 10, 9, "l", 3.0), (2, 20, 4, 2, 100, 9, 50, "js", 5.0), (2, 30, 2, 1, 128, 33, 12, "jl", 0),
+    (1, 20, 4, 2, 40, 8, 5, "js", 0),
 ]
+# Enough blocks for the device's other forms: 64 rows a block, a group's heads in one part, and in two of four.
+LARGE = [(8, 256, 16, 4, 32, "jcsl", 5.0), (8, 250, 16, 16, 64, "jcp", 0), (8, 256, 32, 16, 16, "cd", 9.0), (8, 256, 32, 8, 20, "jcs", 0), (2, 300, 64, 64, 50, "jd", 0)]
 
 
 def inputs(case, dtype, seed=0):
@@ -261,6 +264,11 @@ def check_paged(case, dtype, device, change=None):
     agree(y.numpy(), want, off, dtype, "y")
     assert np.array_equal(k_pages.numpy(), want_k, equal_nan=True) and np.array_equal(v_pages.numpy(), want_v, equal_nan=True)
     assert np.array_equal(x["k_pages"].numpy(), v["k_pages"], equal_nan=True)
+
+
+def past_the_table(v):
+    """More positions before the new tokens than the table has room for."""
+    v["first"][0] = v["table"].shape[1] * v["k_pages"].shape[1] + 5
 
 
 def strange_tables(v):

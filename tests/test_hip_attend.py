@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import rustautograd_amd as rg
-from rustautograd_amd import optim
+from rustautograd_amd import nn, optim, random
 import attention_reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -44,7 +44,78 @@ def test_pages_that_are_not_there(case):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "float64"])
-@pytest.mark.parametrize("sizes", [(1,), (3, 16384, 16385), (100000, 1, 7), tuple(range(1, 131))], ids=len)
+@pytest.mark.parametrize("case", [ref.PAGED[i] for i in (1, 3, 14)], ids=str)
+def test_positions_past_the_table(case, dtype):
+    ref.check_paged(case, dtype, "hip", ref.past_the_table)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("case", ref.LARGE, ids=str)
+def test_attention_of_many_blocks(case, dtype):
+    ref.check(case, dtype, "hip")
+
+
+@pytest.mark.parametrize("length, heads", [(4500, 8), (8400, 2)])
+def test_documents_over_many_stages(length, heads):
+    """Stages without a document of the block's are left out, also past the 64 that are looked at at
+    once; one document comes back at the end."""
+    r = np.random.default_rng(length)
+    case = (1, length, heads, 1, 16, "jcsd", 3.0)
+    ids = np.repeat(np.arange(length // 40 + 1), r.integers(1, 80, length // 40 + 1))[:length]
+    ids = np.concatenate([ids, np.full(length - len(ids), ids.max() + 1)]).astype(np.int32)
+    ids[-20:] = 0
+    ids[500:700] = -1
+    v = {k: r.standard_normal((1, length, n, 16)).astype(F) for k, n in (("q", heads), ("k", 1), ("v", 1), ("dy", heads))}
+    v.update(slopes=np.exp2(-np.arange(1, heads + 1.0)).astype(F), documents=ids[None], prefix=None, lengths=None)
+    x, dy = ref.given(case, v)
+    y = rg.compile(lambda x: ref.call(case, x, v), (x,), validate="none")(x).numpy()
+    grads = rg.compile(lambda x, dy: rg.grad(lambda x: (ref.call(case, x, v) * dy).sum())(x), (x, dy), validate="none")(x, dy)
+    dx = np.split(grads["x"].numpy(), [heads, heads + 1], axis=2)
+    u, dtype, slopes, off_slopes = np.finfo(F).eps / 2, np.dtype(F), np.zeros(heads), np.zeros(heads)
+    for d in np.unique(ids):
+        at = np.flatnonzero(ids == d)
+        if d < 0:
+            assert not y[0, at].any() and not any(g[0, at].any() for g in dx)
+            continue
+        apart = at[:, None] - at[None]
+        want, off = {n: np.zeros((len(at), 16)) for n in "kv"}, {n: np.zeros((len(at), 16)) for n in "kv"}
+        for h in range(heads):
+            args = v["q"][0, at, h], v["k"][0, at, 0], v["v"][0, at, 0], apart >= 0, np.abs(apart).astype(float), 0.25, 3.0, float(v["slopes"][h]), u
+            ref.agree(y[0, at, h], *ref.head(*args), dtype, "y")
+            g, o = ref.head(*args, v["dy"][0, at, h])
+            ref.agree(dx[0][0, at, h], g[0], o[0], dtype, "dq")
+            for n, k in (("k", 1), ("v", 2)):
+                want[n] += g[k]
+                off[n] += o[k]
+            slopes[h] += g[3]
+            off_slopes[h] += o[3]
+        ref.agree(dx[1][0, at, 0], want["k"], off["k"], dtype, "dk")
+        ref.agree(dx[2][0, at, 0], want["v"], off["v"], dtype, "dv")
+    ref.agree(grads["slopes"].numpy(), slopes, off_slopes, dtype, "dslopes")
+
+
+def test_pages_past_32_bits():
+    """A cache of 4.9 GB each way, made on the device, whose last pages the table names: the rows that a
+    small cache of the same values gives."""
+    r = np.random.default_rng(5)
+    page, g, hd, pages = 256, 4, 64, 18700
+    x, base = (rg.tensor(r.standard_normal(s).astype(F)) for s in ((1, 1, 3 * g, hd), (1, page, g, hd)))
+    names = [pages - 1, 3, pages - 2]
+
+    def step(x, base, table, which):
+        cache = tuple(base * s + (which * 2.0 ** -15).reshape(-1, 1, 1, 1) for s in (1.0, -0.5))
+        return rg.paged_attention(x, cache=cache, table=table, first=np.array([700], np.int32), heads=(g, g))[0]
+
+    def at(table, which):
+        args = x, base, rg.tensor(np.array([table], np.int32)), rg.tensor(np.array(which, F))
+        return rg.compile(step, args, validate="none")(*args).numpy()
+
+    # One split more or less sums in another order: a few roundings of values near 1.
+    np.testing.assert_allclose(at(names, np.arange(pages)), at([0, 1, 2], names), rtol=0, atol=2e-6)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("sizes", [(1,), (3, 16384, 16385), (100000, 1, 7), tuple(range(1, 131)), tuple(range(4090, 4400))], ids=len)
 def test_norm(sizes, dtype):
     r = np.random.default_rng(len(sizes))
     parts = [r.standard_normal(n).astype(dtype) for n in sizes]
@@ -215,3 +286,50 @@ def test_tokens_continue_what_attention_reads_at_once():
     want, off = ref.expected(case, v, np.dtype("float32"), False)
     ref.agree(np.concatenate(out, axis=1), want["y"], off["y"], np.dtype("float32"), "y")
     ref.agree(whole, want["y"], off["y"], np.dtype("float32"), "y")
+
+
+def test_a_block_trained_and_then_served():
+    """A block of grouped, capped, turned heads under documents trains with the clip, and is then read
+    over pages, a prompt and single tokens in a captured loop; the device against the oracle."""
+    block = nn.TransformerBlock(48, 6, mlp_ratio=2, kv_heads=2, cap=5.0, rotary=True, distance=True)
+    params = block.init(random.key(1))
+    r = np.random.default_rng(6)
+    x, t = (rg.tensor(r.standard_normal((3, 40, 48)).astype(F)) for _ in range(2))
+    docs = np.sort(r.integers(0, 3, (3, 40)), axis=1).astype(np.int32)
+    opt = optim.sgd(0.1)
+
+    def step(s, data):
+        x, t = data
+        value, grads = rg.value_and_grad(lambda p: nn.mse_loss(block(p, x, documents=docs), t))(s["p"])
+        grads, norm = optim.clip_gradients(grads, 0.2)
+        p, o = opt.update(grads, s["o"], s["p"])
+        return {"p": p, "o": o}, (value, norm)
+
+    def token(s, data):
+        y, cache = block.extend(data["p"], s["x"], s["cache"])
+        return {"x": rg.tanh(y), "cache": cache}
+
+    got = {}
+    for device in ("hip", "cpu"):
+        start = {"p": params, "o": opt.init(params)}
+        run = rg.run(rg.compile(step, (start, (x, t)), validate="none", device=device), start, [(x, t)], steps=3)
+        trained = run.state["p"]
+        lengths = np.array([40, 17, 0], np.int32)
+        read = rg.compile(lambda p, x: block.extend(p, x, block.state(3, 60, page=7), lengths), (trained, x), validate="none", device=device)
+        _, cache = read(trained, x)
+        s = {"x": x[:, :1], "cache": cache}
+        served = rg.run(rg.compile(token, (s, {"p": trained}), validate="none", device=device), s, [{"p": trained}], steps=9).state
+        got[device] = [np.array(run.history["aux.0"]), np.array(run.history["aux.1"]), served["x"].numpy(), served["cache"]["k"].numpy()]
+        assert served["cache"]["pos"].numpy().tolist() == [49, 26, 9]
+    # float32 through three updates and nine tokens of two norms and four products each.
+    for a, b in zip(got["hip"], got["cpu"]):
+        np.testing.assert_allclose(a, b, rtol=1e-4, atol=1e-5)
+
+
+def test_standard_validation_on_the_device():
+    block = nn.TransformerBlock(32, 4, cap=5.0, kv_heads=2)
+    params = block.init(random.key(1))
+    x = random.normal(random.key(2), (2, 20, 32))
+    docs = np.array([[1] * 20, [2] * 15 + [-1] * 5], np.int32)
+    program = rg.compile(lambda p: rg.value_and_grad(lambda p: (block(p, x, documents=docs) ** 2.0).mean())(p), (params,), validate="standard")
+    assert program.report["status"] == "ok", program.report
