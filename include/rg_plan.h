@@ -108,8 +108,9 @@
  *                  (j <= i, or not RG_ATTEND_CAUSAL, or j < prefix) and both have the same document,
  *                  not negative; query head h reads head h G / H of k and v;
  *                  out 0: y[B,T,H,hd], the softmax of s over the keys seen, times v (0 where none is);
- *                  1: the logarithm to base 2 of the softmax's sum, [B,H,T], or the dtype's largest
- *                  value where no key is seen, for the gradient alone
+ *                  1: for the gradient alone, [2,B,H,T]: what scores to base 2 were lowered by before
+ *                  their powers of two were summed, and one over that sum; the dtype's largest value
+ *                  and 0 where no key is seen
  *       _GRAD      in the same, y, result 1, dy; out dq (joined: dx), dk, dv, dslopes
  *     PAGED_ATTENTION in q, k, v or x as above, k and v pages[P,page,G,hd], table[B,N], first[B]
  *                  (, slopes[H]) (, lengths[B]); position p of sequence b lies in row p % page of
@@ -298,7 +299,7 @@ inline Sequence attention_of(int32_t op, const SequenceAttr& at, const std::vect
     if (k >= 0 && s[(size_t)k] != want) fail(what);
   };
   const std::vector<int64_t> keys = {q.batch, q.length, q.keys, q.head}, out = {q.batch, q.length, q.heads, q.head};
-  const std::vector<int64_t> sums = {q.batch, q.heads, q.length};
+  const std::vector<int64_t> sums = {2, q.batch, q.heads, q.length};
   dims(q.k, keys, "k_must_be_batch_length_key_heads_head");
   dims(q.v, keys, "v_must_be_batch_length_key_heads_head");
   dims(q.slopes, {q.heads}, "slopes_must_be_one_per_head");

@@ -294,7 +294,10 @@ void attention(const Operands<T>& o) {
               for (int64_t j : seen) y += s[(size_t)j] * (double)vs(b * L + j, g)[d];
               o.out[0][((b * L + i) * H + h) * hd + d] = (T)y;
             }
-          if (o.out[1]) o.out[1][(b * H + h) * L + i] = seen.empty() ? std::numeric_limits<T>::max() : (T)((top + std::log(sum)) / std::log(2.0));
+          if (o.out[1]) {
+            o.out[1][(b * H + h) * L + i] = seen.empty() ? std::numeric_limits<T>::max() : (T)(top / std::log(2.0));
+            o.out[1][(q.batch * H + b * H + h) * L + i] = seen.empty() ? (T)0 : (T)(1.0 / sum);
+          }
           continue;
         }
         const T* gi = dy + ((b * L + i) * H + h) * hd;

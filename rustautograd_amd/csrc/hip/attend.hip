@@ -7,8 +7,8 @@
 //   dp = dy.v,  ds = p (dp - D),  dslope = -sum ds |i - j|,  du = ds (1 - tanh^2) scale,
 //   dv = p^T dy,  dq = du k,  dk = du^T q.
 //
-// No score is kept: the forward walks the keys once with a running maximum and sum, and leaves the
-// logarithm of each query's sum, from which the backward forms p again.
+// No score is kept: the forward walks the keys once with a running maximum and sum, and leaves both of
+// each query, from which the backward forms p again.
 //
 // A block takes 64 rows (queries, or keys where the gradients of k and v are formed), a wave 16 of
 // them, and the other side passes through LDS, 32 rows at a time for each set of four waves: with
@@ -47,12 +47,17 @@ struct Type<float> {
   static __device__ __forceinline__ acc mfma(float a, float b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
   // The tile row of register r in a lane of group g (its lane number over 16).
   static __device__ __forceinline__ int row_of(int r, int g) { return 4 * g + r; }
+  // Of a tile of results the one of row and column l16, from the lane that holds it.
+  static __device__ __forceinline__ float diagonal(acc x, int l16) {
+    const int r = l16 & 3;
+    return __shfl(r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3], l16 + 16 * (l16 >> 2));
+  }
   static __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
   static __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
   static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
-  // tanh of up to 1 in size: x + x^3 q(x^2), q the polynomial whose largest relative error over
-  // that range is least (4e-9, 1.6 units of 2^-24 with the roundings).
-  static __device__ __forceinline__ float tanh_low(float x) {
+  // What tanh(x) of up to 1 in size lacks of x, as a share of it: z q(z) with z = x^2, q the polynomial
+  // whose largest relative error of the tanh over that range is least (4e-9).
+  static __device__ __forceinline__ float tanh_share(float x) {
     const float z = x * x;
     float q = -3.5334553103893995e-4f;
     q = fmaf(q, z, 2.282229484990239e-3f);
@@ -60,8 +65,7 @@ struct Type<float> {
     q = fmaf(q, z, 2.1464820951223373e-2f);
     q = fmaf(q, z, -5.387091264128685e-2f);
     q = fmaf(q, z, 1.333215981721878e-1f);
-    q = fmaf(q, z, -3.333327770233154e-1f);
-    return fmaf(q, x * z, x);
+    return fmaf(q, z, -3.333327770233154e-1f) * z;
   }
   // Of any size: below 0.7 the fifth convergent of Lambert's continued fraction x / (1 + x^2 / (3 +
   // ...)), off by 2e-9 of it there, from there on (e^2x - 1) / (e^2x + 1), with one division.
@@ -82,10 +86,14 @@ struct Type<double> {
   static constexpr double MOST = __DBL_MAX__;
   static __device__ __forceinline__ acc mfma(double a, double b, acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
   static __device__ __forceinline__ int row_of(int r, int g) { return 4 * r + g; }
+  static __device__ __forceinline__ double diagonal(acc x, int l16) {
+    const int r = l16 >> 2;
+    return __shfl(r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3], l16 + 16 * (l16 & 3));
+  }
   static __device__ __forceinline__ double exp2_of(double x) { return exp2(x); }
   static __device__ __forceinline__ double log2_of(double x) { return log2(x); }
   static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
-  static __device__ __forceinline__ double tanh_low(double x) { return tanh(x); }
+  static __device__ __forceinline__ double tanh_share(double x) { return 0; }  // not called (LOW)
   static __device__ __forceinline__ double tanh_of(double x) { return tanh(x); }
   static constexpr bool LOW = false;
 };
@@ -117,7 +125,7 @@ struct Geo {
   static constexpr bool NARROW = SIZE <= 256;
   static constexpr int WAVES = NARROW ? 8 : 4, SETS = WAVES / RW, NT = 64 * WAVES, ROWS = 16 * RW, STAGE = TILE * SETS;
   // Waves a SIMD that the registers are to leave room for.
-  static constexpr int FORWARD = SIZE <= 256 && sizeof(T) == 4 ? 4 : SIZE <= 512 ? 2 : 1;
+  static constexpr int FORWARD = SIZE <= 256 && sizeof(T) == 4 ? (SIZE == 256 && RW == 2 ? 2 : 4) : SIZE <= 512 ? 2 : 1;
   static constexpr int BACKWARD = SIZE <= 256 && sizeof(T) == 4 ? (SIZE == 256 && RW == 2 ? 2 : 4) : SIZE <= 512 && sizeof(T) == 4 ? 2 : SIZE <= 256 ? 2 : 1;
   // The backward's own rows lie in LDS and not in registers.
   static constexpr bool KEPT = NARROW && sizeof(T) == 4;
@@ -246,18 +254,19 @@ __device__ __forceinline__ constexpr int tile_row(int t, int r) {
   return 16 * t + Type<T>::row_of(r, 0);
 }
 
-// The scores of one head, to base 2: cap log2(e) tanh(dot mul) or dot mul, less slope log2(e) times
-// the distance.
+// The scores of one head, to base 2: cap log2(e) tanh(dot scale / cap) or dot scale log2(e), less slope
+// log2(e) times the distance.
 template <class T>
 struct Scorer {
   typedef typename Type<T>::acc acc;
-  T mul, cap, slope;  // cap and slope times log2(e)
+  T mul, part, cap, slope;  // cap and slope times log2(e); `part`: the scale over the cap
   bool capped, sloped;
   __device__ __forceinline__ Scorer(const AttendArgs& a, uint32_t h) {
     constexpr double LOG2E = 1.4426950408889634;
     capped = a.cap > 0;
     sloped = a.slopes != nullptr;
-    mul = (T)(capped ? a.scale / a.cap : a.scale * LOG2E);
+    mul = (T)(a.scale * LOG2E);
+    part = (T)(capped ? a.scale / a.cap : 0);
     cap = (T)(a.cap * LOG2E);
     slope = sloped ? (T)((double)((const T*)a.slopes)[h] * LOG2E) : (T)0;
   }
@@ -265,35 +274,40 @@ struct Scorer {
   // `apart` is the signed distance between the lane's row and row row_of(0, g) of the tile.
   template <bool TANH>
   __device__ __forceinline__ void operator()(acc* s, acc* bent, int apart) const {
-#pragma unroll
-    for (int t = 0; t < 2; t++) s[t] *= mul;
     if (capped) {
-      // Scores far below the cap, as most are, take the short form.
+      // Scores below the cap, as most are, differ from the uncapped by a share, which spares them two
+      // roundings beside the quotient.
       bool high = !Type<T>::LOW;
       if constexpr (Type<T>::LOW) {
         T most = 0;
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) most = Type<T>::max_of(most, s[t][r] < 0 ? -s[t][r] : s[t][r]);
-        high = __ballot(most > 1) != 0;
+          for (int r = 0; r < 4; r++) most = Type<T>::max_of(most, abs_of(s[t][r]));
+        high = __ballot(most * abs_of(part) > 1) != 0;
       }
       if (high) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) s[t][r] = Type<T>::tanh_of(s[t][r]);
+          for (int r = 0; r < 4; r++) {
+            const T b = Type<T>::tanh_of(s[t][r] * part);
+            if (TANH) bent[t][r] = b;
+            s[t][r] = b * cap;
+          }
       } else {
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) s[t][r] = Type<T>::tanh_low(s[t][r]);
+          for (int r = 0; r < 4; r++) {
+            const T x = s[t][r] * part, u = s[t][r] * mul, share = Type<T>::tanh_share(x);
+            if (TANH) bent[t][r] = fma(x, share, x);
+            s[t][r] = fma(u, share, u);
+          }
       }
+    } else {
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        if (TANH) bent[t] = s[t];
-        s[t] *= cap;
-      }
+      for (int t = 0; t < 2; t++) s[t] *= mul;
     }
     if (sloped) {
       const T d = (T)apart;
@@ -728,9 +742,14 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h;
   const bool none = run.sum == 0 || di < 0;
   if (a.y) put_row<T, HD>((T*)a.y + row * a.head, l.g, a.head, run.out, 1 / run.sum, none);
-  // Of a query that sees nothing the type's largest value, so that the backward forms weights of 0.
-  if (a.sums && l.g == 0)
-    ((T*)a.sums)[((uint64_t)at.b * a.heads + at.h) * a.length + i] = none ? Type<T>::MOST : run.top + Type<T>::log2_of(run.sum);
+  // For the backward, which so forms the weights that were used here: the bound and the sum's
+  // reciprocal; of a query that sees nothing the type's largest value and 0, weights of 0. (With the
+  // logarithm of the sum in their place, 12 of 2^-24 each, the gradient of q was a tenth further off.)
+  if (a.sums && l.g == 0) {
+    const uint64_t stat = ((uint64_t)at.b * a.heads + at.h) * a.length + i;
+    ((T*)a.sums)[stat] = none ? Type<T>::MOST : run.top;
+    ((T*)a.sums)[stat + (uint64_t)a.batch * a.heads * a.length] = none ? (T)0 : 1 / run.sum;
+  }
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others.
@@ -742,7 +761,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
   __shared__ __align__(16) T kept[G::KEPT ? 2 * ROWS * PITCH<T, HD> : 4];
   __shared__ __align__(16) int docs[STAGE];
-  __shared__ T waves[NT / 64];
+  __shared__ T waves[NT / 64], lefts[SETS > 1 ? SETS * ROWS : 1];
   __shared__ uint64_t found[NT / 64];
   T *ks = smem, *vs = smem + STAGE * PITCH<T, HD>;
   const Place at(blockIdx.x, a.batch, a.heads, a.tiles, a.causal, G::BACKWARD * 4 == 2 * G::WAVES);
@@ -763,23 +782,25 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
     T y[HD / 4], x[HD / 4];
     row_frag<T, HD>(di >= 0 ? yb + (int64_t)i * a.heads * a.head : nullptr, l.g, a.head, whole, y);
     row_frag<T, HD>(di >= 0 ? gb + (int64_t)i * a.heads * a.head : nullptr, l.g, a.head, whole, x);
+    // On the matrix instructions in the order of the products dy.v, so that where one key is all that a
+    // query sees both are the same number, and near it nearly so: their difference is the gradient.
+    acc all = {0, 0, 0, 0};
 #pragma unroll
-    for (int n = 0; n < HD / 4; n++) dot += y[n] * x[n];
+    for (int n = 0; n < HD / 4; n++) all = Type<T>::mfma(y[n], x[n], all);
+    dot = Type<T>::diagonal(all, l.l16);
     grad.set(x, l);
     row_frag<T, HD>(di >= 0 ? qb + (int64_t)i * a.q_row : nullptr, l.g, a.head, whole, x);
     own.set(x, l);
   }
-  dot = row_sum(dot);
-  const T sums = di >= 0 ? ((const T*)a.sums_in)[stat] : (T)__builtin_huge_val();
-  if (l.set == 0 && l.g == 0 && i < (int)a.length) ((T*)a.workspace)[stat] = dot;
+  const T top = di >= 0 ? ((const T*)a.sums_in)[stat] : Type<T>::MOST, by = di >= 0 ? ((const T*)a.sums_in)[stat + (uint64_t)a.batch * a.heads * a.length] : (T)0;
   const T *kb = (const T*)a.k + (int64_t)at.b * a.length * a.k_row + kh * a.head, *vb = (const T*)a.v + (int64_t)at.b * a.length * a.k_row + kh * a.head;
-  const int end = (a.dq || a.dslopes_rows) && begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
+  const int end = begin < sight.length ? sight.keys_to(min(begin + ROWS, sight.length)) : 0;
   const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
   Stages<G> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
   acc out[HD / 16];
 #pragma unroll
   for (int n = 0; n < HD / 16; n++) out[n] = acc{0, 0, 0, 0};
-  T dslope = 0;
+  T dslope = 0, left = 0;
   Staged<T, HD, G> next_k(a.k_row, a.head), next_v(a.k_row, a.head);
   int doc = 0;
   auto load = [&](int stage) {
@@ -812,14 +833,31 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
           const int row_in = 16 * t + Type<T>::row_of(r, l.g);
           const bool sees = sight.sees(i, di, first + row_in, sight.in(first + row_in, docs[l.set * TILE + row_in]));
           s[t][r] = sees ? s[t][r] : -(T)__builtin_huge_val();
-          dp[t][r] = sees ? dp[t][r] : dot;
+          dp[t][r] = sees ? dp[t][r] : (T)0;
           if (scorer.capped) bent[t][r] = sees ? bent[t][r] : (T)0;
         }
     }
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) s[t][r] = Type<T>::exp2_of(s[t][r] - sums) * (dp[t][r] - dot);
+      for (int r = 0; r < 4; r++) s[t][r] = Type<T>::exp2_of(s[t][r] - top) * by;
+    if (seen_to <= TILE) {
+      // All keys of the wave's queries are in this tile: dy.y as the mean of the products dy.v that it is
+      // of few, whose roundings then meet in the differences.
+      T mean = 0;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) mean += s[t][r] * (s[t][r] == 0 ? (T)0 : dp[t][r]);
+      dot = row_sum(mean);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        s[t][r] *= dp[t][r] - dot;
+        left += s[t][r];
+      }
     if (scorer.sloped) {
 #pragma unroll
       for (int t = 0; t < 2; t++)
@@ -832,6 +870,17 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
     }
     weigh<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, out);
   }
+  // What the differences leave over goes to dy.y, as the gradients of k and v take it: their sum over a
+  // query's keys is 0.
+  left = row_sum(left);
+  if constexpr (SETS > 1) {
+    lefts[l.set * ROWS + l.row] = left;
+    __syncthreads();
+    left = 0;
+#pragma unroll
+    for (int other = 0; other < SETS; other++) left += lefts[other * ROWS + l.row];
+  }
+  if (l.set == 0 && l.g == 0 && i < (int)a.length) ((T*)a.workspace)[stat] = di < 0 ? (T)0 : dot + left;
   if constexpr (SETS > 1) join<T, HD, G>(out, smem, l.set);
   if (a.dq && l.set == 0 && i < (int)a.length)
     put_row<T, HD>((T*)a.dq + ((int64_t)at.b * a.length + i) * a.q_row + at.h * a.head, l.g, a.head, out, (T)a.scale, di < 0);
@@ -857,6 +906,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   __shared__ __align__(16) T smem[2 * STAGE * PITCH<T, HD>];
   __shared__ __align__(16) T kept[G::KEPT ? 2 * ROWS * PITCH<T, HD> : 4];
   __shared__ __align__(16) int docs[STAGE];
+  __shared__ __align__(16) T tops[STAGE];
   __shared__ __align__(16) T sums[STAGE];
   __shared__ __align__(16) T dots[STAGE];
   __shared__ uint64_t found[NT / 64];
@@ -888,7 +938,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   const uint32_t last = h + per_part;
   Staged<T, HD, G> next_q(a.q_row, a.head), next_g((int64_t)a.heads * a.head, a.head);
   int doc = 0;
-  T sum = 0, dot = 0;
+  T top = 0, sum = 0, dot = 0;
   auto load = [&](uint32_t of, int stage) {
     const int first = stage * STAGE;
     const int64_t t = (int64_t)at.b * a.length + first;
@@ -898,7 +948,8 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
       const int i = first + (int)threadIdx.x;
       doc = sight.document(i);
       const uint64_t stat = ((uint64_t)at.b * a.heads + of) * a.length + min(i, sight.length - 1);
-      sum = ((const T*)a.sums_in)[stat];
+      top = ((const T*)a.sums_in)[stat];
+      sum = ((const T*)a.sums_in)[stat + (uint64_t)a.batch * a.heads * a.length];
       dot = ((const T*)a.workspace)[stat];
     }
   };
@@ -911,7 +962,8 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
     next_q.store(qs);
     next_g.store(gs);
     if (threadIdx.x < STAGE) {
-      sums[threadIdx.x] = doc < 0 ? (T)__builtin_huge_val() : sum;  // weights of 0
+      tops[threadIdx.x] = doc < 0 ? Type<T>::MOST : top;  // weights of 0
+      sums[threadIdx.x] = doc < 0 ? (T)0 : sum;
       dots[threadIdx.x] = doc < 0 ? (T)0 : dot;
     }
     settle<T, HD, G>(sight, k * STAGE, doc, docs, qs, gs);
@@ -939,7 +991,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
           dp[t][r] = 0;
           if (scorer.capped) bent[t][r] = 0;
         }
-        s[t][r] = Type<T>::exp2_of(s[t][r] - sums[row]);
+        s[t][r] = Type<T>::exp2_of(s[t][r] - tops[row]) * sums[row];
         dp[t][r] = s[t][r] * (dp[t][r] - dots[row]);
       }
     if (scorer.capped) {
