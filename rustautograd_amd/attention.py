@@ -3,7 +3,7 @@ its form over a paged cache. Each is one operation of the engine with kernels of
 may be long, since no score is kept. The reference has no counterpart.
 
 Values are float32 or float64, one dtype a call; documents, prefixes, lengths, tables and positions
-are int32. Heads have at most 256 values.
+are int32. Heads have at most 256 values, of float64 on the device at most 128.
 """
 
 import math
@@ -51,8 +51,8 @@ def attention(q, k=None, v=None, heads=None, causal=True, scale=None, cap=None, 
     `slopes` (heads,), lowered by slope * |i - j|. Query i sees key j if j <= i (any j if not
     `causal`), or j < `prefix` (batch,); if both are of the same document of `documents` (batch,
     length), of which a negative one is none; and if both are before `lengths` (batch,). A query that
-    sees nothing gives 0. What lies outside a sequence or a document is not read. Differentiable
-    in q, k, v and the slopes, once."""
+    sees nothing gives 0. Infinities and NaN reach what sees them and nothing else; what lies past the
+    lengths or in no document is not looked at. Differentiable in q, k, v and the slopes, once."""
     operands, pair, flags = _parts(q, k, v, heads)
     index = [x if x is None else _as_index(x) for x in (documents, prefix, lengths)]
     values, mask = _present(operands, (slopes, *index), (_SLOPES, _DOCUMENTS, _PREFIX, _LENGTHS))

@@ -220,7 +220,8 @@ __device__ __forceinline__ void score(const T* lds, int l16, int g, const F& own
 }
 
 // acc of the lane's row += the tile's 32 rows weighed by w[t][r]: value row_of(r, g) HD / 16 + n of the
-// head in acc[n][r].
+// head in acc[n][r]. Keys that are not seen have weights of 0, which would not keep infinities and NaN
+// out: the rows have none (make_finite).
 template <class T, int HD>
 __device__ __forceinline__ void weigh(const T* lds, int l16, int g, const typename Type<T>::acc* w, typename Type<T>::acc* acc) {
   constexpr int ND = HD / 16;
@@ -418,6 +419,61 @@ __device__ __forceinline__ double buffer_value(__amdgpu_buffer_rsrc_t from, uint
   typedef uint32_t words __attribute__((ext_vector_type(2)));
   const words w = __builtin_amdgcn_raw_buffer_load_b64(from, (int)at, 0, 0);
   return __builtin_bit_cast(double, w);
+}
+
+// Makes infinities and NaN among a thread's N vectors 0; whether there were any. Rows to be weighed go
+// through it, and what a seen one of them does is made up for after the loop, in `for_odd_rows`: there is
+// no place for it inside (it cost the forward of heads of 128 a third, in registers).
+template <class T, int N, class... More>
+__device__ __forceinline__ bool make_finite(typename Type<T>::vec (&x)[N], More&... more) {
+  T z = 0;
+  auto look = [&](auto& v) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int j = 0; j < Type<T>::V; j++) z = fma(v[i][j], (T)0, z);
+  };
+  auto clear = [&](auto& v) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+      for (int j = 0; j < Type<T>::V; j++) v[i][j] = v[i][j] * (T)0 == 0 ? v[i][j] : (T)0;
+  };
+  look(x);
+  (look(more), ...);
+  const bool odd = z != z;
+  if (odd) {
+    clear(x);
+    (clear(more), ...);
+  }
+  return odd;
+}
+
+// Calls f(n) for each n of [from, to) whose row at(n) of `head` values holds an infinity or NaN; a wave's
+// lanes look at 64 rows at once. `at` gives nullptr where there is no row.
+template <class At, class F>
+__device__ __forceinline__ void for_odd_rows(int from, int to, uint32_t head, const At& at, const F& f) {
+  for (int base = from; base < to; base += 64) {
+    const int n = base + (int)(threadIdx.x & 63);
+    bool odd = false;
+    if (n < to)
+      if (const auto* row = at(n))
+        for (uint32_t d = 0; d < head; d++) odd |= row[d] * 0 != 0;
+    for (uint64_t left = __ballot(odd); left; left &= left - 1) f(base + (int)__builtin_ctzll(left));
+  }
+}
+// To a lane's share of the result of a row that sees it, a row's infinities and NaN, whatever its weight.
+template <class T, int HD>
+__device__ __forceinline__ void add_odd(const T* row, int g, uint32_t head, typename Type<T>::acc* acc) {
+  constexpr int ND = HD / 16;
+#pragma unroll
+  for (int n = 0; n < ND; n++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const uint32_t d = (uint32_t)(Type<T>::row_of(r, g) * ND + n);
+      const T x = d < head ? row[d] : (T)0;
+      acc[n][r] += x * 0 == 0 ? (T)0 : x;
+    }
 }
 
 // N rows of one operand on their way to LDS, 16 bytes a thread and step. They are read as a buffer that
@@ -644,7 +700,7 @@ template <int RW>
 struct Lane {
   int l16, g, set, row, first;
   __device__ __forceinline__ Lane() {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     l16 = lane & 15;
     g = lane >> 4;
     set = wave / RW;
@@ -702,6 +758,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   const int seen_to = i0 < sight.length ? sight.keys_to(min(i0 + 16, sight.length)) : 0;
   Stages<G> stages(sight, begin, 0, (end + STAGE - 1) / STAGE, found);
   Running<T, HD> run;
+  bool odd = false;
   Staged<T, HD, G> next_k(a.k_row, a.head), next_v(a.k_row, a.head);
   int doc = 0;
   auto load = [&](int stage) {
@@ -714,6 +771,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   if (k < stages.end) load(k);
   while (k < stages.end) {
     __syncthreads();
+    odd |= make_finite<T>(next_v.x);
     next_k.store(ks);
     next_v.store(vs);
     settle<T, HD, G>(sight, k * STAGE, doc, docs, ks, vs);
@@ -738,6 +796,11 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   }
   run.sum = row_sum(run.sum);
   if constexpr (SETS > 1) join<T, HD, G>(run, smem, tops, sums, l.set);
+  if (__syncthreads_or(odd) && l.set == 0) {
+    for_odd_rows(0, seen_to, a.head, [&](int j) { return vb + (int64_t)j * a.k_row; }, [&](int j) {
+      if (sight.sees(i, di, j, sight.document(j))) add_odd<T, HD>(vb + (int64_t)j * a.k_row, l.g, a.head, run.out);
+    });
+  }
   if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)at.b * a.length + i) * a.heads + at.h;
   const bool none = run.sum == 0 || di < 0;
@@ -801,6 +864,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 #pragma unroll
   for (int n = 0; n < HD / 16; n++) out[n] = acc{0, 0, 0, 0};
   T dslope = 0, left = 0;
+  bool odd = false;
   Staged<T, HD, G> next_k(a.k_row, a.head), next_v(a.k_row, a.head);
   int doc = 0;
   auto load = [&](int stage) {
@@ -813,6 +877,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   if (k < stages.end) load(k);
   while (k < stages.end) {
     __syncthreads();
+    odd |= make_finite<T>(next_k.x);
     next_k.store(ks);
     next_v.store(vs);
     settle<T, HD, G>(sight, k * STAGE, doc, docs, ks, vs);
@@ -869,6 +934,16 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
       for (int t = 0; t < 2; t++) s[t] -= s[t] * (bent[t] * bent[t]);
     }
     weigh<T, HD>(ks + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, out);
+  }
+  if (__syncthreads_or(odd)) {
+    // The key's scores are no numbers either: nothing is left of a query that sees one.
+    bool hit = false;
+    for_odd_rows(0, seen_to, a.head, [&](int j) { return kb + (int64_t)j * a.k_row; }, [&](int j) { hit |= sight.sees(i, di, j, sight.document(j)); });
+    if (hit) {
+      left = dslope = (T)__builtin_nan("");
+#pragma unroll
+      for (int n = 0; n < HD / 16; n++) out[n] = acc{left, left, left, left};
+    }
   }
   // What the differences leave over goes to dy.y, as the gradients of k and v take it: their sum over a
   // query's keys is 0.
@@ -939,6 +1014,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   Staged<T, HD, G> next_q(a.q_row, a.head), next_g((int64_t)a.heads * a.head, a.head);
   int doc = 0;
   T top = 0, sum = 0, dot = 0;
+  bool odd = false;
   auto load = [&](uint32_t of, int stage) {
     const int first = stage * STAGE;
     const int64_t t = (int64_t)at.b * a.length + first;
@@ -959,6 +1035,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
   while (some && h < last) {
     if (!G::NARROW) load(h, k);  // its registers are the accumulators' while it computes
     __syncthreads();
+    odd |= make_finite<T>(next_q.x, next_g.x);
     next_q.store(qs);
     next_g.store(gs);
     if (threadIdx.x < STAGE) {
@@ -986,11 +1063,6 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int row = l.set * TILE + 16 * t + Type<T>::row_of(r, l.g);
-        if (!all && !sight.sees(here * STAGE + row, sight.in(here * STAGE + row, docs[row]), j, dj)) {
-          s[t][r] = -(T)__builtin_huge_val();
-          dp[t][r] = 0;
-          if (scorer.capped) bent[t][r] = 0;
-        }
         s[t][r] = Type<T>::exp2_of(s[t][r] - tops[row]) * sums[row];
         dp[t][r] = s[t][r] * (dp[t][r] - dots[row]);
       }
@@ -998,12 +1070,38 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 #pragma unroll
       for (int t = 0; t < 2; t++) dp[t] -= dp[t] * (bent[t] * bent[t]);
     }
+    // After all of it: a query that does not see the key may hold anything.
+    if (!all) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int row = l.set * TILE + 16 * t + Type<T>::row_of(r, l.g);
+          const bool sees = sight.sees(here * STAGE + row, sight.in(here * STAGE + row, docs[row]), j, dj);
+          s[t][r] = sees ? s[t][r] : (T)0;
+          dp[t][r] = sees ? dp[t][r] : (T)0;
+        }
+    }
     weigh<T, HD>(gs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, s, dv);
     weigh<T, HD>(qs + l.set * TILE * PITCH<T, HD>, l.l16, l.g, dp, dk);
   }
   if constexpr (SETS > 1) {
     join<T, HD, G>(dk, smem, l.set);
     join<T, HD, G>(dv, smem, l.set);
+  }
+  if (__syncthreads_or(odd) && l.set == 0) {
+    // Of queries or gradients that are no numbers nothing is left to the keys that they see.
+    bool hit = false;
+    for (uint32_t of = last - per_part; of < last; of++) {
+      auto see = [&](int i) { hit |= sight.sees(i, sight.document(i), j, dj); };
+      for_odd_rows(seen_from, sight.length, a.head, [&](int i) { return (const T*)a.q + ((int64_t)at.b * a.length + i) * a.q_row + of * a.head; }, see);
+      for_odd_rows(seen_from, sight.length, a.head, [&](int i) { return (const T*)a.dy + (((int64_t)at.b * a.length + i) * a.heads + of) * a.head; }, see);
+    }
+    if (hit) {
+      const T none = (T)__builtin_nan("");
+#pragma unroll
+      for (int n = 0; n < HD / 16; n++) dk[n] = dv[n] = acc{none, none, none, none};
+    }
   }
   if (l.set != 0 || j >= (int)a.length) return;
   const bool none = dj < 0;
@@ -1093,6 +1191,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   const int64_t kn = (const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.k_pages;
   const int64_t vn = (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head - (const T*)a.v_pages;
   Running<T, HD> run;
+  bool odd = false;
   Gathered<T, HD, G> next;
   // Where a stage's rows lie is looked up by its first threads a stage before it is loaded, two before
   // it is used, so that no load waits for the table.
@@ -1128,6 +1227,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   }
   for (int stage = from; stage < end; stage += STAGE) {
     __syncthreads();
+    odd |= make_finite<T>(next.y);
     next.store(ks, vs);
     if (looks) there[threadIdx.x] = coming[threadIdx.x];
     leave();
@@ -1167,6 +1267,16 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   }
   run.sum = row_sum(run.sum);
   if constexpr (SETS > 1) join<T, HD, G>(run, smem, tops, sums, l.set);
+  if (__syncthreads_or(odd) && l.set == 0) {
+    auto value = [&](int c) -> const T* {
+      if (c >= cache.past) return (const T*)a.v_pages + vn + (int64_t)(c - cache.past) * a.k_row;
+      const int64_t row = cache.row((uint32_t)c);
+      return row < 0 ? nullptr : (const T*)a.v_pages + (row * a.keys + kh) * a.head;
+    };
+    for_odd_rows(from, end, a.head, value, [&](int c) {
+      if (in && c - cache.past <= i) add_odd<T, HD>(value(c), l.g, a.head, run.out);
+    });
+  }
   if (l.set != 0 || i >= (int)a.length) return;
   const uint64_t row = ((uint64_t)b * a.length + i) * a.heads + h;
   if (a.splits == 1) {
@@ -1196,7 +1306,7 @@ struct FewGeo {
 constexpr int FEW_ROWS = 16;
 
 template <class T, int HD, bool WHOLE>
-__global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(AttendArgs a) {
+__global__ void __launch_bounds__(256, (WHOLE ? FewGeo<T, HD>::TILES + 1 : 2)) k_paged_few(AttendArgs a) {
   typedef typename Type<T>::acc acc;
   typedef typename Type<T>::vec vec;
   constexpr int TILES = FewGeo<T, HD>::TILES, STEP = FewGeo<T, HD>::STEP, ND = HD / 16, V = Type<T>::V;
@@ -1288,9 +1398,23 @@ __global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(A
             if (!(x.there[t] >> Type<T>::row_of(r, g) & 1)) x.v[t][r][n] = 0;
       }
   };
-  // `apart`: the distance of the lane's row from the step's first key.
-  auto work = [&](Rows& x, int apart, bool ordered) {
+  // `apart`: the distance of the lane's row from the step's first key. `news`: the values of the new
+  // tokens, where the step is of them.
+  auto work = [&](Rows& x, int apart, const T* news) {
+    const bool ordered = news != nullptr;
     clear(x);
+    bool odd = false;
+    if (ordered && a.length > 1) {
+      // Of tokens that earlier ones do not see, infinities and NaN are kept out as by make_finite.
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int n = 0; n < ND; n++)
+          if (x.v[0][r][n] * 0 != 0) {
+            odd = true;
+            x.v[0][r][n] = 0;
+          }
+    }
     acc s[2] = {acc{0, 0, 0, 0}, acc{0, 0, 0, 0}};
 #pragma unroll
     for (int n = 0; n < KV; n++)
@@ -1314,6 +1438,9 @@ __global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(A
       for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int n = 0; n < ND; n++) run.out[n] = Type<T>::mfma(x.v[t][r][n], s[t][r], run.out[n]);
+    if (ordered && __ballot(odd) != 0)
+      for (int c = 0; c < cache.count; c++)
+        if (in && c <= i) add_odd<T, HD>(news + c * a.k_row, g, a.head, run.out);
   };
   const T *kp = (const T*)a.k_pages + kh * a.head, *vp = (const T*)a.v_pages + kh * a.head;
   const int64_t pitch = (int64_t)a.keys * a.head;
@@ -1324,13 +1451,14 @@ __global__ void __launch_bounds__(256, (FewGeo<T, HD>::TILES + 1)) k_paged_few(A
   for (; first < end; first += 4 * STEP) {
     fetch(kp, vp, pitch, row, x);
     look(first + 4 * STEP, row);
-    work(x, cache.first + i - first, false);
+    work(x, cache.first + i - first, nullptr);
   }
   if (own && wave == 3) {
 #pragma unroll
     for (int t = 0; t < TILES; t++) row[t] = t == 0 && l16 < cache.count ? l16 : -1;
-    fetch((const T*)a.k + (int64_t)b * a.length * a.k_row + kh * a.head, (const T*)a.v + (int64_t)b * a.length * a.k_row + kh * a.head, a.k_row, row, x);
-    work(x, i, true);
+    const int64_t at = (int64_t)b * a.length * a.k_row + kh * a.head;
+    fetch((const T*)a.k + at, (const T*)a.v + at, a.k_row, row, x);
+    work(x, i, (const T*)a.v + at);
   }
   // The four waves' results, joined in order.
   const T sum = row_sum(run.sum);

@@ -190,6 +190,48 @@ def check(case, dtype, device):
         agree(got[k], want[k], off[k], dtype, "d" + k)
 
 
+# Of CASES, and where values that are no numbers stand: their place as a share of the length.
+ODD = [(CASES[i], at) for i, at in ((5, 0.3), (6, 0.9), (8, 0.6), (9, 0.2), (11, 0.7), (12, 0.3), (14, 0.5), (15, 0.4), (16, 0.8))] + [(LARGE[1], 0.5), (LARGE[3], 0.9)]
+
+
+def check_odd(case, at, bad, dtype, device):
+    """Infinities and NaN in one position of the first sequence reach what sees it and nothing else: its key
+    and value the queries that see it and, through them, the keys that those see; its query and the
+    gradient of its result the keys that it sees."""
+    dtype = np.dtype(dtype)
+    case = (*case[:5], case[5].replace("j", ""), case[6])
+    v, see, p = inputs(case, dtype), seen(case, inputs(case, dtype)), int(at * case[1])
+    assert see[0, p, p]
+    program = rg.compile(lambda x: call(case, x, v), ({k: rg.tensor(v[k]) for k in ("q", "k", "v", "slopes") if v[k] is not None},), validate="none", device=device)
+
+    def agrees(got, want, off, reached, what):
+        agree(np.where(reached[..., None, None], dtype.type(0), got), np.where(reached[..., None, None], 0.0, want), off, dtype, what)
+        if np.isnan(bad):
+            assert np.isnan(got[reached]).all(), what
+
+    for where in (("k", "v"), ("v",), ("q", "dy"), ("dy",)):
+        x = {k: v[k].copy() for k in ("q", "k", "v", "dy", "slopes") if v[k] is not None}
+        for k in where:
+            x[k][0, p, :, 1:] = bad
+        dy, x = rg.tensor(x["dy"]), {k: rg.tensor(a) for k, a in x.items() if k != "dy"}
+        queries = np.zeros(see.shape[:2], bool)
+        queries[0] = see[0, :, p] if "v" in where else np.arange(case[1]) == p
+        keys = (see & queries[:, :, None]).any(1)
+        y, want, off = program(x).numpy(), *expected(case, v, dtype, False)
+        if "dy" in where:
+            agrees(y, want["y"], off["y"], queries & ("q" in where), "y")
+        else:
+            column = 0 if "k" in where else 1  # of values alone the others' columns are as they were
+            agree(y[..., :column], want["y"][..., :column], off["y"][..., :column], dtype, "y")
+            agrees(y[..., column:], want["y"][..., column:], off["y"][..., column:], queries, "y")
+        grads = rg.compile(lambda x, dy: rg.grad(lambda x: (call(case, x, v) * dy).sum())(x), (x, dy), validate="none", device=device)(x, dy)
+        want, off = expected(case, v, dtype, True)
+        for k, reached in (("q", queries), ("k", keys)):
+            agrees(grads[k].numpy(), want[k], off[k], reached, "d" + k)
+        got = grads["v"].numpy()
+        agree(np.where(keys[..., None, None], dtype.type(0), got), np.where(keys[..., None, None], 0.0, want["v"]), off["v"], dtype, "dv")
+
+
 # ---- over a paged cache ------------------------------------------------------------------------------
 
 def paged_inputs(case, dtype, seed=0):
@@ -279,3 +321,22 @@ def strange_tables(v):
     if len(v["first"]) > 1:
         v["table"][-1, :] = np.iinfo(np.int32).min
         v["first"][-1] = -3
+
+
+def check_odd_token(case, bad, dtype, device):
+    """Infinities and NaN in the last new token of the first sequence reach its own row alone."""
+    dtype = np.dtype(dtype)
+    case = (*case[:7], case[7].replace("j", ""), case[8])
+    v = paged_inputs(case, dtype)
+    clean = paged_expected(case, v, dtype)
+    last = case[1] - 1
+    for where in (("k", "v"), ("v",)):
+        x = {k: a.copy() for k, a in v.items() if a is not None}
+        for k in where:
+            x[k][0, last] = bad
+        y, (k_pages, v_pages) = rg.compile(lambda x: paged_call(case, x), (paged_given(case, x),), validate="none", device=device)(paged_given(case, x))
+        got, want = y.numpy(), clean[0].copy()
+        assert not np.isfinite(got[0, last]).any()
+        got[0, last] = want[0, last] = 0
+        agree(got, want, clean[1], dtype, "y")
+        assert np.isfinite(k_pages.numpy()).all() == ("k" not in where) and not np.isfinite(v_pages.numpy()).all()

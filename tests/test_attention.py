@@ -24,6 +24,20 @@ def test_paged_attention(case, dtype):
     ref.check_paged(case, dtype, "cpu")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("case, at", ref.ODD[:-2], ids=str)
+def test_what_is_no_number_reaches_what_sees_it(case, at, bad, dtype):
+    ref.check_odd(case, at, bad, dtype, "cpu")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("case", [ref.PAGED[i] for i in (3, 4, 6, 9, 11, 13)], ids=str)
+def test_a_token_that_is_no_number(case, bad, dtype):
+    ref.check_odd_token(case, bad, dtype, "cpu")
+
+
 @pytest.mark.parametrize("case", [ref.PAGED[i] for i in (1, 2, 3, 6)], ids=str)
 def test_pages_that_are_not_there(case):
     ref.check_paged(case, "float32", "cpu", ref.strange_tables)

@@ -38,6 +38,24 @@ def test_paged_attention(case, dtype):
             ref.check_paged(case, dtype, "hip")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("case, at", ref.ODD, ids=str)
+def test_what_is_no_number_reaches_what_sees_it(case, at, bad, dtype):
+    if not _takes(case[4], dtype):
+        pytest.skip("refused")
+    ref.check_odd(case, at, bad, dtype, "hip")
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float64"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("case", [ref.PAGED[i] for i in (3, 4, 6, 9, 11, 13)], ids=str)
+def test_a_token_that_is_no_number(case, bad, dtype):
+    if not _takes(case[4], dtype):
+        pytest.skip("refused")
+    ref.check_odd_token(case, bad, dtype, "hip")
+
+
 @pytest.mark.parametrize("case", [ref.PAGED[i] for i in (1, 2, 3, 6)], ids=str)
 def test_pages_that_are_not_there(case):
     ref.check_paged(case, "float32", "hip", ref.strange_tables)
