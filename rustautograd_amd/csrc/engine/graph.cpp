@@ -706,7 +706,7 @@ void Graph::check_sequence(const Op& op, const std::vector<uint32_t>& inputs) co
     if (!std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)) fail("INVALID_ARGUMENT", "scale_must_be_finite_and_cap_positive");
     // Scores are divided by the cap and multiplied by it in the dtype.
     if (d == DType::F32 && op.eps > 0 && !(op.eps >= 1e-30 && op.eps <= 1e30)) fail("INVALID_ARGUMENT", "cap_out_of_the_dtypes_range");
-    if (d == DType::F32 && std::fabs(op.base) > 1e30) fail("INVALID_ARGUMENT", "scale_out_of_the_dtypes_range");
+    if (d == DType::F32 && (std::fabs(op.base) > 1e30 || (op.eps > 0 && std::fabs(op.base) > 1e30 * op.eps))) fail("INVALID_ARGUMENT", "scale_out_of_the_dtypes_range");
   }
   const bool rotary = op.kind == RG_OP_ROTARY_NORM || op.kind == RG_OP_ROTARY_NORM_GRAD;
   if (rotary && (!(op.base > 0) || !std::isfinite(op.base) || !(op.eps >= 0) || !std::isfinite(op.eps)))

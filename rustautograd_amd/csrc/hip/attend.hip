@@ -20,6 +20,9 @@
 // the head, spread so that a lane ends with consecutive values of its row.
 //
 // Scores, sums, maxima and results are held in the type, scores to base 2.
+//
+// Times below are of one MI355X, whose fp32 matrix product of 8192^3 reaches 154 TFLOP/s and whose copy
+// of 2 GB 4.9 TB/s. "The causal case" is 2 sequences of 2048, 8 heads of 64, capped: 8.6 GFLOP forward.
 #include "attend.h"
 
 #include <algorithm>
@@ -53,7 +56,6 @@ struct Type<float> {
     return __shfl(r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3], l16 + 16 * (l16 >> 2));
   }
   static __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
-  static __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
   static __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
   // What tanh(x) of up to 1 in size lacks of x, as a share of it: z q(z) with z = x^2, q the polynomial
   // whose largest relative error of the tanh over that range is least (4e-9).
@@ -91,10 +93,31 @@ struct Type<double> {
     return __shfl(r == 0 ? x[0] : r == 1 ? x[1] : r == 2 ? x[2] : x[3], l16 + 16 * (l16 & 3));
   }
   static __device__ __forceinline__ double exp2_of(double x) { return exp2(x); }
-  static __device__ __forceinline__ double log2_of(double x) { return log2(x); }
   static __device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
   static __device__ __forceinline__ double tanh_share(double x) { return 0; }  // not called (LOW)
-  static __device__ __forceinline__ double tanh_of(double x) { return tanh(x); }
+  // (e^2x - 1) / (e^2x + 1), where e^2x - 1 = (2^n - 1) + 2^n (e^y - 1) with y of at most ln 2 / 2 in size,
+  // and e^y - 1 is its Taylor series to the 14th power (off by 2e-19 of it): no digit is lost near 0, where
+  // n = 0. Within 3 of 2^-53 of the tanh; the library's, also within few, takes the forward of 2 x 130 x 4
+  // heads of 32 from 18 to 22 us.
+  static __device__ __forceinline__ double tanh_of(double x) {
+    const double a = fmin(2 * fabs(x), 40.0), n = __builtin_rint(a * 1.4426950408889634);
+    const double y = fma(n, -0.6931471805599453, a);
+    double p = 1.0 / 87178291200.0;
+    p = fma(p, y, 1.0 / 6227020800.0);
+    p = fma(p, y, 1.0 / 479001600.0);
+    p = fma(p, y, 1.0 / 39916800.0);
+    p = fma(p, y, 1.0 / 3628800.0);
+    p = fma(p, y, 1.0 / 362880.0);
+    p = fma(p, y, 1.0 / 40320.0);
+    p = fma(p, y, 1.0 / 5040.0);
+    p = fma(p, y, 1.0 / 720.0);
+    p = fma(p, y, 1.0 / 120.0);
+    p = fma(p, y, 1.0 / 24.0);
+    p = fma(p, y, 1.0 / 6.0);
+    p = fma(p, y, 0.5);
+    const double e = fma(p, y * y, y), two = __builtin_ldexp(1.0, (int)n), up = fma(two, e, two - 1);
+    return copysign(x == x ? up / (up + 2) : x, x);
+  }
   static constexpr bool LOW = false;
 };
 
@@ -733,6 +756,9 @@ struct Own {
   }
 };
 
+// Two products a pair. Bound by the matrix unit and the vector unit, which share a SIMD's issue: of the
+// causal case's 121 us (71 TFLOP/s) the first is busy for 57 % and the second, with some 220 instructions
+// for a wave's 16 x 32 scores, for 33 %. Heads of 128 over 5000 positions: 331 us, 77 TFLOP/s.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_attend(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -815,7 +841,8 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
   }
 }
 
-// The gradient of q, of the slopes, and each query's dy.y for the kernel of the others.
+// The gradient of q, of the slopes, and each query's dy.y for the kernel of the others. Three products a
+// pair, bound as the forward is: 181 us in the causal case, 71 TFLOP/s, the matrix unit busy for 59 %.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dq(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -973,6 +1000,9 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 
 // The gradients of k and v: a block's 64 keys against the queries of the heads that read them, all
 // of a group's or, where that leaves too few blocks, a part of them, whose sums k_attend_parts adds up.
+// Four products a pair: 229 us in the causal case, 75 TFLOP/s, the matrix unit busy for 60 %. Scores and
+// dy.v are formed here a second time; one kernel for all five products would have to add to dq from many
+// blocks, with atomics in an order of their own or a row of partial sums for every 64 keys.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dkv(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -1157,7 +1187,8 @@ struct Cache {
 };
 
 // Rows of a sequence's queries: the heads of one key head side by side, token after token. A block
-// takes 64 of them and a split of the keys.
+// takes 64 of them (32 of heads past 256 bytes) and a split of the keys. Bound as the forward is, at two
+// waves a SIMD: four chunks of 256, 8 heads of 128, over 0 to 3800 positions 176 us in the mean, 58 TFLOP/s.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_paged(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -1296,7 +1327,10 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
 // fourth step of the split's keys, straight from memory into the fragments of both products, while the
 // rows of its next step are looked up. A key's row is read by the four lanes that hold it 16 bytes
 // apart, a value's by sixteen. Three waves a SIMD, with 16 KB on the way each, hide what they wait for;
-// a second step's fragments in registers left room for one (32 us against the 23 of the block's kernel).
+// a second step's fragments in registers left room for one and took three times as long. Bound by memory:
+// 62 MB of 60000 positions, 2 key heads of 64, in 14 to 16 us (4.0 TB/s); by the latency of a split's few
+// steps where there are many sequences: 28 MB of sixteen of 300 to 2300 in 10 to 12 us, for which the
+// kernel of whole tiles takes 23.
 // WHOLE: heads of whole 16 bytes.
 template <class T, int HD>
 struct FewGeo {
@@ -1590,7 +1624,9 @@ __global__ void __launch_bounds__(512) k_paged_finish(AttendArgs a, uint32_t joi
 
 // ---- the joint norm --------------------------------------------------------------------------------
 
-// Values of a block: four 16 bytes a thread of float32 on their way at once.
+// Squares are exact in 64 bits and summed there. Values of a block: four 16 bytes a thread of float32 on
+// their way at once. 19 MB in 64 tensors: 4.3 to 5.3 us (3.7 TB/s or more, from the caches) and 1.8 for the
+// root of the blocks' sums.
 constexpr uint64_t NORM_PER_BLOCK = 4096;
 
 template <class T>
@@ -1665,7 +1701,9 @@ void by_head(int dtype, uint32_t head, uint32_t rows, const F& f) {
 bool wide_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 64u : 32u); }
 bool widest_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 128u : 64u); }
 // Rows of a block: 64, or 32 where those leave fewer than two blocks for every CU, and for heads whose
-// blocks have four waves.
+// blocks have four waves. Forward, dq, dk and dv of the causal case (512 blocks of 64) 121, 181, 229 us, with 32
+// rows 152, 201, 242; of 3 sequences of 777, 6 heads of 44 (234 blocks of 64) 31, 40, 47 with 32 rows, with 64
+// 46, 68, 90.
 uint32_t rows_of(int dtype, const AttendArgs& a) {
   if (widest_head(dtype, a.head)) return 64;
   return wide_head(dtype, a.head) || (uint64_t)a.batch * a.heads * ((a.length + 63) / 64) < 2 * CUS ? 32 : 64;
@@ -1688,12 +1726,14 @@ uint32_t paged_tiles(int dtype, const AttendArgs& a) {
   return (uint32_t)(((uint64_t)a.length * (a.heads / a.keys) + paged_rows(dtype, a) - 1) / paged_rows(dtype, a));
 }
 // Over how many blocks a sequence's keys are split, by the room of its table, since only the device
-// knows how much of it is used: three blocks of few rows for every CU, of whole tiles two, but not so
-// many that a full table leaves one fewer than 128 keys (a step of each wave) or 256.
+// knows how much of it is used: three blocks of few rows for every CU, of whole tiles two (176 us for 4
+// chunks of 256 at 8 heads of 128 over up to 4096 positions; with four of them 193), but not so many that
+// a full table leaves one fewer keys than a stage of the block has (float64, 3 x 17 x 6 heads of 40 over 600
+// positions: 12 us, with 256 at least 27).
 void set_splits(int dtype, AttendArgs& a) {
   const bool few = few_rows(dtype, a);
   const uint64_t keys = (uint64_t)a.table_pages * a.page + (few ? 0 : a.length), blocks = (uint64_t)a.batch * a.keys * (few ? 1 : paged_tiles(dtype, a));
-  const uint64_t least = few ? 128 : 256, want = std::max<uint64_t>(1, (few ? 3 * CUS : 2 * CUS) / blocks);
+  const uint64_t least = few ? 128 : 64, want = std::max<uint64_t>(1, (few ? 3 * CUS : 2 * CUS) / blocks);
   uint64_t per = std::max(least, (keys + want - 1) / want);
   per = (per + least - 1) / least * least;
   a.splits = (uint32_t)((keys + per - 1) / per);
@@ -1701,7 +1741,9 @@ void set_splits(int dtype, AttendArgs& a) {
 
 // A gradient's workspace: dy.y of every query, then the parts of dk and dv.
 uint64_t dots_bytes(int dtype, const AttendArgs& a) { return ((uint64_t)a.batch * a.heads * a.length * size_of(dtype) + 255) / 256 * 256; }
-// Parts of a group's heads: as few as leave two blocks for every CU.
+// Parts of a group's heads: as few as leave two blocks for every CU. Packed documents, 4 sequences of 1024, 8
+// heads on 2 of 64 (128 blocks): 135 us and 6 for the sums of four parts, 445 in one; the 3 of 777 above, 6
+// heads on 3: 47 and 5, 84 in one.
 uint32_t parts_of(int dtype, const AttendArgs& a) {
   const uint32_t group = a.heads / a.keys;
   const uint64_t blocks = (uint64_t)a.batch * a.keys * tiles_of(dtype, a);

@@ -169,6 +169,14 @@ def test_refusals():
         assert _code(fn) == code, n
 
 
+def test_scales_that_float32_does_not_hold_are_refused():
+    q, k = rg.ones((1, 4, 2, 8)), rg.ones((1, 4, 2, 8))
+    for kw in ({"scale": 1e31}, {"cap": 1e-31}, {"cap": 1e31}, {"scale": 1e10, "cap": 1e-25}):
+        with pytest.raises(rg.DiagnosticError, match="INVALID_ARGUMENT"):
+            rg.attention(q, k, k, **kw)
+    assert np.isfinite(rg.attention(q, k, k, scale=1e5, cap=1e-20).numpy()).all()
+
+
 def test_paged_refusals():
     x, pages, table, first = _t(2, 1, 8, 8), _t(6, 4, 2, 8), rg.zeros((2, 3), "int32"), _i(1, 2)
     call = lambda x=x, cache=(pages, pages), table=table, first=first, heads=(4, 2), **kw: rg.paged_attention(x, cache=cache, table=table, first=first, heads=heads, **kw)
