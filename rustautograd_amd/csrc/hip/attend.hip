@@ -757,7 +757,7 @@ struct Own {
 };
 
 // Two products a pair. Bound by the matrix unit and the vector unit, which share a SIMD's issue: of the
-// causal case's 121 us (71 TFLOP/s) the first is busy for 57 % and the second, with some 220 instructions
+// causal case's 122 us (70 TFLOP/s) the first is busy for 57 % and the second, with some 220 instructions
 // for a wave's 16 x 32 scores, for 33 %. Heads of 128 over 5000 positions: 331 us, 77 TFLOP/s.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_attend(AttendArgs a) {
@@ -842,7 +842,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others. Three products a
-// pair, bound as the forward is: 181 us in the causal case, 71 TFLOP/s, the matrix unit busy for 59 %.
+// pair, bound as the forward is: 182 us in the causal case, 71 TFLOP/s, the matrix unit busy for 59 %.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dq(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -1000,7 +1000,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 
 // The gradients of k and v: a block's 64 keys against the queries of the heads that read them, all
 // of a group's or, where that leaves too few blocks, a part of them, whose sums k_attend_parts adds up.
-// Four products a pair: 229 us in the causal case, 75 TFLOP/s, the matrix unit busy for 60 %. Scores and
+// Four products a pair: 230 us in the causal case, 75 TFLOP/s, the matrix unit busy for 60 %. Scores and
 // dy.v are formed here a second time; one kernel for all five products would have to add to dq from many
 // blocks, with atomics in an order of their own or a row of partial sums for every 64 keys.
 template <class T, int HD, int RW>
@@ -1701,7 +1701,7 @@ void by_head(int dtype, uint32_t head, uint32_t rows, const F& f) {
 bool wide_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 64u : 32u); }
 bool widest_head(int dtype, uint32_t head) { return head > (dtype == RG_F32 ? 128u : 64u); }
 // Rows of a block: 64, or 32 where those leave fewer than two blocks for every CU, and for heads whose
-// blocks have four waves. Forward, dq, dk and dv of the causal case (512 blocks of 64) 121, 181, 229 us, with 32
+// blocks have four waves. Forward, dq, dk and dv of the causal case (512 blocks of 64) 122, 182, 230 us, with 32
 // rows 152, 201, 242; of 3 sequences of 777, 6 heads of 44 (234 blocks of 64) 31, 40, 47 with 32 rows, with 64
 // 46, 68, 90.
 uint32_t rows_of(int dtype, const AttendArgs& a) {

@@ -190,6 +190,18 @@ def check(case, dtype, device):
         agree(got[k], want[k], off[k], dtype, "d" + k)
 
 
+def check_each_alone(case, dtype, device):
+    """The gradient in one operand alone is that of all of them."""
+    dtype = np.dtype(dtype)
+    case = (*case[:5], case[5].replace("j", ""), case[6])
+    v = inputs(case, dtype)
+    x, dy = {k: rg.tensor(v[k]) for k in ("q", "k", "v", "slopes")}, rg.tensor(v["dy"])
+    grads = lambda names: rg.compile(lambda x: rg.grad(lambda part: (call(case, {**x, **part}, v) * dy).sum())({k: x[k] for k in names}), (x,), validate="none", device=device)(x)
+    want = grads(tuple(x))
+    for k in x:
+        assert np.array_equal(grads((k,))[k].numpy(), want[k].numpy()), k
+
+
 # Of CASES, and where values that are no numbers stand: their place as a share of the length.
 ODD = [(CASES[i], at) for i, at in ((5, 0.3), (6, 0.9), (8, 0.6), (9, 0.2), (11, 0.7), (12, 0.3), (14, 0.5), (15, 0.4), (16, 0.8))] + [(LARGE[1], 0.5), (LARGE[3], 0.9)]
 

@@ -38,6 +38,12 @@ def test_a_token_that_is_no_number(case, bad, dtype):
     ref.check_odd_token(case, bad, dtype, "cpu")
 
 
+@pytest.mark.parametrize("case", [ref.CASES[i] for i in (6, 11, 18)], ids=str)
+def test_a_gradient_alone(case):
+    case = (*case[:5], case[5] + "s" * ("s" not in case[5]), case[6])
+    ref.check_each_alone(case, "float32", "cpu")
+
+
 @pytest.mark.parametrize("case", [ref.PAGED[i] for i in (1, 2, 3, 6)], ids=str)
 def test_pages_that_are_not_there(case):
     ref.check_paged(case, "float32", "cpu", ref.strange_tables)

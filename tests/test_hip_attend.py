@@ -56,6 +56,12 @@ def test_a_token_that_is_no_number(case, bad, dtype):
     ref.check_odd_token(case, bad, dtype, "hip")
 
 
+@pytest.mark.parametrize("case", [ref.CASES[i] for i in (6, 11, 18)], ids=str)
+def test_a_gradient_alone(case):
+    case = (*case[:5], case[5] + "s" * ("s" not in case[5]), case[6])
+    ref.check_each_alone(case, "float32", "hip")
+
+
 @pytest.mark.parametrize("case", [ref.PAGED[i] for i in (1, 2, 3, 6)], ids=str)
 def test_pages_that_are_not_there(case):
     ref.check_paged(case, "float32", "hip", ref.strange_tables)
@@ -342,6 +348,27 @@ def test_a_block_trained_and_then_served():
     # float32 through three updates and nine tokens of two norms and four products each.
     for a, b in zip(got["hip"], got["cpu"]):
         np.testing.assert_allclose(a, b, rtol=1e-4, atol=1e-5)
+
+
+def test_a_decoder_of_several_layers_carries_its_caches():
+    """Three blocks, each with pages of its own, token by token: one captured loop and single calls."""
+    blocks = [nn.TransformerBlock(32, 4, kv_heads=2, cap=7.0, rotary=True) for _ in range(3)]
+    params = [b.init(k) for b, k in zip(blocks, random.split(random.key(3), 3))]
+
+    def step(s, data):
+        x, caches = s["x"], []
+        for block, p, cache in zip(blocks, data, s["caches"]):
+            x, cache = block.extend(p, x, cache)
+            caches.append(cache)
+        return {"x": rg.tanh(x), "caches": caches}
+
+    start = {"x": random.normal(random.key(4), (2, 1, 32)), "caches": [b.state(2, 40, page=6) for b in blocks]}
+    run = rg.run(rg.compile(step, (start, params), validate="none"), start, [params], steps=21).state
+    want = _one_by_one(step, start, params, 21)
+    _same({"x": run["x"]}, {"x": want["x"]})
+    for got, cache in zip(run["caches"], want["caches"]):
+        _same(got, cache)
+        assert cache["pos"].numpy().tolist() == [21, 21]
 
 
 def test_standard_validation_on_the_device():
