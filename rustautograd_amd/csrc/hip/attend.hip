@@ -224,22 +224,31 @@ struct Kept {
   __device__ __forceinline__ void get(int n, T* out) const { take<4>(at + n * 16, out); }
 };
 
-// Two score tiles (rows 0..15 and 16..31 of `lds` against the lane's row).
+// Two score tiles (rows 0..15 and 16..31 of `lds` against the lane's row), each half of the head summed by
+// itself, which halves the length of the chain of roundings.
 template <class T, int HD, class F>
 __device__ __forceinline__ void score(const T* lds, int l16, int g, const F& own, typename Type<T>::acc* s) {
-  s[0] = s[1] = typename Type<T>::acc{0, 0, 0, 0};
+  constexpr int HALF = HD / 32;
+  typename Type<T>::acc late[2];
+  s[0] = s[1] = late[0] = late[1] = typename Type<T>::acc{0, 0, 0, 0};
 #pragma unroll
-  for (int n = 0; n < HD / 16; n++) {
-    T a[4], b[4], x[4];
-    take<4>(lds + l16 * PITCH<T, HD> + n * 16 + 4 * g, a);
-    take<4>(lds + (16 + l16) * PITCH<T, HD> + n * 16 + 4 * g, b);
-    own.get(n, x);
+  for (int m = 0; m < HALF; m++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      s[0] = Type<T>::mfma(a[j], x[j], s[0]);
-      s[1] = Type<T>::mfma(b[j], x[j], s[1]);
+    for (int half = 0; half < 2; half++) {
+      const int n = half * HALF + m;
+      T a[4], b[4], x[4];
+      take<4>(lds + l16 * PITCH<T, HD> + n * 16 + 4 * g, a);
+      take<4>(lds + (16 + l16) * PITCH<T, HD> + n * 16 + 4 * g, b);
+      own.get(n, x);
+      typename Type<T>::acc* to = half == 0 ? s : late;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        to[0] = Type<T>::mfma(a[j], x[j], to[0]);
+        to[1] = Type<T>::mfma(b[j], x[j], to[1]);
+      }
     }
-  }
+  s[0] += late[0];
+  s[1] += late[1];
 }
 
 // acc of the lane's row += the tile's 32 rows weighed by w[t][r]: value row_of(r, g) HD / 16 + n of the
@@ -874,10 +883,13 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
     row_frag<T, HD>(di >= 0 ? gb + (int64_t)i * a.heads * a.head : nullptr, l.g, a.head, whole, x);
     // On the matrix instructions in the order of the products dy.v, so that where one key is all that a
     // query sees both are the same number, and near it nearly so: their difference is the gradient.
-    acc all = {0, 0, 0, 0};
+    acc all = {0, 0, 0, 0}, late = {0, 0, 0, 0};
 #pragma unroll
-    for (int n = 0; n < HD / 4; n++) all = Type<T>::mfma(y[n], x[n], all);
-    dot = Type<T>::diagonal(all, l.l16);
+    for (int n = 0; n < HD / 8; n++) {
+      all = Type<T>::mfma(y[n], x[n], all);
+      late = Type<T>::mfma(y[n + HD / 8], x[n + HD / 8], late);
+    }
+    dot = Type<T>::diagonal(all + late, l.l16);
     grad.set(x, l);
     row_frag<T, HD>(di >= 0 ? qb + (int64_t)i * a.q_row : nullptr, l.g, a.head, whole, x);
     own.set(x, l);
