@@ -225,7 +225,8 @@ struct Kept {
 };
 
 // Two score tiles (rows 0..15 and 16..31 of `lds` against the lane's row), each half of the head summed by
-// itself, which halves the length of the chain of roundings.
+// itself, which halves the length of the chain of roundings (gradients of heads of 64 a third further off with
+// one; dq of the causal case 182 us for 190).
 template <class T, int HD, class F>
 __device__ __forceinline__ void score(const T* lds, int l16, int g, const F& own, typename Type<T>::acc* s) {
   constexpr int HALF = HD / 32;
@@ -766,8 +767,8 @@ struct Own {
 };
 
 // Two products a pair. Bound by the matrix unit and the vector unit, which share a SIMD's issue: of the
-// causal case's 122 us (70 TFLOP/s) the first is busy for 57 % and the second, with some 220 instructions
-// for a wave's 16 x 32 scores, for 33 %. Heads of 128 over 5000 positions: 331 us, 77 TFLOP/s.
+// causal case's 118 us (73 TFLOP/s) the first is busy for 57 % and the second, with some 220 instructions
+// for a wave's 16 x 32 scores, for 33 %. Heads of 128 over 5000 positions: 332 us, 77 TFLOP/s.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD)) k_attend(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::FORWARD
 }
 
 // The gradient of q, of the slopes, and each query's dy.y for the kernel of the others. Three products a
-// pair, bound as the forward is: 182 us in the causal case, 71 TFLOP/s, the matrix unit busy for 59 %.
+// pair, bound as the forward is: 190 us in the causal case, 68 TFLOP/s, the matrix unit busy for 59 %.
 template <class T, int HD, int RW>
 __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWARD)) k_attend_dq(AttendArgs a) {
   typedef Geo<T, HD, RW> G;
@@ -1012,7 +1013,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 
 // The gradients of k and v: a block's 64 keys against the queries of the heads that read them, all
 // of a group's or, where that leaves too few blocks, a part of them, whose sums k_attend_parts adds up.
-// Four products a pair: 230 us in the causal case, 75 TFLOP/s, the matrix unit busy for 60 %. Scores and
+// Four products a pair: 228 us in the causal case, 75 TFLOP/s, the matrix unit busy for 60 %. Scores and
 // dy.v are formed here a second time; one kernel for all five products would have to add to dq from many
 // blocks, with atomics in an order of their own or a row of partial sums for every 64 keys.
 template <class T, int HD, int RW>
