@@ -19,7 +19,9 @@
 // operand's rows in the same order (`row_of`). Results have 16 rows of the tile's other dimension,
 // the head, spread so that a lane ends with consecutive values of its row.
 //
-// Scores, sums, maxima and results are held in the type, scores to base 2.
+// Scores, sums, maxima and results are held in the type. The logarithm's base enters with the bound that a
+// weight's score is lowered by, 2^(log2(e) s - bound) with one rounding, of a difference that is small where
+// the weight is not: scores kept to base 2, and rounded as such, left the slopes' gradients half again as far off.
 //
 // Times below are of one MI355X, whose fp32 matrix product of 8192^3 reaches 154 TFLOP/s and whose copy
 // of 2 GB 4.9 TB/s. "The causal case" is 2 sequences of 2048, 8 heads of 64, capped: 8.6 GFLOP forward.
@@ -135,6 +137,12 @@ __device__ __forceinline__ T row_sum(T x) {
   rg_swap16(x, &a, &b);
   rg_swap32(a + b, &a, &b);
   return a + b;
+}
+
+// 2^(log2(e) s - bound): a weight.
+template <class T>
+__device__ __forceinline__ T weight(T s, T bound) {
+  return Type<T>::exp2_of(fma(s, (T)1.4426950408889634, -bound));
 }
 
 constexpr int TILE = 32;  // rows of the other side in a wave's tile
@@ -288,21 +296,19 @@ __device__ __forceinline__ constexpr int tile_row(int t, int r) {
   return 16 * t + Type<T>::row_of(r, 0);
 }
 
-// The scores of one head, to base 2: cap log2(e) tanh(dot scale / cap) or dot scale log2(e), less slope
-// log2(e) times the distance.
+// The scores of one head: cap tanh(dot scale / cap) or dot scale, less slope times the distance.
 template <class T>
 struct Scorer {
   typedef typename Type<T>::acc acc;
-  T mul, part, cap, slope;  // cap and slope times log2(e); `part`: the scale over the cap
+  T mul, part, cap, slope;  // the scale, and over the cap
   bool capped, sloped;
   __device__ __forceinline__ Scorer(const AttendArgs& a, uint32_t h) {
-    constexpr double LOG2E = 1.4426950408889634;
     capped = a.cap > 0;
     sloped = a.slopes != nullptr;
-    mul = (T)(a.scale * LOG2E);
+    mul = (T)a.scale;
     part = (T)(capped ? a.scale / a.cap : 0);
-    cap = (T)(a.cap * LOG2E);
-    slope = sloped ? (T)((double)((const T*)a.slopes)[h] * LOG2E) : (T)0;
+    cap = (T)a.cap;
+    slope = sloped ? ((const T*)a.slopes)[h] : (T)0;
   }
   // Makes scores of dot products, and leaves the tanh of each (0 without a cap) where asked to.
   // `apart` is the signed distance between the lane's row and row row_of(0, g) of the tile.
@@ -643,8 +649,8 @@ struct Place {
   }
 };
 
-// The running softmax of a row over its keys: a bound that its scores stay near, the sum (of the
-// lane's own keys until the end) and the weighed values. The bound is the largest score when it was
+// The running softmax of a row over its keys: a bound that its scores stay near (to base 2), the sum (of
+// the lane's own keys until the end) and the weighed values. The bound is the largest score when it was
 // last moved; it moves once a score is more than 2^8 times as heavy, and then what there is is scaled.
 template <class T, int HD>
 struct Running {
@@ -669,7 +675,7 @@ struct Running {
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int r = 0; r < 4; r++) most = Type<T>::max_of(most, s[t][r]);
-    most = row_max(most);
+    most = row_max(most) * (T)1.4426950408889634;
     if (__ballot(most > top + 8) != 0) {
       const T next = Type<T>::max_of(top, most);
       scale(Type<T>::exp2_of(top - base(next)));
@@ -680,7 +686,7 @@ struct Running {
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        s[t][r] = Type<T>::exp2_of(s[t][r] - at);
+        s[t][r] = weight(s[t][r], at);
         sum += s[t][r];
       }
   }
@@ -945,7 +951,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) s[t][r] = Type<T>::exp2_of(s[t][r] - top) * by;
+      for (int r = 0; r < 4; r++) s[t][r] = weight(s[t][r], top) * by;
     if (seen_to <= TILE) {
       // All keys of the wave's queries are in this tile: dy.y as the mean of the products dy.v that it is
       // of few, whose roundings then meet in the differences.
@@ -1106,7 +1112,7 @@ __global__ void __launch_bounds__((Geo<T, HD, RW>::NT), (Geo<T, HD, RW>::BACKWAR
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int row = l.set * TILE + 16 * t + Type<T>::row_of(r, l.g);
-        s[t][r] = Type<T>::exp2_of(s[t][r] - tops[row]) * sums[row];
+        s[t][r] = weight(s[t][r], tops[row]) * sums[row];
         dp[t][r] = s[t][r] * (dp[t][r] - dots[row]);
       }
     if (scorer.capped) {
